@@ -157,6 +157,37 @@ int spd_write_req_to_token(int32_t* req_to_token, const int64_t* req_pool_indice
                            int64_t req_to_token_stride, spd_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * cache rows that move between slots, in all layers' pools by one call.  A set is `planes` buffers of equal shape,
+ * plane_stride bytes apart, of `rows` rows of row_bytes bytes each (row = slot); at most 64 sets per call.  Slots outside
+ * [0, rows), requests and positions outside the page table are left out.  Replaces, for one slot list,
+ * MHATokenToKVPool's per-layer index copies (S/mem_cache/memory_pool.py:254-346).
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  void* base;
+  int64_t plane_stride;
+  int64_t rows;
+  int64_t row_bytes;
+  int32_t planes;
+} spd_kv_planes_t;
+/* row dst[i] = row src[i] in every plane, i < n.  No slot is both a source and a destination, none is a destination twice. */
+int spd_kv_copy(const spd_kv_planes_t* sets, int num_sets, const int64_t* src, const int64_t* dst, int64_t n,
+                spd_stream_t stream);
+/* children[i] becomes a copy of request parents[i] (seq_lens[i] tokens), i < n: their page-table rows share the slots of
+ * the whole runs of run_len tokens, and the tokens behind those are copied to the slots tail_slots[i], tail_slots[i] + 1, ...
+ * requests x max_tokens entries of req_to_token are in use.  No child is a parent or a child twice. */
+int spd_kv_fork(const spd_kv_planes_t* sets, int num_sets, int32_t* req_to_token, int64_t req_to_token_stride, int64_t requests,
+                int64_t max_tokens, const int64_t* parents, const int64_t* children, const int64_t* seq_lens,
+                const int64_t* tail_slots, int64_t n, int run_len, spd_stream_t stream);
+/* Request src_requests[i] goes on, as request dst_requests[i], with the tokens at its positions keep[keep_indptr[i] ..
+ * keep_indptr[i + 1]), in that order: their rows are copied to the slots loc[...] (of no token that is kept), which become the first
+ * entries of the page-table row.  dst_requests NULL: in place; otherwise none of them is a source.  total = keep_indptr[n].
+ * write_table 0: the page table stays as it is (planes that take more than one call). */
+int spd_kv_compact(const spd_kv_planes_t* sets, int num_sets, int32_t* req_to_token, int64_t req_to_token_stride,
+                   int64_t requests, int64_t max_tokens, const int64_t* src_requests, const int64_t* dst_requests,
+                   const int64_t* keep, const int64_t* keep_indptr, const int64_t* loc, int64_t n, int64_t total,
+                   int write_table, spd_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * OPT-family ops (opt-125m: plumbing + logit check).  The reference has no OPT
  * model; these follow torch.nn.LayerNorm / F.relu / the `residual + hidden_states` adds of
  * transformers' modeling_opt.py (OPTDecoderLayer.forward), fp32 math, 16-bit I/O.
@@ -263,6 +294,22 @@ int spd_attn_decode_paged_own(void* out, const void* q, const void* k_pool, cons
                               int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
                               int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace,
                               int64_t workspace_bytes, int sm_budget, spd_stream_t stream);
+/* Decode attention for requests that continue the same tokens.  Rows [group_indptr[g], group_indptr[g + 1]) of the batch
+ * (int32, num_groups + 1 entries, ascending) are a group whose members' req_to_token rows name the same slots in their first
+ * shared_lens[g] positions; max_shared_len is no less than any of those.  The result is spd_attn_decode_paged's: every row of
+ * req_to_token is complete, rows of no group stand alone, seq_lens[b] counts the shared tokens too, and a request of length
+ * 0 gets zeros.  The shared part of a group is read once for all of its queries.
+ * Workspace: spd_attn_decode_shared_workspace_bytes(), zeroed once before its first use (each call leaves its counters at
+ * zero), one per stream.
+ * The reference has no such call; its cascade form is flashinfer's, behind the same wrapper interface as
+ * S/layers/attention/flashinfer_backend.py:454-488. */
+int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_heads, int num_kv_heads, int head_dim);
+int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
+                           const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
+                           const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t max_shared_len,
+                           int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
+                           int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
+                           int sm_budget, spd_stream_t stream);
 /* Plain SIMT implementations of the two calls above (no tensor cores).  Bring-up / on-device
  * cross-check only; the product path never calls them. */
 int spd_attn_prefill_simt(void* out, const void* q, const void* k_pool, const void* v_pool,

@@ -89,6 +89,14 @@ SIGNATURES = {
         _i,
         [_p, _p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i64, _i64, _i64, _f, _i, _p, _i64, _i, _p],
     ),
+    "spd_attn_decode_shared_workspace_bytes": (_i64, [_i64, _i, _i, _i]),
+    "spd_attn_decode_shared": (
+        _i,
+        [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _i, _i, _i64, _i64, _i64, _f, _i, _p, _i64, _i, _p],
+    ),
+    "spd_kv_copy": (_i, [_p, _i, _p, _p, _i64, _p]),
+    "spd_kv_fork": (_i, [_p, _i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _i, _p]),
+    "spd_kv_compact": (_i, [_p, _i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i, _p]),
     "spd_comm_create": (_i, [_i, _i, _i64, C.POINTER(_p), _p]),
     "spd_comm_connect": (_i, [_p, _p]),
     "spd_comm_max_bytes": (_i64, [_p]),
@@ -244,6 +252,11 @@ class RotarySegment(C.Structure):
     _fields_ = [("src", _p), ("bias", _p), ("dst", _p), ("src_row", _i64), ("dst_row", _i64), ("heads", C.c_int32),
                 ("head_dim", C.c_int32), ("rot", C.c_int32), ("src_head", C.c_int32), ("dst_head", C.c_int32),
                 ("to_pool", C.c_int32), ("norm_w", _p), ("norm", C.c_int32), ("norm_eps", _f)]
+
+
+class KVPlaneSet(C.Structure):
+    """spd_kv_planes_t of include/spd.h."""
+    _fields_ = [("base", _p), ("plane_stride", _i64), ("rows", _i64), ("row_bytes", _i64), ("planes", C.c_int32)]
 
 
 def declared_functions(header_path: str = HEADER_PATH):

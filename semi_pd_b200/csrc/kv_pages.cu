@@ -1,0 +1,262 @@
+// Rows of the cache that move between slots, in all layers' pools at once: copying, forking and compacting requests.
+// The pools are "planes" of equally long rows, one row per slot; a request's tokens are its entries of req_to_token.
+//
+// Nothing is computed: a call moves 2 x rows x bytes of a token and should take what those bytes take.  A block owns a few
+// rows of one plane: their slots are looked up once, in parallel, into shared memory, and its threads then walk the rows'
+// 16-byte pieces as one list, kKvUnroll of them loaded before the first is stored.
+#include "common.cuh"
+#include "prefill_tiles.cuh"
+#include "ptx.cuh"
+
+namespace spd {
+
+constexpr int kKvThreads = 256;
+constexpr int kKvRows = 64;    // rows of a block at most
+constexpr int kKvUnroll = 4;
+constexpr int kKvSets = 64;
+
+struct KvSet {
+  char* base;
+  int64_t stride;     // bytes between planes
+  int64_t rows;       // slots
+  int64_t row_bytes;
+  int first;          // planes of the sets before
+  uint32_t pieces_m, pieces_s;  // division by the pieces of a row
+};
+struct KvPlanes {
+  int sets, planes;
+  KvSet set[kKvSets];
+};
+
+// where the rows of a call lie
+struct KvCopyRows {
+  const int64_t *src, *dst;
+  int64_t n;
+};
+struct KvForkRows {
+  const int64_t *parents, *children, *lens, *tail;
+  int32_t* table;
+  int64_t stride, requests, width;
+  int run_len;
+};
+struct KvCompactRows {
+  const int64_t *src, *dst, *keep, *indptr, *loc;
+  int32_t* table;
+  int64_t stride, requests, width, n, total;
+};
+
+// the last request whose first row is not behind row j
+__device__ __forceinline__ int64_t kv_request(const int64_t* indptr, int64_t n, int64_t j) {
+  int64_t lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) >> 1;
+    if (indptr[mid] <= j) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// rows [first, first + count) of this block -> (source, destination) slots; a row with a slot of -1 stays as it is
+__device__ __forceinline__ int kv_rows(const KvCopyRows& r, int per_block, int64_t* src, int64_t* dst) {
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
+  const int count = static_cast<int>(min(static_cast<int64_t>(per_block), r.n - first));
+  for (int i = threadIdx.x; i < count; i += kKvThreads) {
+    src[i] = r.src[first + i];
+    dst[i] = r.dst[first + i];
+  }
+  return count;
+}
+__device__ __forceinline__ int kv_rows(const KvForkRows& r, int per_block, int64_t* src, int64_t* dst) {
+  const int64_t parent = r.parents[blockIdx.z], len = r.lens[blockIdx.z], tail = r.tail[blockIdx.z];
+  if (parent < 0 || parent >= r.requests || len < 0 || len > r.width) return 0;
+  const int64_t full = len / r.run_len * r.run_len, first = static_cast<int64_t>(blockIdx.x) * per_block;
+  const int count = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(per_block), len - full - first)));
+  for (int i = threadIdx.x; i < count; i += kKvThreads) {
+    src[i] = r.table[parent * r.stride + full + first + i];
+    dst[i] = tail + first + i;
+  }
+  return count;
+}
+__device__ __forceinline__ int kv_rows(const KvCompactRows& r, int per_block, int64_t* src, int64_t* dst) {
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
+  const int count = static_cast<int>(min(static_cast<int64_t>(per_block), r.total - first));
+  for (int i = threadIdx.x; i < count; i += kKvThreads) {
+    const int64_t j = first + i, request = r.src[kv_request(r.indptr, r.n, j)], pos = r.keep[j];
+    const bool ok = request >= 0 && request < r.requests && pos >= 0 && pos < r.width;
+    src[i] = ok ? r.table[request * r.stride + pos] : -1;
+    dst[i] = r.loc[j];
+  }
+  return count;
+}
+
+// the page table's part of a call
+__device__ __forceinline__ void kv_table(const KvCopyRows&) {}
+__device__ __forceinline__ void kv_table(const KvForkRows& r) {
+  const int64_t parent = r.parents[blockIdx.z], child = r.children[blockIdx.z], len = r.lens[blockIdx.z], tail = r.tail[blockIdx.z];
+  if (parent < 0 || parent >= r.requests || child < 0 || child >= r.requests || child == parent || len < 0 || len > r.width) return;
+  const int64_t full = len / r.run_len * r.run_len;
+  const int32_t* from = r.table + parent * r.stride;
+  int32_t* to = r.table + child * r.stride;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kKvThreads + threadIdx.x; i < len; i += static_cast<int64_t>(gridDim.x) * kKvThreads)
+    to[i] = i < full ? from[i] : static_cast<int32_t>(tail + i - full);
+}
+__device__ __forceinline__ void kv_table(const KvCompactRows& r) {
+  for (int64_t j = static_cast<int64_t>(blockIdx.x) * kKvThreads + threadIdx.x; j < r.total;
+       j += static_cast<int64_t>(gridDim.x) * kKvThreads) {
+    const int64_t i = kv_request(r.indptr, r.n, j), at = j - r.indptr[i], request = r.dst[i];
+    if (request >= 0 && request < r.requests && at >= 0 && at < r.width) r.table[request * r.stride + at] = static_cast<int32_t>(r.loc[j]);
+  }
+}
+
+// V: the piece that a thread moves at a time, 16 bytes where rows and pointers allow it
+template <typename V, typename Rows>
+__global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_constant__ KvPlanes pl, const Rows rows, int per_block) {
+  __shared__ int64_t s_src[kKvRows], s_dst[kKvRows];
+  griddep_launch_dependents();
+  griddep_wait();
+  if (static_cast<int>(blockIdx.y) == pl.planes) {
+    kv_table(rows);
+    return;
+  }
+  const int count = kv_rows(rows, per_block, s_src, s_dst);
+  if (count <= 0) return;
+  int si = 0;
+  while (si + 1 < pl.sets && static_cast<int>(blockIdx.y) >= pl.set[si + 1].first) ++si;
+  const KvSet& set = pl.set[si];
+  const int pieces = static_cast<int>(set.row_bytes / sizeof(V));
+  char* plane = set.base + (static_cast<int>(blockIdx.y) - set.first) * set.stride;
+  __syncthreads();
+  const int total = count * pieces;
+  for (int i0 = threadIdx.x; i0 < total; i0 += kKvThreads * kKvUnroll) {
+    V v[kKvUnroll];
+    V* to[kKvUnroll];
+#pragma unroll
+    for (int k = 0; k < kKvUnroll; ++k) {
+      const int i = i0 + k * kKvThreads;
+      to[k] = nullptr;
+      if (i < total) {
+        const int row = fastdiv(i, set.pieces_m, set.pieces_s), at = i - row * pieces;
+        const int64_t s = s_src[row], d = s_dst[row];
+        if (s >= 0 && s < set.rows && d >= 0 && d < set.rows) {
+          v[k] = __ldcs(reinterpret_cast<const V*>(plane + s * set.row_bytes) + at);
+          to[k] = reinterpret_cast<V*>(plane + d * set.row_bytes) + at;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kKvUnroll; ++k)
+      if (to[k]) *to[k] = v[k];
+  }
+}
+
+// req_to_token rows of requests that were compacted in place: after the kernel that reads them
+__global__ void __launch_bounds__(kKvThreads) kv_table_kernel(const KvCompactRows rows) {
+  griddep_launch_dependents();
+  griddep_wait();
+  kv_table(rows);
+}
+
+// The plane sets as the kernel takes them, and the bytes of a piece that suits all of them (0 and an error otherwise).
+static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, KvPlanes& pl, int& piece) {
+  SPD_REQUIRE(sets && num_sets > 0 && num_sets <= kKvSets, SPD_E_BADARG, "%s: 1 to %d plane sets (got %d)", fn, kKvSets, num_sets);
+  pl.sets = num_sets;
+  pl.planes = 0;
+  piece = 16;
+  for (int i = 0; i < num_sets; ++i) {
+    const spd_kv_planes_t& s = sets[i];
+    SPD_REQUIRE(s.base && s.planes > 0 && s.rows > 0 && s.row_bytes > 0 && s.plane_stride >= 0, SPD_E_BADARG, "%s: bad plane set", fn);
+    SPD_REQUIRE(s.row_bytes % 2 == 0 && s.row_bytes <= (1 << 20) && s.plane_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(s.base) & 1) == 0,
+                SPD_E_ALIGN, "%s: rows of an even number of bytes, 1 MB at most", fn);
+    const uint64_t bits = reinterpret_cast<uintptr_t>(s.base) | s.row_bytes | s.plane_stride;
+    while (bits % piece) piece >>= 1;
+    pl.set[i].base = static_cast<char*>(s.base);
+    pl.set[i].stride = s.plane_stride;
+    pl.set[i].rows = s.rows;
+    pl.set[i].row_bytes = s.row_bytes;
+    pl.set[i].first = pl.planes;
+    pl.planes += s.planes;
+    SPD_REQUIRE(pl.planes < 65535, SPD_E_SHAPE, "%s: too many planes", fn);
+  }
+  for (int i = 0; i < num_sets; ++i)
+    fastdiv_magic(static_cast<uint32_t>(pl.set[i].row_bytes / piece), pl.set[i].pieces_m, pl.set[i].pieces_s);
+  return 0;
+}
+
+// Rows of a block: 32 KB of them, fewer where the call would not give every SM four blocks, and 4 KB at least.
+static int kv_rows_per_block(const KvPlanes& pl, int64_t rows) {
+  int64_t bytes = 0;
+  for (int i = 0; i < pl.sets; ++i) bytes = bytes > pl.set[i].row_bytes ? bytes : pl.set[i].row_bytes;
+  int64_t per = (32768 + bytes - 1) / bytes;
+  const int64_t spread = rows * pl.planes / (4 * device_sm_count_cached()), least = (4096 + bytes - 1) / bytes;
+  if (per > spread) per = spread;
+  if (per < least) per = least;
+  return static_cast<int>(per < 1 ? 1 : per > kKvRows ? kKvRows : per);
+}
+
+template <typename Rows>
+static int kv_move(const KvPlanes& pl, int piece, const Rows& rows, int64_t n, int per_block, int64_t z, bool table, cudaStream_t st) {
+  const int64_t x = (n + per_block - 1) / per_block;
+  SPD_REQUIRE(x < (1ll << 31) && z < 65536, SPD_E_SHAPE, "kv move: too many rows");
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(pl.planes + (table ? 1 : 0)), static_cast<unsigned>(z));
+#define SPD_KV_MOVE(V) SPD_CUDA(launch(kv_move_kernel<V, Rows>, grid, dim3(kKvThreads), 0, st, pdl_enabled(), pl, rows, per_block))
+  switch (piece) {
+    case 16: SPD_KV_MOVE(uint4); break;
+    case 8: SPD_KV_MOVE(uint2); break;
+    case 4: SPD_KV_MOVE(uint32_t); break;
+    default: SPD_KV_MOVE(unsigned short);
+  }
+#undef SPD_KV_MOVE
+  return 0;
+}
+
+}  // namespace spd
+
+using namespace spd;
+
+extern "C" {
+
+int spd_kv_copy(const spd_kv_planes_t* sets, int num_sets, const int64_t* src, const int64_t* dst, int64_t n, spd_stream_t stream) {
+  KvPlanes pl;
+  int piece;
+  if (int rc = kv_planes("spd_kv_copy", sets, num_sets, pl, piece)) return rc;
+  SPD_REQUIRE(n >= 0 && n < (1ll << 31) && (n == 0 || (src && dst)), SPD_E_BADARG, "spd_kv_copy: bad slots");
+  if (n == 0) return 0;
+  return kv_move(pl, piece, KvCopyRows{src, dst, n}, n, kv_rows_per_block(pl, n), 1, false, as_stream(stream));
+}
+
+int spd_kv_fork(const spd_kv_planes_t* sets, int num_sets, int32_t* req_to_token, int64_t req_to_token_stride, int64_t requests,
+                int64_t max_tokens, const int64_t* parents, const int64_t* children, const int64_t* seq_lens, const int64_t* tail_slots,
+                int64_t n, int run_len, spd_stream_t stream) {
+  KvPlanes pl;
+  int piece;
+  if (int rc = kv_planes("spd_kv_fork", sets, num_sets, pl, piece)) return rc;
+  SPD_REQUIRE(req_to_token && n >= 0 && (n == 0 || (parents && children && seq_lens && tail_slots)) && requests > 0 &&
+                  max_tokens > 0 && run_len > 0 && req_to_token_stride >= max_tokens,
+              SPD_E_BADARG, "spd_kv_fork: bad arguments");
+  SPD_REQUIRE(n < 65536, SPD_E_SHAPE, "spd_kv_fork: at most 65535 children (got %lld)", (long long)n);
+  if (n == 0) return 0;
+  const KvForkRows rows{parents, children, seq_lens, tail_slots, req_to_token, req_to_token_stride, requests, max_tokens, run_len};
+  return kv_move(pl, piece, rows, run_len - 1 > 0 ? run_len - 1 : 1, kv_rows_per_block(pl, n * run_len / 2), n, true, as_stream(stream));
+}
+
+int spd_kv_compact(const spd_kv_planes_t* sets, int num_sets, int32_t* req_to_token, int64_t req_to_token_stride, int64_t requests,
+                   int64_t max_tokens, const int64_t* src_requests, const int64_t* dst_requests, const int64_t* keep,
+                   const int64_t* keep_indptr, const int64_t* loc, int64_t n, int64_t total, int write_table, spd_stream_t stream) {
+  KvPlanes pl;
+  int piece;
+  if (int rc = kv_planes("spd_kv_compact", sets, num_sets, pl, piece)) return rc;
+  SPD_REQUIRE(req_to_token && n >= 0 && total >= 0 && total < (1ll << 31) && requests > 0 && max_tokens > 0 &&
+                  req_to_token_stride >= max_tokens && (n == 0 || total == 0 || (src_requests && keep && keep_indptr && loc)),
+              SPD_E_BADARG, "spd_kv_compact: bad arguments");
+  if (n == 0 || total == 0) return 0;
+  KvCompactRows rows{src_requests, dst_requests, keep, keep_indptr, loc, req_to_token, req_to_token_stride, requests, max_tokens, n, total};
+  if (int rc = kv_move(pl, piece, rows, total, kv_rows_per_block(pl, total), 1, write_table && dst_requests, as_stream(stream))) return rc;
+  if (write_table && !dst_requests) {
+    rows.dst = src_requests;
+    const int64_t blocks = (total + kKvThreads - 1) / kKvThreads;
+    SPD_CUDA(launch(kv_table_kernel, dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), dim3(kKvThreads), 0, as_stream(stream),
+                    pdl_enabled(), rows));
+  }
+  return 0;
+}
+
+}  // extern "C"

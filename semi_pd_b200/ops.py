@@ -9,6 +9,7 @@ torch is plumbing here (device memory + streams); every computation runs in libs
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import functools
 import os
 from typing import Optional
@@ -48,6 +49,14 @@ def _cuda(*ts: torch.Tensor) -> None:
             raise RuntimeError(
                 "libspd ops need CUDA tensors: there is no CPU path (got a tensor on %s)" % t.device
             )
+
+
+def _here(fn: str, *ts: Optional[torch.Tensor]) -> None:
+    """Tensors on the device whose current stream the call goes to."""
+    here = torch._C._cuda_getDevice()
+    for t in ts:
+        if t is not None and t.device.index != here:
+            raise RuntimeError(f"{fn}: a tensor is on {t.device}, the current device is cuda:{here}")
 
 
 # ------------------------------------------------------------------------------------------------
@@ -297,6 +306,114 @@ def write_req_to_token_pool(req_to_token: torch.Tensor, req_pool_indices: torch.
     check(lib.spd_write_req_to_token(req_to_token.data_ptr(), *[a.data_ptr() for a in args],
                                      args[0].numel(), req_to_token.stride(0), _stream()),
           "spd_write_req_to_token")
+
+
+# ------------------------------------------------------------------------------------------------
+# rows of the cache that move between slots, in all layers' pools at once
+# ------------------------------------------------------------------------------------------------
+class KVPlanes:
+    """The buffers of a pool (one row per slot, contiguous; keys, values or latent rows of every layer) as kv_copy, kv_fork
+    and kv_compact take them.  Made once per pool; a buffer that layers share counts once.  Keeps the buffers alive."""
+
+    MAX_SETS = 64  # of a call
+
+    def __init__(self, buffers):
+        seen = {}
+        for b in buffers:
+            if b is not None and b.numel() and (b.data_ptr(), b.numel()) not in seen:
+                seen[b.data_ptr(), b.numel()] = b
+        self.buffers = list(seen.values())
+        if not self.buffers:
+            raise RuntimeError("KVPlanes: no buffers")
+        if any(b.dim() < 2 or not b.is_contiguous() for b in self.buffers):
+            raise RuntimeError("KVPlanes: buffers are contiguous, one row per slot")
+        if len({b.device for b in self.buffers}) > 1:
+            raise RuntimeError("KVPlanes: buffers are on one device")
+        self.device = self.buffers[0].device
+        sets = []  # [base, stride, rows, row_bytes, planes]
+        for b in self.buffers:
+            at, rows, size = b.data_ptr(), b.shape[0], b.numel() // b.shape[0] * b.element_size()
+            last = sets[-1] if sets else None
+            if last is not None and last[2:4] == [rows, size] and (last[4] == 1 and at > last[0] or at == last[0] + last[1] * last[4]):
+                if last[4] == 1:
+                    last[1] = at - last[0]
+                last[4] += 1
+            else:
+                sets.append([at, 0, rows, size, 1])
+        self.token_bytes = sum(s[3] * s[4] for s in sets)
+        self.calls = []  # (address, sets) of every call that an operator makes
+        self._arrays = []
+        for i in range(0, len(sets), self.MAX_SETS):
+            part = sets[i:i + self.MAX_SETS]
+            arr = (_lib.KVPlaneSet * len(part))(*[_lib.KVPlaneSet(*s) for s in part])
+            self._arrays.append(arr)
+            self.calls.append((ctypes.addressof(arr), len(part)))
+
+    def _check(self, fn: str, *ts: torch.Tensor) -> None:
+        _cuda(self.buffers[0], *ts)
+        _here(fn, self.buffers[0], *ts)
+
+
+def _kv_lists(fn: str, **lists: torch.Tensor) -> None:
+    for name, t in lists.items():
+        if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+            raise RuntimeError(f"{fn}: {name} must be a contiguous int64 list")
+
+
+def _kv_table(fn: str, req_to_token: torch.Tensor) -> tuple:
+    if req_to_token.dtype != torch.int32 or req_to_token.dim() != 2 or req_to_token.stride(1) != 1:
+        raise RuntimeError(f"{fn}: req_to_token is int32 with contiguous rows")
+    return req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[0], req_to_token.shape[1]
+
+
+def kv_copy(planes: KVPlanes, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Row dst[i] = row src[i] of every buffer (int64 slots).  No slot is both a source and a destination, none is a
+    destination twice; pairs with a slot outside the pool are left out."""
+    planes._check("kv_copy", src, dst)
+    _kv_lists("kv_copy", src=src, dst=dst)
+    if src.numel() != dst.numel():
+        raise RuntimeError("kv_copy: as many sources as destinations")
+    for at, n in planes.calls:
+        check(lib.spd_kv_copy(at, n, src.data_ptr(), dst.data_ptr(), src.numel(), _stream()), "spd_kv_copy")
+
+
+def kv_fork(planes: KVPlanes, req_to_token: torch.Tensor, parents: torch.Tensor, children: torch.Tensor,
+            seq_lens: torch.Tensor, tail_slots: torch.Tensor, run_len: int) -> None:
+    """Request children[i] becomes a copy of request parents[i], which has seq_lens[i] tokens: their page-table rows share the
+    slots of the whole runs of run_len tokens; the tokens behind those are copied to the slots tail_slots[i] and following.
+    All int64 lists on the device.  No child is a parent or a child twice."""
+    planes._check("kv_fork", req_to_token, parents, children, seq_lens, tail_slots)
+    _kv_lists("kv_fork", parents=parents, children=children, seq_lens=seq_lens, tail_slots=tail_slots)
+    n = parents.numel()
+    if children.numel() != n or seq_lens.numel() != n or tail_slots.numel() != n:
+        raise RuntimeError("kv_fork: one parent, length and tail slot per child")
+    if run_len < 1:
+        raise RuntimeError("kv_fork: run_len must be positive")
+    table = _kv_table("kv_fork", req_to_token)
+    for at, sets in planes.calls:
+        check(lib.spd_kv_fork(at, sets, *table, parents.data_ptr(), children.data_ptr(), seq_lens.data_ptr(),
+                              tail_slots.data_ptr(), n, int(run_len), _stream()), "spd_kv_fork")
+
+
+def kv_compact(planes: KVPlanes, req_to_token: torch.Tensor, src_requests: torch.Tensor, dst_requests: Optional[torch.Tensor],
+               keep: torch.Tensor, keep_indptr: torch.Tensor, loc: torch.Tensor) -> None:
+    """Request src_requests[i] goes on as request dst_requests[i] with a part of its tokens: those at its positions
+    keep[keep_indptr[i]:keep_indptr[i + 1]], in that order, copied to the slots loc[...], which become the first entries of the
+    page-table row.  dst_requests None: in place; otherwise none of them is a source.  No slot of `loc` holds a kept token.
+    All int64 lists on the device."""
+    planes._check("kv_compact", req_to_token, src_requests, keep, keep_indptr, loc, dst_requests)
+    _kv_lists("kv_compact", src_requests=src_requests, keep=keep, keep_indptr=keep_indptr, loc=loc)
+    n = src_requests.numel()
+    if dst_requests is not None:
+        _kv_lists("kv_compact", dst_requests=dst_requests)
+    if (dst_requests is not None and dst_requests.numel() != n) or keep_indptr.numel() != n + 1 or keep.numel() != loc.numel():
+        raise RuntimeError("kv_compact: one destination per request, one more offset, one new slot per kept token")
+    table = _kv_table("kv_compact", req_to_token)
+    dst = dst_requests.data_ptr() if dst_requests is not None else None
+    for at, sets in planes.calls:  # the page table, which all of them read, is written by the last one
+        check(lib.spd_kv_compact(at, sets, *table, src_requests.data_ptr(), dst, keep.data_ptr(), keep_indptr.data_ptr(),
+                                 loc.data_ptr(), n, keep.numel(), 1 if at == planes.calls[-1][0] else 0, _stream()),
+              "spd_kv_compact")
 
 
 # ------------------------------------------------------------------------------------------------
@@ -664,6 +781,61 @@ def attn_decode(q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, num
               "spd_attn_decode_simt")
     else:
         raise ValueError(impl)
+    return out
+
+
+def new_attn_shared_workspace(device, max_batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> torch.Tensor:
+    """Scratch of attn_decode_shared for batches up to max_batch: zeroed here, left so by every call, one stream at a time."""
+    need = lib.spd_attn_decode_shared_workspace_bytes(max_batch, num_q_heads, num_kv_heads, head_dim)
+    return torch.zeros((need,), dtype=torch.uint8, device=device)
+
+
+def attn_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, req_to_token: torch.Tensor,
+                       req_pool_indices: torch.Tensor, seq_lens: torch.Tensor, group_indptr: torch.Tensor,
+                       shared_lens: torch.Tensor, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                       sm_scale: float, out: Optional[torch.Tensor] = None,
+                       workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attn_decode for a batch in which groups of requests continue the same tokens: the rows group_indptr[g] ..
+    group_indptr[g + 1] of the batch (int32 [groups + 1], ascending) have the same slots in the first shared_lens[g] (int64
+    [groups]) entries of their req_to_token rows, which are read once for all of them.  The result is attn_decode's; seq_lens
+    counts the shared tokens too, rows outside every group stand alone.  max_shared_len: a bound of shared_lens that the host
+    knows (in a captured graph: of all replays).  workspace: new_attn_shared_workspace's, zeroed once, never replaced, one
+    stream at a time; without one every call takes and zeroes its own."""
+    _cuda(q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, group_indptr, shared_lens, out, workspace)
+    _here("attn_decode_shared", q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, group_indptr, shared_lens, out, workspace)
+    B, G = seq_lens.numel(), shared_lens.numel()
+    if q.shape[0] != B or req_pool_indices.numel() != B or q.numel() != B * num_q_heads * head_dim:
+        raise RuntimeError("attn_decode_shared: q is [batch, heads * head_dim], one request slot and length per row")
+    if not (q.dtype == k_pool.dtype == v_pool.dtype):
+        raise RuntimeError("attn_decode_shared: q and the pools share a dtype")
+    row = (num_kv_heads, head_dim)
+    if any(t.dim() != 3 or tuple(t.shape[1:]) != row or not t.is_contiguous() for t in (k_pool, v_pool)):
+        raise RuntimeError("attn_decode_shared: the pools are contiguous [slots, kv heads, head_dim]")
+    if req_to_token.dtype != torch.int32 or req_to_token.dim() != 2 or req_to_token.stride(1) != 1:
+        raise RuntimeError("attn_decode_shared: req_to_token is int32 with contiguous rows")
+    if any(t.dtype != torch.int64 or not t.is_contiguous() for t in (req_pool_indices, seq_lens, shared_lens)):
+        raise RuntimeError("attn_decode_shared: req_pool_indices, seq_lens and shared_lens must be contiguous int64")
+    if group_indptr.dtype != torch.int32 or group_indptr.numel() != G + 1 or not group_indptr.is_contiguous():
+        raise RuntimeError("attn_decode_shared: group_indptr must be int32 with one entry more than shared_lens")
+    if max_shared_len < 0:
+        raise RuntimeError("attn_decode_shared: max_shared_len must not be negative")
+    if out is None:
+        out = torch.empty(B, num_q_heads * head_dim, device=q.device, dtype=q.dtype)
+    if out.dtype != q.dtype or out.numel() != q.numel() or out.shape[0] != B:
+        raise RuntimeError("attn_decode_shared: out must have q's shape and dtype")
+    if B == 0:
+        return out
+    q2, o2 = q.view(B, -1), out.view(B, -1)
+    if q2.stride(1) != 1 or o2.stride(1) != 1:
+        raise RuntimeError("attn_decode_shared: q and out must have contiguous rows")
+    if workspace is None:
+        workspace = new_attn_shared_workspace(q.device, B, num_q_heads, num_kv_heads, head_dim)
+    check(lib.spd_attn_decode_shared(o2.data_ptr(), q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), req_to_token.data_ptr(),
+                                     req_pool_indices.data_ptr(), seq_lens.data_ptr(), group_indptr.data_ptr(),
+                                     shared_lens.data_ptr(), B, G, int(max_shared_len), num_q_heads, num_kv_heads, head_dim,
+                                     q2.stride(0), o2.stride(0), req_to_token.stride(0), float(sm_scale), _dt(q),
+                                     workspace.data_ptr(), workspace.numel(), get_sm_budget(), _stream()),
+          "spd_attn_decode_shared")
     return out
 
 
