@@ -44,7 +44,6 @@
 
 #include "common.cuh"
 #include "ptx.cuh"
-#include "shared_groups.cuh"
 #include "tmap.cuh"
 
 namespace spd {
@@ -59,10 +58,7 @@ constexpr int kDcQBytes = 16 * 128 * 2;   // [16 rows x 128 d] as two 2 KB swizz
 constexpr int kDcLenCache = 1024;         // seq_lens cached in smem
 constexpr int kDcQBufs = 4;  // Q staging buffers: item i uses i % 4 (see the loader)
 constexpr int kDcMisc = 1024 + kDcLenCache * 4;
-constexpr int kDcMiscShared = kDcMisc + kShRows * 2 + static_cast<int>(sizeof(SharedPlan));
 constexpr int kDcSmem = kDcStages * 2 * kDcTileBytes + (kDcQBufs + 2) * kDcQBytes + 1024 + kDcMisc;
-constexpr int kDcSmemShared = kDcSmem - kDcMisc + kDcMiscShared;
-static_assert(kDcSmemShared <= 232448 && kShRows == kDcLenCache, "shared memory of one block");
 constexpr int kDcMaxGroup = 8;
 constexpr int kDcItemUnits = 1;   // what an item's epilogue costs, in tiles: it counts in the work split
 constexpr int kDcMinUnits = 2;    // a share shorter than two tiles costs more in merge traffic than it saves in streaming
@@ -84,18 +80,7 @@ struct DecodeParams {
   float* ml_part;  // [2 * grid][G][2]
   int* counters;   // [b][Hk]
   int use_tma;     // 0: always gather (SPD_ATTN_TMA=0)
-  SharedGroups sg;         // kShared: the requests' groups and what attn_shared.cu leaves of them
-  unsigned* wait_expired;  // kShared
 };
-
-// kShared: bounded (see mbar_wait_bounded)
-template <bool kShared>
-__device__ __forceinline__ void dc_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-  if constexpr (kShared)
-    mbar_wait_bounded(bar, parity, dead);
-  else
-    mbar_wait(bar, parity);
-}
 
 __device__ __forceinline__ int dc_len(const DecodeParams& p, const int* s_len, int b) {
   return b < kDcLenCache ? s_len[b] : static_cast<int>(p.seq_lens[b]);
@@ -191,12 +176,7 @@ __device__ __forceinline__ bool softmax_bar_or(bool pred) {
 }
 __device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// kShared: the requests' own tokens behind the keys that their groups share (shared_groups.cuh); lengths and tiles then count
-// from a request's first own token, and an item's result is joined with the parts that attn_shared.cu left.  That kernel
-// is the one before in the stream and waits, before it lets this one in, for all that came before it; so what this kernel
-// reads of the batch and of the pools stands in memory when it starts, and it waits for that kernel (griddep_wait) only
-// before the first join: its CTAs take over the SMs one by one.
-template <typename T, bool kShared>
+template <typename T>
 __global__ void __launch_bounds__(kDcThreads, 1)
 attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const DecodeParams p) {
@@ -221,14 +201,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   uint64_t* o_empty = bars + 21;   // 2
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   int* flag_slot = reinterpret_cast<int*>(tmem_slot + 1);
-  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 2);  // kShared
   float* red = reinterpret_cast<float*>(misc + 256);   // [4 warps][8 heads] scratch (+ 8 totals)
   int* s_len = reinterpret_cast<int*>(misc + 1024);    // seq_lens[0 .. kDcLenCache)
   int* s_scan = reinterpret_cast<int*>(misc + 512);    // [9] warps' units; then the range's start: request, kv head, units before
-
-  uint16_t* s_group = reinterpret_cast<uint16_t*>(misc + kDcMisc);                    // kShared: [kShRows], kNoGroup: none
-  SharedPlan& plan = *reinterpret_cast<SharedPlan*>(misc + kDcMisc + kShRows * 2);  // kShared
-  constexpr uint16_t kNoGroup = 0xffff;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -236,7 +211,6 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 
   if (warp == 8) {
     if (lane == 0) {
-      if constexpr (kShared) *dead = 0;
       for (int i = 0; i < kDcStages; ++i) {
         mbar_init(&k_full[i], 64);
         mbar_init(&k_empty[i], 1);
@@ -270,25 +244,13 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   // wait for the predecessor.  A decode GEMM two kernels downstream can then take over an SM the
   // moment the previous GEMM's CTA leaves it and stream its weights under this kernel.
   griddep_launch_dependents();
-  if constexpr (kShared) {
-    sh_plan<kDcThreads>(p.sg, p.seq_lens, p.batch, p.Hk, plan, [&](int b, int L, int g) {
-      s_len[b] = L;
-      s_group[b] = g >= 0 ? static_cast<uint16_t>(g) : kNoGroup;
-    });
-  } else {
-    griddep_wait();
-  }
-  // keys of request b before its own tokens
-  auto first_own = [&](int b) {
-    if constexpr (!kShared) return 0;
-    return s_group[b] != kNoGroup ? plan.tiles[s_group[b]] * kDcTile : 0;
-  };
+  griddep_wait();
   // this CTA's range of the work list: thread t counts the units of requests [b0, b1)
   const int per_thread = (p.batch + kDcThreads - 1) / kDcThreads;
   const int b0 = threadIdx.x * per_thread, b1 = min(p.batch, b0 + per_thread);
   int sum = 0;
   for (int b = b0; b < b1; ++b) {
-    const int L = kShared ? s_len[b] - first_own(b) : static_cast<int>(p.seq_lens[b]);
+    const int L = static_cast<int>(p.seq_lens[b]);
     if (b < kDcLenCache) s_len[b] = L;
     prefetch_l2(p.req_pool_indices + b);  // read when the range is known
     sum += (dc_tiles(L) + kDcItemUnits) * p.Hk;
@@ -362,9 +324,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       int ts = 0;  // global tile counter of the S stream
       auto issue_s = [&]() {
         const int st = ts % kDcStages, sb = ts & 1;
-        dc_wait<kShared>(&k_full[st], (ts / kDcStages) & 1, dead);
+        mbar_wait(&k_full[st], (ts / kDcStages) & 1);
         fence_proxy_async_smem();  // cp.async (generic proxy) writes -> UMMA operand reads
-        dc_wait<kShared>(&s_empty[sb], ((ts >> 1) & 1) ^ 1, dead);
+        mbar_wait(&s_empty[sb], ((ts >> 1) & 1) ^ 1);
         tc_fence_after_sync();
         const uint32_t ka = k_lo + st * (kDcTileBytes >> 4), qa = q_lo + (cs.iter % kDcQBufs) * (kDcQBytes >> 4);
 #pragma unroll
@@ -382,12 +344,12 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       while (cp.valid) {
         if (cs.valid) issue_s();
         const int st = tp % kDcStages, pb = tp & 1, ob = cp.iter & 1;
-        dc_wait<kShared>(&p_full[pb], (tp >> 1) & 1, dead);
-        dc_wait<kShared>(&v_full[st], (tp / kDcStages) & 1, dead);
+        mbar_wait(&p_full[pb], (tp >> 1) & 1);
+        mbar_wait(&v_full[st], (tp / kDcStages) & 1);
         fence_proxy_async_smem();
         const bool first = cp.tile == cp.tile0;
         if (first) {
-          dc_wait<kShared>(&o_empty[ob], (o_uses[ob] & 1) ^ 1, dead);
+          mbar_wait(&o_empty[ob], (o_uses[ob] & 1) ^ 1);
           ++o_uses[ob];
         }
         tc_fence_after_sync();
@@ -423,15 +385,14 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     // between the two warps, 64 requests of 1088 tokens took 53.1 us, so 51.6.
     // `base` = slot of the tile's first row when the tile is FULL (else -1): the candidate TMA row.
     auto lookup = [&](const DcCursor& cc, int* sl, int& base) {
-      const int64_t req = kShared ? __ldcg(reinterpret_cast<const long long*>(p.req_pool_indices) + cc.b) : p.req_pool_indices[cc.b];
-      const int32_t* rtt0 = p.req_to_token + req * p.rtt_stride + first_own(cc.b);
+      const int32_t* rtt0 = p.req_to_token + p.req_pool_indices[cc.b] * p.rtt_stride;
       const int tile0 = cc.tile * kDcTile;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int tok = tile0 + lane + i * 32;
-        sl[i] = tok < cc.L ? (kShared ? __ldcg(rtt0 + tok) : __ldg(rtt0 + tok)) : -1;
+        sl[i] = tok < cc.L ? __ldg(rtt0 + tok) : -1;
       }
-      base = (p.use_tma && tile0 + kDcTile <= cc.L) ? (kShared ? __ldcg(rtt0 + tile0) : __ldg(rtt0 + tile0)) : -1;
+      base = (p.use_tma && tile0 + kDcTile <= cc.L) ? __ldg(rtt0 + tile0) : -1;
     };
     const CUtensorMap* tmap = is_v ? &tmV : &tmK;
     int slot[4], base = -1;
@@ -448,7 +409,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
       for (int i = 0; i < 4; ++i) contig &= (slot[i] == base + i * 32 + lane);
       contig = __all_sync(0xffffffffu, contig);
-      dc_wait<kShared>(&empty[st], ((t / kDcStages) & 1) ^ 1, dead);
+      mbar_wait(&empty[st], ((t / kDcStages) & 1) ^ 1);
       if (!is_v && load_q) {
         // stage the G query rows of this (request, kv head) as the K-major B operand, in the same
         // cp.async group as the K tile.  Buffer citer % 4 was last read by the S MMAs of item
@@ -497,50 +458,6 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     // ===================== softmax / correction / epilogue =====================
     const int tid = threadIdx.x;  // TMEM lane: kv token within tile (S^T) or head-dim index (O^T)
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    // kShared: an item's (M, sum P v, sum P) over its own keys, joined with the parts over the shared ones, which lie with
-    // the CTAs of attn_shared.cu that had tiles of its query tile's item.  A lane looks at one part's (m, l); then thread
-    // d adds up column d of all of them.
-    auto join = [&](int b, int hk, float (&M)[kDcMaxGroup], float (&num)[kDcMaxGroup], float (&den)[kDcMaxGroup]) {
-      const int grp = s_group[b];
-      if (grp == kNoGroup || plan.tiles[grp] == 0) return;
-      griddep_wait();
-      const int tiles = plan.tiles[grp], member = b - plan.start[grp], mpt = p.sg.mpt;
-      const int pairs = sh_pairs(plan.count[grp], mpt), pair = member / (2 * mpt);
-      const int per_sh = sh_per_cta(plan.unit0[p.sg.groups], p.sg.grid);
-      const int u0 = plan.unit0[grp] + (hk * pairs + pair) * (tiles + kShItemUnits) + kShItemUnits;  // unit of its tile 0
-      const int c0 = u0 / per_sh, parts = (u0 + tiles - 1) / per_sh - c0 + 1;
-      const int64_t at_first = static_cast<int64_t>(b) * p.Hq + hk * G;
-      const int64_t at_next = (static_cast<int64_t>(c0) * 2 + (member / mpt & 1)) * kDcTile + member % mpt * G;  // of part 0, unused
-      for (int i0 = 0; i0 < parts; i0 += 32) {
-        const int mine = i0 + lane, here = min(32, parts - i0);
-        float wt[kDcMaxGroup];
-#pragma unroll
-        for (int g = 0; g < kDcMaxGroup; ++g) {
-          wt[g] = 0.f;
-          if (g < G) {
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (mine < parts)
-              ml = __ldcg(reinterpret_cast<const float2*>(mine == 0 ? p.sg.ml_first : p.sg.ml_next) + g +
-                          (mine == 0 ? at_first : at_next + static_cast<int64_t>(mine) * 2 * kDcTile));
-            const float own = den[g] > 0.f ? M[g] : -INFINITY;
-            const float top = fmaxf(own, warp_max(ml.y > 0.f ? ml.x : -INFINITY));
-            const float keep = den[g] > 0.f ? fast_exp2(M[g] - top) : 0.f;
-            wt[g] = ml.y > 0.f ? fast_exp2(ml.x - top) : 0.f;
-            num[g] *= keep;
-            den[g] = den[g] * keep + warp_sum(wt[g] * ml.y);
-            M[g] = top;
-          }
-        }
-#pragma unroll 4
-        for (int i = 0; i < here; ++i) {
-          const float* src = (i0 + i == 0 ? p.sg.o_first + at_first * kDcD
-                                          : p.sg.o_next + (at_next + static_cast<int64_t>(i0 + i) * 2 * kDcTile) * kDcD) + tid;
-#pragma unroll
-          for (int g = 0; g < kDcMaxGroup; ++g)
-            if (g < G) num[g] = fmaf(__shfl_sync(0xffffffffu, wt[g], i), __ldcg(src + g * kDcD), num[g]);
-        }
-      }
-    };
     int t = 0;  // global tile counter
     while (c.valid) {
       const int ib = c.b, ihk = c.hk, L = c.L, n = c.n, tile0 = c.tile0, ob = c.iter & 1;
@@ -554,7 +471,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         tile = c.tile;
         c.next(p, s_len);
         const int sb = t & 1;
-        dc_wait<kShared>(&s_full[sb], (t >> 1) & 1, dead);
+        mbar_wait(&s_full[sb], (t >> 1) & 1);
         tc_fence_after_sync();
         uint32_t r[16];
         tmem_ld_32x32b_x16(tmem_S + lane_base + sb * kDcN, r);
@@ -593,7 +510,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             // with every PV): this thread waited for the PREVIOUS phase of that barrier at tile t-1,
             // so the parity wait cannot alias — a per-PV barrier that is only waited on now and then
             // (the softmax may run up to two PVs ahead) would.
-            dc_wait<kShared>(&p_empty[(t - 1) & 1], ((t - 1) >> 1) & 1, dead);
+            mbar_wait(&p_empty[(t - 1) & 1], ((t - 1) >> 1) & 1);
             tc_fence_after_sync();
             uint32_t o[16];
             tmem_ld_32x32b_x16(tmem_O + lane_base + ob * kDcN, o);
@@ -608,7 +525,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           softmax_bar();  // `red` may be reused by the next slow path
         }
         // P^T -> smem (B operand, K-major: row = head, col = kv token); row sums stay per thread
-        dc_wait<kShared>(&p_empty[sb], ((t >> 1) & 1) ^ 1, dead);
+        mbar_wait(&p_empty[sb], ((t >> 1) & 1) ^ 1);
         uint8_t* pdst = sP + sb * kDcQBytes;
 #pragma unroll
         for (int g = 0; g < kDcMaxGroup; ++g) {
@@ -633,7 +550,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       for (int g = 0; g < kDcMaxGroup; ++g)
         l_tot[g] = (red[g] + red[8 + g]) + (red[16 + g] + red[24 + g]);
       {
-        dc_wait<kShared>(&p_empty[(t - 1) & 1], ((t - 1) >> 1) & 1, dead);  // last PV of the item complete
+        mbar_wait(&p_empty[(t - 1) & 1], ((t - 1) >> 1) & 1);  // last PV of the item complete
         tc_fence_after_sync();
         uint32_t r[16];
         tmem_ld_32x32b_x16(tmem_O + lane_base + ob * kDcN, r);
@@ -645,7 +562,6 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         for (int g = 0; g < kDcMaxGroup; ++g) o[g] = __uint_as_float(r[g]);
       }
       if (tile0 == 0 && tile + 1 == n) {
-        if constexpr (kShared) join(ib, ihk, m_ref, o, l_tot);
         T* dst = reinterpret_cast<T*>(p.out) + ib * p.out_stride + static_cast<int64_t>(ihk) * G * kDcD + tid;
 #pragma unroll
         for (int g = 0; g < kDcMaxGroup; ++g)
@@ -689,7 +605,6 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 den[g] += wgt * ml.y;
               }
           }
-          if constexpr (kShared) join(ib, ihk, M, num, den);
           T* dst = reinterpret_cast<T*>(p.out) + ib * p.out_stride + static_cast<int64_t>(ihk) * G * kDcD + tid;
 #pragma unroll
           for (int g = 0; g < kDcMaxGroup; ++g)
@@ -701,26 +616,14 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
   }
 
-  if constexpr (kShared) griddep_wait();  // CTAs without a join too: this grid ends after the one before
   tc_fence_before_sync();
   __syncthreads();
-  if constexpr (kShared) {
-    if (*dead) {
-      wait_drain();
-      if (threadIdx.x == 0) wait_report(p.wait_expired);
-    }
-  }
   if (warp == 8) tmem_dealloc(tmem_base, 64);
 }
 
 int check_attn_args(const char* fn, const void* out, const void* q, const void* k_pool,
                     const void* v_pool, const void* rtt, const void* rpi, int Hq, int Hk, int D,
                     int64_t q_stride, int64_t out_stride);
-int attn_decode_own(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
-                    const int64_t* req_pool_indices, const int64_t* seq_lens, int64_t batch, int num_q_heads, int num_kv_heads,
-                    int head_dim, int64_t q_stride, int64_t out_stride, int64_t req_to_token_stride, float sm_scale, int dtype,
-                    void* workspace, int64_t workspace_bytes, const SharedGroups& sg, unsigned* wait_expired, int sm_budget,
-                    cudaStream_t stream);
 
 }  // namespace spd
 
@@ -728,12 +631,11 @@ using namespace spd;
 
 // own_workspace: the workspace is zeroed and this stream's alone at every batch size (spd_attn_decode_paged_own), so items
 // may also be cut where their number fills the SMs; otherwise such a call leaves it untouched.
-// sg (kShared): the batch's groups, whose shared keys attn_shared.cu has been launched for.
 static int attn_decode(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
                        const int64_t* req_pool_indices, const int64_t* seq_lens, int64_t batch, int num_q_heads,
                        int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride, int64_t req_to_token_stride,
                        float sm_scale, int dtype, void* workspace, int64_t workspace_bytes, bool own_workspace,
-                       int sm_budget, spd_stream_t stream, const SharedGroups* sg = nullptr, unsigned* wait_expired = nullptr) {
+                       int sm_budget, spd_stream_t stream) {
   int rc = check_attn_args("spd_attn_decode_paged", out, q, k_pool, v_pool, req_to_token,
                            req_pool_indices, num_q_heads, num_kv_heads, head_dim, q_stride, out_stride);
   if (rc) return rc;
@@ -789,22 +691,8 @@ static int attn_decode(void* out, const void* q, const void* k_pool, const void*
   const uint64_t row_elems = static_cast<uint64_t>(num_kv_heads) * head_dim;
   if ((rc = get_tmap(&tk, k_pool, 1ull << 31, row_elems, row_elems, kDcTile))) return rc;
   if ((rc = get_tmap(&tv, v_pool, 1ull << 31, row_elems, row_elems, kDcTile))) return rc;
-  if (sg) {
-    p.sg = *sg;
-    p.wait_expired = wait_expired;
-    SPD_DISPATCH_DTYPE(dtype, {
-      auto kern = attn_decode_kernel<T, true>;
-      static bool configured = false;
-      if (!configured) {
-        SPD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDcSmemShared));
-        configured = true;
-      }
-      SPD_CUDA(launch(kern, dim3(grid), dim3(kDcThreads), kDcSmemShared, as_stream(stream), pdl_enabled(), tk, tv, p));
-    });
-    return 0;
-  }
   SPD_DISPATCH_DTYPE(dtype, {
-    auto kern = attn_decode_kernel<T, false>;
+    auto kern = attn_decode_kernel<T>;
     static bool configured = false;
     if (!configured) {
       SPD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDcSmem));
@@ -813,16 +701,6 @@ static int attn_decode(void* out, const void* q, const void* k_pool, const void*
     SPD_CUDA(launch(kern, dim3(grid), dim3(kDcThreads), kDcSmem, as_stream(stream), pdl_enabled(), tk, tv, p));
   });
   return 0;
-}
-
-int spd::attn_decode_own(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
-                         const int64_t* req_pool_indices, const int64_t* seq_lens, int64_t batch, int num_q_heads,
-                         int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride, int64_t req_to_token_stride,
-                         float sm_scale, int dtype, void* workspace, int64_t workspace_bytes, const SharedGroups& sg,
-                         unsigned* wait_expired, int sm_budget, cudaStream_t stream) {
-  return attn_decode(out, q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, batch, num_q_heads, num_kv_heads,
-                     head_dim, q_stride, out_stride, req_to_token_stride, sm_scale, dtype, workspace, workspace_bytes, true,
-                     sm_budget, stream, &sg, wait_expired);
 }
 
 extern "C" int spd_attn_decode_paged(void* out, const void* q, const void* k_pool, const void* v_pool,
