@@ -20,11 +20,14 @@
 //
 //   warps 0-3 / 4-7  softmax of query tile 0 / 1: one thread per query row; P goes back into the TMEM columns of its S
 //   warp 8, warp 9   K / V loader: a ring of four 128 x 128 tiles, K_j V_j K_{j+1} ..., by TMA where a tile's slots are
-//                    consecutive, gathered row by row elsewhere
+//                    consecutive, gathered row by row elsewhere; over own keys both, for warpgroup 0 / 1
 //   warp 10, warp 11 MMA issuer of query tile 0 / 1
-// A key tile is taken in two halves of 64 keys, so that a warpgroup's softmax of one half runs beside the MMAs of the other.  Items
-// over own keys have the query heads of one kv head as their only rows (the tensor cores wait for the keys anyhow) and
-// go to the two warpgroups in turn, so that the softmax of one runs beside the other's.
+// Over shared keys a tile is taken in two halves of 64 keys, so that a warpgroup's softmax of one half runs beside the MMAs of
+// the other.  An item over own keys has the few query heads of one kv head as its rows; it is computed the other way round,
+// S^T = K Q^T and O^T = V^T P^T, with a thread per key and P^T in shared memory, as in attn_decode.cu.  (With queries in the
+// rows there too, one warp did all the exponentials: 160 requests of 132 own tokens, 32 / 32 heads, 276 us.)  The items go to
+// the two warpgroups in turn, and each has a loader, an issuer and a ring of three tiles to itself (its half of the ring above and
+// the memory of its query tile): with one ring for both, an item waited for the one before in every role (229 us).
 // Sums, maxima and outputs are fp32 up to the join; P is rounded to the type of the keys, as the tensor cores take it, and l
 // sums the rounded P, so that the rounding of a P that outweighs the others cancels.  The reference maximum is raised when a
 // score passes it by 2^8 (O is then rescaled in TMEM), so a P is at most 2^8.
@@ -49,9 +52,16 @@ constexpr int kSpSlots = 4;
 constexpr int kSpRows = 1024;    // batch rows that a plan holds
 constexpr int kSpGroups = 256;   // groups
 constexpr int kSpMaxTiles = 65535;
-constexpr int kSpOwnQ = 4;       // buffers for the queries of items over own keys: [8 rows x 64 columns] twice
-constexpr int kSpStage = 8 * 2048;  // per softmax warp: 32 rows x 16 fp32 columns of an output on their way to memory
+constexpr int kSpMaxGroup = 8;
+constexpr int kSpN = 16;         // own keys: columns of an MMA (>= kSpMaxGroup)
+constexpr int kSpOwnSlots = 3;   // tiles of a warpgroup's ring over own keys
+constexpr int kSpSmall = 2048;   // own keys: [8 rows x 128] of queries or P^T, in two blocks with the 128-byte swizzle
+// per softmax warp: 32 rows x 16 fp32 columns of an output on their way to memory; or per warpgroup: two buffers of P^T, two of
+// queries
+constexpr int kSpStage = 8 * 2048;
+static_assert(kSpStage == 2 * 4 * kSpSmall, "one memory for both");
 constexpr int kSpBars = 256;
+constexpr int kSpRed = 2 * 2 * kSpMaxGroup * 4 * 4;  // per warpgroup, twice: the maxima or sums of 4 warps for every head
 constexpr float kSpRescale = 8.f;  // exponent of 2 that a score may pass the reference maximum by
 // what the list's entries cost: a key tile for two query tiles, for one; an item's start and end
 constexpr int kCostPair = 3, kCostTile = 2, kCostShared = 4, kCostOwn = 1;
@@ -80,11 +90,12 @@ struct SharedPlan {  // in shared memory
   uint16_t skip[kSpRows];    // its shared tiles
   int unit0[kSpGroups + 1];  // cost of the groups before
   int req[kSpGroups];        // page-table row of a member that is not empty
+  int least[kSpGroups], lead[kSpGroups];
   uint16_t start[kSpGroups], count[kSpGroups], tiles[kSpGroups];
-  int sums[16];
+  int2 sums[kSpThreads / 32];
   int own_row, own_head, own_at, own_req;  // where this CTA's range begins among the own keys
 };
-constexpr int kSpSmem = kSpTileBytes * (2 + kSpSlots) + kSpOwnQ * 2048 + kSpStage + kSpBars + static_cast<int>(sizeof(SharedPlan)) + 1024;
+constexpr int kSpSmem = kSpTileBytes * (2 + kSpSlots) + kSpStage + kSpBars + kSpRed + static_cast<int>(sizeof(SharedPlan)) + 1024;
 static_assert(kSpSmem <= 232448, "shared memory of one block");
 
 __device__ __forceinline__ int sp_pairs(int count, int mpt) { return count <= mpt ? 1 : (count + 2 * mpt - 1) / (2 * mpt); }
@@ -100,34 +111,13 @@ struct SpRange {
   __device__ __forceinline__ bool own() const { return begin < end && end > shared; }  // reaches into the items over own keys
 };
 
-// sum over the threads before this one, and over all (into sums, by warp); a barrier inside
-__device__ __forceinline__ int sp_scan(int v, int* sums, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
-  }
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kSpThreads / 32; ++w) {
-    const int x = sums[w];
-    before += w < warp ? x : 0;
-    total += x;
-  }
-  return before + incl - v;
-}
-
-// The plan, by all threads of the CTA, from the groups' offsets and the lengths.
+// The plan, by all threads of the CTA, from the groups' offsets and the lengths.  It stands before the CTA's first load, so it
+// asks for all that it reads at once and has few barriers.
 __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl) {
-  static_assert(kSpThreads >= kSpGroups && kSpThreads / 32 <= 16, "a thread per group");
-  constexpr int kPer = (kSpRows + kSpThreads - 1) / kSpThreads;
-  const int g = threadIdx.x;
-  // thread t reads rows [b0, b1); everything that the plan reads is requested at once
+  static_assert(kSpThreads >= kSpGroups, "a thread per group");
+  constexpr int kPer = (kSpRows + kSpThreads - 1) / kSpThreads, kWarps = kSpThreads / 32;
+  const int g = threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // thread t reads rows [b0, b0 + rows)
   const int per_thread = (p.batch + kSpThreads - 1) / kSpThreads, b0 = min(p.batch, g * per_thread), rows = min(p.batch, b0 + per_thread) - b0;
   int L[kPer], req[kPer];
 #pragma unroll
@@ -135,15 +125,14 @@ __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl
     L[i] = i < rows ? static_cast<int>(max(0ll, min(static_cast<long long>(p.seq_lens[b0 + i]), static_cast<long long>(INT_MAX - kSpTile)))) : 0;
     req[i] = i < rows ? static_cast<int>(p.req_pool_indices[b0 + i]) : 0;
   }
-  int shared = 0, count = 0;
   if (g < p.groups) {
     const int s = min(max(p.group_indptr[g], 0), p.batch), e = min(max(p.group_indptr[g + 1], s), p.batch);
-    shared = static_cast<int>(max(0ll, min(static_cast<long long>(p.shared_lens[g]), static_cast<long long>(kSpMaxTiles) * kSpTile)));
-    count = e - s;
     pl.start[g] = static_cast<uint16_t>(s);
-    pl.count[g] = static_cast<uint16_t>(count);
-    pl.unit0[g] = INT_MAX;  // for now: the shortest member
-    pl.req[g] = INT_MAX;    // for now: the first member that is not empty
+    pl.count[g] = static_cast<uint16_t>(e - s);
+    // the tiles that its slots allow; the shortest member, and the first that is not empty
+    pl.tiles[g] = static_cast<uint16_t>(max(0ll, min(static_cast<long long>(p.shared_lens[g]) / kSpTile, static_cast<long long>(kSpMaxTiles))));
+    pl.least[g] = INT_MAX;
+    pl.lead[g] = INT_MAX;
   }
   __syncthreads();
   int at[kPer];
@@ -158,42 +147,63 @@ __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl
         if (pl.start[mid] <= b) lo = mid; else hi = mid - 1;
       }
       while (lo > 0 && pl.count[lo] == 0) --lo;  // groups of no rows start where the next one does
-      if (b >= pl.start[lo] && b < pl.start[lo] + pl.count[lo]) {
+      if (pl.count[lo] >= 2 && b >= pl.start[lo] && b < pl.start[lo] + pl.count[lo]) {
         at[i] = lo;
-        atomicMin(&pl.unit0[lo], L[i]);
-        atomicMin(&pl.req[lo], b);
+        atomicMin(&pl.least[lo], L[i]);
+        atomicMin(&pl.lead[lo], b);
       }
     }
   }
   __syncthreads();
-  int cost = 0, tiles = 0;
+  auto tiles_of = [&](int group) {
+    const int least = pl.least[group];
+    return least == INT_MAX ? 0 : min(static_cast<int>(pl.tiles[group]), least / kSpTile);
+  };
+  // costs: of this thread's group, of its rows' own keys
+  int cost = 0, own = 0;
   if (g < p.groups) {
-    const int least = pl.unit0[g];
-    tiles = count >= 2 && least != INT_MAX ? min(shared, least) / kSpTile : 0;
-    pl.tiles[g] = static_cast<uint16_t>(tiles);
+    const int tiles = tiles_of(g), count = pl.count[g];
     cost = tiles > 0 ? p.Hk * sp_pairs(count, p.mpt) * (kCostShared + tiles * sp_cost(count, p.mpt)) : 0;
   }
-  int first[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) first[i] = at[i] >= 0 ? pl.req[at[i]] : -1;
-  SpRange r;
-  const int before = sp_scan(cost, pl.sums, r.shared);  // (its barrier: tiles are there, req has been read)
-  if (g < p.groups) pl.unit0[g] = before;
-  if (g == 0) pl.unit0[p.groups] = r.shared;
-  int own = 0;
+  for (int i = 0; i < kPer; ++i)
+    if (i < rows) {
+      const int skip = at[i] >= 0 ? tiles_of(at[i]) : 0;
+      if (skip > 0 && pl.lead[at[i]] == b0 + i) pl.req[at[i]] = req[i];
+      L[i] -= skip * kSpTile;
+      pl.len[b0 + i] = L[i];
+      pl.skip[b0 + i] = static_cast<uint16_t>(skip);
+      own += sp_own_cost(L[i]) * p.Hk;
+    }
+  int incl = cost, own_incl = own;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (i >= rows) break;
-    if (first[i] == b0 + i) pl.req[at[i]] = req[i];
-    const int skip = at[i] >= 0 ? pl.tiles[at[i]] : 0;
-    L[i] -= skip * kSpTile;
-    pl.len[b0 + i] = L[i];
-    pl.skip[b0 + i] = static_cast<uint16_t>(skip);
-    own += sp_own_cost(L[i]) * p.Hk;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o), y = __shfl_up_sync(0xffffffffu, own_incl, o);
+    if (lane >= o) {
+      incl += x;
+      own_incl += y;
+    }
   }
-  __syncthreads();  // sums have been read
-  int all_own;
-  const int own_before = sp_scan(own, pl.sums, all_own);
+  if (lane == 31) pl.sums[warp] = make_int2(incl, own_incl);
+  __syncthreads();
+  SpRange r;
+  r.shared = 0;
+  int before = incl - cost, own_before = own_incl - own, all_own = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int2 x = pl.sums[w];
+    if (w < warp) {
+      before += x.x;
+      own_before += x.y;
+    }
+    r.shared += x.x;
+    all_own += x.y;
+  }
+  if (g < p.groups) {
+    pl.unit0[g] = before;
+    pl.tiles[g] = static_cast<uint16_t>(tiles_of(g));  // (who reads the tiles as they were has passed the barrier)
+  }
+  if (g == 0) pl.unit0[p.groups] = r.shared;
   const int total = r.shared + all_own;
   r.per = max(kCostMin, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
   r.begin = min(total, r.per * static_cast<int>(blockIdx.x));
@@ -224,93 +234,96 @@ __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl
 }
 
 struct SpItem {
-  bool own;
   int b0, hk;        // batch row of the first member, or of the request; kv head
   int req;           // page-table row
-  int rows0, rows1;  // query rows of the two tiles
-  int skip, keys;    // own: tiles before its first key; keys that the item's tiles hold
+  int rows0, rows1;  // shared keys: query rows of the two tiles
+  int keys;          // keys that the item's tiles hold
+  int s0, tiles;     // the list's position of its first tile; tiles
+  int cost;          // of each
   int tile0, n;      // first key tile of this CTA and how many
-  int buf;           // own: buffer of the queries
-  int c0, parts;     // CTA of the first part and number of parts
+  // tiles that begin in [u, end); the list goes on behind them
+  __device__ __forceinline__ bool cut(int& u, int end) {
+    tile0 = min(tiles, max(0, (u - s0 + cost - 1) / cost));
+    n = min(tiles, max(0, (end - s0 + cost - 1) / cost)) - tile0;
+    u = min(end, s0 + tiles * cost);
+    return n > 0;
+  }
+  // for the join: the CTA of the first part, and how many parts | the row there of a kv head's first query << 16
+  __device__ __forceinline__ int2 note(int per, int row) const {
+    const int c0 = s0 / per;
+    return make_int2(c0, ((s0 + (tiles - 1) * cost) / per - c0 + 1) | row << 16);
+  }
 };
 
-// The items of this CTA, one after another; every role walks for itself.
+// This CTA's items over shared keys, one after another; every role walks for itself.
 struct SpWalk {
-  int u, g;                // position in the list, group
-  int row, head, owns;     // own items: the next one, and how many were before it here
-  int64_t req;             // its page-table row, read when the row before is begun
-  int64_t req_next;
-  __device__ __forceinline__ void init(const SharedParams& p, const SharedPlan& pl, const SpRange& r) {
-    u = r.begin;
+  int u, end, g;  // position in the list, end of the range there, group
+  __device__ __forceinline__ SpWalk(const SharedParams& p, const SharedPlan& pl, const SpRange& r) : u(r.begin), end(min(r.end, r.shared)) {
     int lo = 0, hi = p.groups - 1;  // the last group whose items do not begin behind the range's start
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (pl.unit0[mid] <= u) lo = mid; else hi = mid - 1;
     }
     g = lo;
-    owns = 0;
-    row = head = 0;
-    req = req_next = 0;
-    if (r.own()) {
-      row = pl.own_row;
-      head = pl.own_head;
-      req = pl.own_req;
-      req_next = row + 1 < p.batch ? p.req_pool_indices[row + 1] : 0;
-    }
   }
-  // tiles [t0, t1) of an item whose first tile stands at s0, `cost` each, that begin in [u, end)
-  __device__ __forceinline__ bool cut(const SpRange& r, int s0, int cost, int n, SpItem& it) {
-    it.tile0 = min(n, max(0, (u - s0 + cost - 1) / cost));
-    it.n = min(n, max(0, (r.end - s0 + cost - 1) / cost)) - it.tile0;
-    it.c0 = s0 / r.per;
-    it.parts = (s0 + (n - 1) * cost) / r.per - it.c0 + 1;
-    u = min(r.end, s0 + n * cost);
-    return it.n > 0;
-  }
-  __device__ __forceinline__ bool next(const SharedParams& p, const SharedPlan& pl, const SpRange& r, SpItem& it) {
-    while (u < min(r.end, r.shared)) {
+  __device__ __forceinline__ bool next(const SharedParams& p, const SharedPlan& pl, SpItem& it) {
+    while (u < end) {
       while (pl.unit0[g + 1] <= u) ++g;
-      const int count = pl.count[g], tiles = pl.tiles[g], cost = sp_cost(count, p.mpt), per_item = kCostShared + tiles * cost;
-      const int item = (u - pl.unit0[g]) / per_item, pairs = sp_pairs(count, p.mpt), pair = item % pairs;
-      const int left = count - pair * 2 * p.mpt;
-      it.own = false;
+      const int count = pl.count[g], pairs = sp_pairs(count, p.mpt);
+      it.tiles = pl.tiles[g];
+      it.cost = sp_cost(count, p.mpt);
+      const int per_item = kCostShared + it.tiles * it.cost, item = (u - pl.unit0[g]) / per_item;
       it.hk = item / pairs;
+      const int pair = item - it.hk * pairs, left = count - pair * 2 * p.mpt;
       it.b0 = pl.start[g] + pair * 2 * p.mpt;
       it.req = pl.req[g];
       it.rows0 = min(p.mpt, left) * p.group;
       it.rows1 = min(p.mpt, max(0, left - p.mpt)) * p.group;
-      it.skip = 0;
-      it.keys = tiles * kSpTile;
-      it.buf = 0;
-      if (cut(r, pl.unit0[g] + item * per_item + kCostShared, cost, tiles, it)) return true;
+      it.keys = it.tiles * kSpTile;
+      it.s0 = pl.unit0[g] + item * per_item + kCostShared;
+      if (it.cut(u, end)) return true;
     }
-    while (u < r.end) {
-      const int len = pl.len[row], n = sp_tiles(len);
-      it.own = true;
+    return false;
+  }
+};
+
+// This CTA's items over own keys: every second one, warpgroup w's.
+struct SpOwnWalk {
+  int u, end, row, head, turn;
+  int64_t req, req_next;  // page-table row of the row here and of the one behind it, read ahead
+  __device__ __forceinline__ SpOwnWalk(const SharedParams& p, const SharedPlan& pl, const SpRange& r, int w)
+      : u(0), end(0), row(0), head(0), turn(w), req(0), req_next(0) {
+    if (r.own()) {
+      row = pl.own_row;
+      head = pl.own_head;
+      u = max(r.begin, r.shared) - pl.own_at;  // of the item; its tiles before the range are cut off below
+      end = r.end;
+      req = pl.own_req;
+      req_next = row + 1 < p.batch ? p.req_pool_indices[row + 1] : 0;
+    }
+  }
+  __device__ __forceinline__ bool next(const SharedParams& p, const SharedPlan& pl, const SpRange& r, SpItem& it) {
+    while (u < end) {
+      it.keys = pl.len[row];
       it.hk = head;
       it.b0 = row;
       it.req = static_cast<int>(req);
-      it.skip = pl.skip[row];
-      it.keys = len;
       bool some = false;
-      if (len > 0) {
-        // (the list's position of the item: known for the first one here, the others follow it)
-        const int s0 = (owns == 0 && u == max(r.begin, r.shared) && row == pl.own_row && head == pl.own_head ? u - pl.own_at : u) + kCostOwn;
-        some = cut(r, s0, kCostTile, n, it);
+      if (it.keys > 0) {
+        it.tiles = sp_tiles(it.keys);
+        it.s0 = u + kCostOwn;
+        it.cost = kCostTile;
+        int from = max(u, r.begin);
+        some = it.cut(from, end);
+        u = it.s0 + it.tiles * kCostTile;
       }
-      if (++head == p.Hk || len == 0) {
+      if (++head == p.Hk || it.keys <= 0) {
         head = 0;
         ++row;
         req = req_next;
         req_next = row + 1 < p.batch ? p.req_pool_indices[row + 1] : 0;
       }
-      if (some) {
-        it.rows0 = owns & 1 ? 0 : p.group;
-        it.rows1 = owns & 1 ? p.group : 0;
-        it.buf = owns % kSpOwnQ;
-        ++owns;
-        return true;
-      }
+      if (some && (turn++ & 1) == 0) return true;
     }
     return false;
   }
@@ -321,6 +334,46 @@ __device__ __forceinline__ uint32_t sp_tile_off(int row, int chunk16) {
   return (chunk16 >> 3) * 16384 + row * 128 + (((chunk16 & 7) ^ (row & 7)) << 4);
 }
 
+// of an element of P^T: row (query head), key
+__device__ __forceinline__ uint32_t sp_p_off(int row, int key) {
+  const int chunk = key >> 3;
+  return (chunk >> 3) * 1024 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4) + (key & 7) * 2;
+}
+// barrier of a warpgroup's 128 threads
+__device__ __forceinline__ void sp_bar(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// the two rounded values of a word as fp32.  (bf16 by hand: through the conversion of a pair, a unit's 64 exponentials and
+// sums took 1590 clk, so 716.)
+template <typename T>
+__device__ __forceinline__ float2 sp_unpack(uint32_t w) {
+  if constexpr (umma_fmt<T>::v == 1) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return unpack2<T>(w);
+}
+// One row's 64 scores of a unit: p = exp2(s * scale - m_off), rounded and packed into pk; the sum of the rounded p.
+template <typename T>
+__device__ __forceinline__ float sp_softmax_unit(const uint32_t* ra, const uint32_t* rb, uint32_t* pk, float scale, float m_off) {
+  const uint64_t scale2 = pack_f32x2(scale, scale), neg_m2 = pack_f32x2(-m_off, -m_off);
+#pragma unroll
+  for (int i = 0; i < 64; i += 2) {
+    const uint32_t* r = i < 32 ? ra + i : rb + i - 32;
+    float x0, x1;
+    unpack_f32x2(ffma2(pack_f32x2(__uint_as_float(r[0]), __uint_as_float(r[1])), scale2, neg_m2), x0, x1);
+    pk[i >> 1] = pack2<T>(fast_exp2(x0), fast_exp2(x1));
+  }
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float2 f = sp_unpack<T>(pk[i]);
+    sum[i % 2 * 2] += f.x;
+    sum[i % 2 * 2 + 1] += f.y;
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+// largest value of the warp (not NaN, unless all are)
+__device__ __forceinline__ float sp_warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 template <typename T>
 __global__ void __launch_bounds__(kSpThreads, 1)
 attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQ1,
@@ -330,28 +383,32 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem;                      // 2 tiles
   uint8_t* sKV = smem + 2 * kSpTileBytes;  // ring: position 2t = K of tile t, 2t + 1 = V of tile t
-  // queries of items over own keys: 8 rows of a tile whose other rows are whatever lies behind them, and never looked at
-  uint8_t* sOwnQ = smem + (2 + kSpSlots) * kSpTileBytes;
-  uint8_t* sO = sOwnQ + kSpOwnQ * 2048;
-  static_assert(kSpStage + kSpBars + sizeof(SharedPlan) >= 16384, "the rows behind the last queries are shared memory too");
+  uint8_t* sO = smem + (2 + kSpSlots) * kSpTileBytes;
+  // own keys: the 8 rows of queries or of P^T are half of an operand whose other 8 are whatever lies behind them, and never
+  // looked at
+  auto own_p = [&](int w, int i) { return sO + (w * 4 + i) * kSpSmall; };
+  auto own_q = [&](int w, int i) { return sO + (w * 4 + 2 + i) * kSpSmall; };
   uint64_t* bars = reinterpret_cast<uint64_t*>(sO + kSpStage);
   uint64_t* q_full = bars;                  // 2
-  uint64_t* kv_full = bars + 2;             // kSpSlots
-  uint64_t* kv_empty = kv_full + kSpSlots;  // kSpSlots
-  uint64_t* s_full = kv_empty + kSpSlots;   // 4: [tile][half]
+  uint64_t* kv_full = bars + 2;             // kSpSlots, and the query tiles' memory as slots over own keys
+  uint64_t* kv_empty = kv_full + kSpSlots + 2;
+  uint64_t* s_full = kv_empty + kSpSlots + 2;  // 4: [tile][half]
   uint64_t* p_full = s_full + 4;            // 4
   uint64_t* pv_done = p_full + 4;           // 4
   uint64_t* o_free = pv_done + 4;           // 2
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
+  uint64_t* stage_free = o_free + 2;        // 2: the warpgroup is through with the shared keys
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stage_free + 2);
+  static_assert((4 + 2 * (kSpSlots + 2) + 12 + 4) * 8 <= kSpBars, "barriers");
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  SharedPlan& pl = *reinterpret_cast<SharedPlan*>(reinterpret_cast<uint8_t*>(bars) + kSpBars);
+  float* s_red = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + kSpBars);
+  SharedPlan& pl = *reinterpret_cast<SharedPlan*>(reinterpret_cast<uint8_t*>(s_red) + kSpRed);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   if (warp == 10) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 1);
-      for (int i = 0; i < kSpSlots; ++i) {
+      for (int i = 0; i < kSpSlots + 2; ++i) {
         mbar_init(&kv_full[i], 32);
         mbar_init(&kv_empty[i], 2);
       }
@@ -360,7 +417,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         mbar_init(&p_full[i], 4);
         mbar_init(&pv_done[i], 1);
       }
-      for (int i = 0; i < 2; ++i) mbar_init(&o_free[i], 4);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&o_free[i], 4);
+        mbar_init(&stage_free[i], 4);
+      }
       *dead = 0;
       fence_barrier_init();
     }
@@ -382,27 +442,37 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t tmem_S = tmem_base;        // 2 x (64 + 64) columns; P of a half in the first 32 of its S
   const uint32_t tmem_O = tmem_base + 256;  // 2 x 128 columns
-  SpWalk walk;
-  walk.init(p, pl, range);
+  // Shared keys: tile t of the CTA is in the ring's places 2 t (K) and 2 t + 1 (V), of kSpSlots.  Own keys: tile t of warpgroup
+  // w is in the places 2 t and 2 t + 1 of a ring of three, the slots 2 w and 2 w + 1 of the other ring, whose uses go on
+  // counting, and the memory of the warpgroup's query tile, which is free when its last S over shared keys is complete.
+  struct OwnSlot {
+    int bar, tile;  // barriers; memory, in tiles from the queries' on
+    uint32_t full, empty;  // parities to wait for
+  };
+  auto own_slot = [](int w, uint32_t place, uint32_t shared_tiles) {
+    const uint32_t use = place / kSpOwnSlots, c = place - use * kSpOwnSlots, before = (shared_tiles + 1 - w) / 2;
+    if (c == 2) return OwnSlot{kSpSlots + w, w, use & 1, use & 1};
+    return OwnSlot{2 * w + static_cast<int>(c), 2 + 2 * w + static_cast<int>(c), (before + use) & 1, ((before + use) & 1) ^ 1};
+  };
+  SpWalk walk(p, pl, range);
   SpItem it;
-  bool have = walk.next(p, pl, range, it);
+  uint32_t t_base = 0;  // tiles of all items before
 
   if (warp >= 10) {
     // ===================== MMA issuer of query tile 0 (warp 10) / 1 (warp 11) =====================
     const bool leader = elect_one();
     const int w = warp - 10;
-    constexpr uint32_t idesc_qk = umma_idesc<T>(kSpM, kSpU, 0, 0);  // A, B K-major
-    constexpr uint32_t idesc_pv = umma_idesc<T>(kSpM, kSpD, 0, 1);  // A = P (TMEM), B = V MN-major
+    constexpr uint32_t idesc_qk = umma_idesc<T>(kSpM, kSpU, 0, 0);     // A, B K-major
+    constexpr uint32_t idesc_pv = umma_idesc<T>(kSpM, kSpD, 0, 1);     // A = P (TMEM), B = V MN-major
+    constexpr uint32_t idesc_st = umma_idesc<T>(kSpTile, kSpN, 0, 0);  // own keys: A = K (K-major), B = Q (K-major)
+    constexpr uint32_t idesc_ot = umma_idesc<T>(kSpD, kSpN, 1, 0);     // A = V (MN-major), B = P^T (K-major)
     const uint64_t qd = umma_desc_sw128(smem_u32(sQ + w * kSpTileBytes), 16, 1024);
-    const uint32_t own_q = static_cast<uint32_t>(umma_desc_sw128(smem_u32(sOwnQ), 16, 1024));
     const uint64_t kd0 = umma_desc_sw128(smem_u32(sKV), 16, 1024);
     const uint64_t vd0 = umma_desc_sw128(smem_u32(sKV), 16384, 1024);
     const uint32_t qk_hi = static_cast<uint32_t>(qd >> 32), v_hi = static_cast<uint32_t>(vd0 >> 32);
     const uint32_t q_bytes = static_cast<uint32_t>(p.mpt * p.group) * 256;
-    uint32_t t_base = 0;  // tiles of all items before
-    uint32_t pq = 0;      // PV units issued
-    uint32_t eq = 0;      // items of the tile
-    uint32_t qq = 0;      // of them, items over shared keys
+    uint32_t pq = 0;  // PV units issued: two per tile of shared keys, one per tile of own ones
+    uint32_t eq = 0;  // items of the tile
     bool q_ahead = false;
     auto load_q = [&](const SpItem& i) {
       if (leader) {
@@ -412,39 +482,38 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
       __syncwarp();
     };
+    auto wait_kv = [&](uint32_t pos) { mbar_wait_bounded(&kv_full[pos % kSpSlots], (pos / kSpSlots) & 1, dead); };
+    bool have = walk.next(p, pl, it);
     while (have) {
       SpItem nx;
-      const bool more = walk.next(p, pl, range, nx);
+      const bool more = walk.next(p, pl, nx);
       const int n = it.n, nt = (w == 0 ? it.rows0 : it.rows1) > 0 ? n : 0;
-      if (nt > 0 && !it.own) {
+      if (nt > 0) {
         if (!q_ahead) load_q(it);
         q_ahead = false;
-        mbar_wait_bounded(&q_full[w], qq & 1, dead);
-        ++qq;
+        mbar_wait_bounded(&q_full[w], eq & 1, dead);
       }
-      // S(j, h): P(j - 1, h), which these columns held, has been consumed by PV(j - 1, h), issued earlier by this thread.
-      // (The queries of an item over own keys arrive with its first K tile here.)
-      const uint32_t q_lo = it.own ? own_q + it.buf * (2048 / 16) : static_cast<uint32_t>(qd);
-      const uint32_t q_step = it.own ? (1024 - 96) / 16 : (16384 - 96) / 16;
+      // S(j, h): P(j - 1, h), which these columns held, has been consumed by PV(j - 1, h), issued earlier by this thread
       auto issue_s = [&](int j, int h) {
         const uint32_t pos = 2 * (t_base + j);
-        mbar_wait_bounded(&kv_full[pos % kSpSlots], (pos / kSpSlots) & 1, dead);
+        wait_kv(pos);
         if (h == 0) fence_proxy_async_smem();
         tc_fence_after_sync();
-        uint32_t qa = q_lo;
+        uint32_t qa = static_cast<uint32_t>(qd);
         uint32_t ka = static_cast<uint32_t>(kd0) + (pos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
 #pragma unroll 1
         for (int k = 0; k < kSpD / 16; ++k) {
           umma_ss_if(leader, tmem_S + w * 128 + h * kSpU, qa, ka, qk_hi, idesc_qk, k);
-          qa += k == 3 ? q_step : 2;
-          ka += k == 3 ? (16384 - 96) / 16 : 2;
+          const uint32_t step = k == 3 ? (16384 - 96) / 16 : 2;
+          qa += step;
+          ka += step;
         }
         umma_commit_if(leader, &s_full[w * 2 + h]);
       };
       // a ring slot is released by both issuers; one whose tile has no rows waits for the copy first, to keep to the phases
       auto release_k = [&](int j) {
         const uint32_t pos = 2 * (t_base + j);
-        if (nt == 0) mbar_wait_bounded(&kv_full[pos % kSpSlots], (pos / kSpSlots) & 1, dead);
+        if (nt == 0) wait_kv(pos);
         umma_commit_if(leader, &kv_empty[pos % kSpSlots]);
       };
       if (nt > 0) {
@@ -457,14 +526,14 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (nt > 0) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (j == n - 1 && h == 0 && more && !nx.own && (w == 0 ? nx.rows0 : nx.rows1) > 0) {
+            if (j == n - 1 && h == 0 && more && (w == 0 ? nx.rows0 : nx.rows1) > 0) {
               // the item's last S is under way: once it is complete, Q's memory is free for the next item
               mbar_wait_bounded(&s_full[w * 2 + 1], (pq >> 1) & 1, dead);
               load_q(nx);
               q_ahead = true;
             }
             mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
-            mbar_wait_bounded(&kv_full[vpos % kSpSlots], (vpos / kSpSlots) & 1, dead);
+            wait_kv(vpos);
             if (h == 0) fence_proxy_async_smem();
             if (j == 0 && h == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
             tc_fence_after_sync();
@@ -483,7 +552,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (j + 1 < n) issue_s(j + 1, h);
           }
         } else {
-          mbar_wait_bounded(&kv_full[vpos % kSpSlots], (vpos / kSpSlots) & 1, dead);
+          wait_kv(vpos);
         }
         umma_commit_if(leader, &kv_empty[vpos % kSpSlots]);
         if (j + 1 < n) release_k(j + 1);
@@ -493,174 +562,380 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       it = nx;
       have = more;
     }
-  } else if (warp >= 8) {
-    // ===================== K loader (warp 8, and queries of items over own keys) / V loader (warp 9) =====================
-    const int is_v = warp == 9 ? 1 : 0;
-    const int chunk = lane & 15, rsub = lane >> 4;
-    const T* pool = reinterpret_cast<const T*>(is_v ? p.v_pool : p.k_pool);
-    const CUtensorMap* tmap = is_v ? &tmV : &tmK;
-    const int64_t row_elems = static_cast<int64_t>(p.Hk) * kSpD;
-    // Page-table lookups run one tile ahead of the copies, four rows a lane; -1: behind the item's last key.
-    const int32_t* rtt = nullptr;  // the lane's entry of the next tile's first row
-    int slot[4], j = 0, left = 0;  // left: keys from that tile on
-    auto begin = [&]() {
-      rtt = p.req_to_token + it.req * p.rtt_stride + static_cast<int64_t>(it.skip + it.tile0) * kSpTile + lane;
-      left = it.keys - it.tile0 * kSpTile;
-      j = 0;
-    };
-    auto lookup = [&](int* s) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = lane + i * 32 < left ? rtt[i * 32] : -1;
-      rtt += kSpTile;
-      left -= kSpTile;
-    };
-    if (have) {
-      begin();
-      lookup(slot);
-    }
-    for (uint32_t pos = is_v; have; pos += 2) {
-      const int hk = it.hk;
-      const bool first = j == 0;
-      const int q_buf = !is_v && it.own && first ? it.buf : -1, q_row = it.b0;
-      if (++j == it.n) {
-        have = walk.next(p, pl, range, it);
-        if (have) begin();
+    umma_commit_if(leader, &kv_empty[kSpSlots + w]);  // (twice: an arrival for either issuer)
+    umma_commit_if(leader, &kv_empty[kSpSlots + w]);
+    // ---- own keys: S^T = K Q^T runs a tile ahead of O^T += V^T P^T, across items ----
+    const uint32_t k_lo = static_cast<uint32_t>(umma_desc_sw128(smem_u32(smem), 16, 1024));
+    const uint32_t v_lo = static_cast<uint32_t>(umma_desc_sw128(smem_u32(smem), 16384, 1024));
+    const uint32_t q_lo = static_cast<uint32_t>(umma_desc_sw128(smem_u32(own_q(w, 0)), 16, 1024));
+    const uint32_t p_lo = static_cast<uint32_t>(umma_desc_sw128(smem_u32(own_p(w, 0)), 16, 1024));
+    SpOwnWalk own(p, pl, range, w), own_s = own;
+    SpItem is;
+    uint32_t ks = 0, vs = 0, pu = pq;  // tiles of S and of PV; S units issued
+    int js = 0, qs = 0;                // S: tile of the item, buffer of its queries
+    bool more_s = own_s.next(p, pl, range, is);
+    auto issue_s = [&]() {  // into the buffer of the unit before the last, whose P has been waited for
+      const OwnSlot at = own_slot(w, 2 * ks, t_base);
+      const uint32_t h = pu & 1;
+      mbar_wait_bounded(&kv_full[at.bar], at.full, dead);  // (Q arrives with the item's first tile here)
+      fence_proxy_async_smem();
+      tc_fence_after_sync();
+      uint32_t ka = k_lo + at.tile * (kSpTileBytes / 16), qa = q_lo + qs * (kSpSmall / 16);
+#pragma unroll 1
+      for (int k = 0; k < kSpD / 16; ++k) {
+        umma_ss_if(leader, tmem_S + w * 128 + h * kSpU, ka, qa, qk_hi, idesc_st, k);
+        ka += k == 3 ? (16384 - 96) / 16 : 2;
+        qa += k == 3 ? (1024 - 96) / 16 : 2;
       }
-      int next[4];
-      if (have) lookup(next);
+      umma_commit_if(leader, &kv_empty[at.bar]);
+      umma_commit_if(leader, &kv_empty[at.bar]);
+      umma_commit_if(leader, &s_full[w * 2 + h]);
+      ++pu;
+      ++ks;
+      if (++js == is.n) {
+        js = 0;
+        qs ^= 1;
+        more_s = own_s.next(p, pl, range, is);
+      }
+    };
+    if (more_s) issue_s();
+    while (own.next(p, pl, range, it)) {
+      for (int j = 0; j < it.n; ++j, ++vs) {
+        // the next S goes first, unless its K is still on the way
+        bool later = false;
+        if (more_s) {
+          const OwnSlot at = own_slot(w, 2 * ks, t_base);
+          later = !__any_sync(0xffffffffu, mbar_test(&kv_full[at.bar], at.full));
+          if (!later) issue_s();
+        }
+        const OwnSlot at = own_slot(w, 2 * vs + 1, t_base);
+        const uint32_t h = pq & 1;
+        mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
+        mbar_wait_bounded(&kv_full[at.bar], at.full, dead);
+        fence_proxy_async_smem();
+        if (j == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
+        tc_fence_after_sync();
+        const int steps = min(kSpTile, it.keys - (it.tile0 + j) * kSpTile + 15) / 16;  // of 16 keys
+        uint32_t va = v_lo + at.tile * (kSpTileBytes / 16), pa = p_lo + h * (kSpSmall / 16);
+#pragma unroll 1
+        for (int k = 0; k < steps; ++k) {
+          umma_ss_if(leader, tmem_O + w * kSpD, va, pa, qk_hi, idesc_ot, j + k);
+          va += 2048 / 16;
+          pa += k == 3 ? (1024 - 96) / 16 : 2;
+        }
+        umma_commit_if(leader, &kv_empty[at.bar]);
+        umma_commit_if(leader, &kv_empty[at.bar]);
+        umma_commit_if(leader, &pv_done[w * 2 + h]);
+        ++pq;
+        if (later) issue_s();
+      }
+      ++eq;
+    }
+  } else if (warp >= 8) {
+    // ===================== loaders =====================
+    const int lw = warp - 8;
+    const int chunk = lane & 15, rsub = lane >> 4;
+    const int64_t row_elems = static_cast<int64_t>(p.Hk) * kSpD;
+    // a tile's slots, four rows a lane, from its first row's entry on; -1: behind the item's last key
+    auto lookup = [&](const int32_t* rtt, int left, int* s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = lane + i * 32 < left ? rtt[lane + i * 32] : -1;
+    };
+    // a tile into the memory at `tile`; its barrier gets 32 arrivals
+    auto load = [&](int is_v, int bar, int tile, int hk, const int* slot, int valid) {
+      const CUtensorMap* tmap = is_v ? &tmV : &tmK;
       const int base = __shfl_sync(0xffffffffu, slot[0], 0);
       bool contig = p.use_tma && base > 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) contig &= slot[i] == base + i * 32 + lane;
-      contig = __all_sync(0xffffffffu, contig);
-      const int st = pos % kSpSlots;
-      mbar_wait_bounded(&kv_empty[st], ((pos / kSpSlots) & 1) ^ 1, dead);
-      if (lane == 0 && q_buf >= 0) {
-        // Four items ago this buffer held the queries of an item whose tiles are all older than the one that this slot held
-        // before: its MMAs have finished.
-        mbar_expect_tx_noarrive(&kv_full[st], p.group * 256);
-        tma_load_3d(sOwnQ + q_buf * 2048, &tmQ1, &kv_full[st], 0, hk * p.group, q_row, kEvictNormal);
-        tma_load_3d(sOwnQ + q_buf * 2048 + 1024, &tmQ1, &kv_full[st], 64, hk * p.group, q_row, kEvictNormal);
-      }
-      if (contig) {
+      if (__all_sync(0xffffffffu, contig)) {
         if (lane == 0) {
-          uint8_t* dst = sKV + st * kSpTileBytes;
+          uint8_t* dst = smem + tile * kSpTileBytes;
           fence_proxy_async_smem();  // the slot may last have been written by the gather path
-          mbar_expect_tx_noarrive(&kv_full[st], kSpTileBytes);
-          tma_load_2d(dst, tmap, &kv_full[st], hk * kSpD, base, kEvictNormal);
-          tma_load_2d(dst + 16384, tmap, &kv_full[st], hk * kSpD + 64, base, kEvictNormal);
+          mbar_expect_tx_noarrive(&kv_full[bar], kSpTileBytes);
+          tma_load_2d(dst, tmap, &kv_full[bar], hk * kSpD, base, kEvictNormal);
+          tma_load_2d(dst + 16384, tmap, &kv_full[bar], hk * kSpD + 64, base, kEvictNormal);
         }
         __syncwarp();
-        mbar_arrive(&kv_full[st]);
-      } else {
-        __syncwarp();
-        const uint32_t dst = smem_u32(sKV + st * kSpTileBytes);
-        const T* col = pool + static_cast<int64_t>(hk) * kSpD + chunk * 8;
+        mbar_arrive(&kv_full[bar]);
+        return;
+      }
+      const uint32_t dst = smem_u32(smem + tile * kSpTileBytes);
+      const T* col = reinterpret_cast<const T*>(is_v ? p.v_pool : p.k_pool) + static_cast<int64_t>(hk) * kSpD + chunk * 8;
+      // K rows behind the item's last key stay what they are (their scores are not looked at); V rows up to the next
+      // multiple of 16, an MMA's step, become zeros
+      const int fill = is_v ? min(kSpTile, valid + 15) & ~15 : valid;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const int row = i * 2 + rsub;
-          const int64_t s = __shfl_sync(0xffffffffu, slot[i >> 4], row & 31);
-          cp_async16(dst + sp_tile_off(row, chunk), col + (s >= 0 ? s : 0) * row_elems, s >= 0);
+      for (int i4 = 0; i4 < 4; ++i4) {
+        if (i4 * 32 >= fill) break;
+        // (slots first: a shuffle waited for before every copy made it 35 clk a copy)
+        int s[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = __shfl_sync(0xffffffffu, slot[i4], i * 2 + rsub);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int row = i4 * 32 + i * 2 + rsub;
+          if (i4 * 32 + i * 2 < fill) cp_async16(dst + sp_tile_off(row, chunk), col + max(s[i], 0) * row_elems, s[i] >= 0);
         }
-        cp_async_mbar_arrive_noinc(&kv_full[st]);  // when this lane's copies have landed
+      }
+      cp_async_mbar_arrive_noinc(&kv_full[bar]);  // when this lane's copies have landed
+    };
+    // ---- shared keys: K by warp 8, V by warp 9; lookups run one tile ahead of the copies ----
+    int slot[4], next[4];
+    auto entry = [&](int skip) { return p.req_to_token + it.req * p.rtt_stride + static_cast<int64_t>(skip + it.tile0) * kSpTile; };
+    bool have = walk.next(p, pl, it);
+    if (have) lookup(entry(0), kSpTile, slot);
+    for (int j = 0; have; ++t_base) {
+      const int hk = it.hk;
+      if (++j == it.n) {
+        have = walk.next(p, pl, it);
+        j = 0;
+      }
+      if (have) lookup(entry(0) + j * kSpTile, kSpTile, next);
+      const uint32_t pos = 2 * t_base + lw;
+      mbar_wait_bounded(&kv_empty[pos % kSpSlots], ((pos / kSpSlots) & 1) ^ 1, dead);
+      load(lw, pos % kSpSlots, 2 + pos % kSpSlots, hk, slot, kSpTile);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) slot[i] = next[i];
+    }
+    // ---- own keys: warpgroup lw's, with the queries ----
+    SpOwnWalk own(p, pl, range, lw);
+    uint32_t place = 0;
+    int q_buf = 0;
+    have = own.next(p, pl, range, it);
+    if (have) lookup(entry(pl.skip[it.b0]), it.keys - it.tile0 * kSpTile, slot);
+    // the queries' buffers are memory that the warpgroup's outputs over shared keys pass through
+    if (have) mbar_wait_bounded(&stage_free[lw], 0, dead);
+    for (int j = 0; have;) {
+      const int hk = it.hk, b = it.b0, first = j == 0, valid = min(kSpTile, it.keys - (it.tile0 + j) * kSpTile);
+      if (++j == it.n) {
+        have = own.next(p, pl, range, it);
+        j = 0;
+      }
+      if (have) lookup(entry(pl.skip[it.b0]) + j * kSpTile, it.keys - (it.tile0 + j) * kSpTile, next);
+#pragma unroll
+      for (int is_v = 0; is_v < 2; ++is_v, ++place) {
+        const OwnSlot at = own_slot(lw, place, t_base);
+        mbar_wait_bounded(&kv_empty[at.bar], at.empty, dead);
+        if (is_v == 0 && first) {
+          // The buffer's last queries were those of the item before the last one, whose tiles are no younger than the V tile
+          // that this slot held: its MMAs have finished.
+          if (lane == 0) {
+            mbar_expect_tx_noarrive(&kv_full[at.bar], p.group * 256);
+            tma_load_3d(own_q(lw, q_buf), &tmQ1, &kv_full[at.bar], 0, hk * p.group, b, kEvictNormal);
+            tma_load_3d(own_q(lw, q_buf) + 1024, &tmQ1, &kv_full[at.bar], 64, hk * p.group, b, kEvictNormal);
+          }
+          __syncwarp();
+          q_buf ^= 1;
+        }
+        load(is_v, at.bar, at.tile, hk, slot, valid);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) slot[i] = next[i];
     }
   } else {
-    // ===================== softmax (one thread per query row) =====================
+    // ===================== softmax =====================
     const int w = warp >> 2, row = threadIdx.x & 127, row0 = row & ~31;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem_S + lane_base + w * 128, to = tmem_O + lane_base + w * kSpD;
     const float scale = p.scale_log2, ahead = kSpRescale / scale;
-    uint8_t* stage = sO + warp * 2048;
-    // where this thread's pieces of an output go, by batch row: its own row's (m, l), and the rows 8 i + lane / 4 of its warp
-    const int ml_at = row / p.group * p.Hq + row % p.group;
-    int o_at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = row0 + i * 8 + (lane >> 2);
-      o_at[i] = (r / p.group * p.Hq + r % p.group) * kSpD + (lane & 3) * 4;
-    }
     uint32_t u = 0;  // units of the tile (all items)
-    for (; have; have = walk.next(p, pl, range, it)) {
-      const int rows = w == 0 ? it.rows0 : it.rows1;
-      if (rows == 0) continue;
-      const bool active = row0 < rows;  // (of this warp: the others only keep the barriers' count)
-      float m = -INFINITY, l = 0.f;     // the reference maximum (raw scores) and sum folded into O
-      int key0 = it.tile0 * kSpTile;    // of the unit
-      const uint32_t u0 = u, u1 = u + 2 * it.n;
-      for (; u < u1; ++u, key0 += kSpU) {
+    {
+      // ---- shared keys: a thread per query row ----
+      uint8_t* stage = sO + warp * 2048;
+      // where this thread's pieces of an output go, by batch row: its own row's (m, l), and the rows 8 i + lane / 4 of its warp
+      const int member = row / p.group, ml_at = member * p.Hq + row - member * p.group;
+      int o_at[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = row0 + i * 8 + (lane >> 2), m = r / p.group;
+        o_at[i] = (m * p.Hq + r - m * p.group) * kSpD + (lane & 3) * 4;
+      }
+      while (walk.next(p, pl, it)) {
+        const int rows = w == 0 ? it.rows0 : it.rows1;
+        if (rows == 0) continue;
+        const bool active = row0 < rows;  // (of this warp: the others only keep the barriers' count)
+        float m = -INFINITY, l = 0.f;     // the reference maximum (raw scores) and sum folded into O
+        const uint32_t u0 = u, u1 = u + 2 * it.n;
+        for (; u < u1; ++u) {
+          const int h = u & 1;
+          mbar_wait_bounded(&s_full[w * 2 + h], (u >> 1) & 1, dead);
+          if (active) {
+            tc_fence_after_sync();
+            uint32_t ra[32], rb[32], pk[32];
+            const float mx = softmax_load_max<false, false>(ts + h * kSpU, ra, rb, 0, 0, 0);
+            // The exponentials do not wait for the unit's maximum; where it turns out too large (rarely) they are redone
+            const bool raise = __any_sync(0xffffffffu, mx > m + ahead && row < rows);
+            float alpha = 1.f;
+            if (raise) {
+              const float up = fmaxf(m, mx);
+              alpha = m == -INFINITY ? 0.f : fast_exp2((m - up) * scale);
+              l *= alpha;
+              m = up;
+            }
+            l += sp_softmax_unit<T>(ra, rb, pk, scale, m == -INFINITY ? 0.f : m * scale);
+            tmem_st_32x32b_x32(ts + h * kSpU, pk);
+            if (raise && u > u0) {
+              // O stands still once the PV of the unit before is complete (those before it are: S of this unit was issued
+              // after them)
+              mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
+              tc_fence_after_sync();
+              rescale_row128(to, alpha);
+            }
+            tmem_st_wait();
+            tc_fence_before_sync();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[w * 2 + h]);
+        }
+        // the item's part: O through shared memory, 64 bytes of a row at a time (a thread per row would touch 32 lines a store)
+        if (active) {
+          const bool first = it.tile0 == 0;
+          const int64_t at = first ? static_cast<int64_t>(it.b0 + w * p.mpt) * p.Hq + it.hk * p.group
+                                   : (static_cast<int64_t>(blockIdx.x) * 2 + w) * kSpM;
+          mbar_wait_bounded(&pv_done[w * 2 + 1], ((u - 1) >> 1) & 1, dead);
+          tc_fence_after_sync();
+          float* o = (first ? p.o_first : p.o_next) + at * kSpD;
+#pragma unroll 1
+          for (int c = 0; c < kSpD; c += 16) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(to + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = i * 8 + (lane >> 2);
+              if (row0 + rr < rows)
+                *reinterpret_cast<uint4*>(o + (first ? o_at[i] : (row0 + rr) * kSpD + (lane & 3) * 4) + c) =
+                    *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+            }
+            __syncwarp();
+          }
+          if (row < rows)
+            reinterpret_cast<float2*>(first ? p.ml_first : p.ml_next)[at + (first ? ml_at : row)] = make_float2(m * scale, l);
+          // (an empty request in the middle of a group takes no part)
+          const int b = it.b0 + w * p.mpt + member;
+          if (first && row < rows && row == member * p.group && pl.skip[b] > 0)
+            p.notes[b * p.Hk + it.hk] = it.note(range.per, w * kSpM + row);
+          tc_fence_before_sync();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&o_free[w]);
+      }
+      fence_proxy_async_smem();  // queries are copied into the staging memory
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&stage_free[w]);
+    }
+    // ---- own keys: a thread per key of a tile, then per column of the output ----
+    const int G = p.group;
+    // what the four warps find, [head][warp]; of the tiles alternately, so that one barrier stands between writing and reading
+    float4* red = reinterpret_cast<float4*>(s_red) + w * 2 * kSpMaxGroup;
+    auto put = [&](uint32_t buf, int g, float v) {
+      if (lane == 0) reinterpret_cast<float*>(red + (buf & 1) * kSpMaxGroup + g)[warp & 3] = v;
+    };
+    uint32_t rounds = 0;  // of them
+    SpOwnWalk own(p, pl, range, w);
+    while (own.next(p, pl, range, it)) {
+      float m_ref[kSpMaxGroup], l_thr[kSpMaxGroup];
+#pragma unroll
+      for (int g = 0; g < kSpMaxGroup; ++g) {
+        m_ref[g] = -INFINITY;
+        l_thr[g] = 0.f;
+      }
+      for (int j = 0; j < it.n; ++j, ++u) {
         const int h = u & 1;
         mbar_wait_bounded(&s_full[w * 2 + h], (u >> 1) & 1, dead);
-        if (active) {
-          tc_fence_after_sync();
-          uint32_t ra[32], rb[32], pk[32];
-          const float mx = key0 + kSpU > it.keys ? softmax_load_max<true, false>(ts + h * kSpU, ra, rb, key0, it.keys - 1, 0)
-                                                 : softmax_load_max<false, false>(ts + h * kSpU, ra, rb, 0, 0, 0);
-          const bool raise = __any_sync(0xffffffffu, mx > m + ahead && row < rows);
-          float alpha = 1.f;
-          if (raise) {
-            const float up = fmaxf(m, mx);
-            alpha = m == -INFINITY ? 0.f : fast_exp2((m - up) * scale);
-            l *= alpha;
-            m = up;
+        tc_fence_after_sync();
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(ts + h * kSpU, r);
+        tmem_ld_wait();
+        const bool valid = (it.tile0 + j) * kSpTile + row < it.keys;
+        float s[kSpMaxGroup];
+#pragma unroll
+        for (int g = 0; g < kSpMaxGroup; ++g)
+          if (g < G) {
+            s[g] = valid ? __uint_as_float(r[g]) * scale : -INFINITY;
+            put(rounds, g, sp_warp_max(s[g]));
           }
-          l += softmax_unit<T>(ra, rb, pk, scale, m == -INFINITY ? 0.f : m * scale);
-          tmem_st_32x32b_x32(ts + h * kSpU, pk);
-          if (raise && u > u0) {
-            // O stands still once the PV of the unit before is complete (those before it are: S of this unit was issued after
-            // them)
-            mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
-            tc_fence_after_sync();
-            rescale_row128(to, alpha);
+        sp_bar(1 + w);
+        float alpha[kSpMaxGroup];
+        bool raise = false;  // the same in all threads
+#pragma unroll
+        for (int g = 0; g < kSpMaxGroup; ++g) {
+          alpha[g] = 1.f;
+          if (g < G) {
+            const float4 x = red[(rounds & 1) * kSpMaxGroup + g];
+            const float mx = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+            if (mx > m_ref[g] + kSpRescale) {
+              alpha[g] = m_ref[g] == -INFINITY ? 0.f : fast_exp2(m_ref[g] - mx);
+              l_thr[g] *= alpha[g];
+              m_ref[g] = mx;
+              raise = true;
+            }
           }
-          tmem_st_wait();
-          tc_fence_before_sync();
         }
+        ++rounds;
+        if (raise && j > 0) {
+          mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);  // O stands still
+          tc_fence_after_sync();
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(to, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int g = 0; g < kSpMaxGroup; ++g) o[g] = __float_as_uint(__uint_as_float(o[g]) * alpha[g]);
+          tmem_st_32x32b_x16(to, o);
+          tmem_st_wait();
+        }
+        // the P buffer's last reader is the PV of the unit before the last
+        if (u >= 2) mbar_wait_bounded(&pv_done[w * 2 + h], ((u - 2) >> 1) & 1, dead);
+        uint8_t* pdst = own_p(w, h);
+#pragma unroll
+        for (int g = 0; g < kSpMaxGroup; ++g)
+          if (g < G) {
+            const T pt = from_f32<T>(fast_exp2(s[g] - m_ref[g]));
+            l_thr[g] += to_f32<T>(pt);
+            *reinterpret_cast<T*>(pdst + sp_p_off(g, row)) = pt;
+          }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[w * 2 + h]);
       }
-      // the item's part: O through shared memory, 64 bytes of a row at a time (a thread per row would touch 32 lines a store)
-      if (active) {
-        const bool first = it.tile0 == 0;
-        const int64_t set = it.own ? static_cast<int64_t>(p.batch) * p.Hq : 0;
-        const int64_t at = first ? set + static_cast<int64_t>(it.b0 + (it.own ? 0 : w * p.mpt)) * p.Hq + it.hk * p.group
-                                 : (static_cast<int64_t>(blockIdx.x) * 2 + w) * kSpM;
-        mbar_wait_bounded(&pv_done[w * 2 + 1], ((u - 1) >> 1) & 1, dead);
-        tc_fence_after_sync();
-        float* o = (first ? p.o_first : p.o_next) + at * kSpD;
-#pragma unroll 1
-        for (int c = 0; c < kSpD; c += 16) {
-          uint32_t r[16];
-          tmem_ld_32x32b_x16(to + c, r);
-          tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-          __syncwarp();
+      for (int g = 0; g < kSpMaxGroup; ++g)
+        if (g < G) put(rounds, g, warp_sum(l_thr[g]));
+      sp_bar(1 + w);
+      const bool first = it.tile0 == 0;
+      const int64_t at = first ? static_cast<int64_t>(p.batch + it.b0) * p.Hq + it.hk * G
+                               : (static_cast<int64_t>(blockIdx.x) * 2 + w) * kSpM;
+      if (row == 0) {
+        float2* ml = reinterpret_cast<float2*>(first ? p.ml_first : p.ml_next) + at;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = i * 8 + (lane >> 2);
-            if (row0 + rr < rows)
-              *reinterpret_cast<uint4*>(o + (first ? o_at[i] : (row0 + rr) * kSpD + (lane & 3) * 4) + c) =
-                  *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+        for (int g = 0; g < kSpMaxGroup; ++g)
+          if (g < G) {
+            const float4 x = red[(rounds & 1) * kSpMaxGroup + g];
+            ml[g] = make_float2(m_ref[g], (x.x + x.y) + (x.z + x.w));
           }
-          __syncwarp();
-        }
-        if (row < rows)
-          reinterpret_cast<float2*>(first ? p.ml_first : p.ml_next)[at + (first ? ml_at : row)] = make_float2(m * scale, l);
-        // where the join finds the parts: of a CTA behind the first one, the item is its first, so an own one is in tile 0 there
-        if (first && row < rows && row % p.group == 0) {
-          const int b = it.b0 + (it.own ? 0 : w * p.mpt + row / p.group);
-          if (it.own || pl.skip[b] > 0)  // (an empty request in the middle of a group takes no part)
-            p.notes[((it.own ? p.batch : 0) + b) * p.Hk + it.hk] = make_int2(it.c0, it.parts | (it.own ? 0 : w * kSpM + row) << 16);
-        }
-        tc_fence_before_sync();
-        __syncwarp();
+        // behind the CTA of the first part an item is its CTA's first, so it is warpgroup 0's there
+        if (first) p.notes[(p.batch + it.b0) * p.Hk + it.hk] = it.note(range.per, 0);
       }
+      ++rounds;
+      mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
+      tc_fence_after_sync();
+      uint32_t r[16];
+      tmem_ld_32x32b_x16(to, r);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[w]);
+      float* o = (first ? p.o_first : p.o_next) + at * kSpD + row;
+#pragma unroll
+      for (int g = 0; g < kSpMaxGroup; ++g)
+        if (g < G) o[g * kSpD] = __uint_as_float(r[g]);
     }
   }
 
