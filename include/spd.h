@@ -296,7 +296,7 @@ int spd_attn_decode_paged_own(void* out, const void* q, const void* k_pool, cons
                               int64_t workspace_bytes, int sm_budget, spd_stream_t stream);
 /* Decode attention for requests that continue the same tokens.  Rows [group_indptr[g], group_indptr[g + 1]) of the batch
  * (int32, num_groups + 1 entries, ascending) are a group whose members' req_to_token rows name the same slots in their first
- * shared_lens[g] positions; max_shared_len is no less than any of those.  The result is spd_attn_decode_paged's: every row of
+ * shared_lens[g] positions; max_shared_len is no less than any of those; the pools have pool_slots rows.  The result is spd_attn_decode_paged's: every row of
  * req_to_token is complete, rows of no group stand alone, seq_lens[b] counts the shared tokens too, and a request of length
  * 0 gets zeros.  The shared part of a group is read once for all of its queries.
  * Workspace: spd_attn_decode_shared_workspace_bytes(), zeroed once before its first use (each call leaves its counters at
@@ -307,7 +307,7 @@ int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_head
 int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
                            const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
                            const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t max_shared_len,
-                           int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
+                           int64_t pool_slots, int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
                            int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
                            int sm_budget, spd_stream_t stream);
 /* Plain SIMT implementations of the two calls above (no tensor cores).  Bring-up / on-device

@@ -63,9 +63,9 @@ static_assert(kSpStage == 2 * 4 * kSpSmall, "one memory for both");
 constexpr int kSpBars = 256;
 constexpr int kSpRed = 2 * 2 * kSpMaxGroup * 4 * 4;  // per warpgroup, twice: the maxima or sums of 4 warps for every head
 constexpr float kSpRescale = 8.f;  // exponent of 2 that a score may pass the reference maximum by
-// what the list's entries cost: a key tile for two query tiles, for one; an item's start and end
-constexpr int kCostPair = 3, kCostTile = 2, kCostShared = 4, kCostOwn = 1;
-constexpr int kCostMin = 4;  // of a CTA
+// What the list's entries cost, in 700 clk: a key tile for two query tiles, for one, over own keys; an item's start and end.
+constexpr int kCostPair = 6, kCostOne = 4, kCostOwnTile = 4, kCostShared = 8, kCostOwn = 1;
+constexpr int kCostMin = 8;  // of a CTA
 
 struct SharedParams {
   const void *k_pool, *v_pool;
@@ -79,9 +79,10 @@ struct SharedParams {
   float scale_log2;
   int use_tma;
   // parts.  o: fp32 rows of 128, before the division by l; ml: m (exponent of 2), l
-  float *o_first, *ml_first;  // [2: shared, own][batch][query heads]
-  float *o_next, *ml_next;    // [grid][2 tiles][128]
-  int2* notes;                // [2: shared, own][batch][kv heads]: the CTA of the first part; parts (0: none) | row there << 16
+  float *o_first, *ml_first;  // [3: shared, own, shared keys of warpgroup 1 in a split item][batch][query heads]
+  float *o_next, *ml_next;    // [grid][2 warpgroups][128]
+  // [2: shared, own][batch][kv heads]: the CTA of the first part; CTAs with parts (0: none) | split << 15 | row there << 16
+  int2* notes;
   unsigned* wait_expired;
 };
 
@@ -100,9 +101,12 @@ static_assert(kSpSmem <= 232448, "shared memory of one block");
 
 __device__ __forceinline__ int sp_pairs(int count, int mpt) { return count <= mpt ? 1 : (count + 2 * mpt - 1) / (2 * mpt); }
 // cost of a key tile in an item over shared keys
-__device__ __forceinline__ int sp_cost(int count, int mpt) { return count <= mpt ? kCostTile : kCostPair; }
+__device__ __forceinline__ int sp_cost(int count, int mpt) { return count <= mpt ? kCostOne : kCostPair; }
 __device__ __forceinline__ int sp_tiles(int len) { return (len + kSpTile - 1) / kSpTile; }
-__device__ __forceinline__ int sp_own_cost(int len) { return len > 0 ? kCostOwn + kCostTile * sp_tiles(len) : 0; }
+// of an item over own keys: its last tile costs what its keys do
+__device__ __forceinline__ int sp_own_cost(int len) {
+  return len > 0 ? kCostOwn + kCostOwnTile * ((len - 1) / kSpTile) + ((len - 1) % kSpTile) * kCostOwnTile / kSpTile + 1 : 0;
+}
 
 struct SpRange {
   int begin, end;  // this CTA's part of the list
@@ -236,22 +240,32 @@ __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl
 struct SpItem {
   int b0, hk;        // batch row of the first member, or of the request; kv head
   int req;           // page-table row
-  int rows0, rows1;  // shared keys: query rows of the two tiles
+  // Shared keys: query rows of the two tiles.  Where there is one tile only, the item is split: both warpgroups have it, with
+  // every second key tile each (the ring's slots 2 w and 2 w + 1), and leave a part each.
+  int rows0, rows1;
   int keys;          // keys that the item's tiles hold
   int s0, tiles;     // the list's position of its first tile; tiles
   int cost;          // of each
   int tile0, n;      // first key tile of this CTA and how many
-  // tiles that begin in [u, end); the list goes on behind them
-  __device__ __forceinline__ bool cut(int& u, int end) {
+  // tiles that begin in [u, end)
+  __device__ __forceinline__ bool cut(int u, int end) {
     tile0 = min(tiles, max(0, (u - s0 + cost - 1) / cost));
     n = min(tiles, max(0, (end - s0 + cost - 1) / cost)) - tile0;
-    u = min(end, s0 + tiles * cost);
     return n > 0;
   }
-  // for the join: the CTA of the first part, and how many parts | the row there of a kv head's first query << 16
-  __device__ __forceinline__ int2 note(int per, int row) const {
+  __device__ __forceinline__ bool split() const { return rows1 == 0; }
+  __device__ __forceinline__ int rows(int w) const { return w == 0 || split() ? rows0 : rows1; }
+  __device__ __forceinline__ int member0(int w, int mpt) const { return split() ? b0 : b0 + w * mpt; }
+  // warpgroup w's tiles of this CTA are first, first + step, ..., `count` of them; base: tiles of the items before
+  __device__ __forceinline__ void share(int w, uint32_t base, int& first, int& step, int& count) const {
+    first = split() ? static_cast<int>((base ^ w) & 1) : 0;
+    step = split() ? 2 : 1;
+    count = (n - first + step - 1) / step;
+  }
+  // for the join, see SharedParams
+  __device__ __forceinline__ int2 note(int per, bool halves, int row) const {
     const int c0 = s0 / per;
-    return make_int2(c0, ((s0 + (tiles - 1) * cost) / per - c0 + 1) | row << 16);
+    return make_int2(c0, ((s0 + (tiles - 1) * cost) / per - c0 + 1) | (halves ? 1 << 15 : 0) | row << 16);
   }
 };
 
@@ -281,7 +295,9 @@ struct SpWalk {
       it.rows1 = min(p.mpt, max(0, left - p.mpt)) * p.group;
       it.keys = it.tiles * kSpTile;
       it.s0 = pl.unit0[g] + item * per_item + kCostShared;
-      if (it.cut(u, end)) return true;
+      const bool some = it.cut(u, end);
+      u = min(end, it.s0 + it.tiles * it.cost);
+      if (some) return true;
     }
     return false;
   }
@@ -312,10 +328,9 @@ struct SpOwnWalk {
       if (it.keys > 0) {
         it.tiles = sp_tiles(it.keys);
         it.s0 = u + kCostOwn;
-        it.cost = kCostTile;
-        int from = max(u, r.begin);
-        some = it.cut(from, end);
-        u = it.s0 + it.tiles * kCostTile;
+        it.cost = kCostOwnTile;
+        some = it.cut(max(u, r.begin), end);
+        u += sp_own_cost(it.keys);
       }
       if (++head == p.Hk || it.keys <= 0) {
         head = 0;
@@ -378,6 +393,7 @@ template <typename T>
 __global__ void __launch_bounds__(kSpThreads, 1)
 attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQ1,
                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ CUtensorMap tmK16, const __grid_constant__ CUtensorMap tmV16,
                    const __grid_constant__ SharedParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -477,8 +493,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     auto load_q = [&](const SpItem& i) {
       if (leader) {
         mbar_expect_tx(&q_full[w], q_bytes);
-        tma_load_3d(sQ + w * kSpTileBytes, &tmQ, &q_full[w], 0, i.hk * p.group, i.b0 + w * p.mpt, kEvictNormal);
-        tma_load_3d(sQ + w * kSpTileBytes + 16384, &tmQ, &q_full[w], 64, i.hk * p.group, i.b0 + w * p.mpt, kEvictNormal);
+        const int b = i.member0(w, p.mpt);
+        tma_load_3d(sQ + w * kSpTileBytes, &tmQ, &q_full[w], 0, i.hk * p.group, b, kEvictNormal);
+        tma_load_3d(sQ + w * kSpTileBytes + 16384, &tmQ, &q_full[w], 64, i.hk * p.group, b, kEvictNormal);
       }
       __syncwarp();
     };
@@ -487,13 +504,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     while (have) {
       SpItem nx;
       const bool more = walk.next(p, pl, nx);
-      const int n = it.n, nt = (w == 0 ? it.rows0 : it.rows1) > 0 ? n : 0;
-      if (nt > 0) {
+      int first, step, count, nx_first, nx_step = 0, nx_count = 0;
+      it.share(w, t_base, first, step, count);
+      if (more) nx.share(w, t_base + it.n, nx_first, nx_step, nx_count);
+      if (count > 0) {
         if (!q_ahead) load_q(it);
         q_ahead = false;
         mbar_wait_bounded(&q_full[w], eq & 1, dead);
       }
-      // S(j, h): P(j - 1, h), which these columns held, has been consumed by PV(j - 1, h), issued earlier by this thread
+      // S(j, h): the P which these columns held has been consumed by the PV of this tile's predecessor here, issued earlier by
+      // this thread
       auto issue_s = [&](int j, int h) {
         const uint32_t pos = 2 * (t_base + j);
         wait_kv(pos);
@@ -510,55 +530,54 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         umma_commit_if(leader, &s_full[w * 2 + h]);
       };
-      // a ring slot is released by both issuers; one whose tile has no rows waits for the copy first, to keep to the phases
-      auto release_k = [&](int j) {
-        const uint32_t pos = 2 * (t_base + j);
-        if (nt == 0) wait_kv(pos);
+      // a ring slot gets an arrival from either issuer, or both from the only one that reads it
+      auto release = [&](uint32_t pos) {
         umma_commit_if(leader, &kv_empty[pos % kSpSlots]);
+        if (step == 2) umma_commit_if(leader, &kv_empty[pos % kSpSlots]);
       };
-      if (nt > 0) {
-        issue_s(0, 0);
-        issue_s(0, 1);
+      if (count > 0) {
+        issue_s(first, 0);
+        issue_s(first, 1);
+        release(2 * (t_base + first));
       }
-      release_k(0);
-      for (int j = 0; j < n; ++j) {
+      for (int i = 0; i < count; ++i) {
+        const int j = first + i * step;
         const uint32_t vpos = 2 * (t_base + j) + 1;
-        if (nt > 0) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (j == n - 1 && h == 0 && more && (w == 0 ? nx.rows0 : nx.rows1) > 0) {
-              // the item's last S is under way: once it is complete, Q's memory is free for the next item
-              mbar_wait_bounded(&s_full[w * 2 + 1], (pq >> 1) & 1, dead);
-              load_q(nx);
-              q_ahead = true;
-            }
-            mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
-            wait_kv(vpos);
-            if (h == 0) fence_proxy_async_smem();
-            if (j == 0 && h == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
-            tc_fence_after_sync();
-            uint32_t va = static_cast<uint32_t>(vd0) + (vpos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
-            uint32_t pa = tmem_S + w * 128 + h * kSpU;
-            uint32_t acc = (j > 0 || h > 0) ? 1u : 0u;
-#pragma unroll 1
-            for (int k = 0; k < kSpU / 16; ++k) {
-              umma_ts_if(leader, tmem_O + w * kSpD, pa, va, v_hi, idesc_pv, acc);
-              pa += 8;
-              va += 2048 / 16;
-              acc = 1;
-            }
-            umma_commit_if(leader, &pv_done[w * 2 + h]);
-            ++pq;
-            if (j + 1 < n) issue_s(j + 1, h);
+        for (int h = 0; h < 2; ++h) {
+          if (i == count - 1 && h == 0 && nx_count > 0) {
+            // the item's last S is under way: once it is complete, Q's memory is free for the next item
+            mbar_wait_bounded(&s_full[w * 2 + 1], (pq >> 1) & 1, dead);
+            load_q(nx);
+            q_ahead = true;
           }
-        } else {
+          mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
           wait_kv(vpos);
+          if (h == 0) fence_proxy_async_smem();
+          if (i == 0 && h == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
+          tc_fence_after_sync();
+          uint32_t va = static_cast<uint32_t>(vd0) + (vpos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
+          uint32_t pa = tmem_S + w * 128 + h * kSpU;
+          uint32_t acc = (i > 0 || h > 0) ? 1u : 0u;
+#pragma unroll 1
+          for (int k = 0; k < kSpU / 16; ++k) {
+            umma_ts_if(leader, tmem_O + w * kSpD, pa, va, v_hi, idesc_pv, acc);
+            pa += 8;
+            va += 2048 / 16;
+            acc = 1;
+          }
+          umma_commit_if(leader, &pv_done[w * 2 + h]);
+          ++pq;
+          if (i + 1 < count) issue_s(j + step, h);
         }
-        umma_commit_if(leader, &kv_empty[vpos % kSpSlots]);
-        if (j + 1 < n) release_k(j + 1);
+        release(vpos);
+        if (i + 1 < count) release(2 * (t_base + j + step));
       }
-      if (nt > 0) ++eq;
-      t_base += n;
+      // A split item's other tiles have not been seen here, and a parity tells a phase from the one before only: an item for
+      // both begins when both issuers have waited for all tiles before it.
+      if (step == 2 && more && nx_step == 1) asm volatile("bar.sync 3, 64;" ::: "memory");
+      if (count > 0) ++eq;
+      t_base += it.n;
       it = nx;
       have = more;
     }
@@ -612,10 +631,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const uint32_t h = pq & 1;
         mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
         mbar_wait_bounded(&kv_full[at.bar], at.full, dead);
+        const int valid = min(kSpTile, it.keys - (it.tile0 + j) * kSpTile), steps = (valid + 15) / 16;  // of 16 keys
+        if (valid & 15) {  // V rows that the last step takes in and nobody asked for: their P is 0, they may be anything
+          uint8_t* rows = smem + at.tile * kSpTileBytes + (lane >> 3 & 1) * 16384 + (lane & 7) * 16;
+          for (int r = valid + (lane >> 4); r < steps * 16; r += 2) *reinterpret_cast<uint4*>(rows + r * 128) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         fence_proxy_async_smem();
         if (j == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
         tc_fence_after_sync();
-        const int steps = min(kSpTile, it.keys - (it.tile0 + j) * kSpTile + 15) / 16;  // of 16 keys
         uint32_t va = v_lo + at.tile * (kSpTileBytes / 16), pa = p_lo + h * (kSpSmall / 16);
 #pragma unroll 1
         for (int k = 0; k < steps; ++k) {
@@ -643,18 +668,26 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     };
     // a tile into the memory at `tile`; its barrier gets 32 arrivals
     auto load = [&](int is_v, int bar, int tile, int hk, const int* slot, int valid) {
-      const CUtensorMap* tmap = is_v ? &tmV : &tmK;
       const int base = __shfl_sync(0xffffffffu, slot[0], 0);
       bool contig = p.use_tma && base > 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) contig &= slot[i] == base + i * 32 + lane;
+      for (int i = 0; i < 4; ++i) contig &= lane + i * 32 >= valid || slot[i] == base + i * 32 + lane;
       if (__all_sync(0xffffffffu, contig)) {
+        // Consecutive slots: boxes of 128 rows, or of 16 as far as the valid ones reach.  What stands behind those belongs to
+        // others, or lies past the pool and reads as zeros: the scores of such K rows are not looked at, such V rows are
+        // cleared before the MMA.
+        uint8_t* dst = smem + tile * kSpTileBytes;
+        const int pieces = (valid + 15) / 16;
         if (lane == 0) {
-          uint8_t* dst = smem + tile * kSpTileBytes;
           fence_proxy_async_smem();  // the slot may last have been written by the gather path
-          mbar_expect_tx_noarrive(&kv_full[bar], kSpTileBytes);
-          tma_load_2d(dst, tmap, &kv_full[bar], hk * kSpD, base, kEvictNormal);
-          tma_load_2d(dst + 16384, tmap, &kv_full[bar], hk * kSpD + 64, base, kEvictNormal);
+          mbar_expect_tx_noarrive(&kv_full[bar], pieces * 16 * 256);
+        }
+        __syncwarp();
+        if (pieces == 8) {
+          if (lane < 2) tma_load_2d(dst + lane * 16384, is_v ? &tmV : &tmK, &kv_full[bar], hk * kSpD + lane * 64, base, kEvictNormal);
+        } else if (lane < 2 * pieces) {
+          tma_load_2d(dst + (lane & 1) * 16384 + (lane >> 1) * 2048, is_v ? &tmV16 : &tmK16, &kv_full[bar],
+                      hk * kSpD + (lane & 1) * 64, base + (lane >> 1) * 16, kEvictNormal);
         }
         __syncwarp();
         mbar_arrive(&kv_full[bar]);
@@ -662,12 +695,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
       const uint32_t dst = smem_u32(smem + tile * kSpTileBytes);
       const T* col = reinterpret_cast<const T*>(is_v ? p.v_pool : p.k_pool) + static_cast<int64_t>(hk) * kSpD + chunk * 8;
-      // K rows behind the item's last key stay what they are (their scores are not looked at); V rows up to the next
-      // multiple of 16, an MMA's step, become zeros
-      const int fill = is_v ? min(kSpTile, valid + 15) & ~15 : valid;
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
-        if (i4 * 32 >= fill) break;
+        if (i4 * 32 >= valid) break;
         // (slots first: a shuffle waited for before every copy made it 35 clk a copy)
         int s[16];
 #pragma unroll
@@ -675,7 +705,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int row = i4 * 32 + i * 2 + rsub;
-          if (i4 * 32 + i * 2 < fill) cp_async16(dst + sp_tile_off(row, chunk), col + max(s[i], 0) * row_elems, s[i] >= 0);
+          if (i4 * 32 + i * 2 < valid) cp_async16(dst + sp_tile_off(row, chunk), col + max(s[i], 0) * row_elems, s[i] >= 0);
         }
       }
       cp_async_mbar_arrive_noinc(&kv_full[bar]);  // when this lane's copies have landed
@@ -751,12 +781,13 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int r = row0 + i * 8 + (lane >> 2), m = r / p.group;
         o_at[i] = (m * p.Hq + r - m * p.group) * kSpD + (lane & 3) * 4;
       }
-      while (walk.next(p, pl, it)) {
-        const int rows = w == 0 ? it.rows0 : it.rows1;
-        if (rows == 0) continue;
+      for (; walk.next(p, pl, it); t_base += it.n) {
+        int first_tile, step, count;
+        it.share(w, t_base, first_tile, step, count);
+        const int rows = it.rows(w);
         const bool active = row0 < rows;  // (of this warp: the others only keep the barriers' count)
         float m = -INFINITY, l = 0.f;     // the reference maximum (raw scores) and sum folded into O
-        const uint32_t u0 = u, u1 = u + 2 * it.n;
+        const uint32_t u0 = u, u1 = u + 2 * count;
         for (; u < u1; ++u) {
           const int h = u & 1;
           mbar_wait_bounded(&s_full[w * 2 + h], (u >> 1) & 1, dead);
@@ -791,40 +822,43 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         // the item's part: O through shared memory, 64 bytes of a row at a time (a thread per row would touch 32 lines a store)
         if (active) {
           const bool first = it.tile0 == 0;
-          const int64_t at = first ? static_cast<int64_t>(it.b0 + w * p.mpt) * p.Hq + it.hk * p.group
+          const int b0 = it.member0(w, p.mpt);
+          const int64_t at = first ? static_cast<int64_t>((it.split() && w == 1 ? 2 * p.batch : 0) + b0) * p.Hq + it.hk * p.group
                                    : (static_cast<int64_t>(blockIdx.x) * 2 + w) * kSpM;
-          mbar_wait_bounded(&pv_done[w * 2 + 1], ((u - 1) >> 1) & 1, dead);
-          tc_fence_after_sync();
-          float* o = (first ? p.o_first : p.o_next) + at * kSpD;
+          if (count > 0) {
+            mbar_wait_bounded(&pv_done[w * 2 + 1], ((u - 1) >> 1) & 1, dead);
+            tc_fence_after_sync();
+            float* o = (first ? p.o_first : p.o_next) + at * kSpD;
 #pragma unroll 1
-          for (int c = 0; c < kSpD; c += 16) {
-            uint32_t r[16];
-            tmem_ld_32x32b_x16(to + c, r);
-            tmem_ld_wait();
+            for (int c = 0; c < kSpD; c += 16) {
+              uint32_t r[16];
+              tmem_ld_32x32b_x16(to + c, r);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-            __syncwarp();
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+              __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = i * 8 + (lane >> 2);
-              if (row0 + rr < rows)
-                *reinterpret_cast<uint4*>(o + (first ? o_at[i] : (row0 + rr) * kSpD + (lane & 3) * 4) + c) =
-                    *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+              for (int i = 0; i < 4; ++i) {
+                const int rr = i * 8 + (lane >> 2);
+                if (row0 + rr < rows)
+                  *reinterpret_cast<uint4*>(o + (first ? o_at[i] : (row0 + rr) * kSpD + (lane & 3) * 4) + c) =
+                      *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+              }
+              __syncwarp();
             }
-            __syncwarp();
           }
           if (row < rows)
             reinterpret_cast<float2*>(first ? p.ml_first : p.ml_next)[at + (first ? ml_at : row)] = make_float2(m * scale, l);
-          // (an empty request in the middle of a group takes no part)
-          const int b = it.b0 + w * p.mpt + member;
-          if (first && row < rows && row == member * p.group && pl.skip[b] > 0)
-            p.notes[b * p.Hk + it.hk] = it.note(range.per, w * kSpM + row);
+          // (an empty request in the middle of a group takes no part; without a tile the part is one of sum 0)
+          const int b = b0 + member;
+          if (first && row < rows && row == member * p.group && pl.skip[b] > 0 && (w == 0 || !it.split()))
+            p.notes[b * p.Hk + it.hk] = it.note(range.per, it.split(), w * kSpM + row);
           tc_fence_before_sync();
           __syncwarp();
         }
-        if (lane == 0) mbar_arrive(&o_free[w]);
+        if (lane == 0 && count > 0) mbar_arrive(&o_free[w]);
       }
       fence_proxy_async_smem();  // queries are copied into the staging memory
       __syncwarp();
@@ -921,7 +955,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             ml[g] = make_float2(m_ref[g], (x.x + x.y) + (x.z + x.w));
           }
         // behind the CTA of the first part an item is its CTA's first, so it is warpgroup 0's there
-        if (first) p.notes[(p.batch + it.b0) * p.Hk + it.hk] = it.note(range.per, 0);
+        if (first) p.notes[(p.batch + it.b0) * p.Hk + it.hk] = it.note(range.per, false, 0);
       }
       ++rounds;
       mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
@@ -962,15 +996,15 @@ attn_shared_join_kernel(T* __restrict__ out, int64_t out_stride, const __grid_co
   if (row >= rows) return;
   const int b = row / p.Hq, h = row - b * p.Hq, hk = h / p.group;
   const int2 ns = __ldcg(p.notes + b * p.Hk + hk), no = __ldcg(p.notes + (p.batch + b) * p.Hk + hk);
-  const int shared = ns.y & 0xffff, parts = shared + (no.y & 0xffff);
+  const int halves = ns.y >> 15 & 1, shared = (ns.y & 0x7fff) << halves, parts = shared + (no.y & 0x7fff);
   // the i-th part's row among those by batch row (its first) or by CTA
   auto place = [&](int i, bool& first) {
     const bool own = i >= shared;
     const int2 n = own ? no : ns;
-    const int k = own ? i - shared : i;
+    const int k = own ? i - shared : i >> halves, second = own ? 0 : i & halves;
     first = k == 0;
-    return first ? static_cast<int64_t>(own ? rows : 0) + row
-                 : (static_cast<int64_t>(n.x) + k) * 2 * kSpM + (n.y >> 16) + (h - hk * p.group);
+    return first ? static_cast<int64_t>(own ? 1 : 2 * second) * rows + row
+                 : (static_cast<int64_t>(n.x) + k) * 2 * kSpM + second * kSpM + (n.y >> 16) + (h - hk * p.group);
   };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = -INFINITY, den = 0.f;
@@ -1004,10 +1038,12 @@ attn_shared_join_kernel(T* __restrict__ out, int64_t out_stride, const __grid_co
       for (int k = 0; k < kSjParts; ++k)
         if (j0 + k < here) {
           const float f = __shfl_sync(0xffffffffu, wt, j0 + k);
-          acc.x = fmaf(f, v[k].x, acc.x);
-          acc.y = fmaf(f, v[k].y, acc.y);
-          acc.z = fmaf(f, v[k].z, acc.z);
-          acc.w = fmaf(f, v[k].w, acc.w);
+          if (f != 0.f) {  // (a part of sum 0 has no columns)
+            acc.x = fmaf(f, v[k].x, acc.x);
+            acc.y = fmaf(f, v[k].y, acc.y);
+            acc.z = fmaf(f, v[k].z, acc.z);
+            acc.w = fmaf(f, v[k].w, acc.w);
+          }
         }
     }
   }
@@ -1026,7 +1062,7 @@ static int64_t decode_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
 }
 static int64_t part_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
   const int64_t b = batch < kSpRows ? batch : kSpRows;
-  return (2 * b * num_q_heads + static_cast<int64_t>(device_sm_count_cached()) * 2 * kSpM) * (kSpD + 2) * 4 + 2 * b * num_kv_heads * 8;
+  return (3 * b * num_q_heads + static_cast<int64_t>(device_sm_count_cached()) * 2 * kSpM) * (kSpD + 2) * 4 + 2 * b * num_kv_heads * 8;
 }
 
 }  // namespace spd
@@ -1044,13 +1080,13 @@ int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_head
 int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
                            const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
                            const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t max_shared_len,
-                           int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
+                           int64_t pool_slots, int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
                            int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
                            int sm_budget, spd_stream_t stream) {
   if (int rc = check_attn_args("spd_attn_decode_shared", out, q, k_pool, v_pool, req_to_token, req_pool_indices, num_q_heads,
                                num_kv_heads, head_dim, q_stride, out_stride))
     return rc;
-  SPD_REQUIRE(seq_lens && batch >= 0 && num_groups >= 0 && max_shared_len >= 0 && (num_groups == 0 || (group_indptr && shared_lens)),
+  SPD_REQUIRE(seq_lens && batch >= 0 && num_groups >= 0 && max_shared_len >= 0 && pool_slots > 0 && pool_slots < (1ll << 31) && (num_groups == 0 || (group_indptr && shared_lens)),
               SPD_E_BADARG, "spd_attn_decode_shared: bad lengths or groups");
   SPD_REQUIRE(head_dim == kSpD, SPD_E_SHAPE, "spd_attn_decode_shared: head_dim must be 128 (got %d)", head_dim);
   if (batch == 0) return 0;
@@ -1086,20 +1122,22 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
   p.mpt = kSpM / p.group;
   const int64_t rows = batch * num_q_heads;
   p.o_first = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_bytes(batch, num_q_heads, num_kv_heads));
-  p.o_next = p.o_first + 2 * rows * kSpD;
+  p.o_next = p.o_first + 3 * rows * kSpD;
   p.ml_first = p.o_next + static_cast<int64_t>(sms) * 2 * kSpM * kSpD;
-  p.ml_next = p.ml_first + 2 * rows * 2;
+  p.ml_next = p.ml_first + 3 * rows * 2;
   p.notes = reinterpret_cast<int2*>(p.ml_next + static_cast<int64_t>(sms) * 2 * kSpM * 2);
   // q as [batch][heads][128]: a box of mpt members and a kv head's query heads is a tile of mpt x group rows
-  CUtensorMap tq, tq1, tk, tv;
+  CUtensorMap tq, tq1, tk, tv, tk16, tv16;
   const uint64_t dims[3] = {kSpD, static_cast<uint64_t>(num_q_heads), static_cast<uint64_t>(batch)};
   const uint64_t strides[2] = {kSpD, static_cast<uint64_t>(q_stride)};
   const uint32_t box[3] = {64, static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.mpt)}, box1[3] = {64, box[1], 1};
   if (int rc = make_tmap_sw128(&tq, q, 3, dims, strides, box)) return rc;
   if (int rc = make_tmap_sw128(&tq1, q, 3, dims, strides, box1)) return rc;
-  const uint64_t row_elems = static_cast<uint64_t>(num_kv_heads) * kSpD;
-  if (int rc = get_tmap(&tk, k_pool, 1ull << 31, row_elems, row_elems, kSpTile)) return rc;
-  if (int rc = get_tmap(&tv, v_pool, 1ull << 31, row_elems, row_elems, kSpTile)) return rc;
+  const uint64_t row_elems = static_cast<uint64_t>(num_kv_heads) * kSpD, slots = static_cast<uint64_t>(pool_slots);
+  if (int rc = get_tmap(&tk, k_pool, slots, row_elems, row_elems, kSpTile)) return rc;
+  if (int rc = get_tmap(&tv, v_pool, slots, row_elems, row_elems, kSpTile)) return rc;
+  if (int rc = get_tmap(&tk16, k_pool, slots, row_elems, row_elems, 16)) return rc;
+  if (int rc = get_tmap(&tv16, v_pool, slots, row_elems, row_elems, 16)) return rc;
   SPD_DISPATCH_DTYPE(dtype, {
     auto kern = attn_shared_kernel<T>;
     static bool configured = false;
@@ -1107,7 +1145,7 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
       SPD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpSmem));
       configured = true;
     }
-    SPD_CUDA(launch(kern, dim3(sms), dim3(kSpThreads), kSpSmem, as_stream(stream), pdl_enabled(), tq, tq1, tk, tv, p));
+    SPD_CUDA(launch(kern, dim3(sms), dim3(kSpThreads), kSpSmem, as_stream(stream), pdl_enabled(), tq, tq1, tk, tv, tk16, tv16, p));
     SPD_CUDA(launch(attn_shared_join_kernel<T>, dim3(static_cast<unsigned>((rows + kSjWarps - 1) / kSjWarps)), dim3(kSjWarps * 32), 0,
                     as_stream(stream), pdl_enabled(), static_cast<T*>(out), out_stride, p, static_cast<int>(rows)));
   });

@@ -809,7 +809,8 @@ def attn_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     if not (q.dtype == k_pool.dtype == v_pool.dtype):
         raise RuntimeError("attn_decode_shared: q and the pools share a dtype")
     row = (num_kv_heads, head_dim)
-    if any(t.dim() != 3 or tuple(t.shape[1:]) != row or not t.is_contiguous() for t in (k_pool, v_pool)):
+    if any(t.dim() != 3 or tuple(t.shape[1:]) != row or not t.is_contiguous() for t in (k_pool, v_pool)) or \
+            k_pool.shape[0] != v_pool.shape[0]:
         raise RuntimeError("attn_decode_shared: the pools are contiguous [slots, kv heads, head_dim]")
     if req_to_token.dtype != torch.int32 or req_to_token.dim() != 2 or req_to_token.stride(1) != 1:
         raise RuntimeError("attn_decode_shared: req_to_token is int32 with contiguous rows")
@@ -832,7 +833,7 @@ def attn_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
         workspace = new_attn_shared_workspace(q.device, B, num_q_heads, num_kv_heads, head_dim)
     check(lib.spd_attn_decode_shared(o2.data_ptr(), q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), req_to_token.data_ptr(),
                                      req_pool_indices.data_ptr(), seq_lens.data_ptr(), group_indptr.data_ptr(),
-                                     shared_lens.data_ptr(), B, G, int(max_shared_len), num_q_heads, num_kv_heads, head_dim,
+                                     shared_lens.data_ptr(), B, G, int(max_shared_len), k_pool.shape[0], num_q_heads, num_kv_heads, head_dim,
                                      q2.stride(0), o2.stride(0), req_to_token.stride(0), float(sm_scale), _dt(q),
                                      workspace.data_ptr(), workspace.numel(), get_sm_budget(), _stream()),
           "spd_attn_decode_shared")
