@@ -19,8 +19,8 @@
 // ones, 32 / 8 heads, 48.6 us; each of them starts for 5 us without using the memory.)
 //
 //   warps 0-3 / 4-7  softmax of query tile 0 / 1: one thread per query row; P goes back into the TMEM columns of its S
-//   warp 8, warp 9   K / V loader: a ring of four 128 x 128 tiles, K_j V_j K_{j+1} ..., by TMA where a tile's slots are
-//                    consecutive, gathered row by row elsewhere; over own keys both, for warpgroup 0 / 1
+//   warp 8, warp 9   K / V loader: a ring of four 128 x 128 tiles, K_j V_j K_{j+1} ..., by TMA (single rows where a
+//                    tile's slots are not consecutive); over own keys both, for warpgroup 0 / 1
 //   warp 10, warp 11 MMA issuer of query tile 0 / 1
 // Over shared keys a tile is taken in two halves of 64 keys, so that a warpgroup's softmax of one half runs beside the MMAs of
 // the other.  An item over own keys has the few query heads of one kv head as its rows; it is computed the other way round,
@@ -68,7 +68,6 @@ constexpr int kCostPair = 6, kCostOne = 4, kCostOwnTile = 4, kCostShared = 8, kC
 constexpr int kCostMin = 8;  // of a CTA
 
 struct SharedParams {
-  const void *k_pool, *v_pool;
   const int32_t* req_to_token;
   const int64_t *req_pool_indices, *seq_lens;
   const int32_t* group_indptr;  // [groups + 1]
@@ -77,7 +76,6 @@ struct SharedParams {
   int groups, mpt;              // mpt: members of a query tile, 128 / group
   int64_t rtt_stride;
   float scale_log2;
-  int use_tma;
   // parts.  o: fp32 rows of 128, before the division by l; ml: m (exponent of 2), l
   float *o_first, *ml_first;  // [3: shared, own, shared keys of warpgroup 1 in a split item][batch][query heads]
   float *o_next, *ml_next;    // [grid][2 warpgroups][128]
@@ -344,11 +342,6 @@ struct SpOwnWalk {
   }
 };
 
-// byte offset of (row, 16-byte chunk) inside a tile of two [128 rows x 128 B] blocks with the 128-byte swizzle
-__device__ __forceinline__ uint32_t sp_tile_off(int row, int chunk16) {
-  return (chunk16 >> 3) * 16384 + row * 128 + (((chunk16 & 7) ^ (row & 7)) << 4);
-}
-
 // of an element of P^T: row (query head), key
 __device__ __forceinline__ uint32_t sp_p_off(int row, int key) {
   const int chunk = key >> 3;
@@ -394,6 +387,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQ1,
                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ CUtensorMap tmK16, const __grid_constant__ CUtensorMap tmV16,
+                   const __grid_constant__ CUtensorMap tmK1, const __grid_constant__ CUtensorMap tmV1,
                    const __grid_constant__ SharedParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -517,7 +511,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       auto issue_s = [&](int j, int h) {
         const uint32_t pos = 2 * (t_base + j);
         wait_kv(pos);
-        if (h == 0) fence_proxy_async_smem();
         tc_fence_after_sync();
         uint32_t qa = static_cast<uint32_t>(qd);
         uint32_t ka = static_cast<uint32_t>(kd0) + (pos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
@@ -553,7 +546,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           }
           mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
           wait_kv(vpos);
-          if (h == 0) fence_proxy_async_smem();
           if (i == 0 && h == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
           tc_fence_after_sync();
           uint32_t va = static_cast<uint32_t>(vd0) + (vpos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
@@ -597,7 +589,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const OwnSlot at = own_slot(w, 2 * ks, t_base);
       const uint32_t h = pu & 1;
       mbar_wait_bounded(&kv_full[at.bar], at.full, dead);  // (Q arrives with the item's first tile here)
-      fence_proxy_async_smem();
       tc_fence_after_sync();
       uint32_t ka = k_lo + at.tile * (kSpTileBytes / 16), qa = q_lo + qs * (kSpSmall / 16);
 #pragma unroll 1
@@ -638,7 +629,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
-        fence_proxy_async_smem();
         if (j == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
         tc_fence_after_sync();
         uint32_t va = v_lo + at.tile * (kSpTileBytes / 16), pa = p_lo + h * (kSpSmall / 16);
@@ -659,56 +649,45 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   } else if (warp >= 8) {
     // ===================== loaders =====================
     const int lw = warp - 8;
-    const int chunk = lane & 15, rsub = lane >> 4;
-    const int64_t row_elems = static_cast<int64_t>(p.Hk) * kSpD;
-    // a tile's slots, four rows a lane, from its first row's entry on; -1: behind the item's last key
+    // a tile's slots, rows 4 lane .. 4 lane + 3, from its first row's entry on; -1: behind the item's last key
     auto lookup = [&](const int32_t* rtt, int left, int* s) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = lane + i * 32 < left ? rtt[lane + i * 32] : -1;
+      for (int i = 0; i < 4; ++i) s[i] = lane * 4 + i < left ? rtt[lane * 4 + i] : -1;
     };
-    // a tile into the memory at `tile`; its barrier gets 32 arrivals
+    // A tile into the memory at `tile`; its barrier gets 32 arrivals beside the bytes.  Consecutive slots: one box, or where
+    // only 16 of them are, or a tile ends early, boxes of 16 rows; others: four rows an instruction.  (Scattered rows by 16-byte
+    // cp.async took a warp 4500 clk a tile.)  What stands behind an item's last key in a box belongs to others, or lies past
+    // the pool and reads as zeros: the scores of such K rows are not looked at, such V rows are cleared before the MMA.
     auto load = [&](int is_v, int bar, int tile, int hk, const int* slot, int valid) {
-      const int base = __shfl_sync(0xffffffffu, slot[0], 0);
-      bool contig = p.use_tma && base > 0;
+      uint8_t* dst = smem + tile * kSpTileBytes;
+      const int base = __shfl_sync(0xffffffffu, slot[0], 0), base16 = __shfl_sync(0xffffffffu, slot[0], lane & ~3);
+      bool all = base >= 0, some = base16 >= 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) contig &= lane + i * 32 >= valid || slot[i] == base + i * 32 + lane;
-      if (__all_sync(0xffffffffu, contig)) {
-        // Consecutive slots: boxes of 128 rows, or of 16 as far as the valid ones reach.  What stands behind those belongs to
-        // others, or lies past the pool and reads as zeros: the scores of such K rows are not looked at, such V rows are
-        // cleared before the MMA.
-        uint8_t* dst = smem + tile * kSpTileBytes;
-        const int pieces = (valid + 15) / 16;
-        if (lane == 0) {
-          fence_proxy_async_smem();  // the slot may last have been written by the gather path
-          mbar_expect_tx_noarrive(&kv_full[bar], pieces * 16 * 256);
-        }
-        __syncwarp();
-        if (pieces == 8) {
-          if (lane < 2) tma_load_2d(dst + lane * 16384, is_v ? &tmV : &tmK, &kv_full[bar], hk * kSpD + lane * 64, base, kEvictNormal);
-        } else if (lane < 2 * pieces) {
-          tma_load_2d(dst + (lane & 1) * 16384 + (lane >> 1) * 2048, is_v ? &tmV16 : &tmK16, &kv_full[bar],
-                      hk * kSpD + (lane & 1) * 64, base + (lane >> 1) * 16, kEvictNormal);
-        }
-        __syncwarp();
-        mbar_arrive(&kv_full[bar]);
-        return;
+      for (int i = 0; i < 4; ++i) {
+        all &= slot[i] == base + lane * 4 + i;
+        some &= lane * 4 + i >= valid || slot[i] == base16 + (lane & 3) * 4 + i;
       }
-      const uint32_t dst = smem_u32(smem + tile * kSpTileBytes);
-      const T* col = reinterpret_cast<const T*>(is_v ? p.v_pool : p.k_pool) + static_cast<int64_t>(hk) * kSpD + chunk * 8;
+      all = __all_sync(0xffffffffu, all);
+      some = (__ballot_sync(0xffffffffu, some) >> (lane & ~3) & 15) == 15;
+      const int pieces = (valid + 15) / 16, col = hk * kSpD;
+      if (lane == 0) mbar_expect_tx_noarrive(&kv_full[bar], pieces * 16 * 256);
+      __syncwarp();
+      if (all) {
+        if (lane < 2) tma_load_2d(dst + lane * 16384, is_v ? &tmV : &tmK, &kv_full[bar], col + lane * 64, base, kEvictNormal);
+      } else if (lane >> 2 < pieces) {
+        if (some) {
+          if ((lane & 3) < 2)
+            tma_load_2d(dst + (lane & 1) * 16384 + (lane >> 2) * 2048, is_v ? &tmV16 : &tmK16, &kv_full[bar], col + (lane & 1) * 64,
+                        base16, kEvictNormal);
+        } else {
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        if (i4 * 32 >= valid) break;
-        // (slots first: a shuffle waited for before every copy made it 35 clk a copy)
-        int s[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = __shfl_sync(0xffffffffu, slot[i4], i * 2 + rsub);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int row = i4 * 32 + i * 2 + rsub;
-          if (i4 * 32 + i * 2 < valid) cp_async16(dst + sp_tile_off(row, chunk), col + max(s[i], 0) * row_elems, s[i] >= 0);
+          for (int half = 0; half < 2; ++half)
+            tma_gather4_2d(smem_u32(dst + half * 16384 + lane * 512), is_v ? &tmV1 : &tmK1, &kv_full[bar], col + half * 64, slot[0],
+                           slot[1], slot[2], slot[3], kEvictNormal);
         }
       }
-      cp_async_mbar_arrive_noinc(&kv_full[bar]);  // when this lane's copies have landed
+      __syncwarp();
+      mbar_arrive(&kv_full[bar]);
     };
     // ---- shared keys: K by warp 8, V by warp 9; lookups run one tile ahead of the copies ----
     int slot[4], next[4];
@@ -1103,8 +1082,6 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
                                      workspace_bytes, sm_budget, stream);
   SharedParams p{};
   if (int rc = wait_flag(&p.wait_expired)) return rc;
-  p.k_pool = k_pool;
-  p.v_pool = v_pool;
   p.req_to_token = req_to_token;
   p.req_pool_indices = req_pool_indices;
   p.seq_lens = seq_lens;
@@ -1114,8 +1091,6 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
   p.group = num_q_heads / num_kv_heads;
   p.rtt_stride = req_to_token_stride;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
-  static const bool tma_on = []() { const char* e = getenv("SPD_ATTN_TMA"); return !(e && e[0] == '0'); }();
-  p.use_tma = tma_on ? 1 : 0;
   p.group_indptr = group_indptr;
   p.shared_lens = shared_lens;
   p.groups = static_cast<int>(num_groups);
@@ -1127,7 +1102,7 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
   p.ml_next = p.ml_first + 3 * rows * 2;
   p.notes = reinterpret_cast<int2*>(p.ml_next + static_cast<int64_t>(sms) * 2 * kSpM * 2);
   // q as [batch][heads][128]: a box of mpt members and a kv head's query heads is a tile of mpt x group rows
-  CUtensorMap tq, tq1, tk, tv, tk16, tv16;
+  CUtensorMap tq, tq1, tk, tv, tk16, tv16, tk1, tv1;
   const uint64_t dims[3] = {kSpD, static_cast<uint64_t>(num_q_heads), static_cast<uint64_t>(batch)};
   const uint64_t strides[2] = {kSpD, static_cast<uint64_t>(q_stride)};
   const uint32_t box[3] = {64, static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.mpt)}, box1[3] = {64, box[1], 1};
@@ -1138,6 +1113,8 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
   if (int rc = get_tmap(&tv, v_pool, slots, row_elems, row_elems, kSpTile)) return rc;
   if (int rc = get_tmap(&tk16, k_pool, slots, row_elems, row_elems, 16)) return rc;
   if (int rc = get_tmap(&tv16, v_pool, slots, row_elems, row_elems, 16)) return rc;
+  if (int rc = get_tmap(&tk1, k_pool, slots, row_elems, row_elems, 1)) return rc;
+  if (int rc = get_tmap(&tv1, v_pool, slots, row_elems, row_elems, 1)) return rc;
   SPD_DISPATCH_DTYPE(dtype, {
     auto kern = attn_shared_kernel<T>;
     static bool configured = false;
@@ -1145,7 +1122,7 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
       SPD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpSmem));
       configured = true;
     }
-    SPD_CUDA(launch(kern, dim3(sms), dim3(kSpThreads), kSpSmem, as_stream(stream), pdl_enabled(), tq, tq1, tk, tv, tk16, tv16, p));
+    SPD_CUDA(launch(kern, dim3(sms), dim3(kSpThreads), kSpSmem, as_stream(stream), pdl_enabled(), tq, tq1, tk, tv, tk16, tv16, tk1, tv1, p));
     SPD_CUDA(launch(attn_shared_join_kernel<T>, dim3(static_cast<unsigned>((rows + kSjWarps - 1) / kSjWarps)), dim3(kSjWarps * 32), 0,
                     as_stream(stream), pdl_enabled(), static_cast<T*>(out), out_stride, p, static_cast<int>(rows)));
   });
