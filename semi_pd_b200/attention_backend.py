@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import ops
-from .forward_batch_info import ForwardBatch, ForwardMode
+from .forward_batch_info import ForwardBatch, ForwardMode, SharedPrefix
 
 
 class AttentionBackend(ABC):
@@ -125,7 +125,7 @@ class SpdAttnBackend(AttentionBackend):
         self.num_q_heads = model_runner.model_config.num_attention_heads // model_runner.tp_size
         self.head_dim = model_runner.model_config.head_dim
         self.is_mla = getattr(model_runner.model_config, "model_type", "llama") == "deepseek_v2"
-        self.mla_workspace = self.decode_workspace = None
+        self.mla_workspace = self.decode_workspace = self.shared_workspace = None
         if getattr(model_runner.model_config, "layer_specs", None) is not None:
             # hybrid family: every layer runs the general kernel or a retention mixer, neither of
             # which needs a workspace or a host-side plan
@@ -148,11 +148,18 @@ class SpdAttnBackend(AttentionBackend):
             self.mla_workspace = torch.zeros((need,), dtype=torch.uint8, device=self.device)
             self.decode_workspace = None
             return
-        num_kv_heads = model_runner.model_config.get_num_kv_heads(model_runner.tp_size)
+        num_kv_heads = self.num_kv_heads = model_runner.model_config.get_num_kv_heads(model_runner.tp_size)
         sms = ops.device_sm_count(self.device.index or 0)
         self.split_rows = -(-sms // max(num_kv_heads, 1)) + 1
         need = ops.lib.spd_attn_decode_workspace_bytes(self.split_rows, self.num_q_heads, self.head_dim)
         self.decode_workspace = torch.zeros((need,), dtype=torch.uint8, device=self.device)
+
+    def shares_prefix(self, batch_size: int, shared: SharedPrefix) -> bool:
+        """Whether decode attention takes a batch's shared prefix into account: where reading it once is the faster way."""
+        if self.impl != "tc" or self.is_mla:
+            return False
+        return ops.attn_shared_pays(batch_size, shared.shared_lens.numel(), shared.max_shared_len, self.num_q_heads,
+                                    self.num_kv_heads, self.head_dim)
 
     def init_forward_metadata(self, forward_batch: ForwardBatch):
         if forward_batch.forward_mode.is_extend():
@@ -325,6 +332,17 @@ class SpdAttnBackend(AttentionBackend):
         if layer.general:
             return self._forward_general(q, layer, forward_batch)
         k_buf, v_buf = pool.get_kv_buffer(layer.layer_id)
+        shared = forward_batch.shared_prefix
+        if shared is not None:
+            # not captured (CudaGraphRunner.can_run), so the scratch may grow
+            need = ops.lib.spd_attn_decode_shared_workspace_bytes(forward_batch.batch_size, layer.tp_q_head_num,
+                                                                  layer.tp_k_head_num, layer.head_dim)
+            if self.shared_workspace is None or self.shared_workspace.numel() < need:
+                self.shared_workspace = torch.zeros((need,), dtype=torch.uint8, device=self.device)
+            return ops.attn_decode_shared(
+                q, k_buf, v_buf, forward_batch.req_to_token_pool.req_to_token, forward_batch.req_pool_indices,
+                forward_batch.seq_lens, shared.group_indptr, shared.shared_lens, shared.max_shared_len,
+                layer.tp_q_head_num, layer.tp_k_head_num, layer.head_dim, layer.scaling, workspace=self.shared_workspace)
         return ops.attn_decode(
             q, k_buf, v_buf, forward_batch.req_to_token_pool.req_to_token,
             forward_batch.req_pool_indices, forward_batch.seq_lens, layer.tp_q_head_num,

@@ -1044,6 +1044,25 @@ static int64_t part_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
   return (3 * b * num_q_heads + static_cast<int64_t>(device_sm_count_cached()) * 2 * kSpM) * (kSpD + 2) * 4 + 2 * b * num_kv_heads * 8;
 }
 
+// Whether reading the shared keys once is the faster way, from what the host knows: as if all requests were in groups of one
+// size that share max_shared keys.  In us: a tile of 128 shared keys takes an SM 1.5 here and each member 0.88 there (mostly
+// from L2); requests that there are cut over many SMs cost 0.16 per part and query head in their merge; the longer start, the
+// join and the shorter ranges cost 6 here, and 0.0075 per request and kv head.
+// us by request / shared, own tokens 64, bf16.  32 / 8 heads, one group: 64 members of 256 tokens 18.8 / 25.8, 512: 23.8 / 24.1,
+// 1024: 33.6 / 24.2; 8 of 1024: 14.3 / 17.7, 4096: 25.0 / 24.6, 16384: 59.6 / 35.7; 4 of 4096: 21.7 / 24.1.  Groups of two: 8
+// of 4096: 45.9 / 50.7, of 16384: 160 / 112; 32 of 2048: 61.5 / 83.5, of 4096: 158 / 126.  16 / 2 heads, 2 of 1024: 17.8 / 16.7,
+// of 4096: 44.2 / 21.5.  32 / 32 heads, 16 of 256: 17.7 / 19.3, of 1024: 32.2 / 24.2.
+static bool shared_pays(int64_t batch, int64_t groups, int64_t max_shared, int num_q_heads, int num_kv_heads, int sms) {
+  const double pairs = static_cast<double>(batch) * num_kv_heads, shared = static_cast<double>(max_shared);
+  const double tiles = static_cast<double>(groups) * num_kv_heads * (shared / kSpTile) / sms;  // of an SM
+  double gain = tiles * (0.88 * batch / groups - 1.5);
+  if (pairs < sms) {
+    const double parts = sms / pairs < shared / 256 ? sms / pairs : shared / 256;
+    gain += 0.16 * (num_q_heads / num_kv_heads) * parts;
+  }
+  return gain > 6.0 + 0.0075 * pairs * 148 / sms;
+}
+
 }  // namespace spd
 
 using namespace spd;
@@ -1054,6 +1073,16 @@ int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_head
   if (max_batch < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim != kSpD) return 0;
   // (one behind the other: a call of the one kind leaves the counters of the other at zero)
   return decode_bytes(max_batch, num_q_heads, num_kv_heads) + part_bytes(max_batch, num_q_heads, num_kv_heads);
+}
+
+int spd_attn_decode_shared_pays(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
+                                int head_dim, int sm_budget) {
+  if (batch < 2 || batch > kSpRows || num_groups < 1 || num_groups > kSpGroups || max_shared_len < kSpTile || num_kv_heads < 1 ||
+      num_q_heads < num_kv_heads || head_dim != kSpD)
+    return 0;
+  const int device_sms = device_sm_count_cached();
+  return shared_pays(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads,
+                     sm_budget > 0 && sm_budget < device_sms ? sm_budget : device_sms);
 }
 
 int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
@@ -1074,9 +1103,10 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
               (long long)workspace_bytes);
   const int device_sms = device_sm_count_cached();
   const int sms = sm_budget > 0 && sm_budget < device_sms ? sm_budget : device_sms;
-  // Every request reads its own pages where nothing can be shared, where a plan would not hold the batch, and where the scale
-  // is not positive (the maximum of raw scores serves the scaled ones only there).
-  if (batch < 2 || batch > kSpRows || num_groups < 1 || num_groups > kSpGroups || max_shared_len < kSpTile || !(sm_scale > 0.f))
+  // Every request reads its own pages where nothing can be shared or it does not pay, where a plan would not hold the batch, and
+  // where the scale is not positive (the maximum of raw scores serves the scaled ones only there).
+  if (!(sm_scale > 0.f) ||
+      !spd_attn_decode_shared_pays(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, sm_budget))
     return spd_attn_decode_paged_own(out, q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, batch, num_q_heads,
                                      num_kv_heads, head_dim, q_stride, out_stride, req_to_token_stride, sm_scale, dtype, workspace,
                                      workspace_bytes, sm_budget, stream);

@@ -56,6 +56,16 @@ class ForwardMode(IntEnum):
 
 
 @dataclasses.dataclass
+class SharedPrefix:
+    """Requests of a decode batch that continue the same tokens (ops.attn_decode_shared): rows group_indptr[g] ..
+    group_indptr[g + 1] share the slots of their first shared_lens[g] tokens."""
+
+    group_indptr: torch.Tensor       # [groups + 1] int32, device
+    shared_lens: torch.Tensor        # [groups] int64, device
+    max_shared_len: int
+
+
+@dataclasses.dataclass
 class ModelWorkerBatch:
     """What the scheduler hands the worker (schedule_batch.py:1383-1443)."""
 
@@ -68,6 +78,7 @@ class ModelWorkerBatch:
     seq_lens_sum: int
     # decode
     decode_seq_lens: Optional[torch.Tensor] = None
+    shared_prefix: Optional[SharedPrefix] = None
     # extend
     extend_num_tokens: Optional[int] = None
     extend_seq_lens: Optional[List[int]] = None
@@ -110,6 +121,7 @@ class ForwardBatch:
     extend_logit_rows: Optional[torch.Tensor] = None
     positions: torch.Tensor = None
     decode_seq_lens_cpu: Optional[torch.Tensor] = None
+    shared_prefix: Optional[SharedPrefix] = None
 
     extend_num_tokens: Optional[int] = None
     extend_seq_lens: Optional[torch.Tensor] = None       # int32, device
@@ -155,6 +167,8 @@ class ForwardBatch:
                 ret.positions = ops.clamp_position(batch.seq_lens)
             if ret.decode_seq_lens_cpu is None:
                 ret.decode_seq_lens_cpu = batch.decode_seq_lens
+            if batch.shared_prefix is not None and model_runner.attn_backend.shares_prefix(ret.batch_size, batch.shared_prefix):
+                ret.shared_prefix = batch.shared_prefix
         else:
             # pinned staging so the copies are truly asynchronous
             ret.extend_seq_lens = torch.tensor(batch.extend_seq_lens, dtype=torch.int32,

@@ -20,6 +20,10 @@ that are the point of this build:
    `alloc_decode(seq_lens, last_loc)`), with the bookkeeping on the host so no call synchronises
    with the device.
 
+Requests may share runs: `fork_request` gives the continuations of one prompt its whole runs and a copy of the last, partial
+one; a run is free again when its last holder has let go of it.  `compact_request` lets a request go on with a subset of its
+tokens, in new runs.
+
 HBM layout: per layer, `k_buffer[l]` and `v_buffer[l]` are [size + 1, H_kv, D] 16-bit; all layers
 live in one allocation [2, L, size + 1, H_kv, D] so a 180 GB part is carved once.
 """
@@ -93,6 +97,30 @@ class KVCache(abc.ABC):
     def set_kv_buffer(self, layer, loc: torch.Tensor, cache_k: torch.Tensor,
                       cache_v: torch.Tensor) -> None: ...
 
+    def buffers(self) -> List[Optional[torch.Tensor]]:
+        """Every layer's buffers, one row per slot."""
+        layers = range(self.layer_num)
+        return [self.get_key_buffer(i) for i in layers] + [self.get_value_buffer(i) for i in layers]
+
+    @property
+    def planes(self) -> "ops.KVPlanes":
+        """The buffers as the operators that move rows take them."""
+        if getattr(self, "_planes", None) is None:
+            self._planes = ops.KVPlanes(self.buffers())
+        return self._planes
+
+    def copy_slots(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Rows of every layer from slots to other slots (int64; no slot in both lists)."""
+        ops.kv_copy(self.planes, src, dst)
+
+    def fork_rows(self, parent: int, children: Sequence[int], parent_run: Optional[int], runs: Sequence[int], stage) -> None:
+        """What a fork takes along beside its tokens' rows (`parent_run` and `runs`: the partial runs, None and empty where the
+        parent's tokens fill whole runs)."""
+
+    def compact_refusal(self) -> Optional[str]:
+        """Why requests of this pool cannot go on without some of their tokens (None: they can)."""
+        return None
+
 
 class _PinnedRing:
     """A few reusable pinned staging buffers for the slot-id uploads (a fresh pin_memory()
@@ -153,6 +181,8 @@ class TokenToKVPoolAllocator:
     def clear(self):
         self._free_runs = collections.deque(range(self.num_runs))
         self._used = np.zeros(self.num_runs, dtype=np.int32)
+        self._held = np.zeros(self.num_runs, dtype=np.int32)   # requests that hold the run
+        self._forked = False                                   # some run may have several holders
         self._req_runs: Dict[int, List[int]] = {}   # req_pool_idx -> runs in position order
         self._req_len: Dict[int, int] = {}          # req_pool_idx -> tokens placed
         self.is_not_in_free_group = True
@@ -198,7 +228,7 @@ class TokenToKVPoolAllocator:
                 self._req_runs[idx] = []
             runs = self._req_runs[idx]
             for _ in range(self.runs_needed(pre, seq)):
-                runs.append(self._free_runs.popleft())
+                runs.append(self._take_run())
             pos = np.arange(pre, seq, dtype=np.int64)
             bases = np.asarray(runs, dtype=np.int64) * R + 1
             parts.append(bases[pos // R] + pos % R)
@@ -224,7 +254,7 @@ class TokenToKVPoolAllocator:
             if s != self._req_len[idx]:
                 raise RuntimeError(f"request slot {idx}: length {s} does not match the {self._req_len[idx]} tokens placed")
             if s % R == 0:
-                runs.append(self._free_runs.popleft())
+                runs.append(self._take_run())
             run = runs[s // R]
             out[i] = run * R + 1 + s % R
             self._used[run] += 1
@@ -236,9 +266,87 @@ class TokenToKVPoolAllocator:
         runs = self._req_runs.pop(req_pool_idx, None)
         n = self._req_len.pop(req_pool_idx, 0)
         if runs:
-            self._used[runs] = 0
-            self._free_runs.extend(runs)
+            self._let_go(runs)
         return n
+
+    # ---- requests that share runs --------------------------------------------------------------
+    def _take_run(self) -> int:
+        run = self._free_runs.popleft()
+        self._held[run] = 1
+        return run
+
+    def _let_go(self, runs: List[int]) -> None:
+        """One holder less of each; a run that nobody holds is free."""
+        ids = np.asarray(runs, dtype=np.int64)
+        self._held[ids] -= 1
+        gone = ids[self._held[ids] == 0]
+        self._used[gone] = 0
+        self._free_runs.extend(int(r) for r in gone)
+
+    def req_len(self, req_pool_idx: int) -> int:
+        return self._req_len[req_pool_idx]
+
+    def fork_req(self, parent: int, children: Sequence[int]) -> Optional[np.ndarray]:
+        """`children` share the parent's whole runs and get a run of their own for the tokens behind those: → its first slot per
+        child (0 where there are no such tokens).  None when the free runs do not suffice — nothing is taken then."""
+        if parent not in self._req_runs:
+            raise RuntimeError(f"request slot {parent} holds no tokens")
+        if len(set(children)) != len(children) or any(c == parent or self._req_runs.get(c) for c in children):
+            raise RuntimeError("fork: children must be request slots of their own that hold no runs")
+        R, n, runs = self.run_len, self._req_len[parent], self._req_runs[parent]
+        whole, rest = runs[:n // R], n % R
+        if rest and len(children) > len(self._free_runs):
+            return None
+        out = np.zeros(len(children), dtype=np.int64)
+        for i, c in enumerate(children):
+            mine = list(whole)
+            if whole:
+                self._held[whole] += 1
+                self._forked = True
+            if rest:
+                mine.append(self._take_run())
+                self._used[mine[-1]] = rest
+                out[i] = self._base(mine[-1])
+            self._req_runs[c] = mine
+            self._req_len[c] = n
+        return out
+
+    def rebuild_req(self, req_pool_idx: int, n: int) -> Optional[Tuple[np.ndarray, List[int]]]:
+        """New runs for a request that goes on with n of its tokens: → (their slots, the runs it had, for release_runs once
+        the rows have been copied).  None when the free runs do not suffice."""
+        if not 0 < n <= self._req_len.get(req_pool_idx, 0):
+            raise RuntimeError(f"request slot {req_pool_idx}: cannot keep {n} of {self._req_len.get(req_pool_idx, 0)} tokens")
+        R = self.run_len
+        if -(-n // R) > len(self._free_runs):
+            return None
+        old = self._req_runs[req_pool_idx]
+        self._req_runs[req_pool_idx] = [self._take_run() for _ in range(-(-n // R))]
+        self._req_len[req_pool_idx] = n
+        slots = self.req_slots(req_pool_idx)
+        np.add.at(self._used, (slots - 1) // R, 1)
+        return slots, old
+
+    def release_runs(self, runs: List[int]) -> None:
+        self._let_go(runs)
+
+    def shared_prefix(self, req_pool_indices: Sequence[int]) -> Optional[Tuple[List[int], List[int]]]:
+        """Groups of neighbours in the list that begin with the same runs: → (row offsets, shared tokens per group), rows of no
+        group being groups of one that share nothing.  None when nothing is shared."""
+        if not self._forked or not req_pool_indices:
+            return None
+        self._forked = bool((self._held > 1).any())
+        indptr, lens = [], []
+        lead: List[int] = []    # the runs that the group's members have in common so far
+        for i, idx in enumerate(req_pool_indices):
+            runs = self._req_runs.get(idx, [])
+            same = next((k for k, (a, b) in enumerate(zip(lead, runs)) if a != b), min(len(lead), len(runs)))
+            if same > 0:
+                lead, lens[-1] = lead[:same], same * self.run_len
+            else:
+                indptr.append(i)
+                lens.append(0)
+                lead = runs
+        return (indptr + [len(req_pool_indices)], lens) if any(lens) else None
 
     def req_slots(self, req_pool_idx: int) -> np.ndarray:
         """Slot ids of a request's tokens in position order (host-side view; tests)."""
@@ -272,9 +380,12 @@ class TokenToKVPoolAllocator:
         ids = free_index.detach().to("cpu", torch.int64).numpy()
         ids = ids[ids > 0]
         runs, counts = np.unique((ids - 1) // self.run_len, return_counts=True)
+        if (self._held[runs] > 1).any():
+            raise RuntimeError("KV slots of a run that several requests hold: free the requests")
         self._used[runs] -= counts.astype(np.int32)
         if (self._used[runs] < 0).any():
             raise RuntimeError("KV slots freed twice")
+        self._held[runs[self._used[runs] == 0]] = 0
         self._free_runs.extend(int(r) for r in runs[self._used[runs] == 0])
 
     def free_group_begin(self):
@@ -364,6 +475,9 @@ class MLATokenToKVPool(KVCache):
     def get_kv_size_bytes(self):
         return self._slab.numel() * self._slab.element_size()
 
+    def buffers(self) -> List[Optional[torch.Tensor]]:
+        return list(self.kv_buffer)
+
     def get_key_buffer(self, layer_id: int):
         return self.kv_buffer[layer_id]
 
@@ -377,6 +491,59 @@ class MLATokenToKVPool(KVCache):
         if cache_k.dtype != self.dtype:
             raise RuntimeError("KV cache dtype conversion is not on the semi-PD path")
         ops.kv_write_single(cache_k, self.kv_buffer[layer.layer_id], loc)
+
+
+def fork_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator: TokenToKVPoolAllocator, parent: int,
+                 n: int) -> Optional[List[int]]:
+    """n continuations of a request: new request slots whose page-table rows share the parent's whole runs, its last, partial run
+    copied for each (and its recurrent state, where the model has one).  On the current stream.  → the request slots, or None
+    when slots or runs do not suffice."""
+    children = req_to_token_pool.alloc(n)
+    if children is None:
+        return None
+    try:
+        tails = allocator.fork_req(parent, children)
+    except RuntimeError:
+        req_to_token_pool.free(children)
+        raise
+    if tails is None:
+        req_to_token_pool.free(children)
+        return None
+    length, R = allocator.req_len(parent), allocator.run_len
+    if n == 0:
+        return children
+    lists = np.concatenate([np.full(n, parent), np.asarray(children), np.full(n, length), tails]).astype(np.int64)
+    parents_d, children_d, lens_d, tails_d = allocator._ring.stage(lists, allocator.device).split(n)
+    ops.kv_fork(kv_pool.planes, req_to_token_pool.req_to_token, parents_d, children_d, lens_d, tails_d, R)
+    rest = length % R > 0
+    kv_pool.fork_rows(parent, children, allocator._req_runs[parent][length // R] if rest else None,
+                      [allocator._req_runs[c][-1] for c in children] if rest else [],
+                      lambda rows: allocator._ring.stage(np.asarray(rows, dtype=np.int64), allocator.device))
+    return children
+
+
+def compact_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator: TokenToKVPoolAllocator, req: int,
+                    keep: Sequence[int]) -> bool:
+    """The request goes on with its tokens at the positions `keep` only (ascending, at least one), copied to new runs; keys
+    stay rotated as they are.  On the current stream; what the caller knows of its length is its own.  False when the free
+    runs do not suffice."""
+    why = kv_pool.compact_refusal()
+    if why:
+        raise NotImplementedError(f"compact: {why}")
+    pos = np.asarray(keep, dtype=np.int64)
+    length = allocator.req_len(req)
+    if pos.size == 0 or pos[0] < 0 or pos[-1] >= length or (np.diff(pos) <= 0).any():
+        raise RuntimeError(f"compact: positions must be ascending and below the request's {length} tokens, and at least one")
+    new = allocator.rebuild_req(req, int(pos.size))
+    if new is None:
+        return False
+    slots, old = new
+    n = int(pos.size)
+    lists = allocator._ring.stage(np.concatenate([pos, slots, [req, 0, n]]).astype(np.int64), allocator.device)
+    ops.kv_compact(kv_pool.planes, req_to_token_pool.req_to_token, lists[2 * n:2 * n + 1], None, lists[:n], lists[2 * n + 1:],
+                   lists[n:2 * n])
+    allocator.release_runs(old)  # later writers of these runs come behind the copy, in this stream or by its events
+    return True
 
 
 class RecurrentStatePool:
@@ -416,6 +583,18 @@ class RecurrentStatePool:
 
     def get_shift(self, layer_id: int) -> torch.Tensor:
         return self.shift[layer_id]
+
+    @property
+    def planes(self) -> Optional["ops.KVPlanes"]:
+        """Every layer's states as the operators that move rows take them, one row per request slot."""
+        if getattr(self, "_planes", None) is None:
+            rows = [t for t in self.state + self.shift if t is not None]
+            if self.prev_token is not None:
+                rows.append(self.prev_token.view(-1, 1))
+            if not rows:
+                return None
+            self._planes = ops.KVPlanes(rows)
+        return self._planes
 
 
 class HybridTokenToKVPool(KVCache):
@@ -500,6 +679,21 @@ class HybridTokenToKVPool(KVCache):
 
     def get_blocks(self, layer_id: int) -> Optional[Tuple[int, int, int]]:
         return self._blocks[layer_id]
+
+    def fork_rows(self, parent: int, children: Sequence[int], parent_run: Optional[int], runs: Sequence[int], stage) -> None:
+        """The pooled blocks of the partial run (a run's block rows lie behind the token rows), and the recurrent states."""
+        n = len(children)
+        if runs:
+            for (owner, size), at in {(self.owner[i], b[0]): b for i, b in enumerate(self._blocks) if b}.items():
+                per, base = -(-self.run_len // size), at[2]
+                rows = stage([base + parent_run * per + j for _ in runs for j in range(per)] +
+                             [base + r * per + j for r in runs for j in range(per)])
+                ops.kv_copy(ops.KVPlanes([self.k_buffer[owner], self.v_buffer[owner]]), *rows.split(n * per))
+        if self.state_pool is not None and self.state_pool.planes is not None:
+            ops.kv_copy(self.state_pool.planes, *stage([parent] * n + list(children)).split(n))
+
+    def compact_refusal(self) -> Optional[str]:
+        return "layers of this model hold more than their tokens' rows (states, pooled blocks, windows by position)"
 
     def writes_blocks(self, layer_id: int) -> bool:
         return self._writes_blocks[layer_id]

@@ -277,7 +277,8 @@ class CudaGraphRunner:
             self.capture()
 
     def can_run(self, forward_batch: ForwardBatch) -> bool:
-        return forward_batch.forward_mode.is_decode() and forward_batch.batch_size <= self.max_bs
+        return (forward_batch.forward_mode.is_decode() and forward_batch.batch_size <= self.max_bs
+                and forward_batch.shared_prefix is None)
 
     def capture(self):
         set_current_comm(self.model_runner.tp_comm)

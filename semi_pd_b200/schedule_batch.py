@@ -9,14 +9,15 @@ Sampling is greedy-only; logprobs / grammar / multimodal are off this path
 """
 from __future__ import annotations
 
+import copy
 import dataclasses
 from typing import List, Optional
 
 import torch
 
 from . import ops
-from .forward_batch_info import ForwardMode, ModelWorkerBatch
-from .memory_pool import ReqToTokenPool, TokenToKVPoolAllocator
+from .forward_batch_info import ForwardMode, ModelWorkerBatch, SharedPrefix
+from .memory_pool import ReqToTokenPool, TokenToKVPoolAllocator, fork_request
 
 _bid = 0
 
@@ -109,6 +110,7 @@ class ScheduleBatch:
         self.extend_lens = None
         self.extend_num_tokens = None
         self.decoding_reqs = None
+        self._shared = None   # (groups of the last step, SharedPrefix)
 
     @classmethod
     def init_new(cls, reqs, req_to_token_pool, token_to_kv_pool_allocator, device=None):
@@ -241,6 +243,44 @@ class ScheduleBatch:
         self.seq_lens_host = [s + 1 for s in self.seq_lens_host]
         self.seq_lens_sum += bs
 
+    def fork_req(self, index: int, n: int) -> Optional[List[Req]]:
+        """n more continuations of request `index` of a decode batch, between two steps: requests like it (prompt and output
+        so far) right behind it in the batch, so that neighbours share a prefix.  Their next input token is the parent's until
+        the caller writes another into `output_ids`.  None when request slots or cache do not suffice."""
+        parent = self.reqs[index]
+        slots = fork_request(self.token_to_kv_pool_allocator.get_kvcache(), self.req_to_token_pool,
+                             self.token_to_kv_pool_allocator, parent.req_pool_idx, n)
+        if slots is None:
+            return None
+        children = []
+        for k, slot in enumerate(slots):
+            req = copy.copy(parent)
+            req.rid = f"{parent.rid}.{k + 1}"
+            req.req_pool_idx = slot
+            for name in ("origin_input_ids", "output_ids", "fill_ids", "prefix_indices", "token_times", "prior_output_ids",
+                         "prior_token_times"):
+                setattr(req, name, list(getattr(parent, name)))
+            children.append(req)
+        rows = list(range(index + 1)) + [index] * n + list(range(index + 1, len(self.reqs)))
+        self.reqs = self.reqs[:index + 1] + children + self.reqs[index + 1:]
+        self.seq_lens_host = [self.seq_lens_host[i] for i in rows]
+        self.seq_lens_sum = sum(self.seq_lens_host)
+        self.req_pool_indices = self._h2d([r.req_pool_idx for r in self.reqs], torch.int64)
+        idx = self._h2d(rows, torch.int64)
+        self.seq_lens = self.seq_lens[idx]
+        if self.output_ids is not None:
+            self.output_ids = self.output_ids[idx]
+        return children
+
+    def _shared_prefix(self) -> Optional[SharedPrefix]:
+        groups = self.token_to_kv_pool_allocator.shared_prefix([r.req_pool_idx for r in self.reqs])
+        if groups is None:
+            return None
+        if self._shared is None or self._shared[0] != groups:  # lists of a few steps are the same
+            indptr, lens = groups
+            self._shared = (groups, SharedPrefix(self._h2d(indptr, torch.int32), self._h2d(lens, torch.int64), max(lens)))
+        return self._shared[1]
+
     def filter_batch(self, keep_indices: Optional[List[int]] = None):
         if keep_indices is None:
             keep_indices = [i for i, r in enumerate(self.reqs) if not r.finished()]
@@ -285,6 +325,7 @@ class ScheduleBatch:
             bid=_bid, forward_mode=self.forward_mode, input_ids=self.input_ids,
             req_pool_indices=self.req_pool_indices, seq_lens=self.seq_lens,
             out_cache_loc=self.out_cache_loc, seq_lens_sum=self.seq_lens_sum,
+            shared_prefix=None if extend else self._shared_prefix(),
             extend_num_tokens=self.extend_num_tokens if extend else None,
             extend_seq_lens=self.extend_lens if extend else None,
             extend_prefix_lens=self.prefix_lens if extend else None,
