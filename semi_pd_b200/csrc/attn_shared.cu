@@ -510,11 +510,11 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       // this thread
       auto issue_s = [&](int j, int h) {
         const uint32_t pos = 2 * (t_base + j);
-        wait_kv(pos);
+        if (h == 0) wait_kv(pos);
         tc_fence_after_sync();
         uint32_t qa = static_cast<uint32_t>(qd);
         uint32_t ka = static_cast<uint32_t>(kd0) + (pos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
-#pragma unroll 1
+#pragma unroll
         for (int k = 0; k < kSpD / 16; ++k) {
           umma_ss_if(leader, tmem_S + w * 128 + h * kSpU, qa, ka, qk_hi, idesc_qk, k);
           const uint32_t step = k == 3 ? (16384 - 96) / 16 : 2;
@@ -545,13 +545,13 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             q_ahead = true;
           }
           mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
-          wait_kv(vpos);
+          if (h == 0) wait_kv(vpos);
           if (i == 0 && h == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
           tc_fence_after_sync();
           uint32_t va = static_cast<uint32_t>(vd0) + (vpos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
           uint32_t pa = tmem_S + w * 128 + h * kSpU;
           uint32_t acc = (i > 0 || h > 0) ? 1u : 0u;
-#pragma unroll 1
+#pragma unroll
           for (int k = 0; k < kSpU / 16; ++k) {
             umma_ts_if(leader, tmem_O + w * kSpD, pa, va, v_hi, idesc_pv, acc);
             pa += 8;

@@ -28,18 +28,28 @@ struct KvPlanes {
   KvSet set[kKvSets];
 };
 
+// A block's place in its call: rows [chunk x rows of a block, ...), plane (the last one: the page table), child of a fork.
+// Children run fastest: those of one parent, which stand together in the lists, then find its rows in L2 (16 children each
+// of 8 parents, 568 MB at least: 165 us with the children slowest).
+struct KvPlace {
+  int64_t chunk;
+  int plane, child, chunks;
+};
 // where the rows of a call lie
 struct KvCopyRows {
+  static constexpr bool kChildren = false;
   const int64_t *src, *dst;
   int64_t n;
 };
 struct KvForkRows {
+  static constexpr bool kChildren = true;
   const int64_t *parents, *children, *lens, *tail;
   int32_t* table;
   int64_t stride, requests, width;
   int run_len;
 };
 struct KvCompactRows {
+  static constexpr bool kChildren = false;
   const int64_t *src, *dst, *keep, *indptr, *loc;
   int32_t* table;
   int64_t stride, requests, width, n, total;
@@ -56,8 +66,8 @@ __device__ __forceinline__ int64_t kv_request(const int64_t* indptr, int64_t n, 
 }
 
 // rows [first, first + count) of this block -> (source, destination) slots; a row with a slot of -1 stays as it is
-__device__ __forceinline__ int kv_rows(const KvCopyRows& r, int per_block, int64_t* src, int64_t* dst) {
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
+__device__ __forceinline__ int kv_rows(const KvCopyRows& r, const KvPlace& at, int per_block, int64_t* src, int64_t* dst) {
+  const int64_t first = at.chunk * per_block;
   const int count = static_cast<int>(min(static_cast<int64_t>(per_block), r.n - first));
   for (int i = threadIdx.x; i < count; i += kKvThreads) {
     src[i] = r.src[first + i];
@@ -65,10 +75,10 @@ __device__ __forceinline__ int kv_rows(const KvCopyRows& r, int per_block, int64
   }
   return count;
 }
-__device__ __forceinline__ int kv_rows(const KvForkRows& r, int per_block, int64_t* src, int64_t* dst) {
-  const int64_t parent = r.parents[blockIdx.z], len = r.lens[blockIdx.z], tail = r.tail[blockIdx.z];
+__device__ __forceinline__ int kv_rows(const KvForkRows& r, const KvPlace& at, int per_block, int64_t* src, int64_t* dst) {
+  const int64_t parent = r.parents[at.child], len = r.lens[at.child], tail = r.tail[at.child];
   if (parent < 0 || parent >= r.requests || len < 0 || len > r.width) return 0;
-  const int64_t full = len / r.run_len * r.run_len, first = static_cast<int64_t>(blockIdx.x) * per_block;
+  const int64_t full = len / r.run_len * r.run_len, first = at.chunk * per_block;
   const int count = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(per_block), len - full - first)));
   for (int i = threadIdx.x; i < count; i += kKvThreads) {
     src[i] = r.table[parent * r.stride + full + first + i];
@@ -76,8 +86,8 @@ __device__ __forceinline__ int kv_rows(const KvForkRows& r, int per_block, int64
   }
   return count;
 }
-__device__ __forceinline__ int kv_rows(const KvCompactRows& r, int per_block, int64_t* src, int64_t* dst) {
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
+__device__ __forceinline__ int kv_rows(const KvCompactRows& r, const KvPlace& at, int per_block, int64_t* src, int64_t* dst) {
+  const int64_t first = at.chunk * per_block;
   const int count = static_cast<int>(min(static_cast<int64_t>(per_block), r.total - first));
   for (int i = threadIdx.x; i < count; i += kKvThreads) {
     const int64_t j = first + i, request = r.src[kv_request(r.indptr, r.n, j)], pos = r.keep[j];
@@ -89,21 +99,20 @@ __device__ __forceinline__ int kv_rows(const KvCompactRows& r, int per_block, in
 }
 
 // the page table's part of a call
-__device__ __forceinline__ void kv_table(const KvCopyRows&) {}
-__device__ __forceinline__ void kv_table(const KvForkRows& r) {
-  const int64_t parent = r.parents[blockIdx.z], child = r.children[blockIdx.z], len = r.lens[blockIdx.z], tail = r.tail[blockIdx.z];
+__device__ __forceinline__ void kv_table(const KvCopyRows&, const KvPlace&) {}
+__device__ __forceinline__ void kv_table(const KvForkRows& r, const KvPlace& at) {
+  const int64_t parent = r.parents[at.child], child = r.children[at.child], len = r.lens[at.child], tail = r.tail[at.child];
   if (parent < 0 || parent >= r.requests || child < 0 || child >= r.requests || child == parent || len < 0 || len > r.width) return;
   const int64_t full = len / r.run_len * r.run_len;
   const int32_t* from = r.table + parent * r.stride;
   int32_t* to = r.table + child * r.stride;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kKvThreads + threadIdx.x; i < len; i += static_cast<int64_t>(gridDim.x) * kKvThreads)
+  for (int64_t i = at.chunk * kKvThreads + threadIdx.x; i < len; i += static_cast<int64_t>(at.chunks) * kKvThreads)
     to[i] = i < full ? from[i] : static_cast<int32_t>(tail + i - full);
 }
-__device__ __forceinline__ void kv_table(const KvCompactRows& r) {
-  for (int64_t j = static_cast<int64_t>(blockIdx.x) * kKvThreads + threadIdx.x; j < r.total;
-       j += static_cast<int64_t>(gridDim.x) * kKvThreads) {
-    const int64_t i = kv_request(r.indptr, r.n, j), at = j - r.indptr[i], request = r.dst[i];
-    if (request >= 0 && request < r.requests && at >= 0 && at < r.width) r.table[request * r.stride + at] = static_cast<int32_t>(r.loc[j]);
+__device__ __forceinline__ void kv_table(const KvCompactRows& r, const KvPlace& at) {
+  for (int64_t j = at.chunk * kKvThreads + threadIdx.x; j < r.total; j += static_cast<int64_t>(at.chunks) * kKvThreads) {
+    const int64_t i = kv_request(r.indptr, r.n, j), pos = j - r.indptr[i], request = r.dst[i];
+    if (request >= 0 && request < r.requests && pos >= 0 && pos < r.width) r.table[request * r.stride + pos] = static_cast<int32_t>(r.loc[j]);
   }
 }
 
@@ -113,17 +122,19 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
   __shared__ int64_t s_src[kKvRows], s_dst[kKvRows];
   griddep_launch_dependents();
   griddep_wait();
-  if (static_cast<int>(blockIdx.y) == pl.planes) {
-    kv_table(rows);
+  const KvPlace at = Rows::kChildren ? KvPlace{blockIdx.y, static_cast<int>(blockIdx.z), static_cast<int>(blockIdx.x), static_cast<int>(gridDim.y)}
+                                     : KvPlace{blockIdx.x, static_cast<int>(blockIdx.y), 0, static_cast<int>(gridDim.x)};
+  if (at.plane == pl.planes) {
+    kv_table(rows, at);
     return;
   }
-  const int count = kv_rows(rows, per_block, s_src, s_dst);
+  const int count = kv_rows(rows, at, per_block, s_src, s_dst);
   if (count <= 0) return;
   int si = 0;
-  while (si + 1 < pl.sets && static_cast<int>(blockIdx.y) >= pl.set[si + 1].first) ++si;
+  while (si + 1 < pl.sets && at.plane >= pl.set[si + 1].first) ++si;
   const KvSet& set = pl.set[si];
   const int pieces = static_cast<int>(set.row_bytes / sizeof(V));
-  char* plane = set.base + (static_cast<int>(blockIdx.y) - set.first) * set.stride;
+  char* plane = set.base + (at.plane - set.first) * set.stride;
   __syncthreads();
   const int total = count * pieces;
   for (int i0 = threadIdx.x; i0 < total; i0 += kKvThreads * kKvUnroll) {
@@ -134,11 +145,12 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
       const int i = i0 + k * kKvThreads;
       to[k] = nullptr;
       if (i < total) {
-        const int row = fastdiv(i, set.pieces_m, set.pieces_s), at = i - row * pieces;
+        const int row = fastdiv(i, set.pieces_m, set.pieces_s), piece = i - row * pieces;
         const int64_t s = s_src[row], d = s_dst[row];
         if (s >= 0 && s < set.rows && d >= 0 && d < set.rows) {
-          v[k] = __ldcs(reinterpret_cast<const V*>(plane + s * set.row_bytes) + at);
-          to[k] = reinterpret_cast<V*>(plane + d * set.row_bytes) + at;
+          const V* from = reinterpret_cast<const V*>(plane + s * set.row_bytes) + piece;
+          v[k] = Rows::kChildren ? *from : __ldcs(from);  // (a parent's rows are read again for its next child)
+          to[k] = reinterpret_cast<V*>(plane + d * set.row_bytes) + piece;
         }
       }
     }
@@ -152,7 +164,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
 __global__ void __launch_bounds__(kKvThreads) kv_table_kernel(const KvCompactRows rows) {
   griddep_launch_dependents();
   griddep_wait();
-  kv_table(rows);
+  kv_table(rows, KvPlace{blockIdx.x, 0, 0, static_cast<int>(gridDim.x)});
 }
 
 // The plane sets as the kernel takes them, and the bytes of a piece that suits all of them (0 and an error otherwise).
@@ -193,10 +205,10 @@ static int kv_rows_per_block(const KvPlanes& pl, int64_t rows) {
 }
 
 template <typename Rows>
-static int kv_move(const KvPlanes& pl, int piece, const Rows& rows, int64_t n, int per_block, int64_t z, bool table, cudaStream_t st) {
-  const int64_t x = (n + per_block - 1) / per_block;
-  SPD_REQUIRE(x < (1ll << 31) && z < 65536, SPD_E_SHAPE, "kv move: too many rows");
-  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(pl.planes + (table ? 1 : 0)), static_cast<unsigned>(z));
+static int kv_move(const KvPlanes& pl, int piece, const Rows& rows, int64_t n, int per_block, int64_t children, bool table, cudaStream_t st) {
+  const unsigned chunks = static_cast<unsigned>((n + per_block - 1) / per_block), planes = static_cast<unsigned>(pl.planes + (table ? 1 : 0));
+  const dim3 grid = Rows::kChildren ? dim3(static_cast<unsigned>(children), chunks, planes) : dim3(chunks, planes);
+  SPD_REQUIRE(!Rows::kChildren || chunks < 65536, SPD_E_SHAPE, "spd_kv_fork: runs of too many tokens");
 #define SPD_KV_MOVE(V) SPD_CUDA(launch(kv_move_kernel<V, Rows>, grid, dim3(kKvThreads), 0, st, pdl_enabled(), pl, rows, per_block))
   switch (piece) {
     case 16: SPD_KV_MOVE(uint4); break;
