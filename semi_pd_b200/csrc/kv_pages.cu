@@ -14,6 +14,11 @@ constexpr int kKvThreads = 256;
 constexpr int kKvRows = 64;    // rows of a block at most
 constexpr int kKvUnroll = 4;
 constexpr int kKvSets = 64;
+// Children of a fork whose rows a block stores after loading them once: those of one parent and length, which stand together
+// in the lists, up to a multiple of kKvKin.  They are the fastest index of the grid, so that the next block of the parent finds
+// its rows in L2.  us with 1 / 2 / 4: 8 parents of 16 children, 567 MB at least, 138 / 104 / 107; 64 parents of one child
+// 145 / 134 / 165; one child, 16 MB, 7.2 / 7.1 / 7.7.  With the children slowest and 1: 165 (8 parents of 16).
+constexpr int kKvKin = 2;
 
 struct KvSet {
   char* base;
@@ -29,8 +34,6 @@ struct KvPlanes {
 };
 
 // A block's place in its call: rows [chunk x rows of a block, ...), plane (the last one: the page table), child of a fork.
-// Children run fastest: those of one parent, which stand together in the lists, then find its rows in L2 (16 children each
-// of 8 parents, 568 MB at least: 165 us with the children slowest).
 struct KvPlace {
   int64_t chunk;
   int plane, child, chunks;
@@ -46,7 +49,7 @@ struct KvForkRows {
   const int64_t *parents, *children, *lens, *tail;
   int32_t* table;
   int64_t stride, requests, width;
-  int run_len;
+  int run_len, n;
 };
 struct KvCompactRows {
   static constexpr bool kChildren = false;
@@ -66,7 +69,7 @@ __device__ __forceinline__ int64_t kv_request(const int64_t* indptr, int64_t n, 
 }
 
 // rows [first, first + count) of this block -> (source, destination) slots; a row with a slot of -1 stays as it is
-__device__ __forceinline__ int kv_rows(const KvCopyRows& r, const KvPlace& at, int per_block, int64_t* src, int64_t* dst) {
+__device__ __forceinline__ int kv_rows(const KvCopyRows& r, const KvPlace& at, int, int per_block, int64_t* src, int64_t* dst) {
   const int64_t first = at.chunk * per_block;
   const int count = static_cast<int>(min(static_cast<int64_t>(per_block), r.n - first));
   for (int i = threadIdx.x; i < count; i += kKvThreads) {
@@ -75,18 +78,24 @@ __device__ __forceinline__ int kv_rows(const KvCopyRows& r, const KvPlace& at, i
   }
   return count;
 }
-__device__ __forceinline__ int kv_rows(const KvForkRows& r, const KvPlace& at, int per_block, int64_t* src, int64_t* dst) {
-  const int64_t parent = r.parents[at.child], len = r.lens[at.child], tail = r.tail[at.child];
+// (kin children of one parent and length from at.child on: dst[k x kKvRows + i])
+__device__ __forceinline__ int kv_rows(const KvForkRows& r, const KvPlace& at, int kin, int per_block, int64_t* src, int64_t* dst) {
+  const int64_t parent = r.parents[at.child], len = r.lens[at.child];
+  int64_t tail[kKvKin];  // (read before anything is stored: a store keeps the loads behind it waiting)
+#pragma unroll
+  for (int k = 0; k < kKvKin; ++k) tail[k] = at.child + k < r.n ? r.tail[at.child + k] : -1;
   if (parent < 0 || parent >= r.requests || len < 0 || len > r.width) return 0;
   const int64_t full = len / r.run_len * r.run_len, first = at.chunk * per_block;
   const int count = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(per_block), len - full - first)));
   for (int i = threadIdx.x; i < count; i += kKvThreads) {
     src[i] = r.table[parent * r.stride + full + first + i];
-    dst[i] = tail + first + i;
+#pragma unroll
+    for (int k = 0; k < kKvKin; ++k)
+      if (k < kin) dst[k * kKvRows + i] = tail[k] + first + i;
   }
   return count;
 }
-__device__ __forceinline__ int kv_rows(const KvCompactRows& r, const KvPlace& at, int per_block, int64_t* src, int64_t* dst) {
+__device__ __forceinline__ int kv_rows(const KvCompactRows& r, const KvPlace& at, int, int per_block, int64_t* src, int64_t* dst) {
   const int64_t first = at.chunk * per_block;
   const int count = static_cast<int>(min(static_cast<int64_t>(per_block), r.total - first));
   for (int i = threadIdx.x; i < count; i += kKvThreads) {
@@ -116,10 +125,37 @@ __device__ __forceinline__ void kv_table(const KvCompactRows& r, const KvPlace& 
   }
 }
 
+// How many children from this one on the block stores to: those of its parent and length up to a multiple of kKvKin; 0 where an
+// earlier child's block does it.
+__device__ __forceinline__ int kv_kin(const KvForkRows& r, int child) {
+  const int first = child / kKvKin * kKvKin;
+  int64_t parent[kKvKin], len[kKvKin];
+#pragma unroll
+  for (int k = 0; k < kKvKin; ++k) {
+    parent[k] = first + k < r.n ? r.parents[first + k] : -1;
+    len[k] = first + k < r.n ? r.lens[first + k] : -1;
+  }
+  int kin = 0;
+#pragma unroll
+  for (int k = 0; k < kKvKin; ++k) {
+    if (first + k >= r.n) break;
+    const bool new_run = k == 0 || parent[k] != parent[k - 1] || len[k] != len[k - 1];
+    if (first + k == child) {
+      if (!new_run) return 0;
+      kin = 1;
+    } else if (first + k > child) {
+      if (new_run) break;
+      ++kin;
+    }
+  }
+  return kin;
+}
+template <typename Rows> __device__ __forceinline__ int kv_kin(const Rows&, int) { return 1; }
+
 // V: the piece that a thread moves at a time, 16 bytes where rows and pointers allow it
 template <typename V, typename Rows>
 __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_constant__ KvPlanes pl, const Rows rows, int per_block) {
-  __shared__ int64_t s_src[kKvRows], s_dst[kKvRows];
+  __shared__ int64_t s_src[kKvRows], s_dst[(Rows::kChildren ? kKvKin : 1) * kKvRows];
   griddep_launch_dependents();
   griddep_wait();
   const KvPlace at = Rows::kChildren ? KvPlace{blockIdx.y, static_cast<int>(blockIdx.z), static_cast<int>(blockIdx.x), static_cast<int>(gridDim.y)}
@@ -128,7 +164,9 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
     kv_table(rows, at);
     return;
   }
-  const int count = kv_rows(rows, at, per_block, s_src, s_dst);
+  const int kin = kv_kin(rows, at.child);
+  if (kin == 0) return;
+  const int count = kv_rows(rows, at, kin, per_block, s_src, s_dst);
   if (count <= 0) return;
   int si = 0;
   while (si + 1 < pl.sets && at.plane >= pl.set[si + 1].first) ++si;
@@ -139,24 +177,30 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
   const int total = count * pieces;
   for (int i0 = threadIdx.x; i0 < total; i0 += kKvThreads * kKvUnroll) {
     V v[kKvUnroll];
-    V* to[kKvUnroll];
+    int row[kKvUnroll], piece[kKvUnroll];
 #pragma unroll
     for (int k = 0; k < kKvUnroll; ++k) {
       const int i = i0 + k * kKvThreads;
-      to[k] = nullptr;
+      row[k] = -1;
       if (i < total) {
-        const int row = fastdiv(i, set.pieces_m, set.pieces_s), piece = i - row * pieces;
-        const int64_t s = s_src[row], d = s_dst[row];
-        if (s >= 0 && s < set.rows && d >= 0 && d < set.rows) {
-          const V* from = reinterpret_cast<const V*>(plane + s * set.row_bytes) + piece;
-          v[k] = Rows::kChildren ? *from : __ldcs(from);  // (a parent's rows are read again for its next child)
-          to[k] = reinterpret_cast<V*>(plane + d * set.row_bytes) + piece;
+        const int r = fastdiv(i, set.pieces_m, set.pieces_s);
+        const int64_t s = s_src[r];
+        piece[k] = i - r * pieces;
+        if (s >= 0 && s < set.rows) {
+          row[k] = r;
+          const V* from = reinterpret_cast<const V*>(plane + s * set.row_bytes) + piece[k];
+          v[k] = Rows::kChildren ? *from : __ldcs(from);  // (a parent's rows are read again)
         }
       }
     }
+    for (int c = 0; c < kin; ++c) {
 #pragma unroll
-    for (int k = 0; k < kKvUnroll; ++k)
-      if (to[k]) *to[k] = v[k];
+      for (int k = 0; k < kKvUnroll; ++k) {
+        if (row[k] < 0) continue;
+        const int64_t d = s_dst[c * kKvRows + row[k]];
+        if (d >= 0 && d < set.rows) *(reinterpret_cast<V*>(plane + d * set.row_bytes) + piece[k]) = v[k];
+      }
+    }
   }
 }
 
@@ -246,7 +290,7 @@ int spd_kv_fork(const spd_kv_planes_t* sets, int num_sets, int32_t* req_to_token
               SPD_E_BADARG, "spd_kv_fork: bad arguments");
   SPD_REQUIRE(n < 65536, SPD_E_SHAPE, "spd_kv_fork: at most 65535 children (got %lld)", (long long)n);
   if (n == 0) return 0;
-  const KvForkRows rows{parents, children, seq_lens, tail_slots, req_to_token, req_to_token_stride, requests, max_tokens, run_len};
+  const KvForkRows rows{parents, children, seq_lens, tail_slots, req_to_token, req_to_token_stride, requests, max_tokens, run_len, static_cast<int>(n)};
   return kv_move(pl, piece, rows, run_len - 1 > 0 ? run_len - 1 : 1, kv_rows_per_block(pl, n * run_len / 2), n, true, as_stream(stream));
 }
 

@@ -133,6 +133,19 @@ def test_fork(kind, lens, kids, run):
     assert torch.equal(table, want_table)
 
 
+@pytest.mark.parametrize("order", [0, 1, 2])
+def test_fork_lengths_of_children_differ_and_parents_mix(order):
+    """Children that take less of their parent than the next one does, and lists in which parents do not stand together."""
+    from semi_pd_b200 import ops
+    bufs, table, rows = _fork_case([300, 200, 90], 5, 128, "mha")
+    rows = [(p, c, n - (7 * i) % 11 * (i % 3), base) for i, (p, c, n, base) in enumerate(rows)]
+    rows = [rows[i] for i in torch.randperm(len(rows), generator=torch.Generator().manual_seed(order))] if order else rows
+    want, want_table = _fork_want(bufs, table, rows, 128)
+    ops.kv_fork(ops.KVPlanes(bufs), table, *_lists(rows), 128)
+    _same(bufs, want)
+    assert torch.equal(table, want_table)
+
+
 def test_fork_leaves_bad_requests_alone():
     from semi_pd_b200 import ops
     bufs, table, rows = _fork_case([200], 1, 128, "mha")
