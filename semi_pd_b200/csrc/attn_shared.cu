@@ -16,7 +16,7 @@
 // ("parts"): by batch row where the CTA has the item's first tile, else in a place of the CTA's own, since of all its items
 // only the first can have begun earlier.  A second kernel joins them.
 // (As two kernels, the shared keys' and attn_decode.cu's for the own ones: 64 requests of 130 own tokens behind 8192 shared
-// ones, 32 / 8 heads, 48.6 us; each of them starts for 5 us without using the memory.)
+// ones, 32 / 8 heads, 48.6 us, and 37.6 so; each kernel starts for 5 us without using the memory.)
 //
 //   warps 0-3 / 4-7  softmax of query tile 0 / 1: one thread per query row; P goes back into the TMEM columns of its S
 //   warp 8, warp 9   K / V loader: a ring of four 128 x 128 tiles, K_j V_j K_{j+1} ..., by TMA (single rows where a
@@ -25,9 +25,10 @@
 // Over shared keys a tile is taken in two halves of 64 keys, so that a warpgroup's softmax of one half runs beside the MMAs of
 // the other.  An item over own keys has the few query heads of one kv head as its rows; it is computed the other way round,
 // S^T = K Q^T and O^T = V^T P^T, with a thread per key and P^T in shared memory, as in attn_decode.cu.  (With queries in the
-// rows there too, one warp did all the exponentials: 160 requests of 132 own tokens, 32 / 32 heads, 276 us.)  The items go to
-// the two warpgroups in turn, and each has a loader, an issuer and a ring of three tiles to itself (its half of the ring above and
-// the memory of its query tile): with one ring for both, an item waited for the one before in every role (229 us).
+// rows there too, one warp did all the exponentials: 160 requests of 132 own tokens, 32 / 32 heads, 276 us, and 102 now.)
+// The items go to the two warpgroups in turn, and each has a loader, an issuer and a ring of three tiles to itself (its half of
+// the ring above and the memory of its query tile): with one ring for both, an item waited for the one before in every role
+// (229 us).
 // Sums, maxima and outputs are fp32 up to the join; P is rounded to the type of the keys, as the tensor cores take it, and l
 // sums the rounded P, so that the rounding of a P that outweighs the others cancels.  The reference maximum is raised when a
 // score passes it by 2^8 (O is then rescaled in TMEM), so a P is at most 2^8.
@@ -1045,22 +1046,24 @@ static int64_t part_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
 }
 
 // Whether reading the shared keys once is the faster way, from what the host knows: as if all requests were in groups of one
-// size that share max_shared keys.  In us: a tile of 128 shared keys takes an SM 1.5 here and each member 0.88 there (mostly
-// from L2); requests that there are cut over many SMs cost 0.16 per part and query head in their merge; the longer start, the
-// join and the shorter ranges cost 6 here, and 0.0075 per request and kv head.
-// us by request / shared, own tokens 64, bf16.  32 / 8 heads, one group: 64 members of 256 tokens 18.8 / 25.8, 512: 23.8 / 24.1,
-// 1024: 33.6 / 24.2; 8 of 1024: 14.3 / 17.7, 4096: 25.0 / 24.6, 16384: 59.6 / 35.7; 4 of 4096: 21.7 / 24.1.  Groups of two: 8
-// of 4096: 45.9 / 50.7, of 16384: 160 / 112; 32 of 2048: 61.5 / 83.5, of 4096: 158 / 126.  16 / 2 heads, 2 of 1024: 17.8 / 16.7,
-// of 4096: 44.2 / 21.5.  32 / 32 heads, 16 of 256: 17.7 / 19.3, of 1024: 32.2 / 24.2.
+// size that share max_shared keys.  The weights fit 330 shapes measured both ways (2 to 256 requests in 1 to 32 groups, 128 to
+// 16384 shared tokens, 64 own, bf16, four head layouts): the choice takes 0.5% longer than the better way on average, 18% at
+// worst.  A tile of 128 shared keys costs an SM 1 here and each member 0.57 there (mostly from L2); requests that there are cut
+// over many SMs cost 0.2 per part and query head in their merge; the longer start, the join and the shorter ranges cost 6 here,
+// and 0.002 per request and kv head.
+// us by request / shared.  32 / 8 heads, one group: 64 members of 256 tokens 19.1 / 25.9, 512: 24.3 / 23.9, 1024: 34.0 / 24.2,
+// 16384: 354 / 49.3; 8 of 1024: 14.3 / 17.4, 4096: 25.4 / 24.1, 16384: 58.2 / 36.4; 4 of 4096: 22.0 / 23.9.  Groups of two: 8
+// of 4096: 45.9 / 48.6, of 16384: 162 / 109; 32 of 2048: 60.8 / 80.8, of 4096: 161 / 122.  16 / 2 heads, 2 of 512: 18.1 / 19.9,
+// of 4096: 49.7 / 23.9.  32 / 32 heads, 16 of 256: 17.9 / 19.5, of 1024: 32.6 / 23.8.
 static bool shared_pays(int64_t batch, int64_t groups, int64_t max_shared, int num_q_heads, int num_kv_heads, int sms) {
   const double pairs = static_cast<double>(batch) * num_kv_heads, shared = static_cast<double>(max_shared);
   const double tiles = static_cast<double>(groups) * num_kv_heads * (shared / kSpTile) / sms;  // of an SM
-  double gain = tiles * (0.88 * batch / groups - 1.5);
+  double gain = tiles * (0.57 * batch / groups - 1.0);
   if (pairs < sms) {
     const double parts = sms / pairs < shared / 256 ? sms / pairs : shared / 256;
-    gain += 0.16 * (num_q_heads / num_kv_heads) * parts;
+    gain += 0.2 * (num_q_heads / num_kv_heads) * parts;
   }
-  return gain > 6.0 + 0.0075 * pairs * 148 / sms;
+  return gain > 6.0 + 0.002 * pairs * 148 / sms;
 }
 
 }  // namespace spd
@@ -1103,9 +1106,11 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
               (long long)workspace_bytes);
   const int device_sms = device_sm_count_cached();
   const int sms = sm_budget > 0 && sm_budget < device_sms ? sm_budget : device_sms;
-  // Every request reads its own pages where nothing can be shared or it does not pay, where a plan would not hold the batch, and
-  // where the scale is not positive (the maximum of raw scores serves the scaled ones only there).
-  if (!(sm_scale > 0.f) ||
+  // What the list can cost at most: no request has more tokens than its row of the page table has entries.
+  const int64_t most = batch * num_kv_heads * (kCostOwnTile * (req_to_token_stride / kSpTile + 1) + kCostShared + kCostOwn);
+  // Every request reads its own pages where nothing can be shared or it does not pay, where a plan would not hold the batch or
+  // its 32-bit costs the list, and where the scale is not positive (the maximum of raw scores serves the scaled ones only there).
+  if (!(sm_scale > 0.f) || most > INT_MAX / 2 ||
       !spd_attn_decode_shared_pays(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, sm_budget))
     return spd_attn_decode_paged_own(out, q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, batch, num_q_heads,
                                      num_kv_heads, head_dim, q_stride, out_stride, req_to_token_stride, sm_scale, dtype, workspace,
