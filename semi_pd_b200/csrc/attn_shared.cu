@@ -64,8 +64,9 @@ static_assert(kSpStage == 2 * 4 * kSpSmall, "one memory for both");
 constexpr int kSpBars = 256;
 constexpr int kSpRed = 2 * 2 * kSpMaxGroup * 4 * 4;  // per warpgroup, twice: the maxima or sums of 4 warps for every head
 constexpr float kSpRescale = 8.f;  // exponent of 2 that a score may pass the reference maximum by
-// What the list's entries cost, in 700 clk: a key tile for two query tiles, for one, over own keys; an item's start and end.
-constexpr int kCostPair = 6, kCostOne = 4, kCostOwnTile = 4, kCostShared = 8, kCostOwn = 1;
+// What the list's entries cost, in about 570 clk: a key tile for two query tiles, for one, over own keys (a tile of few keys is
+// bound by the chain of its steps, not by its bytes); an item's start and end.
+constexpr int kCostPair = 7, kCostOne = 4, kCostOwnTile = 4, kCostOwnLeast = 3, kCostShared = 24, kCostOwn = 1;
 constexpr int kCostMin = 8;  // of a CTA
 
 struct SharedParams {
@@ -102,9 +103,10 @@ __device__ __forceinline__ int sp_pairs(int count, int mpt) { return count <= mp
 // cost of a key tile in an item over shared keys
 __device__ __forceinline__ int sp_cost(int count, int mpt) { return count <= mpt ? kCostOne : kCostPair; }
 __device__ __forceinline__ int sp_tiles(int len) { return (len + kSpTile - 1) / kSpTile; }
-// of an item over own keys: its last tile costs what its keys do
+// of an item over own keys
 __device__ __forceinline__ int sp_own_cost(int len) {
-  return len > 0 ? kCostOwn + kCostOwnTile * ((len - 1) / kSpTile) + ((len - 1) % kSpTile) * kCostOwnTile / kSpTile + 1 : 0;
+  return len > 0 ? kCostOwn + kCostOwnTile * ((len - 1) / kSpTile) + max(kCostOwnLeast, ((len - 1) % kSpTile) * kCostOwnTile / kSpTile + 1)
+                 : 0;
 }
 
 struct SpRange {
@@ -357,6 +359,11 @@ __device__ __forceinline__ float2 sp_unpack(uint32_t w) {
   if constexpr (umma_fmt<T>::v == 1) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   return unpack2<T>(w);
 }
+__device__ __forceinline__ float fmax3(float a, float b, float c) {  // NaN where all are
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // One row's 64 scores of a unit: p = exp2(s * scale - m_off), rounded and packed into pk; the sum of the rounded p.
 template <typename T>
 __device__ __forceinline__ float sp_softmax_unit(const uint32_t* ra, const uint32_t* rb, uint32_t* pk, float scale, float m_off) {
@@ -368,14 +375,16 @@ __device__ __forceinline__ float sp_softmax_unit(const uint32_t* ra, const uint3
     unpack_f32x2(ffma2(pack_f32x2(__uint_as_float(r[0]), __uint_as_float(r[1])), scale2, neg_m2), x0, x1);
     pk[i >> 1] = pack2<T>(fast_exp2(x0), fast_exp2(x1));
   }
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  uint64_t sum[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const float2 f = sp_unpack<T>(pk[i]);
-    sum[i % 2 * 2] += f.x;
-    sum[i % 2 * 2 + 1] += f.y;
+    sum[i & 1] = fadd2(sum[i & 1], pack_f32x2(f.x, f.y));
   }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  float a, b, c, d;
+  unpack_f32x2(sum[0], a, b);
+  unpack_f32x2(sum[1], c, d);
+  return (a + b) + (c + d);
 }
 // largest value of the warp (not NaN, unless all are)
 __device__ __forceinline__ float sp_warp_max(float v) {
@@ -383,12 +392,13 @@ __device__ __forceinline__ float sp_warp_max(float v) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+struct SpBoxes {
+  CUtensorMap rows[5];  // of the keys or values: boxes of 128, 64, 32, 16 rows and one row, by 64 columns
+};
 template <typename T>
 __global__ void __launch_bounds__(kSpThreads, 1)
 attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQ1,
-                   const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const __grid_constant__ CUtensorMap tmK16, const __grid_constant__ CUtensorMap tmV16,
-                   const __grid_constant__ CUtensorMap tmK1, const __grid_constant__ CUtensorMap tmV1,
+                   const __grid_constant__ SpBoxes tmK, const __grid_constant__ SpBoxes tmV,
                    const __grid_constant__ SharedParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -420,7 +430,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 1);
       for (int i = 0; i < kSpSlots + 2; ++i) {
-        mbar_init(&kv_full[i], 32);
+        mbar_init(&kv_full[i], 1);
         mbar_init(&kv_empty[i], 2);
       }
       for (int i = 0; i < 4; ++i) {
@@ -442,8 +452,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   if (warp == 11 && lane == 0) {
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmQ1);
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmK.rows[0]);
+    tma_prefetch_desc(&tmV.rows[0]);
   }
   griddep_launch_dependents();
   griddep_wait();
@@ -655,40 +665,48 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i] = lane * 4 + i < left ? rtt[lane * 4 + i] : -1;
     };
-    // A tile into the memory at `tile`; its barrier gets 32 arrivals beside the bytes.  Consecutive slots: one box, or where
-    // only 16 of them are, or a tile ends early, boxes of 16 rows; others: four rows an instruction.  (Scattered rows by 16-byte
-    // cp.async took a warp 4500 clk a tile.)  What stands behind an item's last key in a box belongs to others, or lies past
-    // the pool and reads as zeros: the scores of such K rows are not looked at, such V rows are cleared before the MMA.
-    auto load = [&](int is_v, int bar, int tile, int hk, const int* slot, int valid) {
+    // A tile into the memory at `tile`; its barrier gets one arrival beside the bytes.  Consecutive slots: as few boxes as make
+    // up its rows, in steps of 16; else boxes of 16 rows where those are consecutive; others four rows an instruction.
+    // (Scattered rows by 16-byte cp.async took a warp 4500 clk a tile.  A TMA instruction takes it about 100: with boxes of 16
+    // rows wherever a tile was not full, and an arrival of every lane, 160 requests of 132 own tokens, 32 / 32 heads, took
+    // 93 us.)  What stands behind an item's last key in a box belongs to others, or lies past the pool and reads as zeros: the
+    // scores of such K rows are not looked at, such V rows are cleared before the MMA.
+    auto load = [&](const SpBoxes& tm, int bar, int tile, int hk, const int* slot, int valid) {
       uint8_t* dst = smem + tile * kSpTileBytes;
       const int base = __shfl_sync(0xffffffffu, slot[0], 0), base16 = __shfl_sync(0xffffffffu, slot[0], lane & ~3);
-      bool all = base >= 0, some = base16 >= 0;
+      bool all = true, some = true;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        all &= slot[i] == base + lane * 4 + i;
-        some &= lane * 4 + i >= valid || slot[i] == base16 + (lane & 3) * 4 + i;
+        const bool behind = lane * 4 + i >= valid;
+        all &= behind || slot[i] == base + lane * 4 + i;
+        some &= behind || slot[i] == base16 + (lane & 3) * 4 + i;
       }
       all = __all_sync(0xffffffffu, all);
-      some = (__ballot_sync(0xffffffffu, some) >> (lane & ~3) & 15) == 15;
-      const int pieces = (valid + 15) / 16, col = hk * kSpD;
-      if (lane == 0) mbar_expect_tx_noarrive(&kv_full[bar], pieces * 16 * 256);
+      const int pieces = (valid + 15) / 16, col = hk * kSpD;  // of 16 rows
+      if (lane == 0) mbar_expect_tx(&kv_full[bar], pieces * 16 * 256);
       __syncwarp();
       if (all) {
-        if (lane < 2) tma_load_2d(dst + lane * 16384, is_v ? &tmV : &tmK, &kv_full[bar], col + lane * 64, base, kEvictNormal);
-      } else if (lane >> 2 < pieces) {
-        if (some) {
-          if ((lane & 3) < 2)
-            tma_load_2d(dst + (lane & 1) * 16384 + (lane >> 2) * 2048, is_v ? &tmV16 : &tmK16, &kv_full[bar], col + (lane & 1) * 64,
-                        base16, kEvictNormal);
-        } else {
+        // lanes 2 b and 2 b + 1: the box of 128 >> b rows, if it is one of those that make up the pieces, behind the larger ones
+        const int half = lane & 1, b = lane >> 1, size = 8 >> b;
+        if (b < 4 && (pieces & size)) {
+          const int row = (pieces & ~(2 * size - 1)) * 16;
+          tma_load_2d(dst + half * 16384 + row * 128, &tm.rows[b], &kv_full[bar], col + half * 64, base + row, kEvictNormal);
+        }
+      } else {
+        some = (__ballot_sync(0xffffffffu, some) >> (lane & ~3) & 15) == 15;
+        if (lane >> 2 < pieces) {
+          if (some) {
+            if ((lane & 3) < 2)
+              tma_load_2d(dst + (lane & 1) * 16384 + (lane >> 2) * 2048, &tm.rows[3], &kv_full[bar], col + (lane & 1) * 64, base16,
+                          kEvictNormal);
+          } else {
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-            tma_gather4_2d(smem_u32(dst + half * 16384 + lane * 512), is_v ? &tmV1 : &tmK1, &kv_full[bar], col + half * 64, slot[0],
-                           slot[1], slot[2], slot[3], kEvictNormal);
+            for (int half = 0; half < 2; ++half)
+              tma_gather4_2d(smem_u32(dst + half * 16384 + lane * 512), &tm.rows[4], &kv_full[bar], col + half * 64, slot[0], slot[1],
+                             slot[2], slot[3], kEvictNormal);
+          }
         }
       }
-      __syncwarp();
-      mbar_arrive(&kv_full[bar]);
     };
     // ---- shared keys: K by warp 8, V by warp 9; lookups run one tile ahead of the copies ----
     int slot[4], next[4];
@@ -704,7 +722,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (have) lookup(entry(0) + j * kSpTile, kSpTile, next);
       const uint32_t pos = 2 * t_base + lw;
       mbar_wait_bounded(&kv_empty[pos % kSpSlots], ((pos / kSpSlots) & 1) ^ 1, dead);
-      load(lw, pos % kSpSlots, 2 + pos % kSpSlots, hk, slot, kSpTile);
+      load(lw ? tmV : tmK, pos % kSpSlots, 2 + pos % kSpSlots, hk, slot, kSpTile);
 #pragma unroll
       for (int i = 0; i < 4; ++i) slot[i] = next[i];
     }
@@ -738,7 +756,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           __syncwarp();
           q_buf ^= 1;
         }
-        load(is_v, at.bar, at.tile, hk, slot, valid);
+        load(is_v ? tmV : tmK, at.bar, at.tile, hk, slot, valid);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) slot[i] = next[i];
@@ -774,7 +792,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           if (active) {
             tc_fence_after_sync();
             uint32_t ra[32], rb[32], pk[32];
-            const float mx = softmax_load_max<false, false>(ts + h * kSpU, ra, rb, 0, 0, 0);
+            tmem_ld_32x32b_x32(ts + h * kSpU, ra);
+            tmem_ld_32x32b_x32(ts + h * kSpU + 32, rb);
+            tmem_ld_wait();
+            float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              m0 = fmax3(m0, __uint_as_float(ra[i]), __uint_as_float(ra[i + 1]));
+              m1 = fmax3(m1, __uint_as_float(rb[i]), __uint_as_float(rb[i + 1]));
+            }
+            const float mx = fmaxf(m0, m1);
             // The exponentials do not wait for the unit's maximum; where it turns out too large (rarely) they are redone
             const bool raise = __any_sync(0xffffffffu, mx > m + ahead && row < rows);
             float alpha = 1.f;
@@ -1137,19 +1164,19 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
   p.ml_next = p.ml_first + 3 * rows * 2;
   p.notes = reinterpret_cast<int2*>(p.ml_next + static_cast<int64_t>(sms) * 2 * kSpM * 2);
   // q as [batch][heads][128]: a box of mpt members and a kv head's query heads is a tile of mpt x group rows
-  CUtensorMap tq, tq1, tk, tv, tk16, tv16, tk1, tv1;
+  CUtensorMap tq, tq1;
+  SpBoxes tk, tv;
   const uint64_t dims[3] = {kSpD, static_cast<uint64_t>(num_q_heads), static_cast<uint64_t>(batch)};
   const uint64_t strides[2] = {kSpD, static_cast<uint64_t>(q_stride)};
   const uint32_t box[3] = {64, static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.mpt)}, box1[3] = {64, box[1], 1};
   if (int rc = make_tmap_sw128(&tq, q, 3, dims, strides, box)) return rc;
   if (int rc = make_tmap_sw128(&tq1, q, 3, dims, strides, box1)) return rc;
   const uint64_t row_elems = static_cast<uint64_t>(num_kv_heads) * kSpD, slots = static_cast<uint64_t>(pool_slots);
-  if (int rc = get_tmap(&tk, k_pool, slots, row_elems, row_elems, kSpTile)) return rc;
-  if (int rc = get_tmap(&tv, v_pool, slots, row_elems, row_elems, kSpTile)) return rc;
-  if (int rc = get_tmap(&tk16, k_pool, slots, row_elems, row_elems, 16)) return rc;
-  if (int rc = get_tmap(&tv16, v_pool, slots, row_elems, row_elems, 16)) return rc;
-  if (int rc = get_tmap(&tk1, k_pool, slots, row_elems, row_elems, 1)) return rc;
-  if (int rc = get_tmap(&tv1, v_pool, slots, row_elems, row_elems, 1)) return rc;
+  constexpr int kBoxes[5] = {128, 64, 32, 16, 1};
+  for (int i = 0; i < 5; ++i) {
+    if (int rc = get_tmap(&tk.rows[i], k_pool, slots, row_elems, row_elems, kBoxes[i])) return rc;
+    if (int rc = get_tmap(&tv.rows[i], v_pool, slots, row_elems, row_elems, kBoxes[i])) return rc;
+  }
   SPD_DISPATCH_DTYPE(dtype, {
     auto kern = attn_shared_kernel<T>;
     static bool configured = false;
@@ -1157,7 +1184,7 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
       SPD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpSmem));
       configured = true;
     }
-    SPD_CUDA(launch(kern, dim3(sms), dim3(kSpThreads), kSpSmem, as_stream(stream), pdl_enabled(), tq, tq1, tk, tv, tk16, tv16, tk1, tv1, p));
+    SPD_CUDA(launch(kern, dim3(sms), dim3(kSpThreads), kSpSmem, as_stream(stream), pdl_enabled(), tq, tq1, tk, tv, p));
     SPD_CUDA(launch(attn_shared_join_kernel<T>, dim3(static_cast<unsigned>((rows + kSjWarps - 1) / kSjWarps)), dim3(kSjWarps * 32), 0,
                     as_stream(stream), pdl_enabled(), static_cast<T*>(out), out_stride, p, static_cast<int>(rows)));
   });
