@@ -16,7 +16,7 @@
 // ("parts"): by batch row where the CTA has the item's first tile, else in a place of the CTA's own, since of all its items
 // only the first can have begun earlier.  A second kernel joins them.
 // (As two kernels, the shared keys' and attn_decode.cu's for the own ones: 64 requests of 130 own tokens behind 8192 shared
-// ones, 32 / 8 heads, 48.6 us, and 37.6 so; each kernel starts for 5 us without using the memory.)
+// ones, 32 / 8 heads, 48.6 us, and 34.0 so; each kernel starts for 5 us without using the memory.)
 //
 //   warps 0-3 / 4-7  softmax of query tile 0 / 1: one thread per query row; P goes back into the TMEM columns of its S
 //   warp 8, warp 9   K / V loader: a ring of four 128 x 128 tiles, K_j V_j K_{j+1} ..., by TMA (single rows where a
@@ -25,7 +25,7 @@
 // Over shared keys a tile is taken in two halves of 64 keys, so that a warpgroup's softmax of one half runs beside the MMAs of
 // the other.  An item over own keys has the few query heads of one kv head as its rows; it is computed the other way round,
 // S^T = K Q^T and O^T = V^T P^T, with a thread per key and P^T in shared memory, as in attn_decode.cu.  (With queries in the
-// rows there too, one warp did all the exponentials: 160 requests of 132 own tokens, 32 / 32 heads, 276 us, and 102 now.)
+// rows there too, one warp did all the exponentials: 160 requests of 132 own tokens, 32 / 32 heads, 276 us, and 86 now.)
 // The items go to the two warpgroups in turn, and each has a loader, an issuer and a ring of three tiles to itself (its half of
 // the ring above and the memory of its query tile): with one ring for both, an item waited for the one before in every role
 // (229 us).
@@ -33,6 +33,10 @@
 // sums the rounded P, so that the rounding of a P that outweighs the others cancels.  The reference maximum is raised when a
 // score passes it by 2^8 (O is then rescaled in TMEM), so a P is at most 2^8.
 // Every mbarrier wait is bounded (see mbar_wait_bounded, spd_wait_status).
+// The roles run side by side, so their code together competes for the instruction cache: long waits are out of the way, and
+// loops are not unrolled where that gains nothing.  (With the waits unrolled in place the kernel had 217 KB; 48 requests of 134
+// own tokens in 8 groups took 46.3 us, with 126 KB 38.9; 256 query rows by 32768 keys 369 and 337.  The MMAs over own keys
+// unrolled: 352.)
 #include <cuda.h>
 #include <limits.h>
 
@@ -263,10 +267,10 @@ struct SpItem {
     step = split() ? 2 : 1;
     count = (n - first + step - 1) / step;
   }
-  // for the join, see SharedParams
-  __device__ __forceinline__ int2 note(int per, bool halves, int row) const {
-    const int c0 = s0 / per;
-    return make_int2(c0, ((s0 + (tiles - 1) * cost) / per - c0 + 1) | (halves ? 1 << 15 : 0) | row << 16);
+  // for the join, see SharedParams; by the CTA that has the item's first tile
+  __device__ __forceinline__ int2 note(const SpRange& r, bool halves, int row) const {
+    const int c0 = blockIdx.x, last = s0 + (tiles - 1) * cost;
+    return make_int2(c0, (last < r.end ? 1 : last / r.per - c0 + 1) | (halves ? 1 << 15 : 0) | row << 16);
   }
 };
 
@@ -304,12 +308,14 @@ struct SpWalk {
   }
 };
 
-// This CTA's items over own keys: every second one, warpgroup w's.
+// This CTA's items over own keys: every second one, warpgroup w's.  A step is on the way of every role of the CTA, so what the
+// heads of a request share is looked up once for all of them.
 struct SpOwnWalk {
   int u, end, row, head, turn;
+  int keys, tiles, cost;  // of the row's items
   int64_t req, req_next;  // page-table row of the row here and of the one behind it, read ahead
   __device__ __forceinline__ SpOwnWalk(const SharedParams& p, const SharedPlan& pl, const SpRange& r, int w)
-      : u(0), end(0), row(0), head(0), turn(w), req(0), req_next(0) {
+      : u(0), end(0), row(0), head(0), turn(w), keys(0), tiles(0), cost(0), req(0), req_next(0) {
     if (r.own()) {
       row = pl.own_row;
       head = pl.own_head;
@@ -317,34 +323,57 @@ struct SpOwnWalk {
       end = r.end;
       req = pl.own_req;
       req_next = row + 1 < p.batch ? p.req_pool_indices[row + 1] : 0;
+      enter(pl);
     }
+  }
+  __device__ __forceinline__ void enter(const SharedPlan& pl) {
+    keys = pl.len[row];
+    tiles = sp_tiles(keys);
+    cost = sp_own_cost(keys);
   }
   __device__ __forceinline__ bool next(const SharedParams& p, const SharedPlan& pl, const SpRange& r, SpItem& it) {
     while (u < end) {
-      it.keys = pl.len[row];
-      it.hk = head;
-      it.b0 = row;
-      it.req = static_cast<int>(req);
-      bool some = false;
-      if (it.keys > 0) {
-        it.tiles = sp_tiles(it.keys);
-        it.s0 = u + kCostOwn;
-        it.cost = kCostOwnTile;
-        some = it.cut(max(u, r.begin), end);
-        u += sp_own_cost(it.keys);
-      }
-      if (++head == p.Hk || it.keys <= 0) {
+      while (keys <= 0 || head == p.Hk) {  // (the list goes on, so there is a row with keys)
         head = 0;
         ++row;
         req = req_next;
         req_next = row + 1 < p.batch ? p.req_pool_indices[row + 1] : 0;
+        enter(pl);
       }
-      if (some && (turn++ & 1) == 0) return true;
+      const int s0 = u + kCostOwn, begin = max(r.begin, r.shared);
+      const int tile0 = s0 >= begin ? 0 : min(tiles, (begin - s0 + kCostOwnTile - 1) / kCostOwnTile);
+      const int n = (end - s0 >= tiles * kCostOwnTile ? tiles : min(tiles, max(0, (end - s0 + kCostOwnTile - 1) / kCostOwnTile))) - tile0;
+      u += cost;
+      const int hk = head++;
+      if (n > 0 && (turn++ & 1) == 0) {
+        it.b0 = row;
+        it.hk = hk;
+        it.req = static_cast<int>(req);
+        it.keys = keys;
+        it.s0 = s0;
+        it.tiles = tiles;
+        it.cost = kCostOwnTile;
+        it.tile0 = tile0;
+        it.n = n;
+        return true;
+      }
     }
     return false;
   }
 };
 
+// mbar_wait_bounded, out of the way but for the first try
+__device__ __noinline__ void sp_wait_long(uint64_t* bar, uint32_t parity, volatile int* dead) {
+#pragma unroll 1
+  for (int i = 0; i < kMbarWaitTries; ++i) {
+    if (mbar_try_wait(bar, parity)) return;
+    if (*dead) return;
+  }
+  *dead = 1;
+}
+__device__ __forceinline__ void sp_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  if (!mbar_try_wait(bar, parity)) sp_wait_long(bar, parity, dead);
+}
 // of an element of P^T: row (query head), key
 __device__ __forceinline__ uint32_t sp_p_off(int row, int key) {
   const int chunk = key >> 3;
@@ -504,7 +533,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
       __syncwarp();
     };
-    auto wait_kv = [&](uint32_t pos) { mbar_wait_bounded(&kv_full[pos % kSpSlots], (pos / kSpSlots) & 1, dead); };
+    auto wait_kv = [&](uint32_t pos) { sp_wait(&kv_full[pos % kSpSlots], (pos / kSpSlots) & 1, dead); };
     bool have = walk.next(p, pl, it);
     while (have) {
       SpItem nx;
@@ -515,7 +544,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (count > 0) {
         if (!q_ahead) load_q(it);
         q_ahead = false;
-        mbar_wait_bounded(&q_full[w], eq & 1, dead);
+        sp_wait(&q_full[w], eq & 1, dead);
       }
       // S(j, h): the P which these columns held has been consumed by the PV of this tile's predecessor here, issued earlier by
       // this thread
@@ -551,13 +580,13 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         for (int h = 0; h < 2; ++h) {
           if (i == count - 1 && h == 0 && nx_count > 0) {
             // the item's last S is under way: once it is complete, Q's memory is free for the next item
-            mbar_wait_bounded(&s_full[w * 2 + 1], (pq >> 1) & 1, dead);
+            sp_wait(&s_full[w * 2 + 1], (pq >> 1) & 1, dead);
             load_q(nx);
             q_ahead = true;
           }
-          mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
+          sp_wait(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
           if (h == 0) wait_kv(vpos);
-          if (i == 0 && h == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
+          if (i == 0 && h == 0) sp_wait(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
           tc_fence_after_sync();
           uint32_t va = static_cast<uint32_t>(vd0) + (vpos % kSpSlots) * (kSpTileBytes / 16) + h * (kSpU * 128 / 16);
           uint32_t pa = tmem_S + w * 128 + h * kSpU;
@@ -599,7 +628,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     auto issue_s = [&]() {  // into the buffer of the unit before the last, whose P has been waited for
       const OwnSlot at = own_slot(w, 2 * ks, t_base);
       const uint32_t h = pu & 1;
-      mbar_wait_bounded(&kv_full[at.bar], at.full, dead);  // (Q arrives with the item's first tile here)
+      sp_wait(&kv_full[at.bar], at.full, dead);  // (Q arrives with the item's first tile here)
       tc_fence_after_sync();
       uint32_t ka = k_lo + at.tile * (kSpTileBytes / 16), qa = q_lo + qs * (kSpSmall / 16);
 #pragma unroll 1
@@ -631,8 +660,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         const OwnSlot at = own_slot(w, 2 * vs + 1, t_base);
         const uint32_t h = pq & 1;
-        mbar_wait_bounded(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
-        mbar_wait_bounded(&kv_full[at.bar], at.full, dead);
+        sp_wait(&p_full[w * 2 + h], (pq >> 1) & 1, dead);
+        sp_wait(&kv_full[at.bar], at.full, dead);
         const int valid = min(kSpTile, it.keys - (it.tile0 + j) * kSpTile), steps = (valid + 15) / 16;  // of 16 keys
         if (valid & 15) {  // V rows that the last step takes in and nobody asked for: their P is 0, they may be anything
           uint8_t* rows = smem + at.tile * kSpTileBytes + (lane >> 3 & 1) * 16384 + (lane & 7) * 16;
@@ -640,7 +669,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (j == 0) mbar_wait_bounded(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
+        if (j == 0) sp_wait(&o_free[w], (eq & 1) ^ 1, dead);  // the previous item's O has been read
         tc_fence_after_sync();
         uint32_t va = v_lo + at.tile * (kSpTileBytes / 16), pa = p_lo + h * (kSpSmall / 16);
 #pragma unroll 1
@@ -710,18 +739,21 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     };
     // ---- shared keys: K by warp 8, V by warp 9; lookups run one tile ahead of the copies ----
     int slot[4], next[4];
-    auto entry = [&](int skip) { return p.req_to_token + it.req * p.rtt_stride + static_cast<int64_t>(skip + it.tile0) * kSpTile; };
-    bool have = walk.next(p, pl, it);
-    if (have) lookup(entry(0), kSpTile, slot);
+    auto entry = [&](int skip, int j) {
+      return p.req_to_token + it.req * p.rtt_stride + static_cast<int64_t>(skip + it.tile0 + j) * kSpTile;
+    };
+    int hk = 0, j = 0;
+    bool first = false, more = true, have = walk.next(p, pl, it);
+    if (have) lookup(entry(0, 0), kSpTile, slot);
     for (int j = 0; have; ++t_base) {
       const int hk = it.hk;
       if (++j == it.n) {
         have = walk.next(p, pl, it);
         j = 0;
       }
-      if (have) lookup(entry(0) + j * kSpTile, kSpTile, next);
+      if (have) lookup(entry(0, j), kSpTile, next);
       const uint32_t pos = 2 * t_base + lw;
-      mbar_wait_bounded(&kv_empty[pos % kSpSlots], ((pos / kSpSlots) & 1) ^ 1, dead);
+      sp_wait(&kv_empty[pos % kSpSlots], ((pos / kSpSlots) & 1) ^ 1, dead);
       load(lw ? tmV : tmK, pos % kSpSlots, 2 + pos % kSpSlots, hk, slot, kSpTile);
 #pragma unroll
       for (int i = 0; i < 4; ++i) slot[i] = next[i];
@@ -729,22 +761,24 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     // ---- own keys: warpgroup lw's, with the queries ----
     SpOwnWalk own(p, pl, range, lw);
     uint32_t place = 0;
-    int q_buf = 0;
-    have = own.next(p, pl, range, it);
-    if (have) lookup(entry(pl.skip[it.b0]), it.keys - it.tile0 * kSpTile, slot);
-    // the queries' buffers are memory that the warpgroup's outputs over shared keys pass through
-    if (have) mbar_wait_bounded(&stage_free[lw], 0, dead);
-    for (int j = 0; have;) {
-      const int hk = it.hk, b = it.b0, first = j == 0, valid = min(kSpTile, it.keys - (it.tile0 + j) * kSpTile);
-      if (++j == it.n) {
-        have = own.next(p, pl, range, it);
+    int q_buf = 0, b = 0, valid = 0;
+    have = false;
+    more = true;
+    it.n = j = 0;
+#pragma unroll 1
+    while (more) {
+      if (j == it.n) {
+        more = own.next(p, pl, range, it);
         j = 0;
       }
-      if (have) lookup(entry(pl.skip[it.b0]) + j * kSpTile, it.keys - (it.tile0 + j) * kSpTile, next);
-#pragma unroll
-      for (int is_v = 0; is_v < 2; ++is_v, ++place) {
+      const int left = it.keys - (it.tile0 + j) * kSpTile;
+      if (more) lookup(entry(pl.skip[it.b0], j), left, next);
+      // the queries' buffers are memory that the warpgroup's outputs over shared keys pass through
+      if (!have) sp_wait(&stage_free[lw], 0, dead);
+#pragma unroll 1
+      for (int is_v = 0; have && is_v < 2; ++is_v, ++place) {
         const OwnSlot at = own_slot(lw, place, t_base);
-        mbar_wait_bounded(&kv_empty[at.bar], at.empty, dead);
+        sp_wait(&kv_empty[at.bar], at.empty, dead);
         if (is_v == 0 && first) {
           // The buffer's last queries were those of the item before the last one, whose tiles are no younger than the V tile
           // that this slot held: its MMAs have finished.
@@ -758,6 +792,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         load(is_v ? tmV : tmK, at.bar, at.tile, hk, slot, valid);
       }
+      have = more;
+      hk = it.hk;
+      b = it.b0;
+      first = j == 0;
+      valid = min(kSpTile, left);
+      ++j;
 #pragma unroll
       for (int i = 0; i < 4; ++i) slot[i] = next[i];
     }
@@ -788,7 +828,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const uint32_t u0 = u, u1 = u + 2 * count;
         for (; u < u1; ++u) {
           const int h = u & 1;
-          mbar_wait_bounded(&s_full[w * 2 + h], (u >> 1) & 1, dead);
+          sp_wait(&s_full[w * 2 + h], (u >> 1) & 1, dead);
           if (active) {
             tc_fence_after_sync();
             uint32_t ra[32], rb[32], pk[32];
@@ -816,7 +856,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (raise && u > u0) {
               // O stands still once the PV of the unit before is complete (those before it are: S of this unit was issued
               // after them)
-              mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
+              sp_wait(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
               tc_fence_after_sync();
               rescale_row128(to, alpha);
             }
@@ -833,7 +873,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           const int64_t at = first ? static_cast<int64_t>((it.split() && w == 1 ? 2 * p.batch : 0) + b0) * p.Hq + it.hk * p.group
                                    : (static_cast<int64_t>(blockIdx.x) * 2 + w) * kSpM;
           if (count > 0) {
-            mbar_wait_bounded(&pv_done[w * 2 + 1], ((u - 1) >> 1) & 1, dead);
+            sp_wait(&pv_done[w * 2 + 1], ((u - 1) >> 1) & 1, dead);
             tc_fence_after_sync();
             float* o = (first ? p.o_first : p.o_next) + at * kSpD;
 #pragma unroll 1
@@ -861,7 +901,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           // (an empty request in the middle of a group takes no part; without a tile the part is one of sum 0)
           const int b = b0 + member;
           if (first && row < rows && row == member * p.group && pl.skip[b] > 0 && (w == 0 || !it.split()))
-            p.notes[b * p.Hk + it.hk] = it.note(range.per, it.split(), w * kSpM + row);
+            p.notes[b * p.Hk + it.hk] = it.note(range, it.split(), w * kSpM + row);
           tc_fence_before_sync();
           __syncwarp();
         }
@@ -889,7 +929,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
       for (int j = 0; j < it.n; ++j, ++u) {
         const int h = u & 1;
-        mbar_wait_bounded(&s_full[w * 2 + h], (u >> 1) & 1, dead);
+        sp_wait(&s_full[w * 2 + h], (u >> 1) & 1, dead);
         tc_fence_after_sync();
         uint32_t r[16];
         tmem_ld_32x32b_x16(ts + h * kSpU, r);
@@ -921,7 +961,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         ++rounds;
         if (raise && j > 0) {
-          mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);  // O stands still
+          sp_wait(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);  // O stands still
           tc_fence_after_sync();
           uint32_t o[16];
           tmem_ld_32x32b_x16(to, o);
@@ -932,7 +972,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           tmem_st_wait();
         }
         // the P buffer's last reader is the PV of the unit before the last
-        if (u >= 2) mbar_wait_bounded(&pv_done[w * 2 + h], ((u - 2) >> 1) & 1, dead);
+        if (u >= 2) sp_wait(&pv_done[w * 2 + h], ((u - 2) >> 1) & 1, dead);
         uint8_t* pdst = own_p(w, h);
 #pragma unroll
         for (int g = 0; g < kSpMaxGroup; ++g)
@@ -962,10 +1002,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             ml[g] = make_float2(m_ref[g], (x.x + x.y) + (x.z + x.w));
           }
         // behind the CTA of the first part an item is its CTA's first, so it is warpgroup 0's there
-        if (first) p.notes[(p.batch + it.b0) * p.Hk + it.hk] = it.note(range.per, false, 0);
+        if (first) p.notes[(p.batch + it.b0) * p.Hk + it.hk] = it.note(range, false, 0);
       }
       ++rounds;
-      mbar_wait_bounded(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
+      sp_wait(&pv_done[w * 2 + ((u - 1) & 1)], ((u - 1) >> 1) & 1, dead);
       tc_fence_after_sync();
       uint32_t r[16];
       tmem_ld_32x32b_x16(to, r);
@@ -1073,24 +1113,24 @@ static int64_t part_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
 }
 
 // Whether reading the shared keys once is the faster way, from what the host knows: as if all requests were in groups of one
-// size that share max_shared keys.  The weights fit 330 shapes measured both ways (2 to 256 requests in 1 to 32 groups, 128 to
-// 16384 shared tokens, 64 own, bf16, four head layouts): the choice takes 0.5% longer than the better way on average, 18% at
-// worst.  A tile of 128 shared keys costs an SM 1 here and each member 0.57 there (mostly from L2); requests that there are cut
-// over many SMs cost 0.2 per part and query head in their merge; the longer start, the join and the shorter ranges cost 6 here,
-// and 0.002 per request and kv head.
-// us by request / shared.  32 / 8 heads, one group: 64 members of 256 tokens 19.1 / 25.9, 512: 24.3 / 23.9, 1024: 34.0 / 24.2,
-// 16384: 354 / 49.3; 8 of 1024: 14.3 / 17.4, 4096: 25.4 / 24.1, 16384: 58.2 / 36.4; 4 of 4096: 22.0 / 23.9.  Groups of two: 8
-// of 4096: 45.9 / 48.6, of 16384: 162 / 109; 32 of 2048: 60.8 / 80.8, of 4096: 161 / 122.  16 / 2 heads, 2 of 512: 18.1 / 19.9,
-// of 4096: 49.7 / 23.9.  32 / 32 heads, 16 of 256: 17.9 / 19.5, of 1024: 32.6 / 23.8.
+// size that share max_shared keys.  The weights fit 325 shapes measured both ways (2 to 256 requests in 1 to 32 groups, 128 to
+// 16384 shared tokens, 64 own, bf16, four head layouts): the choice takes 0.6% longer than the better way on average, 19% at
+// worst.  A tile of 128 shared keys costs an SM 1.2 here and each member 0.7 there (mostly from L2); requests that there are cut
+// over many SMs cost 0.4 per part and query head in their merge; the longer start, the join and the shorter ranges cost 6 here,
+// and 0.0008 per request and kv head.
+// us by request / shared.  32 / 8 heads, one group: 64 members of 256 tokens 18.8 / 18.9, 512: 24.1 / 21.3, 1024: 33.8 / 22.0,
+// 16384: 388 / 41.5; 8 of 1024: 14.3 / 15.5, 4096: 25.1 / 22.7, 16384: 57.0 / 31.2; 4 of 4096: 21.6 / 22.0.  Groups of two: 8
+// of 4096: 46.3 / 39.8, of 16384: 164 / 100; 32 of 2048: 62.3 / 67.9, of 4096: 161 / 107.  16 / 2 heads, 2 of 512: 17.6 / 15.1,
+// of 4096: 53.1 / 24.6.  32 / 32 heads, 16 of 256: 17.7 / 17.6, of 1024: 32.3 / 21.3.
 static bool shared_pays(int64_t batch, int64_t groups, int64_t max_shared, int num_q_heads, int num_kv_heads, int sms) {
   const double pairs = static_cast<double>(batch) * num_kv_heads, shared = static_cast<double>(max_shared);
   const double tiles = static_cast<double>(groups) * num_kv_heads * (shared / kSpTile) / sms;  // of an SM
-  double gain = tiles * (0.57 * batch / groups - 1.0);
+  double gain = tiles * (0.7 * batch / groups - 1.2);
   if (pairs < sms) {
     const double parts = sms / pairs < shared / 256 ? sms / pairs : shared / 256;
-    gain += 0.2 * (num_q_heads / num_kv_heads) * parts;
+    gain += 0.4 * (num_q_heads / num_kv_heads) * parts;
   }
-  return gain > 6.0 + 0.002 * pairs * 148 / sms;
+  return gain > 6.0 + 0.0008 * pairs * 148 / sms;
 }
 
 }  // namespace spd
@@ -1124,7 +1164,8 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
   if (int rc = check_attn_args("spd_attn_decode_shared", out, q, k_pool, v_pool, req_to_token, req_pool_indices, num_q_heads,
                                num_kv_heads, head_dim, q_stride, out_stride))
     return rc;
-  SPD_REQUIRE(seq_lens && batch >= 0 && num_groups >= 0 && max_shared_len >= 0 && pool_slots > 0 && pool_slots < (1ll << 31) && (num_groups == 0 || (group_indptr && shared_lens)),
+  SPD_REQUIRE(seq_lens && batch >= 0 && num_groups >= 0 && max_shared_len >= 0 && pool_slots > 0 && pool_slots < (1ll << 31) &&
+                  (num_groups == 0 || (group_indptr && shared_lens)),
               SPD_E_BADARG, "spd_attn_decode_shared: bad lengths or groups");
   SPD_REQUIRE(head_dim == kSpD, SPD_E_SHAPE, "spd_attn_decode_shared: head_dim must be 128 (got %d)", head_dim);
   if (batch == 0) return 0;
