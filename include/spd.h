@@ -40,8 +40,8 @@ typedef void* spd_stream_t; /* cudaStream_t */
  * ------------------------------------------------------------------------------------------- */
 int spd_version(void);
 const char* spd_last_error_string(void);
-/* Waits inside spd_attn_mla, spd_attn_mla_prefill and spd_retention_extend are bounded (seconds).  One that runs out sets a
- * word in host memory when its kernel ends; what that kernel wrote is not to be trusted (a recurrent state is kept as it was before the tokens
+/* Waits inside spd_attn_mla, spd_attn_mla_prefill, spd_attn_decode_shared and spd_retention_extend are bounded (seconds).  One
+ * that runs out sets a word in host memory when its kernel ends; what that kernel wrote is not to be trusted (a recurrent state is kept as it was before the tokens
  * the wait stood for), and those calls return SPD_E_TIMEOUT from then on.  spd_wait_status reads the word without
  * synchronising: call it where a kernel's results are known to have arrived.  clear != 0 resets it. */
 int spd_wait_status(int* expired, int clear);
@@ -296,9 +296,11 @@ int spd_attn_decode_paged_own(void* out, const void* q, const void* k_pool, cons
                               int64_t workspace_bytes, int sm_budget, spd_stream_t stream);
 /* Decode attention for requests that continue the same tokens.  Rows [group_indptr[g], group_indptr[g + 1]) of the batch
  * (int32, num_groups + 1 entries, ascending) are a group whose members' req_to_token rows name the same slots in their first
- * shared_lens[g] positions; max_shared_len is no less than any of those; the pools have pool_slots rows.  The result is spd_attn_decode_paged's: every row of
- * req_to_token is complete, rows of no group stand alone, seq_lens[b] counts the shared tokens too, and a request of length
- * 0 gets zeros.  The shared part of a group is read once for all of its queries.
+ * shared_lens[g] positions; max_shared_len is no less than any of those; the pools have pool_slots rows.  The result is
+ * spd_attn_decode_paged's: every row of req_to_token is complete, rows of no group stand alone, seq_lens[b] counts the shared
+ * tokens too, and a request of length 0 gets zeros.  The shared part of a group is read once for all of its queries.
+ * head_dim 128, at most 8 query heads per kv head; batches of more than 1024 requests or 256 groups are read as
+ * spd_attn_decode_paged reads them.
  * Workspace: spd_attn_decode_shared_workspace_bytes(), zeroed once before its first use (each call leaves its counters at
  * zero), one per stream.  spd_attn_decode_shared_pays: 1 where a call of these sizes takes the kernel that shares, 0 where
  * spd_attn_decode_paged serves it as well (decided on the host, without a launch).
