@@ -31,7 +31,7 @@ from __future__ import annotations
 
 import abc
 import collections
-from typing import Dict, List, Optional, Sequence, Tuple, Union
+from typing import Deque, Dict, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -40,6 +40,46 @@ from . import ops
 
 GB = 1024 ** 3
 DEFAULT_RUN_LEN = 128
+
+
+class _FreeList:
+    """Free items, in the order they came back.  What comes back while copies that read it may still run (fork_request,
+    compact_request) is free once they have, since its next writer may be on another stream."""
+
+    def __init__(self, items):
+        self.items: Deque[int] = collections.deque(items)
+        self.copies: List["torch.cuda.Event"] = []
+        self.waiting: Deque[Tuple[list, List[int]]] = collections.deque()
+
+    def copying(self) -> None:
+        """Copies that read what is not free have been launched on the current stream."""
+        if torch.cuda.is_available():
+            event = torch.cuda.Event()
+            event.record()
+            self.copies.append(event)
+
+    def give(self, items: Sequence[int]) -> None:
+        self.copies = [e for e in self.copies if not e.query()]
+        if self.copies:
+            self.waiting.append((list(self.copies), list(items)))
+        else:
+            self.items.extend(items)
+
+    def enough(self, need: int) -> bool:
+        """Whether `need` items are free, if necessary after waiting for the copies that read some of them."""
+        while self.waiting and (need > len(self.items) or all(e.query() for e in self.waiting[0][0])):
+            events, items = self.waiting.popleft()
+            for e in events:
+                if not e.query():
+                    e.synchronize()
+            self.items.extend(items)
+        return need <= len(self.items)
+
+    def take(self) -> int:
+        return self.items.popleft()
+
+    def __len__(self) -> int:
+        return len(self.items) + sum(len(items) for _, items in self.waiting)
 
 
 class ReqToTokenPool:
@@ -61,9 +101,9 @@ class ReqToTokenPool:
         return len(self._free)
 
     def alloc(self, need_size: int) -> Optional[List[int]]:
-        if need_size > len(self._free):
+        if not self._free.enough(need_size):
             return None
-        out = [self._free.popleft() for _ in range(need_size)]
+        out = [self._free.take() for _ in range(need_size)]
         self._live.update(out)
         return out
 
@@ -72,15 +112,19 @@ class ReqToTokenPool:
             if i not in self._live:
                 raise RuntimeError(f"request slot {i} freed twice")
             self._live.discard(i)
-            self._free.append(i)
+            self._free.give([i])
+
+    def copying(self) -> None:
+        """See _FreeList.copying: of a request's page-table row, or of what its slot stands for."""
+        self._free.copying()
 
     def clear(self):
-        self._free = collections.deque(range(self.size))
+        self._free = _FreeList(range(self.size))
         self._live = set()
 
     @property
     def free_slots(self) -> List[int]:
-        return list(self._free)
+        return list(self._free.items)
 
 
 class KVCache(abc.ABC):
@@ -179,7 +223,7 @@ class TokenToKVPoolAllocator:
 
     # ---- bookkeeping ---------------------------------------------------------------------------
     def clear(self):
-        self._free_runs = collections.deque(range(self.num_runs))
+        self._free_runs = _FreeList(range(self.num_runs))
         self._used = np.zeros(self.num_runs, dtype=np.int32)
         self._held = np.zeros(self.num_runs, dtype=np.int32)   # requests that hold the run
         self._forked = False                                   # some run may have several holders
@@ -217,7 +261,7 @@ class TokenToKVPoolAllocator:
             if pre != have:
                 raise RuntimeError(f"request slot {idx}: prefix {pre} does not match the {have} tokens placed")
             need += self.runs_needed(pre, seq)
-        if need > len(self._free_runs):
+        if not self._free_runs.enough(need):
             return None
         R = self.run_len
         parts = []
@@ -240,7 +284,7 @@ class TokenToKVPoolAllocator:
     def can_alloc_decode(self, seq_lens_before: Sequence[int]) -> bool:
         """One more token for every request of the batch (lens BEFORE the step)."""
         R = self.run_len
-        return sum(1 for s in seq_lens_before if s % R == 0) <= len(self._free_runs)
+        return self._free_runs.enough(sum(1 for s in seq_lens_before if s % R == 0))
 
     def alloc_decode(self, req_pool_indices: Sequence[int], seq_lens_before: Sequence[int]
                      ) -> Optional[torch.Tensor]:
@@ -271,7 +315,7 @@ class TokenToKVPoolAllocator:
 
     # ---- requests that share runs --------------------------------------------------------------
     def _take_run(self) -> int:
-        run = self._free_runs.popleft()
+        run = self._free_runs.take()
         self._held[run] = 1
         return run
 
@@ -281,7 +325,11 @@ class TokenToKVPoolAllocator:
         self._held[ids] -= 1
         gone = ids[self._held[ids] == 0]
         self._used[gone] = 0
-        self._free_runs.extend(int(r) for r in gone)
+        self._free_runs.give([int(r) for r in gone])
+
+    def copying(self) -> None:
+        """See _FreeList.copying: of rows that requests hold."""
+        self._free_runs.copying()
 
     def req_len(self, req_pool_idx: int) -> int:
         return self._req_len[req_pool_idx]
@@ -295,7 +343,7 @@ class TokenToKVPoolAllocator:
             raise RuntimeError("fork: children must be request slots of their own that hold no runs")
         R, n, runs = self.run_len, self._req_len[parent], self._req_runs[parent]
         whole, rest = runs[:n // R], n % R
-        if rest and len(children) > len(self._free_runs):
+        if rest and not self._free_runs.enough(len(children)):
             return None
         out = np.zeros(len(children), dtype=np.int64)
         for i, c in enumerate(children):
@@ -317,7 +365,7 @@ class TokenToKVPoolAllocator:
         if not 0 < n <= self._req_len.get(req_pool_idx, 0):
             raise RuntimeError(f"request slot {req_pool_idx}: cannot keep {n} of {self._req_len.get(req_pool_idx, 0)} tokens")
         R = self.run_len
-        if -(-n // R) > len(self._free_runs):
+        if not self._free_runs.enough(-(-n // R)):
             return None
         old = self._req_runs[req_pool_idx]
         self._req_runs[req_pool_idx] = [self._take_run() for _ in range(-(-n // R))]
@@ -360,9 +408,9 @@ class TokenToKVPoolAllocator:
         stays reserved until the slots next to it are freed."""
         R = self.run_len
         n_runs = -(-need_size // R)
-        if n_runs > len(self._free_runs):
+        if not self._free_runs.enough(n_runs):
             return None
-        runs = [self._free_runs.popleft() for _ in range(n_runs)]
+        runs = [self._free_runs.take() for _ in range(n_runs)]
         pos = np.arange(need_size, dtype=np.int64)
         flat = (np.asarray(runs, dtype=np.int64)[pos // R] * R + 1 + pos % R) if need_size else pos
         if need_size:
@@ -386,7 +434,7 @@ class TokenToKVPoolAllocator:
         if (self._used[runs] < 0).any():
             raise RuntimeError("KV slots freed twice")
         self._held[runs[self._used[runs] == 0]] = 0
-        self._free_runs.extend(int(r) for r in runs[self._used[runs] == 0])
+        self._free_runs.give([int(r) for r in runs[self._used[runs] == 0]])
 
     def free_group_begin(self):
         self.is_not_in_free_group = False
@@ -519,6 +567,8 @@ def fork_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator:
     kv_pool.fork_rows(parent, children, allocator._req_runs[parent][length // R] if rest else None,
                       [allocator._req_runs[c][-1] for c in children] if rest else [],
                       lambda rows: allocator._ring.stage(np.asarray(rows, dtype=np.int64), allocator.device))
+    allocator.copying()
+    req_to_token_pool.copying()
     return children
 
 
@@ -542,7 +592,8 @@ def compact_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocat
     lists = allocator._ring.stage(np.concatenate([pos, slots, [req, 0, n]]).astype(np.int64), allocator.device)
     ops.kv_compact(kv_pool.planes, req_to_token_pool.req_to_token, lists[2 * n:2 * n + 1], None, lists[:n], lists[2 * n + 1:],
                    lists[n:2 * n])
-    allocator.release_runs(old)  # later writers of these runs come behind the copy, in this stream or by its events
+    allocator.copying()
+    allocator.release_runs(old)
     return True
 
 

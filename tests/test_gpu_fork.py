@@ -183,3 +183,37 @@ def test_attention_over_a_compacted_request():
     spread = torch.einsum("hn,nhd->hd", p, (vv.repeat_interleave(2, 1) - want).abs())
     u = 2.0 ** -8   # weights and output rounded to bf16, half a step each
     assert bool(((out.double().view(4, 128) - want).abs() <= 1.02 * u * (spread + want.abs()) + 1e-4).all())
+
+
+@pytest.mark.parametrize("what", ["fork", "compact"])
+def test_what_a_copy_reads_is_not_written_by_another_stream(what):
+    """A request that is let go right after it was forked (or compacted), its runs and slots asked for on another stream while the
+    copy has not begun."""
+    from semi_pd_b200.memory_pool import compact_request, fork_request
+    pool, table, alloc = _pools("mha", runs=8, reqs=3)
+    parent = _place(table, alloc, 500)            # four of eight runs
+    before = _rows(pool, table.req_to_token, parent, 500)
+    torch.cuda.synchronize()
+    one, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(one):
+        torch.cuda._sleep(200_000_000)            # about 0.1 s
+        if what == "fork":
+            (req,) = fork_request(pool, table, alloc, parent, 1)
+            alloc.free_req(parent)
+            table.free(parent)
+            keep = list(range(500))
+        else:
+            keep = list(range(3, 500, 2))
+            assert compact_request(pool, table, alloc, parent, keep)
+            req = parent
+    with torch.cuda.stream(other):
+        while table.available_size() and alloc.available_size():
+            (idx,) = table.alloc(1)
+            n = min(alloc.available_size(), 256)
+            slots = alloc.alloc_extend([idx], [0], [n])
+            table.req_to_token[idx] = -1
+            for b in pool.planes.buffers:
+                b[slots] = 0
+    torch.cuda.synchronize()
+    for a, b in zip(_rows(pool, table.req_to_token, req, len(keep)), before):
+        assert torch.equal(a, b[keep])
