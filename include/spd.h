@@ -303,12 +303,15 @@ int spd_attn_decode_paged_own(void* out, const void* q, const void* k_pool, cons
  * spd_attn_decode_paged reads them.
  * Workspace: spd_attn_decode_shared_workspace_bytes(), zeroed once before its first use (each call leaves its counters at
  * zero), one per stream.  spd_attn_decode_shared_pays: 1 where a call of these sizes takes the kernel that shares, 0 where
- * spd_attn_decode_paged serves it as well (decided on the host, without a launch).
+ * spd_attn_decode_paged serves it as well (decided on the host, without a launch); _saves: about how many us the call saves
+ * then, rounded up (0 where it does not pay).
  * The reference has no such call; its cascade form is flashinfer's, behind the same wrapper interface as
  * S/layers/attention/flashinfer_backend.py:454-488. */
 int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_heads, int num_kv_heads, int head_dim);
 int spd_attn_decode_shared_pays(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
                                 int head_dim, int sm_budget);
+int spd_attn_decode_shared_saves(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
+                                 int head_dim, int sm_budget);
 int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
                            const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
                            const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t max_shared_len,

@@ -91,6 +91,7 @@ SIGNATURES = {
     ),
     "spd_attn_decode_shared_workspace_bytes": (_i64, [_i64, _i, _i, _i]),
     "spd_attn_decode_shared_pays": (_i, [_i64, _i64, _i64, _i, _i, _i, _i]),
+    "spd_attn_decode_shared_saves": (_i, [_i64, _i64, _i64, _i, _i, _i, _i]),
     "spd_attn_decode_shared": (
         _i,
         [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i64, _i64, _i64, _f, _i, _p, _i64, _i, _p],

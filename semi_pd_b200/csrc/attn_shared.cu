@@ -1122,7 +1122,7 @@ static int64_t part_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
 // 16384: 388 / 41.5; 8 of 1024: 14.3 / 15.5, 4096: 25.1 / 22.7, 16384: 57.0 / 31.2; 4 of 4096: 21.6 / 22.0.  Groups of two: 8
 // of 4096: 46.3 / 39.8, of 16384: 164 / 100; 32 of 2048: 62.3 / 67.9, of 4096: 161 / 107.  16 / 2 heads, 2 of 512: 17.6 / 15.1,
 // of 4096: 53.1 / 24.6.  32 / 32 heads, 16 of 256: 17.7 / 17.6, of 1024: 32.3 / 21.3.
-static bool shared_pays(int64_t batch, int64_t groups, int64_t max_shared, int num_q_heads, int num_kv_heads, int sms) {
+static double shared_saves(int64_t batch, int64_t groups, int64_t max_shared, int num_q_heads, int num_kv_heads, int sms) {
   const double pairs = static_cast<double>(batch) * num_kv_heads, shared = static_cast<double>(max_shared);
   const double tiles = static_cast<double>(groups) * num_kv_heads * (shared / kSpTile) / sms;  // of an SM
   double gain = tiles * (0.7 * batch / groups - 1.2);
@@ -1130,7 +1130,7 @@ static bool shared_pays(int64_t batch, int64_t groups, int64_t max_shared, int n
     const double parts = sms / pairs < shared / 256 ? sms / pairs : shared / 256;
     gain += 0.4 * (num_q_heads / num_kv_heads) * parts;
   }
-  return gain > 6.0 + 0.0008 * pairs * 148 / sms;
+  return gain - (6.0 + 0.0008 * pairs * 148 / sms);
 }
 
 }  // namespace spd
@@ -1145,14 +1145,20 @@ int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_head
   return decode_bytes(max_batch, num_q_heads, num_kv_heads) + part_bytes(max_batch, num_q_heads, num_kv_heads);
 }
 
-int spd_attn_decode_shared_pays(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
-                                int head_dim, int sm_budget) {
+int spd_attn_decode_shared_saves(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
+                                 int head_dim, int sm_budget) {
   if (batch < 2 || batch > kSpRows || num_groups < 1 || num_groups > kSpGroups || max_shared_len < kSpTile || num_kv_heads < 1 ||
       num_q_heads < num_kv_heads || head_dim != kSpD)
     return 0;
   const int device_sms = device_sm_count_cached();
-  return shared_pays(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads,
-                     sm_budget > 0 && sm_budget < device_sms ? sm_budget : device_sms);
+  const double us = shared_saves(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads,
+                                 sm_budget > 0 && sm_budget < device_sms ? sm_budget : device_sms);
+  return us <= 0. ? 0 : us >= 1e9 ? 1000000000 : static_cast<int>(us) + 1;
+}
+
+int spd_attn_decode_shared_pays(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
+                                int head_dim, int sm_budget) {
+  return spd_attn_decode_shared_saves(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, sm_budget) > 0;
 }
 
 int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,

@@ -791,13 +791,18 @@ def new_attn_shared_workspace(device, max_batch: int, num_q_heads: int, num_kv_h
 
 
 @functools.lru_cache(maxsize=1024)
-def _attn_shared_pays(batch: int, groups: int, max_shared_len: int, hq: int, hk: int, d: int, sm_budget: int) -> bool:
-    return lib.spd_attn_decode_shared_pays(batch, groups, max_shared_len, hq, hk, d, sm_budget) == 1
+def _attn_shared_saves(batch: int, groups: int, max_shared_len: int, hq: int, hk: int, d: int, sm_budget: int) -> int:
+    return lib.spd_attn_decode_shared_saves(batch, groups, max_shared_len, hq, hk, d, sm_budget)
+
+
+def attn_shared_saves(batch: int, groups: int, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """About how many us attn_decode_shared saves by reading such a batch's shared keys once, 0 where it reads them per request."""
+    return _attn_shared_saves(batch, groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, get_sm_budget())
 
 
 def attn_shared_pays(batch: int, groups: int, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> bool:
     """Whether attn_decode_shared reads such a batch's shared keys once (attn_decode serves it as well otherwise)."""
-    return _attn_shared_pays(batch, groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, get_sm_budget())
+    return attn_shared_saves(batch, groups, max_shared_len, num_q_heads, num_kv_heads, head_dim) > 0
 
 
 def attn_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, req_to_token: torch.Tensor,

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from semi_pd_b200 import _lib, ops
-from semi_pd_b200.memory_pool import TokenToKVPoolAllocator
+from semi_pd_b200.memory_pool import ReqToTokenPool, TokenToKVPoolAllocator
 
 R = 16
 
@@ -207,3 +207,64 @@ def test_c_abi_refuses_before_any_cuda_call():
     ((1025, 1, 8192, 32, 8, 128, 148), 0), ((1024, 257, 8192, 32, 8, 128, 148), 0), ((64, 1, 8192, 32, 8, 64, 148), 0)])
 def test_when_sharing_pays(args, pays):
     assert _lib.lib.spd_attn_decode_shared_pays(*args) == pays
+    assert (_lib.lib.spd_attn_decode_shared_saves(*args) > 0) == bool(pays)
+
+
+def test_a_graph_is_given_up_only_for_more_than_it_saves():
+    from semi_pd_b200 import ops
+    from semi_pd_b200.attention_backend import SpdAttnBackend
+    from semi_pd_b200.forward_batch_info import SharedPrefix
+    backend = SpdAttnBackend.__new__(SpdAttnBackend)
+    backend.impl, backend.is_mla, backend.num_q_heads, backend.num_kv_heads, backend.head_dim = "tc", False, 32, 8, 128
+    shared = lambda n: SharedPrefix(torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int64), n)  # noqa: E731
+    few = next(n for n in range(128, 1 << 16, 128) if ops.attn_shared_pays(64, 1, n, 32, 8, 128))
+    assert 0 < ops.attn_shared_saves(64, 1, few, 32, 8, 128) <= SpdAttnBackend.GRAPH_SAVES < ops.attn_shared_saves(64, 1, 8192, 32, 8, 128)
+    for most, want in ((0, True), (63, True), (64, False)):
+        backend.graph_max_bs = most
+        assert backend.shares_prefix(64, shared(few)) is want
+        assert backend.shares_prefix(64, shared(8192))
+
+
+class _Event:
+    def __init__(self):
+        self.done, self.waited = False, False
+
+    def query(self):
+        return self.done
+
+    def synchronize(self):
+        self.done = self.waited = True
+
+
+def test_what_a_copy_reads_is_free_when_it_has_run():
+    """Runs and request slots that come back while a copy may still read them are not handed out before it has run."""
+    pool = ReqToTokenPool(4, 64, "cpu")
+    alloc = TokenToKVPoolAllocator(6 * 8, torch.float32, "cpu", None, run_len=8)
+    (a,) = pool.alloc(1)
+    alloc.alloc_extend([a], [0], [20])          # three of six runs
+    held = set(alloc._req_runs[a])
+    event = _Event()
+    alloc._free_runs.copies.append(event)
+    pool._free.copies.append(event)
+    alloc.free_req(a)
+    pool.free(a)
+    assert alloc.available_size() == 48 and pool.available_size() == 4
+    b = pool.alloc(3)
+    assert a not in b
+    alloc.alloc_extend(b[:1], [0], [24])        # the other three
+    assert not held & set(alloc._req_runs[b[0]]) and not event.waited
+    assert alloc.can_alloc_decode([8]) and event.waited   # a fourth one waits for the copy
+    alloc.alloc_extend(b[1:2], [0], [24])
+    assert set(alloc._req_runs[b[1]]) == held and alloc.available_size() == 0
+    assert pool.alloc(1) == [a]
+    alloc.free_req(b[0])                        # no copy runs any more
+    assert alloc.alloc_extend([a], [0], [24]) is not None
+    alloc.clear()
+    pool.clear()
+    assert alloc.available_size() == 48 and pool.available_size() == 4
+    event = _Event()
+    alloc._free_runs.copies.append(event)
+    alloc.alloc_extend([a], [0], [20])
+    alloc.free_req(a)
+    event.done = True
+    assert alloc.alloc_extend([a], [0], [48]) is not None and not event.waited
