@@ -233,12 +233,6 @@ __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl
     }
   }
   __syncthreads();
-  // rows without a shared or without an own part: the join looks at their notes too
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
-    for (int hk = threadIdx.x; hk < p.Hk; hk += kSpThreads) {
-      if (pl.skip[b] == 0) p.notes[b * p.Hk + hk] = make_int2(0, 0);
-      if (pl.len[b] == 0) p.notes[(p.batch + b) * p.Hk + hk] = make_int2(0, 0);
-    }
   return r;
 }
 
@@ -803,6 +797,14 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
   } else {
     // ===================== softmax =====================
+    // Rows without a shared or without an own part: the join looks at their notes too.  (The first scores are a while off.)
+#pragma unroll 1
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
+#pragma unroll 1
+      for (int hk = threadIdx.x; hk < p.Hk; hk += 2 * kSpM) {
+        if (pl.skip[b] == 0) p.notes[b * p.Hk + hk] = make_int2(0, 0);
+        if (pl.len[b] == 0) p.notes[(p.batch + b) * p.Hk + hk] = make_int2(0, 0);
+      }
     const int w = warp >> 2, row = threadIdx.x & 127, row0 = row & ~31;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem_S + lane_base + w * 128, to = tmem_O + lane_base + w * kSpD;
