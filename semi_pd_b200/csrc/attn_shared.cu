@@ -16,7 +16,7 @@
 // ("parts"): by batch row where the CTA has the item's first tile, else in a place of the CTA's own, since of all its items
 // only the first can have begun earlier.  A second kernel joins them.
 // (As two kernels, the shared keys' and attn_decode.cu's for the own ones: 64 requests of 130 own tokens behind 8192 shared
-// ones, 32 / 8 heads, 48.6 us, and 34.0 so; each kernel starts for 5 us without using the memory.)
+// ones, 32 / 8 heads, 48.6 us, and 31.7 so; each kernel starts for 5 us without using the memory.)
 //
 //   warps 0-3 / 4-7  softmax of query tile 0 / 1: one thread per query row; P goes back into the TMEM columns of its S
 //   warp 8, warp 9   K / V loader: a ring of four 128 x 128 tiles, K_j V_j K_{j+1} ..., by TMA (single rows where a
@@ -25,7 +25,7 @@
 // Over shared keys a tile is taken in two halves of 64 keys, so that a warpgroup's softmax of one half runs beside the MMAs of
 // the other.  An item over own keys has the few query heads of one kv head as its rows; it is computed the other way round,
 // S^T = K Q^T and O^T = V^T P^T, with a thread per key and P^T in shared memory, as in attn_decode.cu.  (With queries in the
-// rows there too, one warp did all the exponentials: 160 requests of 132 own tokens, 32 / 32 heads, 276 us, and 86 now.)
+// rows there too, one warp did all the exponentials: 160 requests of 132 own tokens, 32 / 32 heads, 276 us, and 81 now.)
 // The items go to the two warpgroups in turn, and each has a loader, an issuer and a ring of three tiles to itself (its half of
 // the ring above and the memory of its query tile): with one ring for both, an item waited for the one before in every role
 // (229 us).
@@ -71,7 +71,12 @@ constexpr float kSpRescale = 8.f;  // exponent of 2 that a score may pass the re
 // What the list's entries cost, in about 570 clk: a key tile for two query tiles, for one, over own keys (a tile of few keys is
 // bound by the chain of its steps, not by its bytes); an item's start and end.
 constexpr int kCostPair = 7, kCostOne = 4, kCostOwnTile = 4, kCostOwnLeast = 3, kCostShared = 24, kCostOwn = 1;
-constexpr int kCostMin = 8;  // of a CTA
+// of a range that begins among shared items for two query tiles (256 rows of output to keep).  64 requests behind 8192 tokens,
+// 130 of their own, 32 / 8 heads: 33.3 us with 0, 32.2 with 16, 31.7 with 20; 160 behind 1408, 32 / 32: 84.7, 83.2, 81.1.  For
+// items of one query tile 0 and 16 take 38.6 and 41.2 (8 groups of 6).  Half a mean range at most: where there is little to do,
+// few such parts are written at once (128 requests behind 128 tokens, 8 / 1 heads: 16.6 with 0, 22.5 with 20).
+constexpr int kCostPart = 20;
+constexpr int kCostMin = 7;    // of a range, and one more
 
 struct SharedParams {
   const int32_t* req_to_token;
@@ -116,8 +121,27 @@ __device__ __forceinline__ int sp_own_cost(int len) {
 struct SpRange {
   int begin, end;  // this CTA's part of the list
   int shared;      // cost of all items over shared keys, which come first
-  int per;
+  int per, per_shared, shared_ctas;  // length of a range: the first shared_ctas ones, which begin among the shared items; others
   __device__ __forceinline__ bool own() const { return begin < end && end > shared; }  // reaches into the items over own keys
+  __device__ __forceinline__ int start(int cta) const { return min(cta, shared_ctas) * per_shared + max(0, cta - shared_ctas) * per; }
+  __device__ __forceinline__ int cta(int u) const {
+    const int first = shared_ctas * per_shared;
+    return u < first ? u / per_shared : shared_ctas + (u - first) / per;
+  }
+  // Every CTA costs the same: a range among the shared items also `part` for a part's beginning and end.  With n ranges of x over
+  // A of them, (N - n) of x + part over the rest, n x = A:  N x^2 + (N part - total) x = A part.
+  __device__ __forceinline__ void divide(int total, int ctas, int part) {
+    const float N = ctas, b = N * part - total;
+    const float x = part > 0 ? (sqrtf(b * b + 4.f * N * part * shared) - b) / (2.f * N) : total / N;
+    per_shared = max(kCostMin, static_cast<int>(x));
+    do {  // (rounding, and shared items that leave the last of their ranges partly empty)
+      ++per_shared;
+      per = per_shared + part;
+      shared_ctas = (shared + per_shared - 1) / per_shared;
+    } while (shared_ctas > ctas || start(ctas) < total);
+    begin = min(total, start(blockIdx.x));
+    end = min(total, start(blockIdx.x + 1));
+  }
 };
 
 // The plan, by all threads of the CTA, from the groups' offsets and the lengths.  It stands before the CTA's first load, so it
@@ -194,7 +218,7 @@ __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl
     }
   }
   if (lane == 31) pl.sums[warp] = make_int2(incl, own_incl);
-  __syncthreads();
+  const bool pairs = __syncthreads_or(cost > 0 && pl.count[g] > p.mpt);
   SpRange r;
   r.shared = 0;
   int before = incl - cost, own_before = own_incl - own, all_own = 0;
@@ -214,9 +238,7 @@ __device__ __forceinline__ SpRange sp_plan(const SharedParams& p, SharedPlan& pl
   }
   if (g == 0) pl.unit0[p.groups] = r.shared;
   const int total = r.shared + all_own;
-  r.per = max(kCostMin, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  r.begin = min(total, r.per * static_cast<int>(blockIdx.x));
-  r.end = min(total, r.begin + r.per);
+  r.divide(total, gridDim.x, pairs ? min(kCostPart, total / (2 * static_cast<int>(gridDim.x))) : 0);
   // where the range begins among the own items: found by the thread whose rows it is in
   int rem = max(r.begin, r.shared) - r.shared - own_before;
   if (r.own() && rem >= 0 && rem < own) {
@@ -264,7 +286,7 @@ struct SpItem {
   // for the join, see SharedParams; by the CTA that has the item's first tile
   __device__ __forceinline__ int2 note(const SpRange& r, bool halves, int row) const {
     const int c0 = blockIdx.x, last = s0 + (tiles - 1) * cost;
-    return make_int2(c0, (last < r.end ? 1 : last / r.per - c0 + 1) | (halves ? 1 << 15 : 0) | row << 16);
+    return make_int2(c0, (last < r.end ? 1 : r.cta(last) - c0 + 1) | (halves ? 1 << 15 : 0) | row << 16);
   }
 };
 
@@ -1116,7 +1138,7 @@ static int64_t part_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
 
 // Whether reading the shared keys once is the faster way, from what the host knows: as if all requests were in groups of one
 // size that share max_shared keys.  The weights fit 325 shapes measured both ways (2 to 256 requests in 1 to 32 groups, 128 to
-// 16384 shared tokens, 64 own, bf16, four head layouts): the choice takes 0.6% longer than the better way on average, 19% at
+// 16384 shared tokens, 64 own, bf16, four head layouts): the choice takes 0.5% longer than the better way on average, 24% at
 // worst.  A tile of 128 shared keys costs an SM 1.2 here and each member 0.7 there (mostly from L2); requests that there are cut
 // over many SMs cost 0.4 per part and query head in their merge; the longer start, the join and the shorter ranges cost 6 here,
 // and 0.0008 per request and kv head.
