@@ -11,8 +11,8 @@
 // no query of the shared part needs a mask.
 //
 // ONE list of work: items (group, kv head, pair of query tiles) over the shared keys, then items (request, kv head) over the own
-// ones, each with its key tiles one after another.  Tiles and items count what they cost, and every CTA takes an equal range
-// of the list, so CTAs at the tensor cores' limit run beside CTAs at the memory's.  An item's sums are kept per CTA
+// ones, each with its key tiles one after another.  Tiles and items count what they cost, and every CTA takes a range of the
+// list that costs the same, so CTAs at the tensor cores' limit run beside CTAs at the memory's.  An item's sums are kept per CTA
 // ("parts"): by batch row where the CTA has the item's first tile, else in a place of the CTA's own, since of all its items
 // only the first can have begun earlier.  A second kernel joins them.
 // (As two kernels, the shared keys' and attn_decode.cu's for the own ones: 64 requests of 130 own tokens behind 8192 shared
@@ -33,6 +33,10 @@
 // sums the rounded P, so that the rounding of a P that outweighs the others cancels.  The reference maximum is raised when a
 // score passes it by 2^8 (O is then rescaled in TMEM), so a P is at most 2^8.
 // Every mbarrier wait is bounded (see mbar_wait_bounded, spd_wait_status).
+// Measured, both kernels, caches cold: 64 requests of 130 own tokens behind 8192, 32 / 8 heads, 33 us (68.5 MB: 10.4 at the rate
+// of a copy); 8 groups of 6, 134 behind 2944, 40 / 8 heads, 39 us (114 MB: 17.4); 160 of 132 behind 1408, 32 / 32 heads, 82 us
+// (370 MB: 56); 256 of 300 behind 32768, 64 / 8 heads, 328 - 412 us as the power cap has it (277 GFLOP: 0.67 - 0.85 PFLOP/s).
+// Start, the parts' way to memory and the join are 10 of the 33 us.
 // The roles run side by side, so their code together competes for the instruction cache: long waits are out of the way, and
 // loops are not unrolled where that gains nothing.  (With the waits unrolled in place the kernel had 217 KB; 48 requests of 134
 // own tokens in 8 groups took 46.3 us, with 126 KB 38.9; 256 query rows by 32768 keys 369 and 337.  The MMAs over own keys

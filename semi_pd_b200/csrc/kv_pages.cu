@@ -4,6 +4,8 @@
 // Nothing is computed: a call moves 2 x rows x bytes of a token and should take what those bytes take.  A block owns a few
 // rows of one plane: their slots are looked up once, in parallel, into shared memory, and its threads then walk the rows'
 // 16-byte pieces as one list, kKvUnroll of them loaded before the first is stored.
+// Measured: 12001 latent rows in 27 layers (747 MB) copied in 118 us, 6.3 TB/s; 16 requests' fp32 rows compacted (1.89 GB) in 292,
+// 6.5; 8 parents with 16 children each forked (568 MB, nearly all of it written) in 110, 5.2.  A plain copy has 6.56.
 #include "common.cuh"
 #include "prefill_tiles.cuh"
 #include "ptx.cuh"
