@@ -299,6 +299,7 @@ int spd_attn_decode_paged_own(void* out, const void* q, const void* k_pool, cons
  * shared_lens[g] positions; max_shared_len is no less than any of those; the pools have pool_slots rows.  The result is
  * spd_attn_decode_paged's: every row of req_to_token is complete, rows of no group stand alone, seq_lens[b] counts the shared
  * tokens too, and a request of length 0 gets zeros.  The shared part of a group is read once for all of its queries.
+ * Scores of -inf weigh nothing; a NaN or +inf among a request's scores, or nothing but -inf, makes its output NaN.
  * head_dim 128, at most 8 query heads per kv head; batches of more than 1024 requests or 256 groups are read as
  * spd_attn_decode_paged reads them.
  * Workspace: spd_attn_decode_shared_workspace_bytes(), zeroed once before its first use (each call leaves its counters at

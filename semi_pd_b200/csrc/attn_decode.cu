@@ -41,6 +41,7 @@
 // (tile::gather4, 4 rows x 128 B per instruction, was built and measured: correct,
 // but ~1 instruction per 27 clk per SM -> 36 GB/s per SM, below the cp.async gather's 47.)
 #include <cuda.h>
+#include <float.h>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -464,7 +465,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       const int unit0 = u_end - c.left - c.tile;  // unit of the item's tile 0
       float m_ref[kDcMaxGroup], l_thr[kDcMaxGroup];
 #pragma unroll
-      for (int g = 0; g < kDcMaxGroup; ++g) { m_ref[g] = L > 0 ? -INFINITY : 0.f; l_thr[g] = 0.f; }
+      for (int g = 0; g < kDcMaxGroup; ++g) { m_ref[g] = -FLT_MAX; l_thr[g] = 0.f; }  // (-inf - -inf is not -inf)
       int tile = tile0;
       for (bool end = false; !end; ++t) {
         end = c.ends();
@@ -500,8 +501,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
           for (int g = 0; g < kDcMaxGroup; ++g) {
             const float mt = fmaxf(fmaxf(red[g], red[8 + g]), fmaxf(red[16 + g], red[24 + g]));
-            const float m_new = fmaxf(m_ref[g], mt);  // finite: every tile has >= 1 valid token
-            alpha[g] = (m_ref[g] == -INFINITY) ? 0.f : fast_exp2(m_ref[g] - m_new);
+            const float m_new = fmaxf(m_ref[g], mt);  // -FLT_MAX as long as all scores are -inf
+            alpha[g] = fast_exp2(m_ref[g] - m_new);
             l_thr[g] *= alpha[g];
             m_ref[g] = m_new;
           }
@@ -565,7 +566,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         T* dst = reinterpret_cast<T*>(p.out) + ib * p.out_stride + static_cast<int64_t>(ihk) * G * kDcD + tid;
 #pragma unroll
         for (int g = 0; g < kDcMaxGroup; ++g)
-          if (g < G) dst[g * kDcD] = from_f32<T>(l_tot[g] > 0.f ? o[g] / l_tot[g] : 0.f);
+          if (g < G) dst[g * kDcD] = from_f32<T>(L > 0 ? o[g] / l_tot[g] : 0.f);  // (NaN where no score has any weight)
         softmax_bar();  // `red` is rewritten by the next item
       } else {
         const int64_t part = static_cast<int64_t>(2 * cta + (tile0 > 0 ? 0 : 1)) * G;
@@ -600,7 +601,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
               if (g < G) {
                 const float2 ml = __ldcg(reinterpret_cast<const float2*>(&p.ml_part[(at(i) + g) * 2]));
                 const float ov = __ldcg(&p.o_part[(at(i) + g) * kDcD + tid]);
-                const float wgt = ml.y > 0.f ? fast_exp2(ml.x - M[g]) : 0.f;
+                const float wgt = ml.y != 0.f ? fast_exp2(ml.x - M[g]) : 0.f;
                 num[g] += wgt * ov;
                 den[g] += wgt * ml.y;
               }
@@ -608,7 +609,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           T* dst = reinterpret_cast<T*>(p.out) + ib * p.out_stride + static_cast<int64_t>(ihk) * G * kDcD + tid;
 #pragma unroll
           for (int g = 0; g < kDcMaxGroup; ++g)
-            if (g < G) dst[g * kDcD] = from_f32<T>(den[g] > 0.f ? num[g] / den[g] : 0.f);
+            if (g < G) dst[g * kDcD] = from_f32<T>(num[g] / den[g]);  // (only requests with keys are cut)
           if (tid == 0) p.counters[ib * p.Hk + ihk] = 0;  // re-arm for the next launch
         }
         softmax_bar();  // flag_slot / red are reused by the next item

@@ -42,6 +42,7 @@
 // own tokens in 8 groups took 46.3 us, with 126 KB 38.9; 256 query rows by 32768 keys 369 and 337.  The MMAs over own keys
 // unrolled: 352.)
 #include <cuda.h>
+#include <float.h>
 #include <limits.h>
 
 #include "common.cuh"
@@ -952,7 +953,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       float m_ref[kSpMaxGroup], l_thr[kSpMaxGroup];
 #pragma unroll
       for (int g = 0; g < kSpMaxGroup; ++g) {
-        m_ref[g] = -INFINITY;
+        m_ref[g] = -FLT_MAX;  // as long as all scores are -inf, which weigh nothing: -inf - -inf is not -inf
         l_thr[g] = 0.f;
       }
       for (int j = 0; j < it.n; ++j, ++u) {
@@ -980,7 +981,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const float4 x = red[(rounds & 1) * kSpMaxGroup + g];
             const float mx = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
             if (mx > m_ref[g] + kSpRescale) {
-              alpha[g] = m_ref[g] == -INFINITY ? 0.f : fast_exp2(m_ref[g] - mx);
+              alpha[g] = fast_exp2(m_ref[g] - mx);
               l_thr[g] *= alpha[g];
               m_ref[g] = mx;
               raise = true;
@@ -1059,6 +1060,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
 // out = the join of a query head's parts, over the shared and over the own keys.  A warp per row of the output, four columns a
 // lane; a lane looks at one part's (m, l).  Latency bounds it, so a row's loads are requested before the first is waited for.
+// A part of sum 0 has scores of -inf only, or no tile at all, and takes no part; a sum that is not a number does.  0 / 0 where
+// no part is left, 0 where there was none.
 constexpr int kSjWarps = 8;
 constexpr int kSjParts = 8;  // of a row at a time
 template <typename T>
@@ -1102,10 +1105,10 @@ attn_shared_join_kernel(T* __restrict__ out, int64_t out_stride, const __grid_co
           v[k] = __ldcg(reinterpret_cast<const float4*>((first ? p.o_first : p.o_next) + at * kSpD) + lane);
         }
       if (j0 == 0) {
-        const float top = fmaxf(M, warp_max(ml.y > 0.f ? ml.x : -INFINITY));
-        const float keep = den > 0.f ? fast_exp2(M - top) : 0.f;
-        wt = ml.y > 0.f ? fast_exp2(ml.x - top) : 0.f;
-        den = den * keep + warp_sum(wt * ml.y);
+        const float top = fmaxf(M, warp_max(ml.y != 0.f ? ml.x : -INFINITY));
+        const float keep = den != 0.f ? fast_exp2(M - top) : 0.f;
+        wt = ml.y != 0.f ? fast_exp2(ml.x - top) : -1.f;
+        den = den * keep + warp_sum(ml.y != 0.f ? wt * ml.y : 0.f);
         acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
         M = top;
       }
@@ -1113,7 +1116,7 @@ attn_shared_join_kernel(T* __restrict__ out, int64_t out_stride, const __grid_co
       for (int k = 0; k < kSjParts; ++k)
         if (j0 + k < here) {
           const float f = __shfl_sync(0xffffffffu, wt, j0 + k);
-          if (f != 0.f) {  // (a part of sum 0 has no columns)
+          if (!(f < 0.f)) {  // (a part of sum 0 may have no columns)
             acc.x = fmaf(f, v[k].x, acc.x);
             acc.y = fmaf(f, v[k].y, acc.y);
             acc.z = fmaf(f, v[k].z, acc.z);
@@ -1122,7 +1125,7 @@ attn_shared_join_kernel(T* __restrict__ out, int64_t out_stride, const __grid_co
         }
     }
   }
-  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const float inv = parts > 0 ? 1.f / den : 0.f;
   *reinterpret_cast<uint2*>(out + b * out_stride + static_cast<int64_t>(h) * kSpD + lane * 4) =
       make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
 }
