@@ -3,7 +3,9 @@
 //
 // Nothing is computed: a call moves 2 x rows x bytes of a token and should take what those bytes take.  A block owns a few
 // rows of one plane: their slots are looked up once, in parallel, into shared memory, and its threads then walk the rows'
-// 16-byte pieces as one list, kKvUnroll of them loaded before the first is stored.
+// 16-byte pieces as one list, kKvUnroll of them loaded before the first is stored.  Rows of more than kKvPart bytes (a request's
+// recurrent state is one row) are taken in parts, each as a plane of its own, so that they too are spread over the SMs (one
+// request's states of 2 MB in 24 layers, 101 MB: 16.2 us, 6.2 TB/s).
 // Measured: 12001 latent rows in 27 layers (747 MB) copied in 118 us, 6.3 TB/s; 16 requests' fp32 rows compacted (1.89 GB) in 292,
 // 6.5; 8 parents with 16 children each forked (568 MB, nearly all of it written) in 110, 5.2.  A plain copy has 6.56.
 #include "common.cuh"
@@ -16,6 +18,8 @@ constexpr int kKvThreads = 256;
 constexpr int kKvRows = 64;    // rows of a block at most
 constexpr int kKvUnroll = 4;
 constexpr int kKvSets = 64;
+constexpr int kKvPart = 32768;       // bytes of a row that a block takes at most, a multiple of any piece
+constexpr int64_t kKvRow = 1 << 30;  // of a row
 // Children of a fork whose rows a block stores after loading them once: those of one parent and length, which stand together
 // in the lists, up to a multiple of kKvKin.  They are the fastest index of the grid, so that the next block of the parent finds
 // its rows in L2.  us with 1 / 2 / 4: 8 parents of 16 children, 567 MB at least, 138 / 104 / 107; 64 parents of one child
@@ -28,10 +32,11 @@ struct KvSet {
   int64_t rows;       // slots
   int64_t row_bytes;
   int first;          // planes of the sets before
-  uint32_t pieces_m, pieces_s;  // division by the pieces of a row
+  int parts;          // planes that a buffer's rows are taken in
+  uint32_t pieces_m, pieces_s;  // division by the pieces of a row, or of a part
 };
 struct KvPlanes {
-  int sets, planes;
+  int sets, planes;   // (parts count as planes)
   KvSet set[kKvSets];
 };
 
@@ -173,8 +178,11 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
   int si = 0;
   while (si + 1 < pl.sets && at.plane >= pl.set[si + 1].first) ++si;
   const KvSet& set = pl.set[si];
-  const int pieces = static_cast<int>(set.row_bytes / sizeof(V));
-  char* plane = set.base + (at.plane - set.first) * set.stride;
+  const int rel = at.plane - set.first, buffer = set.parts == 1 ? rel : rel / set.parts, part = rel - buffer * set.parts;
+  const int pieces = static_cast<int>((set.parts == 1 ? set.row_bytes : static_cast<int64_t>(kKvPart)) / sizeof(V));
+  // (the last part is shorter)
+  const int last = static_cast<int>(min(static_cast<int64_t>(pieces), (set.row_bytes - static_cast<int64_t>(part) * kKvPart) / static_cast<int64_t>(sizeof(V))));
+  char* plane = set.base + buffer * set.stride + static_cast<int64_t>(part) * kKvPart;
   __syncthreads();
   const int total = count * pieces;
   for (int i0 = threadIdx.x; i0 < total; i0 += kKvThreads * kKvUnroll) {
@@ -188,7 +196,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
         const int r = fastdiv(i, set.pieces_m, set.pieces_s);
         const int64_t s = s_src[r];
         piece[k] = i - r * pieces;
-        if (s >= 0 && s < set.rows) {
+        if (s >= 0 && s < set.rows && piece[k] < last) {
           row[k] = r;
           const V* from = reinterpret_cast<const V*>(plane + s * set.row_bytes) + piece[k];
           v[k] = Rows::kChildren ? *from : __ldcs(from);  // (a parent's rows are read again)
@@ -222,8 +230,9 @@ static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, 
   for (int i = 0; i < num_sets; ++i) {
     const spd_kv_planes_t& s = sets[i];
     SPD_REQUIRE(s.base && s.planes > 0 && s.rows > 0 && s.row_bytes > 0 && s.plane_stride >= 0, SPD_E_BADARG, "%s: bad plane set", fn);
-    SPD_REQUIRE(s.row_bytes % 2 == 0 && s.row_bytes <= (1 << 20) && s.plane_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(s.base) & 1) == 0,
-                SPD_E_ALIGN, "%s: rows of an even number of bytes, 1 MB at most", fn);
+    SPD_REQUIRE(s.row_bytes % 2 == 0 && s.plane_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(s.base) & 1) == 0, SPD_E_ALIGN,
+                "%s: rows of an even number of bytes", fn);
+    SPD_REQUIRE(s.row_bytes <= kKvRow, SPD_E_SHAPE, "%s: rows of 1 GB at most", fn);
     const uint64_t bits = reinterpret_cast<uintptr_t>(s.base) | s.row_bytes | s.plane_stride;
     while (bits % piece) piece >>= 1;
     pl.set[i].base = static_cast<char*>(s.base);
@@ -231,11 +240,14 @@ static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, 
     pl.set[i].rows = s.rows;
     pl.set[i].row_bytes = s.row_bytes;
     pl.set[i].first = pl.planes;
-    pl.planes += s.planes;
-    SPD_REQUIRE(pl.planes < 65535, SPD_E_SHAPE, "%s: too many planes", fn);
+    pl.set[i].parts = static_cast<int>((s.row_bytes + kKvPart - 1) / kKvPart);
+    const int64_t planes = pl.planes + static_cast<int64_t>(s.planes) * pl.set[i].parts;
+    SPD_REQUIRE(planes < 65535, SPD_E_SHAPE, "%s: too many planes (a row of more than %d bytes counts once for every %d)", fn, kKvPart,
+                kKvPart);
+    pl.planes = static_cast<int>(planes);
   }
   for (int i = 0; i < num_sets; ++i)
-    fastdiv_magic(static_cast<uint32_t>(pl.set[i].row_bytes / piece), pl.set[i].pieces_m, pl.set[i].pieces_s);
+    fastdiv_magic(static_cast<uint32_t>((pl.set[i].parts == 1 ? pl.set[i].row_bytes : kKvPart) / piece), pl.set[i].pieces_m, pl.set[i].pieces_s);
   return 0;
 }
 
@@ -243,6 +255,7 @@ static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, 
 static int kv_rows_per_block(const KvPlanes& pl, int64_t rows) {
   int64_t bytes = 0;
   for (int i = 0; i < pl.sets; ++i) bytes = bytes > pl.set[i].row_bytes ? bytes : pl.set[i].row_bytes;
+  if (bytes > kKvPart) bytes = kKvPart;
   int64_t per = (32768 + bytes - 1) / bytes;
   const int64_t spread = rows * pl.planes / (4 * device_sm_count_cached()), least = (4096 + bytes - 1) / bytes;
   if (per > spread) per = spread;
