@@ -374,6 +374,11 @@ class TokenToKVPoolAllocator:
         np.add.at(self._used, (slots - 1) // R, 1)
         return slots, old
 
+    def restore_req(self, req_pool_idx: int, runs: List[int], n: int) -> None:
+        """Takes a rebuild_req back: the request holds its n tokens in the runs that it had."""
+        new, self._req_runs[req_pool_idx], self._req_len[req_pool_idx] = self._req_runs[req_pool_idx], runs, n
+        self._let_go(new)
+
     def release_runs(self, runs: List[int]) -> None:
         self._let_go(runs)
 
@@ -545,7 +550,7 @@ def fork_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator:
                  n: int) -> Optional[List[int]]:
     """n continuations of a request: new request slots whose page-table rows share the parent's whole runs, its last, partial run
     copied for each (and its recurrent state, where the model has one).  On the current stream.  → the request slots, or None
-    when slots or runs do not suffice."""
+    when slots or runs do not suffice.  Where a copy is refused, everything is as it was."""
     children = req_to_token_pool.alloc(n)
     if children is None:
         return None
@@ -560,15 +565,23 @@ def fork_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator:
     length, R = allocator.req_len(parent), allocator.run_len
     if n == 0:
         return children
-    lists = np.concatenate([np.full(n, parent), np.asarray(children), np.full(n, length), tails]).astype(np.int64)
-    parents_d, children_d, lens_d, tails_d = allocator._ring.stage(lists, allocator.device).split(n)
-    ops.kv_fork(kv_pool.planes, req_to_token_pool.req_to_token, parents_d, children_d, lens_d, tails_d, R)
-    rest = length % R > 0
-    kv_pool.fork_rows(parent, children, allocator._req_runs[parent][length // R] if rest else None,
-                      [allocator._req_runs[c][-1] for c in children] if rest else [],
-                      lambda rows: allocator._ring.stage(np.asarray(rows, dtype=np.int64), allocator.device))
-    allocator.copying()
-    req_to_token_pool.copying()
+    done = False
+    try:
+        lists = np.concatenate([np.full(n, parent), np.asarray(children), np.full(n, length), tails]).astype(np.int64)
+        parents_d, children_d, lens_d, tails_d = allocator._ring.stage(lists, allocator.device).split(n)
+        ops.kv_fork(kv_pool.planes, req_to_token_pool.req_to_token, parents_d, children_d, lens_d, tails_d, R)
+        rest = length % R > 0
+        kv_pool.fork_rows(parent, children, allocator._req_runs[parent][length // R] if rest else None,
+                          [allocator._req_runs[c][-1] for c in children] if rest else [],
+                          lambda rows: allocator._ring.stage(np.asarray(rows, dtype=np.int64), allocator.device))
+        done = True
+    finally:
+        allocator.copying()
+        req_to_token_pool.copying()
+        if not done:  # what was taken goes back, once the copies that were launched have run
+            for c in children:
+                allocator.free_req(c)
+            req_to_token_pool.free(children)
     return children
 
 
@@ -576,7 +589,7 @@ def compact_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocat
                     keep: Sequence[int]) -> bool:
     """The request goes on with its tokens at the positions `keep` only (ascending, at least one), copied to new runs; keys
     stay rotated as they are.  On the current stream; what the caller knows of its length is its own.  False when the free
-    runs do not suffice."""
+    runs do not suffice.  Where the copy is refused, the request is as it was."""
     why = kv_pool.compact_refusal()
     if why:
         raise NotImplementedError(f"compact: {why}")
@@ -589,10 +602,16 @@ def compact_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocat
         return False
     slots, old = new
     n = int(pos.size)
-    lists = allocator._ring.stage(np.concatenate([pos, slots, [req, 0, n]]).astype(np.int64), allocator.device)
-    ops.kv_compact(kv_pool.planes, req_to_token_pool.req_to_token, lists[2 * n:2 * n + 1], None, lists[:n], lists[2 * n + 1:],
-                   lists[n:2 * n])
-    allocator.copying()
+    done = False
+    try:
+        lists = allocator._ring.stage(np.concatenate([pos, slots, [req, 0, n]]).astype(np.int64), allocator.device)
+        ops.kv_compact(kv_pool.planes, req_to_token_pool.req_to_token, lists[2 * n:2 * n + 1], None, lists[:n], lists[2 * n + 1:],
+                       lists[n:2 * n])
+        done = True
+    finally:
+        allocator.copying()
+        if not done:  # (the page table is written last)
+            allocator.restore_req(req, old, length)
     allocator.release_runs(old)
     return True
 
