@@ -610,6 +610,7 @@ def compact_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocat
         done = True
     finally:
         allocator.copying()
+        req_to_token_pool.copying()
         if not done:  # (the page table is written last)
             allocator.restore_req(req, old, length)
     allocator.release_runs(old)
