@@ -79,6 +79,8 @@ class ModelWorkerBatch:
     # decode
     decode_seq_lens: Optional[torch.Tensor] = None
     shared_prefix: Optional[SharedPrefix] = None
+    # [bs] int64: how far every request's positions are ahead of its cache's length (compacted requests)
+    position_offsets: Optional[torch.Tensor] = None
     # extend
     extend_num_tokens: Optional[int] = None
     extend_seq_lens: Optional[List[int]] = None
@@ -122,6 +124,7 @@ class ForwardBatch:
     positions: torch.Tensor = None
     decode_seq_lens_cpu: Optional[torch.Tensor] = None
     shared_prefix: Optional[SharedPrefix] = None
+    position_offsets: Optional[torch.Tensor] = None
 
     extend_num_tokens: Optional[int] = None
     extend_seq_lens: Optional[torch.Tensor] = None       # int32, device
@@ -165,6 +168,9 @@ class ForwardBatch:
         if ret.forward_mode.is_decode():
             if ret.positions is None:
                 ret.positions = ops.clamp_position(batch.seq_lens)
+                ret.position_offsets = batch.position_offsets
+                if ret.position_offsets is not None:
+                    ret.positions += ret.position_offsets
             if ret.decode_seq_lens_cpu is None:
                 ret.decode_seq_lens_cpu = batch.decode_seq_lens
             if batch.shared_prefix is not None and model_runner.attn_backend.shares_prefix(ret.batch_size, batch.shared_prefix):

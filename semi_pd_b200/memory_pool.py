@@ -587,9 +587,10 @@ def fork_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator:
 
 def compact_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator: TokenToKVPoolAllocator, req: int,
                     keep: Sequence[int]) -> bool:
-    """The request goes on with its tokens at the positions `keep` only (ascending, at least one), copied to new runs; keys
-    stay rotated as they are.  On the current stream; what the caller knows of its length is its own.  False when the free
-    runs do not suffice.  Where the copy is refused, the request is as it was."""
+    """The request goes on with its tokens at `keep` only (ascending indices into what it has cached, at least one), copied to new
+    runs.  Keys stay rotated as they are, so the next tokens' positions go on where they were: for a request in a batch
+    ScheduleBatch.compact_req carries that (ModelWorkerBatch.position_offsets).  On the current stream; what the caller knows
+    of its length is its own.  False when the free runs do not suffice.  Where the copy is refused, the request is as it was."""
     why = kv_pool.compact_refusal()
     if why:
         raise NotImplementedError(f"compact: {why}")

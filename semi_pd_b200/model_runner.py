@@ -278,7 +278,7 @@ class CudaGraphRunner:
 
     def can_run(self, forward_batch: ForwardBatch) -> bool:
         return (forward_batch.forward_mode.is_decode() and forward_batch.batch_size <= self.max_bs
-                and forward_batch.shared_prefix is None)
+                and forward_batch.shared_prefix is None and forward_batch.position_offsets is None)
 
     def capture(self):
         set_current_comm(self.model_runner.tp_comm)

@@ -11,13 +11,13 @@ from __future__ import annotations
 
 import copy
 import dataclasses
-from typing import List, Optional
+from typing import List, Optional, Sequence
 
 import torch
 
 from . import ops
 from .forward_batch_info import ForwardMode, ModelWorkerBatch, SharedPrefix
-from .memory_pool import ReqToTokenPool, TokenToKVPoolAllocator, fork_request
+from .memory_pool import ReqToTokenPool, TokenToKVPoolAllocator, compact_request, fork_request
 
 _bid = 0
 
@@ -48,6 +48,8 @@ class Req:
         self.finished_reason: Optional[str] = None
         # tokens whose computation has been launched (>= len(output_ids) under the overlap loop)
         self.launched_tokens = 0
+        # tokens that compactions took out of the cache: the next one's position is that many ahead of the cache's length
+        self.dropped_tokens = 0
         # timing (host clock, seconds)
         self.arrival_time = arrival_time
         self.first_token_time: Optional[float] = None
@@ -87,6 +89,7 @@ class Req:
         self.extend_input_len = 0
         self.is_retracted = True
         self.req_pool_idx = None
+        self.dropped_tokens = 0
 
 
 class ScheduleBatch:
@@ -111,6 +114,7 @@ class ScheduleBatch:
         self.extend_num_tokens = None
         self.decoding_reqs = None
         self._shared = None   # (groups of the last step, SharedPrefix)
+        self._compacted = False   # some request may have dropped tokens
 
     @classmethod
     def init_new(cls, reqs, req_to_token_pool, token_to_kv_pool_allocator, device=None):
@@ -147,6 +151,8 @@ class ScheduleBatch:
         self.forward_mode = ForwardMode.EXTEND
         bs = len(self.reqs)
         reqs = self.reqs
+        if any(r.dropped_tokens for r in reqs):
+            raise NotImplementedError("a request whose cache was compacted takes no further prompt tokens")
         input_ids = [r.fill_ids[len(r.prefix_indices):] for r in reqs]
         extend_num_tokens = sum(len(ids) for ids in input_ids)
         seq_lens = [len(r.fill_ids) for r in reqs]
@@ -272,6 +278,29 @@ class ScheduleBatch:
             self.output_ids = self.output_ids[idx]
         return children
 
+    def compact_req(self, index: int, keep: Sequence[int]) -> bool:
+        """Request `index` of a decode batch goes on, between two steps, with its cached tokens at `keep` only (ascending indices
+        into what is cached; memory_pool.compact_request).  Its next tokens stand at the positions that they would have had:
+        the keys that are left are rotated for those.  A step with such a request runs without its CUDA graph.  False when the
+        cache does not suffice."""
+        req = self.reqs[index]
+        if req.finished():
+            raise RuntimeError(f"compact: request {req.rid} has finished")
+        if not compact_request(self.token_to_kv_pool_allocator.get_kvcache(), self.req_to_token_pool,
+                               self.token_to_kv_pool_allocator, req.req_pool_idx, keep):
+            return False
+        req.dropped_tokens += self.seq_lens_host[index] - len(keep)
+        self.seq_lens_host[index] = len(keep)
+        self.seq_lens_sum = sum(self.seq_lens_host)
+        self.seq_lens = self._h2d(self.seq_lens_host, torch.int64)  # (a new one: a launched step may read the old)
+        self._compacted = True
+        return True
+
+    def _position_offsets(self) -> Optional[torch.Tensor]:
+        dropped = [r.dropped_tokens for r in self.reqs] if self._compacted else []
+        self._compacted = any(dropped)
+        return self._h2d(dropped, torch.int64) if self._compacted else None
+
     def _shared_prefix(self) -> Optional[SharedPrefix]:
         groups = self.token_to_kv_pool_allocator.shared_prefix([r.req_pool_idx for r in self.reqs])
         if groups is None:
@@ -302,6 +331,7 @@ class ScheduleBatch:
         self.seq_lens_sum = sum(self.seq_lens_host)
 
     def merge_batch(self, other: "ScheduleBatch"):
+        self._compacted |= other._compacted
         if self.is_empty():
             self.reqs = list(other.reqs)
             self.req_pool_indices, self.seq_lens = other.req_pool_indices, other.seq_lens
@@ -326,6 +356,7 @@ class ScheduleBatch:
             req_pool_indices=self.req_pool_indices, seq_lens=self.seq_lens,
             out_cache_loc=self.out_cache_loc, seq_lens_sum=self.seq_lens_sum,
             shared_prefix=None if extend else self._shared_prefix(),
+            position_offsets=None if extend else self._position_offsets(),
             extend_num_tokens=self.extend_num_tokens if extend else None,
             extend_seq_lens=self.extend_lens if extend else None,
             extend_prefix_lens=self.prefix_lens if extend else None,
