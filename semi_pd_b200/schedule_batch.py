@@ -50,6 +50,7 @@ class Req:
         self.launched_tokens = 0
         # tokens that compactions took out of the cache: the next one's position is that many ahead of the cache's length
         self.dropped_tokens = 0
+        self.num_forks = 0   # continuations forked off (their rids are numbered)
         # timing (host clock, seconds)
         self.arrival_time = arrival_time
         self.first_token_time: Optional[float] = None
@@ -252,8 +253,13 @@ class ScheduleBatch:
     def fork_req(self, index: int, n: int) -> Optional[List[Req]]:
         """n more continuations of request `index` of a decode batch, between two steps: requests like it (prompt and output
         so far) right behind it in the batch, so that neighbours share a prefix.  Their next input token is the parent's until
-        the caller writes another into `output_ids`.  None when request slots or cache do not suffice."""
+        the caller writes another into `output_ids` (and into their own lists).  What the parent's launched steps gave has to
+        have been read: the children take over its output as it is known.  None when request slots or cache do not suffice."""
         parent = self.reqs[index]
+        if parent.finished():
+            raise RuntimeError(f"fork: request {parent.rid} has finished")
+        if parent.launched_tokens > len(parent.output_ids):
+            raise RuntimeError(f"fork: request {parent.rid} has launched steps whose results are unread; drain them first")
         slots = fork_request(self.token_to_kv_pool_allocator.get_kvcache(), self.req_to_token_pool,
                              self.token_to_kv_pool_allocator, parent.req_pool_idx, n)
         if slots is None:
@@ -261,12 +267,14 @@ class ScheduleBatch:
         children = []
         for k, slot in enumerate(slots):
             req = copy.copy(parent)
-            req.rid = f"{parent.rid}.{k + 1}"
+            req.rid = f"{parent.rid}.{parent.num_forks + k + 1}"
+            req.num_forks = 0
             req.req_pool_idx = slot
             for name in ("origin_input_ids", "output_ids", "fill_ids", "prefix_indices", "token_times", "prior_output_ids",
                          "prior_token_times"):
                 setattr(req, name, list(getattr(parent, name)))
             children.append(req)
+        parent.num_forks += n
         rows = list(range(index + 1)) + [index] * n + list(range(index + 1, len(self.reqs)))
         self.reqs = self.reqs[:index + 1] + children + self.reqs[index + 1:]
         self.seq_lens_host = [self.seq_lens_host[i] for i in rows]

@@ -509,6 +509,7 @@ class SemiPDDecodeScheduler(SemiPDScheduler):
                 new_req = self.handle_generate_request(msg)
                 # history the continuation must report when it finishes (stitched in _release)
                 new_req.retracted_from = req
+                new_req.num_forks = req.num_forks
                 new_req.prior_output_ids = req.prior_output_ids + req.output_ids
                 new_req.prior_token_times = req.prior_token_times + req.token_times
                 new_req.first_token_time = req.first_token_time
@@ -519,6 +520,15 @@ class SemiPDDecodeScheduler(SemiPDScheduler):
                                        self.min_new_token_ratio)
         batch.prepare_for_decode()
         return batch
+
+    def fork_running(self, rid: str, n: int) -> Optional[List[Req]]:
+        """n more continuations of a decoding request (ScheduleBatch.fork_req), which run and finish as requests of their own.
+        On this loop's thread between two steps (under TP on every rank in the same iteration), not from a token callback.
+        None when the request is not decoding (any more), or request slots or cache do not suffice."""
+        self._drain_results(all_of_them=True)  # a step that is still unread would not reach the children
+        batch = self.running_batch
+        index = next((i for i, r in enumerate(batch.reqs) if r.rid == rid and not r.finished()), None)
+        return None if index is None else batch.fork_req(index, n)
 
     def get_next_batch_to_run(self) -> Optional[ScheduleBatch]:
         if self.running_batch.is_empty():
