@@ -305,7 +305,12 @@ int spd_attn_decode_paged_own(void* out, const void* q, const void* k_pool, cons
  * Workspace: spd_attn_decode_shared_workspace_bytes(), zeroed once before its first use (each call leaves its counters at
  * zero), one per stream.  spd_attn_decode_shared_pays: 1 where a call of these sizes takes the kernel that shares, 0 where
  * spd_attn_decode_paged serves it as well (decided on the host, without a launch); _saves: about how many us the call saves
- * then, rounded up (0 where it does not pay).
+ * then, rounded up (0 where it does not pay).  They take all requests to be in groups of one size that share max_shared_len tokens.
+ * The _tokens forms decide by what the host knows of unequal groups, and of batches in which requests of no group stand beside
+ * them: group_tokens, the sum of the groups' shared tokens, member_tokens, the sum of members x shared tokens, both over groups
+ * of two members and more, in whole tiles of 128 tokens; own_tokens, what is left of the sum of seq_lens; and the longest of
+ * seq_lens.  (Requests of no group may be left out of the lists at both
+ * ends, and are one group of shared_lens 0 between two others.)
  * The reference has no such call; its cascade form is flashinfer's, behind the same wrapper interface as
  * S/layers/attention/flashinfer_backend.py:454-488. */
 int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_heads, int num_kv_heads, int head_dim);
@@ -319,6 +324,15 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
                            int64_t pool_slots, int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
                            int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
                            int sm_budget, spd_stream_t stream);
+int spd_attn_decode_shared_saves_tokens(int64_t batch, int64_t num_groups, int64_t group_tokens, int64_t member_tokens,
+                                        int64_t own_tokens, int64_t longest, int num_q_heads, int num_kv_heads, int head_dim,
+                                        int sm_budget);
+int spd_attn_decode_shared_tokens(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
+                                  const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
+                                  const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t group_tokens,
+                                  int64_t member_tokens, int64_t own_tokens, int64_t longest, int64_t pool_slots, int num_q_heads,
+                                  int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride, int64_t req_to_token_stride, float sm_scale, int dtype,
+                                  void* workspace, int64_t workspace_bytes, int sm_budget, spd_stream_t stream);
 /* Plain SIMT implementations of the two calls above (no tensor cores).  Bring-up / on-device
  * cross-check only; the product path never calls them. */
 int spd_attn_prefill_simt(void* out, const void* q, const void* k_pool, const void* v_pool,

@@ -96,6 +96,11 @@ SIGNATURES = {
         _i,
         [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i64, _i64, _i64, _f, _i, _p, _i64, _i, _p],
     ),
+    "spd_attn_decode_shared_saves_tokens": (_i, [_i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i]),
+    "spd_attn_decode_shared_tokens": (
+        _i,
+        [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i64, _i64, _i64, _f, _i, _p, _i64, _i, _p],
+    ),
     "spd_kv_copy": (_i, [_p, _i, _p, _p, _i64, _p]),
     "spd_kv_fork": (_i, [_p, _i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _i, _p]),
     "spd_kv_compact": (_i, [_p, _i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i, _p]),

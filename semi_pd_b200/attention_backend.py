@@ -165,7 +165,7 @@ class SpdAttnBackend(AttentionBackend):
         if self.impl != "tc" or self.is_mla:
             return False
         saved = ops.attn_shared_saves(batch_size, shared.shared_lens.numel(), shared.max_shared_len, self.num_q_heads,
-                                      self.num_kv_heads, self.head_dim)
+                                      self.num_kv_heads, self.head_dim, shared.tokens)
         return saved > (self.GRAPH_SAVES if batch_size <= self.graph_max_bs else 0)
 
     def init_forward_metadata(self, forward_batch: ForwardBatch):
@@ -349,7 +349,8 @@ class SpdAttnBackend(AttentionBackend):
             return ops.attn_decode_shared(
                 q, k_buf, v_buf, forward_batch.req_to_token_pool.req_to_token, forward_batch.req_pool_indices,
                 forward_batch.seq_lens, shared.group_indptr, shared.shared_lens, shared.max_shared_len,
-                layer.tp_q_head_num, layer.tp_k_head_num, layer.head_dim, layer.scaling, workspace=self.shared_workspace)
+                layer.tp_q_head_num, layer.tp_k_head_num, layer.head_dim, layer.scaling, workspace=self.shared_workspace,
+                shared_tokens=shared.tokens)
         return ops.attn_decode(
             q, k_buf, v_buf, forward_batch.req_to_token_pool.req_to_token,
             forward_batch.req_pool_indices, forward_batch.seq_lens, layer.tp_q_head_num,

@@ -1143,25 +1143,39 @@ static int64_t part_bytes(int64_t batch, int num_q_heads, int num_kv_heads) {
   return (3 * b * num_q_heads + static_cast<int64_t>(device_sm_count_cached()) * 2 * kSpM) * (kSpD + 2) * 4 + 2 * b * num_kv_heads * 8;
 }
 
-// Whether reading the shared keys once is the faster way, from what the host knows: as if all requests were in groups of one
-// size that share max_shared keys.  The weights fit 325 shapes measured both ways (2 to 256 requests in 1 to 32 groups, 128 to
-// 16384 shared tokens, 64 own, bf16, four head layouts): the choice takes 0.5% longer than the better way on average, 24% at
-// worst.  A tile of 128 shared keys costs an SM 1.2 here and each member 0.7 there (mostly from L2); requests that there are cut
-// over many SMs cost 0.4 per part and query head in their merge; the longer start, the join and the shorter ranges cost 6 here,
-// and 0.0008 per request and kv head.
+// Whether reading the shared keys once is the faster way, from what the host knows.
+struct SharedTokens {
+  int64_t group, member;  // that the groups share; that their members would read of them one by one
+  int64_t own, longest;   // that every request reads by itself either way; of the longest request
+};
+// The weights fit 325 shapes of equal groups measured both ways (2 to 256 requests in 1 to 32 groups, 128 to 16384 shared tokens,
+// 64 own, bf16, four head layouts): the choice takes 0.5% longer than the better way on average, 24% at worst.  A tile of 128
+// shared keys costs an SM 1.2 here and each member 0.7 there (mostly from L2); requests that there are cut over many SMs cost 0.4
+// per part and query head in their merge; the longer start, the join and the shorter ranges cost 6 here, and 0.0008 per request
+// and kv head.  A tile of own keys beyond the 64 costs 0.25 more here, 1.46 there.  There, items that are not cut (attn_decode.cu
+// has the rule) wait for the longest one, 0.7 a tile; here the list is cut evenly.
+// 620 batches of unequal groups beside up to 400 requests of no group (2 to 100 members, 128 to 32768 shared tokens, own ones of 1
+// to 16000, seven head layouts): 0.9% longer than the better way on average, 74% at worst (57 requests on 2 kv heads, one of 13176 tokens).
 // us by request / shared.  32 / 8 heads, one group: 64 members of 256 tokens 18.8 / 18.9, 512: 24.1 / 21.3, 1024: 33.8 / 22.0,
 // 16384: 388 / 41.5; 8 of 1024: 14.3 / 15.5, 4096: 25.1 / 22.7, 16384: 57.0 / 31.2; 4 of 4096: 21.6 / 22.0.  Groups of two: 8
 // of 4096: 46.3 / 39.8, of 16384: 164 / 100; 32 of 2048: 62.3 / 67.9, of 4096: 161 / 107.  16 / 2 heads, 2 of 512: 17.6 / 15.1,
-// of 4096: 53.1 / 24.6.  32 / 32 heads, 16 of 256: 17.7 / 17.6, of 1024: 32.3 / 21.3.
-static double shared_saves(int64_t batch, int64_t groups, int64_t max_shared, int num_q_heads, int num_kv_heads, int sms) {
-  const double pairs = static_cast<double>(batch) * num_kv_heads, shared = static_cast<double>(max_shared);
-  const double tiles = static_cast<double>(groups) * num_kv_heads * (shared / kSpTile) / sms;  // of an SM
-  double gain = tiles * (0.7 * batch / groups - 1.2);
+// of 4096: 53.1 / 24.6.  32 / 32 heads, 16 of 256: 17.7 / 17.6, of 1024: 32.3 / 21.3.  64 of 8192 beside n requests of 500 tokens,
+// 32 / 8 heads: n = 0 184 / 39, 64: 197 / 64, 100: 209 / 78, 400: 305 / 188; 16 of 8192 beside 100: 86 / 78; 8 of 4096 beside 100
+// of 2000: 143 / 170; 126 of 128 and 2 of 16384: 113 / 57.
+static double shared_saves(int64_t batch, const SharedTokens& t, int num_q_heads, int num_kv_heads, int sms) {
+  const double pairs = static_cast<double>(batch) * num_kv_heads, per_sm = static_cast<double>(num_kv_heads) / kSpTile / sms;
+  double there = per_sm * 0.7 * t.member;
   if (pairs < sms) {
-    const double parts = sms / pairs < shared / 256 ? sms / pairs : shared / 256;
-    gain += 0.4 * (num_q_heads / num_kv_heads) * parts;
+    const double parts = sms / pairs < t.longest / 256. ? sms / pairs : t.longest / 256.;
+    there += 0.4 * (num_q_heads / num_kv_heads) * parts;
+  } else {
+    const double units = pairs + static_cast<double>(num_kv_heads) * (t.member + t.own) / kSpTile;
+    const double rounds = static_cast<double>((static_cast<int64_t>(pairs) + sms - 1) / sms);
+    const double chain = 0.7 * t.longest / kSpTile - per_sm * 1.46 * t.own;
+    if ((rounds / pairs - 1. / sms) * units < 18. && chain > there) there = chain;
   }
-  return gain - (6.0 + 0.0008 * pairs * 148 / sms);
+  const double own = static_cast<double>(t.own) - 64. * batch;
+  return there - per_sm * (1.2 * t.group + (own > 0. ? 0.25 * own : 0.)) - (6.0 + 0.0008 * pairs * 148 / sms);
 }
 
 }  // namespace spd
@@ -1176,15 +1190,25 @@ int64_t spd_attn_decode_shared_workspace_bytes(int64_t max_batch, int num_q_head
   return decode_bytes(max_batch, num_q_heads, num_kv_heads) + part_bytes(max_batch, num_q_heads, num_kv_heads);
 }
 
-int spd_attn_decode_shared_saves(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
-                                 int head_dim, int sm_budget) {
-  if (batch < 2 || batch > kSpRows || num_groups < 1 || num_groups > kSpGroups || max_shared_len < kSpTile || num_kv_heads < 1 ||
-      num_q_heads < num_kv_heads || head_dim != kSpD)
+int spd_attn_decode_shared_saves_tokens(int64_t batch, int64_t num_groups, int64_t group_tokens, int64_t member_tokens,
+                                        int64_t own_tokens, int64_t longest, int num_q_heads, int num_kv_heads, int head_dim,
+                                        int sm_budget) {
+  if (batch < 2 || batch > kSpRows || num_groups < 1 || num_groups > kSpGroups || group_tokens < kSpTile || member_tokens < group_tokens ||
+      num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim != kSpD)
     return 0;
   const int device_sms = device_sm_count_cached();
-  const double us = shared_saves(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads,
+  const double us = shared_saves(batch, SharedTokens{group_tokens, member_tokens, own_tokens, longest}, num_q_heads, num_kv_heads,
                                  sm_budget > 0 && sm_budget < device_sms ? sm_budget : device_sms);
   return us <= 0. ? 0 : us >= 1e9 ? 1000000000 : static_cast<int>(us) + 1;
+}
+
+// as if all requests were in groups of one size that share max_shared_len tokens, with 64 of their own
+int spd_attn_decode_shared_saves(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
+                                 int head_dim, int sm_budget) {
+  if (batch < 2 || batch > kSpRows || num_groups < 1 || num_groups > batch || max_shared_len < kSpTile) return 0;
+  const int64_t most = max_shared_len < (1ll << 40) ? max_shared_len : 1ll << 40;
+  return spd_attn_decode_shared_saves_tokens(batch, num_groups, num_groups * most, batch * most, 64 * batch, most, num_q_heads,
+                                             num_kv_heads, head_dim, sm_budget);
 }
 
 int spd_attn_decode_shared_pays(int64_t batch, int64_t num_groups, int64_t max_shared_len, int num_q_heads, int num_kv_heads,
@@ -1192,16 +1216,18 @@ int spd_attn_decode_shared_pays(int64_t batch, int64_t num_groups, int64_t max_s
   return spd_attn_decode_shared_saves(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, sm_budget) > 0;
 }
 
-int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
-                           const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
-                           const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t max_shared_len,
-                           int64_t pool_slots, int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
-                           int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
-                           int sm_budget, spd_stream_t stream) {
+}  // extern "C"
+
+static int attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
+                              const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
+                              const int64_t* shared_lens, int64_t batch, int64_t num_groups, bool pays, int64_t pool_slots,
+                              int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
+                              int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
+                              int sm_budget, spd_stream_t stream) {
   if (int rc = check_attn_args("spd_attn_decode_shared", out, q, k_pool, v_pool, req_to_token, req_pool_indices, num_q_heads,
                                num_kv_heads, head_dim, q_stride, out_stride))
     return rc;
-  SPD_REQUIRE(seq_lens && batch >= 0 && num_groups >= 0 && max_shared_len >= 0 && pool_slots > 0 && pool_slots < (1ll << 31) &&
+  SPD_REQUIRE(seq_lens && batch >= 0 && num_groups >= 0 && pool_slots > 0 && pool_slots < (1ll << 31) &&
                   (num_groups == 0 || (group_indptr && shared_lens)),
               SPD_E_BADARG, "spd_attn_decode_shared: bad lengths or groups");
   SPD_REQUIRE(head_dim == kSpD, SPD_E_SHAPE, "spd_attn_decode_shared: head_dim must be 128 (got %d)", head_dim);
@@ -1215,8 +1241,7 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
   const int64_t most = batch * num_kv_heads * (kCostOwnTile * (req_to_token_stride / kSpTile + 1) + kCostShared + kCostOwn);
   // Every request reads its own pages where nothing can be shared or it does not pay, where a plan would not hold the batch or
   // its 32-bit costs the list, and where the scale is not positive (the maximum of raw scores serves the scaled ones only there).
-  if (!(sm_scale > 0.f) || most > INT_MAX / 2 ||
-      !spd_attn_decode_shared_pays(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, sm_budget))
+  if (!(sm_scale > 0.f) || most > INT_MAX / 2 || !pays)
     return spd_attn_decode_paged_own(out, q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, batch, num_q_heads,
                                      num_kv_heads, head_dim, q_stride, out_stride, req_to_token_stride, sm_scale, dtype, workspace,
                                      workspace_bytes, sm_budget, stream);
@@ -1267,6 +1292,35 @@ int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const v
                     as_stream(stream), pdl_enabled(), static_cast<T*>(out), out_stride, p, static_cast<int>(rows)));
   });
   return 0;
+}
+
+extern "C" {
+
+int spd_attn_decode_shared(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
+                           const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
+                           const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t max_shared_len,
+                           int64_t pool_slots, int num_q_heads, int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride,
+                           int64_t req_to_token_stride, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
+                           int sm_budget, spd_stream_t stream) {
+  SPD_REQUIRE(max_shared_len >= 0, SPD_E_BADARG, "spd_attn_decode_shared: bad max_shared_len");
+  return attn_decode_shared(out, q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, group_indptr, shared_lens, batch, num_groups,
+                            spd_attn_decode_shared_pays(batch, num_groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, sm_budget),
+                            pool_slots, num_q_heads, num_kv_heads, head_dim, q_stride, out_stride, req_to_token_stride, sm_scale, dtype,
+                            workspace, workspace_bytes, sm_budget, stream);
+}
+
+int spd_attn_decode_shared_tokens(void* out, const void* q, const void* k_pool, const void* v_pool, const int32_t* req_to_token,
+                                  const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* group_indptr,
+                                  const int64_t* shared_lens, int64_t batch, int64_t num_groups, int64_t group_tokens,
+                                  int64_t member_tokens, int64_t own_tokens, int64_t longest, int64_t pool_slots, int num_q_heads,
+                                  int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride, int64_t req_to_token_stride, float sm_scale, int dtype,
+                                  void* workspace, int64_t workspace_bytes, int sm_budget, spd_stream_t stream) {
+  SPD_REQUIRE(group_tokens >= 0 && member_tokens >= 0 && own_tokens >= 0 && longest >= 0, SPD_E_BADARG, "spd_attn_decode_shared: bad token counts");
+  return attn_decode_shared(out, q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, group_indptr, shared_lens, batch, num_groups,
+                            spd_attn_decode_shared_saves_tokens(batch, num_groups, group_tokens, member_tokens, own_tokens, longest,
+                                                                num_q_heads, num_kv_heads, head_dim, sm_budget) > 0,
+                            pool_slots, num_q_heads, num_kv_heads, head_dim, q_stride, out_stride, req_to_token_stride, sm_scale, dtype,
+                            workspace, workspace_bytes, sm_budget, stream);
 }
 
 }  // extern "C"

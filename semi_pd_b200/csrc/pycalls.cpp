@@ -87,7 +87,7 @@ struct Call<int(A...)> {
   X(spd_embed_norm_streams) X(spd_streams_mix_norm) X(spd_rotary_bias_store) X(spd_matrix_memory) X(spd_attn_general_ex) \
   X(spd_embed_pair) X(spd_residual_tanh_norm) X(spd_heads_gate) X(spd_residual_postnorm) X(spd_softcap_f32) \
   X(spd_attn_general_blocks) X(spd_attn_general_keys) X(spd_attn_general_sms) X(spd_pool_key_blocks) X(spd_head_decay) \
-  X(spd_short_conv) X(spd_gated_group_norm) X(spd_attn_decode_shared) X(spd_kv_copy) X(spd_kv_fork) X(spd_kv_compact)
+  X(spd_short_conv) X(spd_gated_group_norm) X(spd_attn_decode_shared) X(spd_attn_decode_shared_tokens) X(spd_kv_copy) X(spd_kv_fork) X(spd_kv_compact)
 
 PyMethodDef calls[] = {
 #define X(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&Call<decltype(name)>::run)), METH_FASTCALL, nullptr},

@@ -63,6 +63,7 @@ class SharedPrefix:
     group_indptr: torch.Tensor       # [groups + 1] int32, device
     shared_lens: torch.Tensor        # [groups] int64, device
     max_shared_len: int
+    tokens: Optional[ops.SharedTokens] = None
 
 
 @dataclasses.dataclass

@@ -12,7 +12,7 @@ import contextlib
 import ctypes
 import functools
 import os
-from typing import Optional
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -790,31 +790,53 @@ def new_attn_shared_workspace(device, max_batch: int, num_q_heads: int, num_kv_h
     return torch.zeros((need,), dtype=torch.uint8, device=device)
 
 
-@functools.lru_cache(maxsize=1024)
-def _attn_shared_saves(batch: int, groups: int, max_shared_len: int, hq: int, hk: int, d: int, sm_budget: int) -> int:
-    return lib.spd_attn_decode_shared_saves(batch, groups, max_shared_len, hq, hk, d, sm_budget)
+class SharedTokens(NamedTuple):
+    """What the host knows of a batch that shares prefixes, by which attn_decode_shared decides whether to read them once."""
+    group: int    # tokens that the groups share
+    member: int   # tokens of them that their members would read one by one
+    own: int      # tokens that every request reads by itself either way
+    longest: int  # request
 
 
-def attn_shared_saves(batch: int, groups: int, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
-    """About how many us attn_decode_shared saves by reading such a batch's shared keys once, 0 where it reads them per request."""
-    return _attn_shared_saves(batch, groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, get_sm_budget())
+def attn_shared_tokens(group_indptr: Sequence[int], shared_lens: Sequence[int], seq_lens: Sequence[int]) -> SharedTokens:
+    """Of the batch's lists, as the host has them; groups of two members and more count in whole tiles of 128 tokens."""
+    group = member = 0
+    for start, end, n in zip(group_indptr, group_indptr[1:], shared_lens):
+        if end - start >= 2:
+            n = n // 128 * 128
+            group += n
+            member += (end - start) * n
+    return SharedTokens(group, member, max(0, sum(seq_lens) - member), max(seq_lens, default=0))
 
 
-def attn_shared_pays(batch: int, groups: int, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> bool:
+def attn_shared_saves(batch: int, groups: int, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                      shared_tokens: Optional[SharedTokens] = None) -> int:
+    """About how many us attn_decode_shared saves by reading such a batch's shared keys once, 0 where it reads them per request.
+    shared_tokens: attn_shared_tokens of the groups; without it all requests are taken to be in groups of one size that share
+    max_shared_len tokens."""
+    if shared_tokens is None:
+        return lib.spd_attn_decode_shared_saves(batch, groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, get_sm_budget())
+    return lib.spd_attn_decode_shared_saves_tokens(batch, groups, *shared_tokens, num_q_heads, num_kv_heads, head_dim, get_sm_budget())
+
+
+def attn_shared_pays(batch: int, groups: int, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                     shared_tokens: Optional[SharedTokens] = None) -> bool:
     """Whether attn_decode_shared reads such a batch's shared keys once (attn_decode serves it as well otherwise)."""
-    return attn_shared_saves(batch, groups, max_shared_len, num_q_heads, num_kv_heads, head_dim) > 0
+    return attn_shared_saves(batch, groups, max_shared_len, num_q_heads, num_kv_heads, head_dim, shared_tokens) > 0
 
 
 def attn_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, req_to_token: torch.Tensor,
                        req_pool_indices: torch.Tensor, seq_lens: torch.Tensor, group_indptr: torch.Tensor,
                        shared_lens: torch.Tensor, max_shared_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
-                       sm_scale: float, out: Optional[torch.Tensor] = None,
-                       workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                       sm_scale: float, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                       shared_tokens: Optional[SharedTokens] = None) -> torch.Tensor:
     """attn_decode for a batch in which groups of requests continue the same tokens: the rows group_indptr[g] ..
     group_indptr[g + 1] of the batch (int32 [groups + 1], ascending) have the same slots in the first shared_lens[g] (int64
     [groups]) entries of their req_to_token rows, which are read once for all of them.  The result is attn_decode's; seq_lens
     counts the shared tokens too, rows outside every group stand alone.  max_shared_len: a bound of shared_lens that the host
-    knows (in a captured graph: of all replays).  workspace: new_attn_shared_workspace's, zeroed once, never replaced, one
+    knows (in a captured graph: of all replays).  By it the call decides whether to share, as if all requests were in groups of one
+    size; shared_tokens (attn_shared_tokens) says it of unequal groups and of batches with rows outside them, which may be left
+    out of the lists at both ends and are one group of length 0 between two others.  workspace: new_attn_shared_workspace's, zeroed once, never replaced, one
     stream at a time; without one every call takes and zeroes its own."""
     _cuda(q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, group_indptr, shared_lens, out, workspace)
     _here("attn_decode_shared", q, k_pool, v_pool, req_to_token, req_pool_indices, seq_lens, group_indptr, shared_lens, out, workspace)
@@ -846,11 +868,12 @@ def attn_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
         raise RuntimeError("attn_decode_shared: q and out must have contiguous rows")
     if workspace is None:
         workspace = new_attn_shared_workspace(q.device, B, num_q_heads, num_kv_heads, head_dim)
-    check(lib.spd_attn_decode_shared(o2.data_ptr(), q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), req_to_token.data_ptr(),
-                                     req_pool_indices.data_ptr(), seq_lens.data_ptr(), group_indptr.data_ptr(),
-                                     shared_lens.data_ptr(), B, G, int(max_shared_len), k_pool.shape[0], num_q_heads, num_kv_heads, head_dim,
-                                     q2.stride(0), o2.stride(0), req_to_token.stride(0), float(sm_scale), _dt(q),
-                                     workspace.data_ptr(), workspace.numel(), get_sm_budget(), _stream()),
+    call, known = (lib.spd_attn_decode_shared, (int(max_shared_len),)) if shared_tokens is None else \
+        (lib.spd_attn_decode_shared_tokens, tuple(map(int, shared_tokens)))
+    check(call(o2.data_ptr(), q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), req_to_token.data_ptr(), req_pool_indices.data_ptr(),
+               seq_lens.data_ptr(), group_indptr.data_ptr(), shared_lens.data_ptr(), B, G, *known, k_pool.shape[0], num_q_heads,
+               num_kv_heads, head_dim, q2.stride(0), o2.stride(0), req_to_token.stride(0), float(sm_scale), _dt(q),
+               workspace.data_ptr(), workspace.numel(), get_sm_budget(), _stream()),
           "spd_attn_decode_shared")
     return out
 

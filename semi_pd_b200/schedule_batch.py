@@ -114,7 +114,7 @@ class ScheduleBatch:
         self.extend_lens = None
         self.extend_num_tokens = None
         self.decoding_reqs = None
-        self._shared = None   # (groups of the last step, SharedPrefix)
+        self._shared = None   # (groups of the last step, SharedPrefix, its lists)
         self._compacted = False   # some request may have dropped tokens
 
     @classmethod
@@ -314,9 +314,10 @@ class ScheduleBatch:
         if groups is None:
             return None
         if self._shared is None or self._shared[0] != groups:  # lists of a few steps are the same
-            indptr, lens = groups
-            self._shared = (groups, SharedPrefix(self._h2d(indptr, torch.int32), self._h2d(lens, torch.int64), max(lens)))
-        return self._shared[1]
+            indptr, lens = _joined_alone(*groups)
+            self._shared = (groups, SharedPrefix(self._h2d(indptr, torch.int32), self._h2d(lens, torch.int64), max(lens)), indptr, lens)
+        _, shared, indptr, lens = self._shared
+        return dataclasses.replace(shared, tokens=ops.attn_shared_tokens(indptr, lens, self.seq_lens_host))
 
     def filter_batch(self, keep_indices: Optional[List[int]] = None):
         if keep_indices is None:
@@ -371,6 +372,20 @@ class ScheduleBatch:
             extend_logprob_start_lens=[0] * len(self.reqs) if extend else None,
             gather_logits=getattr(self, "gather_logits", True),
             extend_logit_rows=getattr(self, "extend_logit_rows", None) if extend else None)
+
+
+def _joined_alone(indptr, lens):
+    """Group lists without requests that share nothing at both ends, those between two groups as one: a plan holds so many."""
+    out, sizes = [], []
+    for start, n in zip(indptr, lens):
+        if n or (sizes and sizes[-1]):
+            out.append(start)
+            sizes.append(n)
+    end = indptr[-1]
+    if sizes and not sizes[-1]:
+        end = out.pop()
+        sizes.pop()
+    return out + [end], sizes
 
 
 def _cumsum(xs):
