@@ -197,6 +197,50 @@ class _PinnedRing:
         return out
 
 
+def _common_runs(a: Sequence[int], b: Sequence[int]) -> int:
+    """How many runs two requests have in common.  They come from one fork, so all before a common one are common too."""
+    lo, hi = 0, min(len(a), len(b))
+    while lo < hi:
+        mid = (lo + hi) // 2
+        if a[mid] == b[mid]:
+            lo = mid + 1
+        else:
+            hi = mid
+    return lo
+
+
+def _best_groups(common: List[int], start: int, end: int) -> List[Tuple[int, int]]:
+    """Rows [start, end), each with something in common with the one before it, cut into groups of neighbours: → (end, shared runs)
+    of each.  A group of n saves the reads of shared x (0.7 n - 1.2) runs, as measured for decode attention; the cut that saves
+    most is taken, and of equal ones the one of larger groups.  (Without cuts one shallow relative would cost a group of deep
+    ones all that they share.)"""
+    rows = range(start + 1, end)
+    if end - start == 1:
+        return [(end, 0)]
+    if all(common[i] == common[start + 1] for i in rows):
+        return [(end, common[start + 1])]
+    # A row inside a stretch of equals never begins a group: its neighbours' group would gain by taking the others.
+    at = [start] + [i for i in rows if common[i] != common[i - 1] or i + 1 == end or common[i] != common[i + 1]] + [end]
+    first, none = np.asarray(at, dtype=np.int64), np.int64(1 << 40)
+    least = np.zeros(len(at), dtype=np.int64)     # what the rows from at[p] to here have in common
+    best = np.zeros(len(at), dtype=np.int64)      # of the rows before at[p]
+    cut = [0] * len(at)
+    for q in range(len(at) - 1):
+        inner = min(common[at[q] + 1:at[q + 1]], default=none)
+        least[:q] = np.minimum(least[:q], min(inner, common[at[q]]))
+        least[q] = inner
+        n = first[q + 1] - first[:q + 1]
+        total = best[:q + 1] + np.where(n > 1, (7 * n - 12) * least[:q + 1], 0)
+        cut[q + 1] = int(np.argmax(total))
+        best[q + 1] = total[cut[q + 1]]
+    groups, q = [], len(at) - 1
+    while q:
+        p = cut[q]
+        groups.append((at[q], min(common[at[p] + 1:at[q]], default=0)))
+        q = p
+    return groups[::-1]
+
+
 class TokenToKVPoolAllocator:
     """Run allocator behind the token-granular contract (see the module docstring).
 
@@ -388,18 +432,20 @@ class TokenToKVPoolAllocator:
         if not self._forked or not req_pool_indices:
             return None
         self._forked = bool((self._held > 1).any())
-        indptr, lens = [], []
-        lead: List[int] = []    # the runs that the group's members have in common so far
-        for i, idx in enumerate(req_pool_indices):
-            runs = self._req_runs.get(idx, [])
-            same = next((k for k, (a, b) in enumerate(zip(lead, runs)) if a != b), min(len(lead), len(runs)))
-            if same > 0:
-                lead, lens[-1] = lead[:same], same * self.run_len
-            else:
-                indptr.append(i)
-                lens.append(0)
-                lead = runs
-        return (indptr + [len(req_pool_indices)], lens) if any(lens) else None
+        return self._find_groups(req_pool_indices) if self._forked else None
+
+    def _find_groups(self, req_pool_indices: Sequence[int]) -> Optional[Tuple[List[int], List[int]]]:
+        runs = [self._req_runs.get(idx, ()) for idx in req_pool_indices]
+        common = [0] + [_common_runs(a, b) for a, b in zip(runs, runs[1:])]  # of a row and the one before it
+        if not any(common):
+            return None
+        starts = [i for i, c in enumerate(common) if c == 0] + [len(runs)]
+        indptr, lens = [0], []
+        for s, e in zip(starts, starts[1:]):
+            for end, n in _best_groups(common, s, e):
+                indptr.append(end)
+                lens.append(n * self.run_len)
+        return indptr, lens
 
     def req_slots(self, req_pool_idx: int) -> np.ndarray:
         """Slot ids of a request's tokens in position order (host-side view; tests)."""
