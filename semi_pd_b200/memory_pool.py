@@ -271,6 +271,7 @@ class TokenToKVPoolAllocator:
         self._used = np.zeros(self.num_runs, dtype=np.int32)
         self._held = np.zeros(self.num_runs, dtype=np.int32)   # requests that hold the run
         self._forked = False                                   # some run may have several holders
+        self._groups = None                                    # (requests, their groups), see shared_prefix
         self._req_runs: Dict[int, List[int]] = {}   # req_pool_idx -> runs in position order
         self._req_len: Dict[int, int] = {}          # req_pool_idx -> tokens placed
         self.is_not_in_free_group = True
@@ -365,6 +366,7 @@ class TokenToKVPoolAllocator:
 
     def _let_go(self, runs: List[int]) -> None:
         """One holder less of each; a run that nobody holds is free."""
+        self._groups = None
         ids = np.asarray(runs, dtype=np.int64)
         self._held[ids] -= 1
         gone = ids[self._held[ids] == 0]
@@ -385,6 +387,7 @@ class TokenToKVPoolAllocator:
             raise RuntimeError(f"request slot {parent} holds no tokens")
         if len(set(children)) != len(children) or any(c == parent or self._req_runs.get(c) for c in children):
             raise RuntimeError("fork: children must be request slots of their own that hold no runs")
+        self._groups = None
         R, n, runs = self.run_len, self._req_len[parent], self._req_runs[parent]
         whole, rest = runs[:n // R], n % R
         if rest and not self._free_runs.enough(len(children)):
@@ -411,6 +414,7 @@ class TokenToKVPoolAllocator:
         R = self.run_len
         if not self._free_runs.enough(-(-n // R)):
             return None
+        self._groups = None
         old = self._req_runs[req_pool_idx]
         self._req_runs[req_pool_idx] = [self._take_run() for _ in range(-(-n // R))]
         self._req_len[req_pool_idx] = n
@@ -431,8 +435,11 @@ class TokenToKVPoolAllocator:
         group being groups of one that share nothing.  None when nothing is shared."""
         if not self._forked or not req_pool_indices:
             return None
-        self._forked = bool((self._held > 1).any())
-        return self._find_groups(req_pool_indices) if self._forked else None
+        # a run that gets its first token is nobody else's: only forks, compactions and frees change what is shared
+        if self._groups is None or self._groups[0] != list(req_pool_indices):
+            self._forked = bool((self._held > 1).any())
+            self._groups = (list(req_pool_indices), self._find_groups(req_pool_indices) if self._forked else None)
+        return self._groups[1]
 
     def _find_groups(self, req_pool_indices: Sequence[int]) -> Optional[Tuple[List[int], List[int]]]:
         runs = [self._req_runs.get(idx, ()) for idx in req_pool_indices]

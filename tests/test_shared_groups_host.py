@@ -1,4 +1,4 @@
-"""How a batch is cut into groups that share a prefix: by what sharing saves."""
+"""How a batch is cut into groups that share a prefix: by what sharing saves, found again only when it may have changed."""
 import itertools
 import random
 import time
@@ -80,6 +80,32 @@ def test_common_runs():
         a = list(range(k)) + [1000 + i for i in range(n - k)]
         b = list(range(k)) + [5000 + i for i in range(m - k)]
         assert _common_runs(a, b) == k == _common_runs(b, a)
+
+
+def test_groups_are_found_again_only_when_they_may_have_changed(monkeypatch):
+    a = _alloc()
+    found = []
+    real = TokenToKVPoolAllocator._find_groups
+    monkeypatch.setattr(TokenToKVPoolAllocator, "_find_groups", lambda self, rows: (found.append(1), real(self, rows))[1])
+    a.alloc_extend([0], [0], [5 * R])
+    assert a.shared_prefix([0]) is None and not found     # nothing was ever forked
+    a.fork_req(0, [1, 2])
+    want = ([0, 3], [5 * R])
+    for step in range(3 * R):
+        assert a.shared_prefix([0, 1, 2]) == want
+        a.alloc_decode([0, 1, 2], [5 * R + step] * 3)
+    assert len(found) == 1
+    assert a.shared_prefix([0, 1]) == ([0, 2], [5 * R]) and len(found) == 2          # other members
+    a.alloc_extend([7], [0], [R])
+    assert a.shared_prefix([7, 0, 1]) == ([0, 1, 3], [0, 5 * R]) and len(found) == 3
+    a.fork_req(0, [3])
+    assert a.shared_prefix([0, 3, 1]) == ([0, 3], [5 * R])           # (0.7 x 3 - 1.2) x 5 runs, of two (0.7 x 2 - 1.2) x 8
+    assert a.shared_prefix([0, 3]) == ([0, 2], [8 * R])
+    a.rebuild_req(3, R)
+    assert a.shared_prefix([0, 3, 1]) is None
+    a.free_req(1)
+    a.alloc_extend([1], [0], [5 * R])                                                 # the slot's next request
+    assert a.shared_prefix([0, 1]) is None and a.shared_prefix([0, 2]) == ([0, 2], [5 * R])
 
 
 def test_a_request_is_not_mistaken_for_its_slots_last_owner():
