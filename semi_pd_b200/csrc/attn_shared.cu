@@ -763,8 +763,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     auto entry = [&](int skip, int j) {
       return p.req_to_token + it.req * p.rtt_stride + static_cast<int64_t>(skip + it.tile0 + j) * kSpTile;
     };
-    int hk = 0, j = 0;
-    bool first = false, more = true, have = walk.next(p, pl, it);
+    bool have = walk.next(p, pl, it);
     if (have) lookup(entry(0, 0), kSpTile, slot);
     for (int j = 0; have; ++t_base) {
       const int hk = it.hk;
@@ -782,10 +781,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     // ---- own keys: warpgroup lw's, with the queries ----
     SpOwnWalk own(p, pl, range, lw);
     uint32_t place = 0;
-    int q_buf = 0, b = 0, valid = 0;
+    int q_buf = 0, b = 0, valid = 0, hk = 0, j = 0;
+    bool first = false, more = true;
     have = false;
-    more = true;
-    it.n = j = 0;
+    it.n = 0;
 #pragma unroll 1
     while (more) {
       if (j == it.n) {
@@ -871,7 +870,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
               m1 = fmax3(m1, __uint_as_float(rb[i]), __uint_as_float(rb[i + 1]));
             }
             const float mx = fmaxf(m0, m1);
-            // The exponentials do not wait for the unit's maximum; where it turns out too large (rarely) they are redone
+            // The reference maximum is raised before the exponentials, where a score passes it by 2^8 (rarely but for the first
+            // unit); O is rescaled when the PV of the unit before is complete
             const bool raise = __any_sync(0xffffffffu, mx > m + ahead && row < rows);
             float alpha = 1.f;
             if (raise) {
