@@ -302,8 +302,8 @@ int spd_attn_decode_paged_own(void* out, const void* q, const void* k_pool, cons
  * Scores of -inf weigh nothing; a NaN or +inf among a request's scores, or nothing but -inf, makes its output NaN.
  * head_dim 128, at most 8 query heads per kv head; batches of more than 1024 requests or 256 groups are read as
  * spd_attn_decode_paged reads them.
- * Workspace: spd_attn_decode_shared_workspace_bytes(), zeroed once before its first use (each call leaves its counters at
- * zero), one per stream.  spd_attn_decode_shared_pays: 1 where a call of these sizes takes the kernel that shares, 0 where
+ * Workspace: spd_attn_decode_shared_workspace_bytes(), 16-byte aligned, zeroed once before its first use (each call leaves its
+ * counters at zero), one per stream.  spd_attn_decode_shared_pays: 1 where a call of these sizes takes the kernel that shares, 0 where
  * spd_attn_decode_paged serves it as well (decided on the host, without a launch); _saves: about how many us the call saves
  * then, rounded up (0 where it does not pay).  They take all requests to be in groups of one size that share max_shared_len tokens.
  * The _tokens forms decide by what the host knows of unequal groups, and of batches in which requests of no group stand beside

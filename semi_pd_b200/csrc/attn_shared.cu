@@ -1235,6 +1235,7 @@ static int attn_decode_shared(void* out, const void* q, const void* k_pool, cons
   const int64_t need = spd_attn_decode_shared_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim);
   SPD_REQUIRE(workspace && workspace_bytes >= need, SPD_E_WORKSPACE, "spd_attn_decode_shared: workspace too small (%lld bytes)",
               (long long)workspace_bytes);
+  SPD_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, SPD_E_ALIGN, "spd_attn_decode_shared: workspace must be 16-B aligned");
   const int device_sms = device_sm_count_cached();
   const int sms = sm_budget > 0 && sm_budget < device_sms ? sm_budget : device_sms;
   // What the list can cost at most: no request has more tokens than its row of the page table has entries.

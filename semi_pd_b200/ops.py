@@ -868,12 +868,14 @@ def attn_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
         raise RuntimeError("attn_decode_shared: q and out must have contiguous rows")
     if workspace is None:
         workspace = new_attn_shared_workspace(q.device, B, num_q_heads, num_kv_heads, head_dim)
+    if not workspace.is_contiguous():
+        raise RuntimeError("attn_decode_shared: workspace must be contiguous")
     call, known = (lib.spd_attn_decode_shared, (int(max_shared_len),)) if shared_tokens is None else \
         (lib.spd_attn_decode_shared_tokens, tuple(map(int, shared_tokens)))
     check(call(o2.data_ptr(), q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), req_to_token.data_ptr(), req_pool_indices.data_ptr(),
                seq_lens.data_ptr(), group_indptr.data_ptr(), shared_lens.data_ptr(), B, G, *known, k_pool.shape[0], num_q_heads,
                num_kv_heads, head_dim, q2.stride(0), o2.stride(0), req_to_token.stride(0), float(sm_scale), _dt(q),
-               workspace.data_ptr(), workspace.numel(), get_sm_budget(), _stream()),
+               workspace.data_ptr(), workspace.numel() * workspace.element_size(), get_sm_budget(), _stream()),
           "spd_attn_decode_shared")
     return out
 

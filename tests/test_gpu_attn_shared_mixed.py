@@ -43,3 +43,18 @@ def test_refused_counts():
     for bad in ((-1, 0, 0, 0), (0, -1, 0, 0), (0, 0, -1, 0), (0, 0, 0, -1)):
         with pytest.raises(RuntimeError, match="token counts"):
             _call(c, d, ops.SharedTokens(*bad))
+
+
+def test_refused_workspaces():
+    from semi_pd_b200 import ops
+    c = make_case([(300, [20, 21])], [], 8, 2)
+    d = device(c)
+    need = ops.new_attn_shared_workspace(torch.device("cuda", 0), 2, 8, 2, D).numel()
+    wide = torch.zeros(2 * need + 16, dtype=torch.uint8, device="cuda")
+    for bad, match in ((wide[::2], "contiguous"), (wide[4:], "aligned"), (wide[:need - 16], "too small")):
+        with pytest.raises(RuntimeError, match=match):
+            ops.attn_decode_shared(d["q"], d["k"], d["v"], d["table"], d["rpi"], d["seq"], d["indptr"], d["shared"], 300, 8, 2, D, 0.1,
+                                   workspace=bad)
+    # counted in bytes
+    ops.attn_decode_shared(d["q"], d["k"], d["v"], d["table"], d["rpi"], d["seq"], d["indptr"], d["shared"], 300, 8, 2, D, 0.1,
+                           workspace=torch.zeros(need // 4 + 4, dtype=torch.float32, device="cuda"))
