@@ -47,19 +47,19 @@ struct KvPlace {
 };
 // where the rows of a call lie
 struct KvCopyRows {
-  static constexpr bool kChildren = false;
+  static constexpr bool kChildren = false, kParts = true;
   const int64_t *src, *dst;
   int64_t n;
 };
 struct KvForkRows {
-  static constexpr bool kChildren = true;
+  static constexpr bool kChildren = true, kParts = false;  // (tokens' rows are short, and the parts cost 8 of 106 us)
   const int64_t *parents, *children, *lens, *tail;
   int32_t* table;
   int64_t stride, requests, width;
   int run_len, n;
 };
 struct KvCompactRows {
-  static constexpr bool kChildren = false;
+  static constexpr bool kChildren = false, kParts = true;
   const int64_t *src, *dst, *keep, *indptr, *loc;
   int32_t* table;
   int64_t stride, requests, width, n, total;
@@ -178,11 +178,18 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
   int si = 0;
   while (si + 1 < pl.sets && at.plane >= pl.set[si + 1].first) ++si;
   const KvSet& set = pl.set[si];
-  const int rel = at.plane - set.first, buffer = set.parts == 1 ? rel : rel / set.parts, part = rel - buffer * set.parts;
-  const int pieces = static_cast<int>((set.parts == 1 ? set.row_bytes : static_cast<int64_t>(kKvPart)) / sizeof(V));
-  // (the last part is shorter)
-  const int last = static_cast<int>(min(static_cast<int64_t>(pieces), (set.row_bytes - static_cast<int64_t>(part) * kKvPart) / static_cast<int64_t>(sizeof(V))));
-  char* plane = set.base + buffer * set.stride + static_cast<int64_t>(part) * kKvPart;
+  int pieces, last;
+  char* plane;
+  if constexpr (Rows::kParts) {
+    const int rel = at.plane - set.first, buffer = set.parts == 1 ? rel : rel / set.parts, part = rel - buffer * set.parts;
+    pieces = static_cast<int>((set.parts == 1 ? set.row_bytes : static_cast<int64_t>(kKvPart)) / sizeof(V));
+    // (the last part is shorter)
+    last = static_cast<int>(min(static_cast<int64_t>(pieces), (set.row_bytes - static_cast<int64_t>(part) * kKvPart) / static_cast<int64_t>(sizeof(V))));
+    plane = set.base + buffer * set.stride + static_cast<int64_t>(part) * kKvPart;
+  } else {
+    pieces = last = static_cast<int>(set.row_bytes / sizeof(V));
+    plane = set.base + (at.plane - set.first) * set.stride;
+  }
   __syncthreads();
   const int total = count * pieces;
   for (int i0 = threadIdx.x; i0 < total; i0 += kKvThreads * kKvUnroll) {
@@ -196,7 +203,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_move_kernel(const __grid_consta
         const int r = fastdiv(i, set.pieces_m, set.pieces_s);
         const int64_t s = s_src[r];
         piece[k] = i - r * pieces;
-        if (s >= 0 && s < set.rows && piece[k] < last) {
+        if (s >= 0 && s < set.rows && (!Rows::kParts || piece[k] < last)) {
           row[k] = r;
           const V* from = reinterpret_cast<const V*>(plane + s * set.row_bytes) + piece[k];
           v[k] = Rows::kChildren ? *from : __ldcs(from);  // (a parent's rows are read again)
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_table_kernel(const KvCompactRow
 }
 
 // The plane sets as the kernel takes them, and the bytes of a piece that suits all of them (0 and an error otherwise).
-static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, KvPlanes& pl, int& piece) {
+static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, bool parts, KvPlanes& pl, int& piece) {
   SPD_REQUIRE(sets && num_sets > 0 && num_sets <= kKvSets, SPD_E_BADARG, "%s: 1 to %d plane sets (got %d)", fn, kKvSets, num_sets);
   pl.sets = num_sets;
   pl.planes = 0;
@@ -240,7 +247,7 @@ static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, 
     pl.set[i].rows = s.rows;
     pl.set[i].row_bytes = s.row_bytes;
     pl.set[i].first = pl.planes;
-    pl.set[i].parts = static_cast<int>((s.row_bytes + kKvPart - 1) / kKvPart);
+    pl.set[i].parts = parts ? static_cast<int>((s.row_bytes + kKvPart - 1) / kKvPart) : 1;
     const int64_t planes = pl.planes + static_cast<int64_t>(s.planes) * pl.set[i].parts;
     SPD_REQUIRE(planes < 65535, SPD_E_SHAPE, "%s: too many planes (a row of more than %d bytes counts once for every %d)", fn, kKvPart,
                 kKvPart);
@@ -255,7 +262,7 @@ static int kv_planes(const char* fn, const spd_kv_planes_t* sets, int num_sets, 
 static int kv_rows_per_block(const KvPlanes& pl, int64_t rows) {
   int64_t bytes = 0;
   for (int i = 0; i < pl.sets; ++i) bytes = bytes > pl.set[i].row_bytes ? bytes : pl.set[i].row_bytes;
-  if (bytes > kKvPart) bytes = kKvPart;
+  if (bytes > kKvPart) bytes = kKvPart;  // (a part; without parts it is one row a block either way)
   int64_t per = (32768 + bytes - 1) / bytes;
   const int64_t spread = rows * pl.planes / (4 * device_sm_count_cached()), least = (4096 + bytes - 1) / bytes;
   if (per > spread) per = spread;
@@ -288,7 +295,7 @@ extern "C" {
 int spd_kv_copy(const spd_kv_planes_t* sets, int num_sets, const int64_t* src, const int64_t* dst, int64_t n, spd_stream_t stream) {
   KvPlanes pl;
   int piece;
-  if (int rc = kv_planes("spd_kv_copy", sets, num_sets, pl, piece)) return rc;
+  if (int rc = kv_planes("spd_kv_copy", sets, num_sets, KvCopyRows::kParts, pl, piece)) return rc;
   SPD_REQUIRE(n >= 0 && n < (1ll << 31) && (n == 0 || (src && dst)), SPD_E_BADARG, "spd_kv_copy: bad slots");
   if (n == 0) return 0;
   return kv_move(pl, piece, KvCopyRows{src, dst, n}, n, kv_rows_per_block(pl, n), 1, false, as_stream(stream));
@@ -299,7 +306,7 @@ int spd_kv_fork(const spd_kv_planes_t* sets, int num_sets, int32_t* req_to_token
                 int64_t n, int run_len, spd_stream_t stream) {
   KvPlanes pl;
   int piece;
-  if (int rc = kv_planes("spd_kv_fork", sets, num_sets, pl, piece)) return rc;
+  if (int rc = kv_planes("spd_kv_fork", sets, num_sets, KvForkRows::kParts, pl, piece)) return rc;
   SPD_REQUIRE(req_to_token && n >= 0 && (n == 0 || (parents && children && seq_lens && tail_slots)) && requests > 0 &&
                   max_tokens > 0 && run_len > 0 && req_to_token_stride >= max_tokens,
               SPD_E_BADARG, "spd_kv_fork: bad arguments");
@@ -314,7 +321,7 @@ int spd_kv_compact(const spd_kv_planes_t* sets, int num_sets, int32_t* req_to_to
                    const int64_t* keep_indptr, const int64_t* loc, int64_t n, int64_t total, int write_table, spd_stream_t stream) {
   KvPlanes pl;
   int piece;
-  if (int rc = kv_planes("spd_kv_compact", sets, num_sets, pl, piece)) return rc;
+  if (int rc = kv_planes("spd_kv_compact", sets, num_sets, KvCompactRows::kParts, pl, piece)) return rc;
   SPD_REQUIRE(req_to_token && n >= 0 && total >= 0 && total < (1ll << 31) && requests > 0 && max_tokens > 0 &&
                   req_to_token_stride >= max_tokens && (n == 0 || total == 0 || (src_requests && keep && keep_indptr && loc)),
               SPD_E_BADARG, "spd_kv_compact: bad arguments");

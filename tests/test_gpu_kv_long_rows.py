@@ -34,6 +34,30 @@ def test_copy(kind, n):
         assert torch.equal(b, w)
 
 
+@pytest.mark.parametrize("kind", ["1 MB + 16", "odd", "mixed"])
+def test_fork_and_compact(kind):
+    """Pools of such rows: the partial run of a fork, and what a compaction keeps."""
+    from semi_pd_b200 import ops
+    run, slots = 4, 25
+    g = torch.Generator(device=DEV).manual_seed(3)
+    bufs = [torch.randn(slots, size, generator=g, device=DEV).to(dtype) for size, dtype in ROWS[kind]]
+    planes = ops.KVPlanes(bufs)
+    table = torch.zeros(4, 12, dtype=torch.int32, device=DEV)
+    table[1, :7] = torch.tensor([5, 6, 7, 8, 13, 14, 15], dtype=torch.int32, device=DEV)
+    i64 = lambda *x: torch.tensor(x, device=DEV)  # noqa: E731
+    want = [b.clone() for b in bufs]
+    for w in want:
+        w[17:20] = w[13:16]
+        w[21:24] = w[13:16]
+        w[1:4] = w[i64(5, 8, 15)]
+    ops.kv_fork(planes, table, i64(1, 1), i64(0, 3), i64(7, 7), i64(17, 21), run)
+    ops.kv_compact(planes, table, i64(1), i64(2), i64(0, 3, 6), i64(0, 3), i64(1, 2, 3))
+    for b, w in zip(bufs, want):
+        assert torch.equal(b, w)
+    assert table[0, :7].tolist() == [5, 6, 7, 8, 17, 18, 19] and table[3, :7].tolist() == [5, 6, 7, 8, 21, 22, 23]
+    assert table[2, :3].tolist() == [1, 2, 3]
+
+
 @pytest.mark.parametrize("heads,dim,v_dim", [(32, 128, 128), (64, 64, 128), (5, 256, 259)])
 def test_fork_of_large_states(heads, dim, v_dim):
     """States of 2 MB a request, and of an odd number of floats above 1 MB."""
