@@ -47,6 +47,10 @@ class AttentionBackend(ABC):
     def get_cuda_graph_seq_len_fill_value(self):
         raise NotImplementedError()
 
+    def shares_prefix(self, batch_size: int, shared: SharedPrefix) -> bool:
+        """Whether decode attention takes a batch's shared prefix into account (forward_batch.shared_prefix is set then)."""
+        return False
+
     def forward(self, q, k, v, layer: "RadixAttention", forward_batch: ForwardBatch,
                 save_kv_cache: bool = True):
         if forward_batch.forward_mode.is_decode():

@@ -126,3 +126,13 @@ def test_the_lists_say_more_than_the_longest_prefix():
     plain = SharedPrefix(torch.zeros(102, dtype=torch.int32), torch.zeros(101, dtype=torch.int64), 8192)
     known = SharedPrefix(plain.group_indptr[:2], plain.shared_lens[:1], 8192, ops.SharedTokens(8192, 64 * 8192, 60000, 8400))
     assert not backend.shares_prefix(shared=plain, **lists) and backend.shares_prefix(shared=known, **lists)
+
+
+def test_a_backend_without_such_a_form_reads_by_request():
+    from semi_pd_b200.attention_backend import AttentionBackend
+
+    class Plain(AttentionBackend):
+        def init_forward_metadata(self, forward_batch):
+            pass
+
+    assert Plain().shares_prefix(64, SharedPrefix(torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int64), 8192)) is False
