@@ -622,7 +622,8 @@ def fork_request(kv_pool: KVCache, req_to_token_pool: ReqToTokenPool, allocator:
     try:
         lists = np.concatenate([np.full(n, parent), np.asarray(children), np.full(n, length), tails]).astype(np.int64)
         parents_d, children_d, lens_d, tails_d = allocator._ring.stage(lists, allocator.device).split(n)
-        ops.kv_fork(kv_pool.planes, req_to_token_pool.req_to_token, parents_d, children_d, lens_d, tails_d, R)
+        if any(b is not None and b.numel() for b in kv_pool.buffers()):  # (none where all layers are recurrent: nothing reads the slots)
+            ops.kv_fork(kv_pool.planes, req_to_token_pool.req_to_token, parents_d, children_d, lens_d, tails_d, R)
         rest = length % R > 0
         kv_pool.fork_rows(parent, children, allocator._req_runs[parent][length // R] if rest else None,
                           [allocator._req_runs[c][-1] for c in children] if rest else [],

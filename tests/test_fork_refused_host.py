@@ -12,6 +12,9 @@ class _Pool:
     """What fork_request and compact_request ask of a pool; its second copy is refused."""
     planes = None
 
+    def buffers(self):
+        return [torch.zeros(4, 1)]
+
     def fork_rows(self, *args):
         raise RuntimeError("refused behind the first copy")
 
@@ -90,3 +93,15 @@ def test_compact(monkeypatch):
     alloc.free_req(req)
     alloc.free_req(5)
     assert alloc.available_size() == 20 * R and (alloc._held == 0).all() and (alloc._used == 0).all()
+
+
+def test_a_model_without_cached_tokens_forks_its_states(monkeypatch):
+    """All layers recurrent: there are no rows of tokens to copy, the states of the request slots are."""
+    states = memory_pool.RecurrentStatePool(6, [(2, 4, 4), (1, 4, 8)], "cpu")
+    pool = memory_pool.HybridTokenToKVPool(20 * R, 1, torch.float32, [None, None], "cpu", state_pool=states, run_len=R)
+    table, alloc, parent = _setup(40)
+    copied = []
+    monkeypatch.setattr(ops, "kv_fork", _refuse)
+    monkeypatch.setattr(ops, "kv_copy", lambda planes, src, dst: copied.append((planes is states.planes, src.tolist(), dst.tolist())))
+    children = fork_request(pool, table, alloc, parent, 2)
+    assert len(children) == 2 and copied == [(True, [parent] * 2, children)]
