@@ -274,7 +274,7 @@ class ScheduleBatch:
                          "prior_token_times"):
                 setattr(req, name, list(getattr(parent, name)))
             children.append(req)
-        parent.num_forks += n
+        parent.num_forks += len(children)
         rows = list(range(index + 1)) + [index] * n + list(range(index + 1, len(self.reqs)))
         self.reqs = self.reqs[:index + 1] + children + self.reqs[index + 1:]
         self.seq_lens_host = [self.seq_lens_host[i] for i in rows]

@@ -62,6 +62,7 @@ def test_a_finished_request_is_not_forked():
     reqs, _, _ = gs.extend([[1, 2, 3, 4, 5, 6]])
     first, second = gs.batch.fork_req(0, 2), gs.batch.fork_req(0, 1)
     assert len({r.rid for r in reqs + first + second}) == 4 and len({r.rid for r in gs.batch.fork_req(1, 2)} | {r.rid for r in gs.batch.reqs}) == 6
+    assert gs.batch.fork_req(0, 0) == [] and len(gs.batch.reqs) == 6
     reqs[0].finished_reason = "stop"
     with pytest.raises(RuntimeError, match="finished"):
         gs.batch.fork_req(0, 1)
