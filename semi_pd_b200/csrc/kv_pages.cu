@@ -7,7 +7,7 @@
 // recurrent state is one row) are taken in parts, each as a plane of its own, so that they too are spread over the SMs (one
 // request's states of 2 MB in 24 layers, 101 MB: 16.2 us, 6.2 TB/s).
 // Measured: 12001 latent rows in 27 layers (747 MB) copied in 118 us, 6.3 TB/s; 16 requests' fp32 rows compacted (1.89 GB) in 292,
-// 6.5; 8 parents with 16 children each forked (568 MB, nearly all of it written) in 110, 5.2.  A plain copy has 6.56.
+// 6.5; 8 parents with 16 children each forked (568 MB, nearly all of it written) in 104 - 110, 5.2.  A plain copy has 6.56.
 #include "common.cuh"
 #include "prefill_tiles.cuh"
 #include "ptx.cuh"
