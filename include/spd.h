@@ -25,6 +25,7 @@ typedef void* spd_stream_t; /* cudaStream_t */
 /* element types of activations / weights / KV pool */
 #define SPD_BF16 0
 #define SPD_F16 1
+#define SPD_I8 3  /* operands of spd_linear_logprobs (spd_int8_scaled_mm has no others) */
 #define SPD_F32 2 /* the operators of the "32-bit capable ops" section only */
 
 /* argument-check error codes (CUDA errors are returned as positive cudaError_t values) */
@@ -888,6 +889,35 @@ int spd_short_conv(void* out, const void* x, const void* w, const void* bias, fl
  * (y fp32 [rows, groups * part], z rows of stride z_stride, w [groups * part]) */
 int spd_gated_group_norm(void* out, const float* y, const void* z, const void* w, int64_t rows, int groups, int part,
                          int64_t z_stride, float eps, int dtype, spd_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * models served in 8-bit integers
+ * replaces int8_scaled_mm (K/csrc/gemm/int8_gemm_kernel.cu:562-590) and per_token_quant_int8
+ * (S/layers/quantization/int8_kernel.py), as w8a8_int8 layers call them (S/layers/quantization/w8a8_int8.py)
+ * ------------------------------------------------------------------------------------------- */
+/* q [rows, dim] and scales [rows]: scales = max(max |y|, 1e-10) / 127 over a row, q = y / scales to the nearest integer.
+ *   weight and residual NULL, silu_mul 0:  y = x                        (16-bit y: halves go away from zero)
+ *   weight (dtype, [dim]):                 y = x / rms(x) * weight      in 32 bits
+ *   residual too (rows at x_stride):       residual = x + residual, y its norm, of the sum before it is rounded
+ *   silu_mul 1:                            y = SiLU(x[:dim]) * x[dim:2 dim], in 32 bits
+ * x is bf16 or fp16.  dim: a multiple of 16, at most 32768; x_stride a multiple of 8.  A row with a NaN or an infinity gets a
+ * scale that is none of the numbers (NaN or infinite). */
+int spd_quant_int8(int8_t* q, float* scales, const void* x, void* residual, const void* weight, int64_t rows, int64_t dim,
+                   int64_t x_stride, float eps, int silu_mul, int dtype, spd_stream_t stream);
+/* out[m][n] = scales_a[m] * scales_b[n] * sum_k a[m][k] b[n][k] + bias[n], rounded once to dtype (bf16 or fp16; bias of that type
+ * or NULL).  a [M, K], b [N, K] int8, their sums exact.  K, lda, ldb multiples of 16, N and ldc of 8; K <= 131072.
+ * older_w: as SPD_EPI_OLDER_W.  No workspace. */
+int spd_int8_scaled_mm(void* out, const int8_t* a, const int8_t* b, const float* scales_a, const float* scales_b, const void* bias,
+                       int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int dtype, int older_w,
+                       int sm_budget, spd_stream_t stream);
+/* The log-softmax of x w^T over the V rows of w at one of them for every row of x, without the products reaching memory:
+ * lse[m] = log sum_v exp l[m][v], logprobs[m] = l[m][targets[m]] - lse[m]; a target outside [0, V) asks for nothing and gets 0.
+ * (S/layers/logits_processor.py: input_token_logprobs.)  l is the fp32 accumulator; SPD_I8: times scales_x[m] scales_w[v].
+ * Rows of x and w are multiples of 16 bytes.  The workspace need not be cleared and is free when the call has run. */
+int64_t spd_linear_logprobs_workspace_bytes(int64_t M, int64_t V);
+int spd_linear_logprobs(float* logprobs, float* lse, const void* x, const void* w, const float* scales_x, const float* scales_w,
+                        const int64_t* targets, int64_t M, int64_t V, int64_t K, int64_t ldx, int64_t ldw, int dtype, int older_w,
+                        void* workspace, int64_t workspace_bytes, int sm_budget, spd_stream_t stream);
 
 #ifdef __cplusplus
 }

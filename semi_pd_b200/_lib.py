@@ -20,6 +20,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "spd.h")
 SPD_BF16 = 0
 SPD_F16 = 1
 SPD_F32 = 2
+SPD_I8 = 3
 SPD_EPI_NONE = 0
 SPD_EPI_SILU_MUL = 1
 SPD_EPI_GELU = 2
@@ -104,6 +105,10 @@ SIGNATURES = {
     "spd_kv_copy": (_i, [_p, _i, _p, _p, _i64, _p]),
     "spd_kv_fork": (_i, [_p, _i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _i, _p]),
     "spd_kv_compact": (_i, [_p, _i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i, _p]),
+    "spd_quant_int8": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _i, _i, _p]),
+    "spd_int8_scaled_mm": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _p]),
+    "spd_linear_logprobs_workspace_bytes": (_i64, [_i64, _i64]),
+    "spd_linear_logprobs": (_i, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _i, _p, _i64, _i, _p]),
     "spd_comm_create": (_i, [_i, _i, _i64, C.POINTER(_p), _p]),
     "spd_comm_connect": (_i, [_p, _p]),
     "spd_comm_max_bytes": (_i64, [_p]),

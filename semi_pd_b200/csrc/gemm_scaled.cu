@@ -1,0 +1,755 @@
+// Products whose epilogue works on the accumulator as it comes out of TMEM, in two families of tiles on CTA PAIRS:
+//
+//   int8_scaled_mm    C[m][n] = s_a[m] s_b[n] sum_k a[m][k] b[n][k] + bias[n]     8-bit integers, exact sums in 32-bit integers
+//   linear_logprobs   lse[m] = log sum_v exp l[m][v], logprob[m] = l[m][target[m]] - lse[m],  l = x w^T (8-bit: with both scales),
+//                     without l ever reaching memory: a tile leaves (maximum, sum of exponentials) per token, a second kernel joins
+//                     the tiles of a token
+//
+// 8-bit operands take tcgen05.mma kind::i8, whose instruction covers 32 bytes of K as kind::f16's does, at the same rate: a k-block
+// is 128 bytes of a row in either, and one pipeline serves both.
+//
+// Tokens on N (few_tokens_kernel): D[256 weight rows x n tokens] = W A^T, n a multiple of 32 up to 256.  A cluster of 2 S CTAs has one
+// tile, pair s the k-blocks [s kb / S, (s + 1) kb / S); pairs leave their sums in their own idle ring, and after a cluster barrier each
+// adds all of them for its share of the tokens.  Sums of integers have no order, so nothing depends on S.  Two such CTAs share an SM
+// (their rings together 200 KB in flight): one's start and end run under the other's stream.
+// Tokens on M (many_tokens_kernel): 256 tokens x 256 columns, persistent, two accumulators: a tile's epilogue runs under the next
+// tile's MMAs.
+#include <cuda.h>
+#include <atomic>
+
+#include "common.cuh"
+#include "pair.cuh"
+#include "ptx.cuh"
+#include "row_stage.cuh"
+#include "tmap.cuh"
+
+namespace spd {
+
+enum GemmKind { kInt8 = 0, kKindBf16 = 1, kKindF16 = 2 };
+enum GemmEnd { kScaled = 0, kLogprob = 1 };
+
+constexpr int kGsBlock = 128;                   // bytes of K in a k-block
+constexpr int kGsHalf = 128 * kGsBlock;         // 128 rows of one operand
+constexpr int kGsMaxSmem = 232448;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Instruction descriptor: sums in 32-bit integers of signed 8-bit operands, or in fp32 of 16-bit ones; both operands K-major.
+template <int kKind>
+__device__ __forceinline__ constexpr uint32_t gs_idesc(uint32_t M, uint32_t N) {
+  return (kKind == kInt8 ? (2u << 4) | (1u << 7) | (1u << 10) : kKind == kKindBf16 ? (1u << 4) | (1u << 7) | (1u << 10) : 1u << 4) |
+         ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+template <int kKind>
+__device__ __forceinline__ void gs_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (kKind == kInt8)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    umma_ss_2cta(d, a, b, idesc, accumulate);
+}
+template <int kKind>
+__device__ __forceinline__ float gs_value(uint32_t r) {
+  return kKind == kInt8 ? static_cast<float>(static_cast<int>(r)) : __uint_as_float(r);
+}
+
+struct ScaledParams {
+  void* out;           // kScaled: [m_rows, n_cols]
+  int64_t ldc;
+  const void* bias;    // [n_cols] or null
+  const float* sa;     // a token's scale (8-bit operands)
+  const float* sb;     // a weight row's
+  float2* part;        // kLogprob: [tiles][m_rows] (maximum, sum of exponentials over it)
+  float* hit;          // [m_rows]: the target's logit
+  const int64_t* target;
+  int n_cols, m_rows;
+  int kblocks;
+  int tok_tiles, n;    // tokens on N: token tiles, MMA columns of each
+  int stages, slot;
+  int x_tiles, y_tiles, panel;  // tokens on M
+  int early;           // the weights are older than the kernel before this one: the first of them are fetched before it has ended
+  unsigned* wait_expired;
+};
+
+// (maximum, sum of 2^((v - maximum) log2 e)) of values taken in, in fp32.  An infinite maximum counts as 0: a sum over nothing but
+// -inf stays 0, one with +inf becomes inf, and NaN stays NaN, as in the formula.
+struct LogSum {
+  float m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ static float base(float m) { return fabsf(m) == INFINITY ? 0.f : m * kLog2e; }
+  __device__ __forceinline__ void join(float m2, float s2) {
+    const float t = fmaxf(m, m2), b = base(t);
+    s = (s == 0.f ? 0.f : s * fast_exp2(base(m) - b)) + (s2 == 0.f ? 0.f : s2 * fast_exp2(base(m2) - b));
+    m = t;
+  }
+};
+
+// ------------------------------------------------------------------------------------------------
+// tokens on N
+// ------------------------------------------------------------------------------------------------
+constexpr int kFewThreads = 192;  // warps 0-3: epilogue, 4: TMA, 5: MMA and TMEM
+constexpr int kFewStages = 12;    // at most
+constexpr int kFewFixed = 1024 + 256 + 2048;  // alignment, barriers, a scale and a target for each token
+constexpr int kMaxSplit = 4;
+
+__device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// The maximum (kMax) or sum over the warp's 32 lanes of 32 values each: lane t gets that of value t.
+template <bool kMax>
+__device__ __forceinline__ float warp_reduce_32(float (&v)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < o; ++j) {
+      const float keep = up ? v[j + o] : v[j], send = up ? v[j] : v[j + o];
+      const float got = __shfl_xor_sync(0xffffffffu, send, o);
+      v[j] = kMax ? fmaxf(keep, got) : keep + got;
+    }
+  }
+  return v[0];
+}
+
+template <int kKind, int kEnd, typename T>
+__global__ void __launch_bounds__(kFewThreads, 2)
+few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const ScaledParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * p.slot);  // [stages]  (the leaders' are the live ones)
+  uint64_t* empty = full + kFewStages;
+  uint64_t* tfull = empty + kFewStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* tok_scale = reinterpret_cast<float*>(smem + p.stages * p.slot + 256);  // [256]
+  int* tok_target = reinterpret_cast<int*>(tok_scale + 256);                    // [256]: row of this CTA, or none
+  float2* share = reinterpret_cast<float2*>(smem);                              // [4][256], when the ring is idle
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank(), rank = crank & 1, leader = crank & ~1u;
+  const int S = static_cast<int>(cluster_nctarank() >> 1), s = static_cast<int>(crank >> 1);
+  const int tile = blockIdx.x / (2 * S), wt = tile / p.tok_tiles, tt = tile - wt * p.tok_tiles;
+  const int kb0 = s * p.kblocks / S, kb1 = (s + 1) * p.kblocks / S;
+  const int half = p.n >> 1, tmem_cols = p.n <= 32 ? 32 : p.n <= 64 ? 64 : p.n <= 128 ? 128 : 256;
+  const int tok_base = tt * p.n, tokens = min(p.n, p.m_rows - tok_base);
+  const int row_base = wt * 256 + static_cast<int>(rank) * 128;
+
+  if (warp == 4 && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmA);
+    *dead = 0;
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(tfull, 1);
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc_2cta(tmem_slot, tmem_cols);
+    tmem_relinquish_2cta();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the pair's barriers exist before any cross-CTA signal
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch_dependents();
+
+  if (warp == 4) {
+    if (elect_one()) {
+      const uint32_t lead_full0 = map_to_rank(smem_u32(full), leader);
+      const uint32_t bytes = 2 * (kGsHalf + half * kGsBlock);
+      auto load_w = [&](int stage, int kb) {
+        tma_load_2d_2cta(smem + stage * p.slot, &tmW, lead_full0 + stage * 8, kb * (kGsBlock / 2), row_base,
+                         p.tok_tiles > 1 ? kEvictNormal : kEvictFirst);
+      };
+      const int ahead = min(p.stages, kb1 - kb0);
+      if (!p.early) griddep_wait();
+      for (int i = 0; i < ahead; ++i) {
+        if (rank == 0) mbar_expect_tx(&full[i], bytes);
+        load_w(i, kb0 + i);
+      }
+      if (p.early) griddep_wait();
+      int stage = 0, phase = 0;
+      const int a_row = tok_base + static_cast<int>(rank) * half;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (kb - kb0 >= ahead) {
+          mbar_wait_bounded(&empty[stage], phase ^ 1, dead);
+          if (rank == 0) mbar_expect_tx(&full[stage], bytes);
+          load_w(stage, kb);
+        }
+        tma_load_2d_2cta(smem + stage * p.slot + kGsHalf, &tmA, lead_full0 + stage * 8, kb * (kGsBlock / 2), a_row, kEvictLast);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = gs_idesc<kKind>(256, p.n);
+      const uint16_t both = static_cast<uint16_t>(0b11 << leader);
+      int stage = 0, phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        mbar_wait_bounded(&full[stage], phase, dead);
+        tc_fence_after_sync();
+        const uint32_t wa = smem_u32(smem + stage * p.slot), aa = wa + kGsHalf;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          gs_mma<kKind>(tmem, umma_desc_sw128(wa + k * 32, 16, 1024), umma_desc_sw128(aa + k * 32, 16, 1024), idesc,
+                        (kb > kb0 || k > 0) ? 1u : 0u);
+        umma_commit_2cta_mc(&empty[stage], both);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+      umma_commit_2cta_mc(tfull, both);
+    }
+    __syncwarp();
+  }
+  if (warp < 4) {
+    griddep_wait();  // the tokens' scales and what is written from here on
+    const int row = warp * 32 + lane;
+    const int64_t col = row_base + row;
+    const bool have = col < p.n_cols;
+    const float sb = kKind == kInt8 && have ? p.sb[col] : 1.f;
+    float bias = 0.f;
+    if constexpr (kEnd == kScaled) {
+      if (p.bias && have) bias = to_f32<T>(reinterpret_cast<const T*>(p.bias)[col]);
+    }
+    for (int t = threadIdx.x; t < p.n; t += 128) {
+      tok_scale[t] = kKind == kInt8 && t < tokens ? p.sa[tok_base + t] : 1.f;
+      if constexpr (kEnd == kLogprob) {
+        const int64_t at = t < tokens ? p.target[tok_base + t] : -1;
+        tok_target[t] = at >= row_base && at < row_base + 128 ? static_cast<int>(at - row_base) : -1;
+      }
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    mbar_wait_bounded(tfull, 0, dead);  // every MMA of the pair is done: both rings are idle
+    tc_fence_after_sync();
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+#pragma unroll 1
+    for (int c = 0; c < tokens; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(taddr + c, r);
+      tmem_ld_wait();
+      if constexpr (kEnd == kScaled) {
+        if (S > 1) {
+          uint32_t* part = reinterpret_cast<uint32_t*>(smem) + row;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part[(c + j) * 128] = r[j];
+        } else {
+          T* part = reinterpret_cast<T*>(smem) + row;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part[(c + j) * 128] = from_f32<T>(fmaf(gs_value<kKind>(r[j]) * tok_scale[c + j], sb, bias));
+        }
+      } else {
+        float v[32], e[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          v[j] = kKind == kInt8 ? gs_value<kKind>(r[j]) * tok_scale[c + j] * sb : __uint_as_float(r[j]);
+          if (tok_target[c + j] == row && have) p.hit[tok_base + c + j] = v[j];
+          if (!have) v[j] = -INFINITY;
+          e[j] = v[j];
+        }
+        const float top = warp_reduce_32<true>(e, lane);  // of token c + lane
+        const float base = LogSum::base(top);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = fast_exp2(fmaf(v[j], kLog2e, -__shfl_sync(0xffffffffu, base, j)));
+        const float sum = warp_reduce_32<false>(v, lane);
+        share[warp * 256 + c + lane] = make_float2(top, sum);
+      }
+    }
+    tc_fence_before_sync();
+    if constexpr (kEnd == kScaled) {
+      if (S == 1) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int piece = (threadIdx.x & 15) * 8;  // 16 bytes of a token's 128 columns
+        T* out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(tok_base) * p.ldc + row_base + piece;
+        if (row_base + piece < p.n_cols)
+#pragma unroll 4
+          for (int t = threadIdx.x >> 4; t < tokens; t += 8)
+            *reinterpret_cast<uint4*>(out + t * p.ldc) = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(smem) + t * 128 + piece);
+      }
+    } else {
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int t = threadIdx.x; t < tokens; t += 128) {
+        LogSum all;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) all.join(share[w * 256 + t].x, share[w * 256 + t].y);
+        p.part[static_cast<int64_t>(wt * 2 + rank) * p.m_rows + tok_base + t] = make_float2(all.m, all.s);
+      }
+    }
+  }
+  if (kEnd == kScaled && S > 1) {
+    if (warp >= 4) griddep_wait();  // they write C too
+    __syncwarp();
+    cluster_sync_all();  // all pairs' sums are in place
+    const int tok0 = s * p.n / S, tok1 = min((s + 1) * p.n / S, tokens);
+    const uint32_t base = smem_u32(smem);
+    uint32_t src[kMaxSplit];
+#pragma unroll
+    for (int i = 0; i < kMaxSplit; ++i) src[i] = map_to_rank(base, (i < S ? i : 0) * 2 + rank);
+    const int col = row_base + lane * 4;
+    if (col < p.n_cols) {
+      const float4 sb = make_float4(p.sb[col], p.sb[col + 1], p.sb[col + 2], p.sb[col + 3]);
+      float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p.bias) {
+        const T* b = reinterpret_cast<const T*>(p.bias) + col;
+        bias = make_float4(to_f32<T>(b[0]), to_f32<T>(b[1]), to_f32<T>(b[2]), to_f32<T>(b[3]));
+      }
+#pragma unroll 4
+      for (int t = tok0 + warp; t < tok1; t += kFewThreads / 32) {
+        int4 f[kMaxSplit];
+#pragma unroll
+        for (int i = 0; i < kMaxSplit; ++i)
+          if (i < S) f[i] = ld_cluster_s32x4(src[i] + (t * 128 + lane * 4) * 4);
+        int4 v = f[0];
+#pragma unroll
+        for (int i = 1; i < kMaxSplit; ++i)
+          if (i < S) {
+            v.x += f[i].x;
+            v.y += f[i].y;
+            v.z += f[i].z;
+            v.w += f[i].w;
+          }
+        const float sa = tok_scale[t];
+        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + static_cast<int64_t>(tok_base + t) * p.ldc + col) =
+            make_uint2(pack2<T>(fmaf(static_cast<float>(v.x) * sa, sb.x, bias.x), fmaf(static_cast<float>(v.y) * sa, sb.y, bias.y)),
+                       pack2<T>(fmaf(static_cast<float>(v.z) * sa, sb.z, bias.z), fmaf(static_cast<float>(v.w) * sa, sb.w, bias.w)));
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*dead) {
+    wait_drain();
+    if (threadIdx.x == 0) wait_report(p.wait_expired);
+  }
+  cluster_sync_all();  // nobody leaves while a peer may still read its shared memory or signal its barriers
+  if (warp == 5) tmem_dealloc_2cta(tmem, tmem_cols);
+}
+
+// ------------------------------------------------------------------------------------------------
+// tokens on M
+// ------------------------------------------------------------------------------------------------
+constexpr int kManyThreads = 256;  // warp 0: TMA, 1: MMA, 2: TMEM, 4-7: epilogue
+constexpr int kManyStages = 6;
+constexpr int kManyRing = kManyStages * 2 * kGsHalf;
+constexpr int kManySmem = kManyRing + 4 * kStageWarp + 2 * 256 * 8 + 256 + 1024;
+static_assert(kManySmem <= kGsMaxSmem, "shared memory of a CTA");
+
+__device__ __forceinline__ void many_tile(const ScaledParams& p, int tile, int& xt, int& yt) {
+  const int per_panel = p.x_tiles * p.panel, pn = tile / per_panel, r = tile - pn * per_panel;
+  const int y0 = pn * p.panel, q = min(p.panel, p.y_tiles - y0);
+  xt = r / q;
+  yt = y0 + r - xt * q;
+}
+
+template <int kKind, int kEnd, typename T>
+__global__ void __launch_bounds__(kManyThreads, 1)
+many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const ScaledParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sOut = smem + kManyRing;                                          // kStageWarp per epilogue warp
+  float2* cols = reinterpret_cast<float2*>(sOut + 4 * kStageWarp);           // [2][256] (scale, bias) of a tile's columns
+  uint64_t* full = reinterpret_cast<uint64_t*>(cols + 512);                  // [stages]  (the leader's are the live ones)
+  uint64_t* empty = full + kManyStages;                                      // [stages]
+  uint64_t* tfull = empty + kManyStages;                                     // [2]
+  uint64_t* tempty = tfull + 2;                                              // [2]       (the leader's)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1, num_tiles = p.x_tiles * p.y_tiles;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+    *dead = 0;
+  }
+  if (warp == 1 && lane == 0) {
+    for (int i = 0; i < kManyStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 8);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    tmem_alloc_2cta(tmem_slot, 512);
+    tmem_relinquish_2cta();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA signal
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0, phase = 0;
+      const uint32_t lead_full0 = map_to_rank(smem_u32(full), 0);
+      for (int tile = pair; tile < num_tiles; tile += npairs) {
+        int xt, yt;
+        many_tile(p, tile, xt, yt);
+        const int a_row = xt * 256 + static_cast<int>(rank) * 128, w_row = yt * 256 + static_cast<int>(rank) * 128;
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          mbar_wait_bounded(&empty[stage], phase ^ 1, dead);
+          if (rank == 0) mbar_expect_tx(&full[stage], 4 * kGsHalf);
+          tma_load_2d_2cta(smem + stage * 2 * kGsHalf, &tmA, lead_full0 + stage * 8, kb * (kGsBlock / 2), a_row, kEvictNormal);
+          tma_load_2d_2cta(smem + stage * 2 * kGsHalf + kGsHalf, &tmW, lead_full0 + stage * 8, kb * (kGsBlock / 2), w_row, kEvictNormal);
+          if (++stage == kManyStages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = gs_idesc<kKind>(256, 256);
+      int stage = 0, phase = 0, n = 0;
+      for (int tile = pair; tile < num_tiles; tile += npairs, ++n) {
+        const int as = n & 1;
+        mbar_wait_bounded(&tempty[as], ((n >> 1) & 1) ^ 1, dead);  // both CTAs have drained this accumulator
+        tc_fence_after_sync();
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          mbar_wait_bounded(&full[stage], phase, dead);
+          tc_fence_after_sync();
+          const uint32_t aa = smem_u32(smem + stage * 2 * kGsHalf), wa = aa + kGsHalf;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            gs_mma<kKind>(tmem + as * 256, umma_desc_sw128(aa + k * 32, 16, 1024), umma_desc_sw128(wa + k * 32, 16, 1024), idesc,
+                          (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit_2cta_mc(&empty[stage], 0b11);
+          if (++stage == kManyStages) { stage = 0; phase ^= 1; }
+        }
+        umma_commit_2cta_mc(&tfull[as], 0b11);
+      }
+    }
+  } else if (warp >= 4) {
+    const int q = warp & 3, et = threadIdx.x - 128;
+    uint8_t* stage = sOut + q * kStageWarp;
+    const uint32_t lead_tempty0 = map_to_rank(smem_u32(tempty), 0);
+    int n = 0;
+    for (int tile = pair; tile < num_tiles; tile += npairs, ++n) {
+      int xt, yt;
+      many_tile(p, tile, xt, yt);
+      const int as = n & 1, n0 = yt * 256;
+      const int64_t m0 = static_cast<int64_t>(xt) * 256 + rank * 128 + q * 32;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m_rows - m0));
+      const float2* col = cols + as * 256;
+      if constexpr (kKind == kInt8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = n0 + et + i * 128;
+          float2 sb = make_float2(0.f, 0.f);
+          if (c < p.n_cols) {
+            sb.x = p.sb[c];
+            if (kEnd == kScaled && p.bias) sb.y = to_f32<T>(reinterpret_cast<const T*>(p.bias)[c]);
+          }
+          cols[as * 256 + et + i * 128] = sb;
+        }
+        // (one barrier a tile: a warp that is a tile ahead writes the other half, and cannot get two ahead)
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      const float sa = kKind == kInt8 && lane < rows ? p.sa[m0 + lane] : 1.f;
+      mbar_wait_bounded(&tfull[as], (n >> 1) & 1, dead);
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + as * 256;
+      if constexpr (kEnd == kScaled) {
+        auto values = [&](int c, float (&v)[32]) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(taddr + c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(col + c + j);
+            v[j] = fmaf(gs_value<kKind>(r[j]) * sa, f.x, f.y);
+            v[j + 1] = fmaf(gs_value<kKind>(r[j + 1]) * sa, f.z, f.w);
+          }
+        };
+#pragma unroll 1
+        for (int c = 0; c < 256; c += 64) {
+          if (n0 + c >= p.n_cols) break;
+          float v[32];
+          values(c, v);
+          stage_put16<T>(stage, lane, 0, v);
+          values(c + 32, v);
+          stage_put16<T>(stage, lane, 1, v);
+          stage_out(stage, lane, reinterpret_cast<uint8_t*>(p.out) + (m0 * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
+                    min(64, p.n_cols - n0 - c) * 2);
+        }
+      } else {
+        const int64_t target = lane < rows ? p.target[m0 + lane] - n0 : -1;
+        LogSum all;
+#pragma unroll 1
+        for (int c = 0; c < 256; c += 32) {
+          if (n0 + c >= p.n_cols) break;
+          uint32_t r[32];
+          float v[32], top = -INFINITY;
+          tmem_ld_32x32b_x32(taddr + c, r);
+          tmem_ld_wait();
+          const int valid = p.n_cols - n0 - c;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            v[j] = kKind == kInt8 ? gs_value<kKind>(r[j]) * sa * col[c + j].x : __uint_as_float(r[j]);
+            if (j >= valid) v[j] = -INFINITY;
+            top = fmaxf(top, v[j]);
+          }
+          if (target >= c && target < c + 32 && target < c + valid) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (target == c + j) p.hit[m0 + lane] = v[j];
+          }
+          const float base = LogSum::base(top);
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            s0 += fast_exp2(fmaf(v[j], kLog2e, -base));
+            s1 += fast_exp2(fmaf(v[j + 1], kLog2e, -base));
+          }
+          all.join(top, s0 + s1);
+        }
+        if (lane < rows) p.part[static_cast<int64_t>(yt) * p.m_rows + m0 + lane] = make_float2(all.m, all.s);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote_release(lead_tempty0 + as * 8);
+    }
+  }
+
+  __syncwarp();  // the warps of the elected lanes come together before the barriers, which count whole warps
+  griddep_launch_dependents();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*dead) {
+    wait_drain();
+    if (threadIdx.x == 0) wait_report(p.wait_expired);
+  }
+  cluster_sync_all();  // the peer may still read this CTA's shared memory / signal its barriers
+  if (warp == 2) tmem_dealloc_2cta(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------
+// the tiles of a token joined
+// ------------------------------------------------------------------------------------------------
+constexpr int kJoinThreads = 256;
+
+// `width` tokens of a CTA beside one another (a power of two up to 32), kJoinThreads / width shares of the tiles for each
+__global__ void __launch_bounds__(kJoinThreads)
+logprob_join_kernel(float* __restrict__ logprobs, float* __restrict__ lse, const float2* __restrict__ part, const float* __restrict__ hit,
+                    const int64_t* __restrict__ target, int tokens, int tiles, int vocab, int width) {
+  __shared__ float2 sums[kJoinThreads];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int t = blockIdx.x * width + (threadIdx.x & (width - 1)), shares = kJoinThreads / width;
+  LogSum all;
+  if (t < tokens)
+    for (int i = threadIdx.x / width; i < tiles; i += shares) {
+      const float2 f = part[static_cast<int64_t>(i) * tokens + t];
+      all.join(f.x, f.y);
+    }
+  sums[threadIdx.x] = make_float2(all.m, all.s);
+  for (int o = shares >> 1; o > 0; o >>= 1) {
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < o * width) {
+      const float2 f = sums[threadIdx.x + o * width];
+      all.join(f.x, f.y);
+      sums[threadIdx.x] = make_float2(all.m, all.s);
+    }
+  }
+  if (static_cast<int>(threadIdx.x) < width && t < tokens) {
+    const float z = (LogSum::base(all.m) + log2f(all.s)) * kLn2;
+    const int64_t at = target[t];
+    lse[t] = z;
+    logprobs[t] = at >= 0 && at < vocab ? hit[t] - z : 0.f;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------
+// the kernel's limit of shared memory, once on every device
+template <typename K>
+static int allow_smem(K kern, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  SPD_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    SPD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGsMaxSmem));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return 0;
+}
+
+template <typename K>
+static int launch_pairs(K kern, std::atomic<uint64_t>& done, int ctas, int cluster, int threads, int smem, cudaStream_t stream,
+                        const CUtensorMap& t0, const CUtensorMap& t1, const ScaledParams& p) {
+  if (int rc = allow_smem(kern, done)) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  SPD_CUDA(cudaLaunchKernelEx(&cfg, kern, t0, t1, p));
+  return 0;
+}
+
+// How a product is cut: token tiles and pairs of a tile for tokens on N, or tiles of 256 x 256 (tok_tiles 0).
+struct ScaledPlan {
+  int tok_tiles, split, smem;
+};
+
+static ScaledPlan scaled_plan(int64_t M, int64_t N, int kblocks, int sms, bool may_split) {
+  ScaledPlan plan{0, 1, 0};
+  if (M > 256) return plan;
+  plan.tok_tiles = 1;
+  const int n = static_cast<int>(32 * (((M + 31) / 32 + plan.tok_tiles - 1) / plan.tok_tiles));
+  const int64_t w_tiles = (N + 255) / 256;
+  if (may_split)
+    for (int s = 2; s <= kMaxSplit; ++s)
+      if (w_tiles * plan.tok_tiles * 2 * s <= (n <= 160 ? 2 * sms : sms) && kblocks >= 4 * s && s != 3) plan.split = s;
+  plan.smem = (n <= 160 || plan.split == 1) && w_tiles * plan.tok_tiles * 2 * plan.split > sms ? 115712 : kGsMaxSmem;
+  return plan;
+}
+
+// ring slots for tokens on N; the sums (of one pair: the results) have to fit the ring
+static void few_ring(ScaledParams& p, const ScaledPlan& plan) {
+  p.slot = kGsHalf + p.n / 2 * kGsBlock;
+  const int fit = (plan.smem - kFewFixed) / p.slot, most = (p.kblocks + plan.split - 1) / plan.split;
+  const int sums = (p.n * (plan.split > 1 ? 512 : 256) + p.slot - 1) / p.slot;
+  p.stages = fit < kFewStages ? fit : kFewStages;
+  if (p.stages > most) p.stages = most < sums ? sums : most;
+}
+
+template <int kKind, int kEnd, typename T>
+static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, int64_t kbytes, int64_t a_stride, int64_t w_stride,
+                          ScaledParams p, const ScaledPlan& plan, int sms, cudaStream_t stream) {
+  // rows as 16-bit elements: the copies move bytes
+  CUtensorMap ta, tw;
+  p.n_cols = static_cast<int>(N);
+  p.m_rows = static_cast<int>(M);
+  p.kblocks = static_cast<int>((kbytes + kGsBlock - 1) / kGsBlock);
+  if (int rc = wait_flag(&p.wait_expired)) return rc;
+  p.tok_tiles = plan.tok_tiles;
+  if (plan.tok_tiles > 0) {
+    p.n = static_cast<int>(32 * (((M + 31) / 32 + plan.tok_tiles - 1) / plan.tok_tiles));
+    few_ring(p, plan);
+    if (int rc = make_tmap_2d_sw128(&tw, w, N, kbytes / 2, w_stride / 2, 128, kGsBlock / 2)) return rc;
+    if (int rc = make_tmap_2d_sw128(&ta, a, M, kbytes / 2, a_stride / 2, p.n / 2, kGsBlock / 2)) return rc;
+    static std::atomic<uint64_t> done{0};
+    const int ctas = static_cast<int>((N + 255) / 256) * plan.tok_tiles * 2 * plan.split;
+    return launch_pairs(few_tokens_kernel<kKind, kEnd, T>, done, ctas, 2 * plan.split, kFewThreads, p.stages * p.slot + kFewFixed, stream,
+                        tw, ta, p);
+  }
+  if (int rc = make_tmap_2d_sw128(&tw, w, N, kbytes / 2, w_stride / 2, 128, kGsBlock / 2)) return rc;
+  if (int rc = make_tmap_2d_sw128(&ta, a, M, kbytes / 2, a_stride / 2, 128, kGsBlock / 2)) return rc;
+  p.x_tiles = static_cast<int>((M + 255) / 256);
+  p.y_tiles = static_cast<int>((N + 255) / 256);
+  // weight tiles of a rasterisation panel: as many as stay in L2 beside what else passes (gemm.cu)
+  const int64_t q = (40ll << 20) / (256 * kbytes);
+  p.panel = static_cast<int>(q < 1 ? 1 : q < p.y_tiles ? q : p.y_tiles);
+  const int64_t tiles = static_cast<int64_t>(p.x_tiles) * p.y_tiles;
+  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  static std::atomic<uint64_t> done{0};
+  return launch_pairs(many_tokens_kernel<kKind, kEnd, T>, done, 2 * pairs, 2, kManyThreads, kManySmem, stream, ta, tw, p);
+}
+
+static int budget(int sm_budget) {
+  const int sms = sm_budget > 0 ? sm_budget : device_sm_count_cached();
+  return sms < 2 ? 2 : sms;
+}
+
+}  // namespace spd
+
+using namespace spd;
+
+extern "C" {
+
+int spd_int8_scaled_mm(void* out, const int8_t* a, const int8_t* b, const float* scales_a, const float* scales_b, const void* bias,
+                       int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int dtype, int older_w, int sm_budget,
+                       spd_stream_t stream) {
+  SPD_REQUIRE(M >= 0 && N > 0 && K > 0 && M <= 0x7fffff00 && N <= 0x7fffff00, SPD_E_BADARG, "spd_int8_scaled_mm: bad sizes");
+  SPD_REQUIRE(K <= 131072, SPD_E_SHAPE, "spd_int8_scaled_mm: sums of more than 131072 products may not fit 32 bits");
+  SPD_REQUIRE(dtype == SPD_BF16 || dtype == SPD_F16, SPD_E_BADARG, "spd_int8_scaled_mm: bad dtype %d", dtype);
+  SPD_REQUIRE(K % 16 == 0 && N % 8 == 0 && lda % 16 == 0 && ldb % 16 == 0 && ldc % 8 == 0, SPD_E_ALIGN,
+              "spd_int8_scaled_mm: K, lda and ldb must be multiples of 16, N and ldc of 8");
+  SPD_REQUIRE(lda >= K && ldb >= K && ldc >= N, SPD_E_BADARG, "spd_int8_scaled_mm: leading dimension too small");
+  if (M == 0) return 0;
+  SPD_REQUIRE(out && a && b && scales_a && scales_b, SPD_E_BADARG, "spd_int8_scaled_mm: null pointer");
+  SPD_REQUIRE(aligned16(out) && aligned16(a) && aligned16(b), SPD_E_ALIGN, "spd_int8_scaled_mm: pointers must be 16-byte aligned");
+  ScaledParams p{};
+  p.out = out;
+  p.ldc = ldc;
+  p.bias = bias;
+  p.sa = scales_a;
+  p.sb = scales_b;
+  p.early = older_w;
+  const int sms = budget(sm_budget);
+  const ScaledPlan plan = scaled_plan(M, N, static_cast<int>((K + kGsBlock - 1) / kGsBlock), sms, true);
+  SPD_DISPATCH_DTYPE(dtype, { return (scaled_product<kInt8, kScaled, T>(a, b, M, N, K, lda, ldb, p, plan, sms, as_stream(stream))); });
+}
+
+int64_t spd_linear_logprobs_workspace_bytes(int64_t M, int64_t V) {
+  if (M < 0 || V <= 0) return SPD_E_BADARG;
+  return M * ((V + 255) / 256 * 16 + 4);  // two parts of every 256 vocabulary rows, the target's logit
+}
+
+int spd_linear_logprobs(float* logprobs, float* lse, const void* x, const void* w, const float* scales_x, const float* scales_w,
+                        const int64_t* targets, int64_t M, int64_t V, int64_t K, int64_t ldx, int64_t ldw, int dtype, int older_w,
+                        void* workspace, int64_t workspace_bytes, int sm_budget, spd_stream_t stream) {
+  SPD_REQUIRE(M >= 0 && V > 0 && K > 0 && M <= 0x7fffff00 && V <= 0x7fffff00, SPD_E_BADARG, "spd_linear_logprobs: bad sizes");
+  SPD_REQUIRE(dtype == SPD_BF16 || dtype == SPD_F16 || dtype == SPD_I8, SPD_E_BADARG, "spd_linear_logprobs: bad dtype %d", dtype);
+  const int size = dtype == SPD_I8 ? 1 : 2;
+  SPD_REQUIRE(dtype != SPD_I8 || K <= 131072, SPD_E_SHAPE, "spd_linear_logprobs: sums of more than 131072 products may not fit 32 bits");
+  SPD_REQUIRE(K * size % 16 == 0 && ldx * size % 16 == 0 && ldw * size % 16 == 0, SPD_E_ALIGN,
+              "spd_linear_logprobs: rows must be multiples of 16 bytes");
+  SPD_REQUIRE(ldx >= K && ldw >= K, SPD_E_BADARG, "spd_linear_logprobs: leading dimension too small");
+  if (M == 0) return 0;
+  SPD_REQUIRE(logprobs && lse && x && w && targets && workspace, SPD_E_BADARG, "spd_linear_logprobs: null pointer");
+  SPD_REQUIRE((dtype == SPD_I8) == (scales_x != nullptr) && (dtype == SPD_I8) == (scales_w != nullptr), SPD_E_BADARG,
+              "spd_linear_logprobs: 8-bit operands and no others have scales");
+  SPD_REQUIRE(aligned16(x) && aligned16(w) && aligned16(workspace), SPD_E_ALIGN, "spd_linear_logprobs: pointers must be 16-byte aligned");
+  SPD_REQUIRE(workspace_bytes >= spd_linear_logprobs_workspace_bytes(M, V), SPD_E_WORKSPACE, "spd_linear_logprobs: workspace too small");
+  const int sms = budget(sm_budget);
+  ScaledParams p{};
+  p.sa = scales_x;
+  p.sb = scales_w;
+  p.target = targets;
+  p.part = reinterpret_cast<float2*>(workspace);
+  p.early = older_w;
+  const int64_t kbytes = K * size;
+  const ScaledPlan plan = scaled_plan(M, V, static_cast<int>((kbytes + kGsBlock - 1) / kGsBlock), sms, false);
+  const int tiles = static_cast<int>((V + 255) / 256) * (plan.tok_tiles > 0 ? 2 : 1);
+  p.hit = reinterpret_cast<float*>(p.part + tiles * M);
+  cudaStream_t st = as_stream(stream);
+  int rc;
+  if (dtype == SPD_I8) rc = scaled_product<kInt8, kLogprob, __nv_bfloat16>(x, w, M, V, kbytes, ldx, ldw, p, plan, sms, st);
+  else if (dtype == SPD_BF16) rc = scaled_product<kKindBf16, kLogprob, __nv_bfloat16>(x, w, M, V, kbytes, 2 * ldx, 2 * ldw, p, plan, sms, st);
+  else rc = scaled_product<kKindF16, kLogprob, __half>(x, w, M, V, kbytes, 2 * ldx, 2 * ldw, p, plan, sms, st);
+  if (rc) return rc;
+  int width = 1;
+  while (width < 32 && width < M) width *= 2;
+  SPD_CUDA(launch(logprob_join_kernel, dim3(static_cast<unsigned>((M + width - 1) / width)), dim3(kJoinThreads), 0, st, pdl_enabled(), logprobs,
+                  lse, p.part, p.hit, targets, static_cast<int>(M), tiles, static_cast<int>(V), width));
+  return 0;
+}
+
+}  // extern "C"

@@ -12,7 +12,7 @@ import contextlib
 import ctypes
 import functools
 import os
-from typing import NamedTuple, Optional, Sequence
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -57,6 +57,15 @@ def _here(fn: str, *ts: Optional[torch.Tensor]) -> None:
     for t in ts:
         if t is not None and t.device.index != here:
             raise RuntimeError(f"{fn}: a tensor is on {t.device}, the current device is cuda:{here}")
+
+
+def _all_here(fn: str, *ts: Optional[torch.Tensor]) -> None:
+    """_cuda and _here in one pass (0.05 us a tensor)."""
+    here = torch._C._cuda_getDevice()
+    for t in ts:
+        if t is not None and t.get_device() != here:
+            _cuda(t)
+            _here(fn, t)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -482,6 +491,121 @@ def _silu_fused(M: int, N: int, K: int, sm_budget: int) -> bool:
 def silu_fused(x: torch.Tensor, weight: torch.Tensor) -> bool:
     """Whether linear(x, weight, epilogue=SPD_EPI_SILU_MUL) serves as well as linear and silu_and_mul."""
     return _silu_fused(x.shape[0], weight.shape[0] // 2, x.shape[1], get_sm_budget())
+
+
+# ------------------------------------------------------------------------------------------------
+# models served in 8-bit integers
+# ------------------------------------------------------------------------------------------------
+def _quant_int8(fn: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
+                silu_mul: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    _all_here(fn, x, residual, weight)
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise RuntimeError(f"{fn}: the input is 2-D with a contiguous last dimension")
+    rows, cols = x.shape
+    dim = cols // 2 if silu_mul else cols
+    if weight is not None and (weight.dtype != x.dtype or weight.dim() != 1 or weight.numel() != dim or not weight.is_contiguous()):
+        raise RuntimeError(f"{fn}: the weight is a contiguous [{dim}] of the input's type")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape
+                                 or not (residual.is_contiguous() and x.is_contiguous())):
+        raise RuntimeError(f"{fn}: input and residual are contiguous, of one shape and type")
+    if silu_mul and cols % 2:
+        raise RuntimeError(f"{fn}: the last dimension is gate || up, halves of one size")
+    q = torch.empty((rows, dim), device=x.device, dtype=torch.int8)
+    scales = torch.empty((rows, 1), device=x.device, dtype=torch.float32)
+    check(lib.spd_quant_int8(q.data_ptr(), scales.data_ptr(), x.data_ptr(), residual.data_ptr() if residual is not None else None,
+                             weight.data_ptr() if weight is not None else None, rows, dim, x.stride(0) if rows > 1 else cols,
+                             float(eps), silu_mul, _dt(x), _stream()), "spd_quant_int8")
+    return q, scales
+
+
+def per_token_quant_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q int8 [M, K], scales f32 [M, 1]): scales = max(max |x|, 1e-10) / 127 of a row, q = x / scales to the nearest integer, halves
+    away from zero (S/layers/quantization/int8_kernel.py: per_token_quant_int8).  x bf16 / fp16, rows may be strided."""
+    return _quant_int8("per_token_quant_int8", x, None, None, 0.0, 0)
+
+
+def rmsnorm_quant_int8(input: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """per_token_quant_int8 of rmsnorm(input, weight, eps) in one pass, the norm kept in 32 bits."""
+    return _quant_int8("rmsnorm_quant_int8", input, None, weight, eps, 0)
+
+
+def fused_add_rmsnorm_quant_int8(input: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6
+                                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """residual += input in place, and per_token_quant_int8 of its norm in one pass; `input` stays as it is."""
+    return _quant_int8("fused_add_rmsnorm_quant_int8", input, residual, weight, eps, 0)
+
+
+def silu_and_mul_quant_int8(input: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """per_token_quant_int8 of silu(input[:, :d]) * input[:, d:] in one pass, the product kept in 32 bits."""
+    return _quant_int8("silu_and_mul_quant_int8", input, None, None, 0.0, 1)
+
+
+def int8_scaled_mm(mat_a: torch.Tensor, mat_b: torch.Tensor, scales_a: torch.Tensor, scales_b: torch.Tensor, out_dtype: torch.dtype,
+                   bias: Optional[torch.Tensor] = None, older_weight: bool = False) -> torch.Tensor:
+    """scales_a[m] scales_b[n] (mat_a mat_b)[m, n] + bias[n], rounded once (sgl-kernel/python/sgl_kernel/gemm.py: int8_scaled_mm).
+    mat_a int8 [M, K] with contiguous rows; mat_b int8 [K, N] with contiguous columns (`weight.t()`); scales_a fp32, M of them;
+    scales_b fp32, N; bias [N] of out_dtype, bf16 or fp16.  K is a multiple of 16, N of 8.  older_weight: as in `linear`."""
+    _all_here("int8_scaled_mm", mat_a, mat_b, scales_a, scales_b, bias)
+    if mat_a.dim() != 2 or mat_b.dim() != 2:
+        raise RuntimeError("int8_scaled_mm: mat_a and mat_b must be 2-D")
+    M, K = mat_a.shape
+    N = mat_b.shape[1]
+    if mat_a.dtype != torch.int8 or mat_b.dtype != torch.int8:
+        raise RuntimeError("int8_scaled_mm: mat_a and mat_b must be int8")
+    if mat_a.stride(1) != 1 or mat_b.stride(0) != 1:
+        raise RuntimeError("int8_scaled_mm: mat_a must be row-major, mat_b column-major")
+    if mat_b.shape[0] != K:
+        raise RuntimeError(f"int8_scaled_mm: mat_a is [{M}, {K}], mat_b {list(mat_b.shape)}")
+    if (scales_a.dtype != torch.float32 or scales_b.dtype != torch.float32 or scales_a.numel() != M or scales_b.numel() != N
+            or not scales_a.is_contiguous() or not scales_b.is_contiguous()):
+        raise RuntimeError("int8_scaled_mm: scales are contiguous fp32, one for each row of mat_a and each column of mat_b")
+    if out_dtype not in _DTYPE:
+        raise RuntimeError(f"int8_scaled_mm: out_dtype is bfloat16 or float16, got {out_dtype}")
+    if bias is not None and (bias.dtype != out_dtype or bias.numel() != N or not bias.is_contiguous()):
+        raise RuntimeError("int8_scaled_mm: bias is a contiguous [N] of out_dtype")
+    out = torch.empty((M, N), device=mat_a.device, dtype=out_dtype)
+    check(lib.spd_int8_scaled_mm(out.data_ptr(), mat_a.data_ptr(), mat_b.data_ptr(), scales_a.data_ptr(), scales_b.data_ptr(),
+                                 bias.data_ptr() if bias is not None else None, M, N, K, mat_a.stride(0) if M > 1 else K,
+                                 mat_b.stride(1) if N > 1 else K, N, _DTYPE[out_dtype], 1 if older_weight else 0, get_sm_budget(),
+                                 _stream()), "spd_int8_scaled_mm")
+    return out
+
+
+def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, x_scales: Optional[torch.Tensor] = None,
+                    weight_scales: Optional[torch.Tensor] = None, older_weight: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(logprobs f32 [M], logsumexp f32 [M]) of the logits x @ weight.T [M, V], which are never stored: log-softmax over the rows of
+    `weight` at targets[m] (int64); a target outside [0, V) asks for nothing and gets 0.  x and weight are bf16 or fp16, or both
+    int8 with fp32 scales for each row of either.  older_weight: as in `linear`."""
+    _all_here("linear_logprobs", x, weight, targets, x_scales, weight_scales)
+    if x.dim() != 2 or weight.dim() != 2 or x.stride(1) != 1 or weight.stride(1) != 1 or x.shape[1] != weight.shape[1]:
+        raise RuntimeError("linear_logprobs: x [M, K] and weight [V, K] with contiguous last dimension")
+    if x.dtype != weight.dtype:
+        raise RuntimeError("linear_logprobs: x and weight must have the same dtype")
+    M, K = x.shape
+    V = weight.shape[0]
+    if targets.dtype != torch.int64 or targets.shape != (M,) or not targets.is_contiguous():
+        raise RuntimeError("linear_logprobs: targets is a contiguous int64 list, one for each row of x")
+    if x.dtype == torch.int8:
+        if (x_scales is None or weight_scales is None or x_scales.dtype != torch.float32 or weight_scales.dtype != torch.float32
+                or x_scales.numel() != M or weight_scales.numel() != V or not x_scales.is_contiguous()
+                or not weight_scales.is_contiguous()):
+            raise RuntimeError("linear_logprobs: int8 operands come with contiguous fp32 scales, one for each row of x and of weight")
+        dtype = _lib.SPD_I8
+    else:
+        if x_scales is not None or weight_scales is not None:
+            raise RuntimeError("linear_logprobs: scales belong to int8 operands")
+        dtype = _dt(x)
+    out = torch.empty((2, M), device=x.device, dtype=torch.float32)
+    if M == 0:
+        return out[0], out[1]
+    need = lib.spd_linear_logprobs_workspace_bytes(M, V)
+    ws = torch.empty((need,), device=x.device, dtype=torch.uint8)
+    check(lib.spd_linear_logprobs(out.data_ptr(), out[1].data_ptr(), x.data_ptr(), weight.data_ptr(),
+                                  x_scales.data_ptr() if x_scales is not None else None,
+                                  weight_scales.data_ptr() if weight_scales is not None else None, targets.data_ptr(), M, V, K,
+                                  x.stride(0) if M > 1 else K, weight.stride(0) if V > 1 else K, dtype, 1 if older_weight else 0,
+                                  ws.data_ptr(), need, get_sm_budget(), _stream()), "spd_linear_logprobs")
+    return out[0], out[1]
 
 
 def linear_block_diag(x: torch.Tensor, weight: torch.Tensor, num_groups: int, k: int, n: int,
