@@ -56,6 +56,12 @@ __device__ __forceinline__ float gs_value(uint32_t r) {
   return kKind == kInt8 ? static_cast<float>(static_cast<int>(r)) : __uint_as_float(r);
 }
 
+// All threads of the cluster are here; nothing that they wrote is meant to be seen.  (With release semantics the barrier waits for
+// every store to global memory that is still on its way: 1 us at a kernel's end.)
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
 struct ScaledParams {
   void* out;           // kScaled: [m_rows, n_cols]
   int64_t ldc;
@@ -223,7 +229,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       tok_scale[t] = kKind == kInt8 && t < tokens ? p.sa[tok_base + t] : 1.f;
       if constexpr (kEnd == kLogprob) {
         const int64_t at = t < tokens ? p.target[tok_base + t] : -1;
-        tok_target[t] = at >= row_base && at < row_base + 128 ? static_cast<int>(at - row_base) : -1;
+        tok_target[t] = at >= row_base && at < min(row_base + 128, p.n_cols) ? static_cast<int>(at - row_base) : -1;
       }
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -235,6 +241,11 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       uint32_t r[32];
       tmem_ld_32x32b_x32(taddr + c, r);
       tmem_ld_wait();
+      float sa[32];  // read before the first store: a load between two stores to shared memory waits for its turn, 1 us a chunk
+      auto scales = [&]() {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(sa + j) = *reinterpret_cast<const float4*>(tok_scale + c + j);
+      };
       if constexpr (kEnd == kScaled) {
         if (S > 1) {
           uint32_t* part = reinterpret_cast<uint32_t*>(smem) + row;
@@ -242,15 +253,20 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
           for (int j = 0; j < 32; ++j) part[(c + j) * 128] = r[j];
         } else {
           T* part = reinterpret_cast<T*>(smem) + row;
+          scales();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) part[(c + j) * 128] = from_f32<T>(fmaf(gs_value<kKind>(r[j]) * tok_scale[c + j], sb, bias));
+          for (int j = 0; j < 32; ++j) part[(c + j) * 128] = from_f32<T>(fmaf(gs_value<kKind>(r[j]) * sa[j], sb, bias));
         }
       } else {
         float v[32], e[32];
+        if constexpr (kKind == kInt8) scales();
+        int hit[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) *reinterpret_cast<int4*>(hit + j) = *reinterpret_cast<const int4*>(tok_target + c + j);
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          v[j] = kKind == kInt8 ? gs_value<kKind>(r[j]) * tok_scale[c + j] * sb : __uint_as_float(r[j]);
-          if (tok_target[c + j] == row && have) p.hit[tok_base + c + j] = v[j];
+          v[j] = kKind == kInt8 ? gs_value<kKind>(r[j]) * sa[j] * sb : __uint_as_float(r[j]);
+          if (hit[j] == row) p.hit[tok_base + c + j] = v[j];
           if (!have) v[j] = -INFINITY;
           e[j] = v[j];
         }
@@ -330,7 +346,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     wait_drain();
     if (threadIdx.x == 0) wait_report(p.wait_expired);
   }
-  cluster_sync_all();  // nobody leaves while a peer may still read its shared memory or signal its barriers
+  cluster_sync_relaxed();  // nobody leaves while a peer may still read its shared memory or signal its barriers
   if (warp == 5) tmem_dealloc_2cta(tmem, tmem_cols);
 }
 
@@ -534,7 +550,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     wait_drain();
     if (threadIdx.x == 0) wait_report(p.wait_expired);
   }
-  cluster_sync_all();  // the peer may still read this CTA's shared memory / signal its barriers
+  cluster_sync_relaxed();  // the peer may still read this CTA's shared memory / signal its barriers
   if (warp == 2) tmem_dealloc_2cta(tmem, 512);
 }
 
@@ -543,7 +559,9 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 // ------------------------------------------------------------------------------------------------
 constexpr int kJoinThreads = 256;
 
-// `width` tokens of a CTA beside one another (a power of two up to 32), kJoinThreads / width shares of the tiles for each
+// `width` tokens of a CTA beside one another (1, 2 or 4: 32 bytes of every tile), kJoinThreads / width shares of the tiles for each.
+// Bound by the latency of its loads, so a share is short and takes four tiles at a time (32 tokens, 1002 parts: 30 us with 8 shares a
+// token).
 __global__ void __launch_bounds__(kJoinThreads)
 logprob_join_kernel(float* __restrict__ logprobs, float* __restrict__ lse, const float2* __restrict__ part, const float* __restrict__ hit,
                     const int64_t* __restrict__ target, int tokens, int tiles, int vocab, int width) {
@@ -553,9 +571,13 @@ logprob_join_kernel(float* __restrict__ logprobs, float* __restrict__ lse, const
   const int t = blockIdx.x * width + (threadIdx.x & (width - 1)), shares = kJoinThreads / width;
   LogSum all;
   if (t < tokens)
-    for (int i = threadIdx.x / width; i < tiles; i += shares) {
-      const float2 f = part[static_cast<int64_t>(i) * tokens + t];
-      all.join(f.x, f.y);
+    for (int i = threadIdx.x / width; i < tiles; i += 4 * shares) {
+      float2 f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = i + j * shares < tiles ? part[static_cast<int64_t>(i + j * shares) * tokens + t] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) all.join(f[j].x, f[j].y);
     }
   sums[threadIdx.x] = make_float2(all.m, all.s);
   for (int o = shares >> 1; o > 0; o >>= 1) {
@@ -616,27 +638,86 @@ static int launch_pairs(K kern, std::atomic<uint64_t>& done, int ctas, int clust
 struct ScaledPlan {
   int tok_tiles, split, smem;
 };
+constexpr int kHalfSmem = 113 * 1024;  // of a CTA that shares its SM with another
 
-static ScaledPlan scaled_plan(int64_t M, int64_t N, int kblocks, int sms, bool may_split) {
+// Shared memory for the ring of a CTA with tokens on N: `slots` of what it takes for n tokens
+static int few_slots(int n, int smem) {
+  const int slots = (smem - kFewFixed) / (kGsHalf + n / 2 * kGsBlock);
+  return slots < kFewStages ? slots : kFewStages;
+}
+
+// Clusters of 2 S CTAs that run at once, one CTA an SM (a partition: by its share of the SMs)
+static int clusters_at_once(int S, int sms) {
+  static const int b200[kMaxSplit + 1] = {0, 74, 33, 22, 15};
+  const int share = b200[S] * sms / 148, most = sms / (2 * S);
+  return share < most ? share : most;
+}
+
+// Every form's time in us as fitted to 162 products (1 - 3000 tokens; 1024 x 8192, 4096 x 4096 to 4096 x 14336, 5000 x 1360, 5632 x 1024,
+// 6144 x 4096, 8192 x 8192, 16384 x 2048, 28672 x 4096), weights out of L2; the form chosen took 1.02 times the fastest one's time in the
+// mean, 1.19 at most.  Tokens on N, all tiles at once: a k-block of 128 bytes takes a pair 0.18 to 0.26 (half the ring: 1.5 times
+// that), two pairs on an SM 0.13 to 0.30 each, the weights 7.7 GB/ms; then the epilogue, longer where two CTAs on an SM are in it
+// at once, and the pairs' sums.  Tokens on M: 0.29 a k-block and 1.9 a tile.
+static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
+  const int64_t w_tiles = (N + 255) / 256, waves = ((M + 255) / 256 * w_tiles + sms / 2 - 1) / (sms / 2);
   ScaledPlan plan{0, 1, 0};
-  if (M > 256) return plan;
-  plan.tok_tiles = 1;
-  const int n = static_cast<int>(32 * (((M + 31) / 32 + plan.tok_tiles - 1) / plan.tok_tiles));
-  const int64_t w_tiles = (N + 255) / 256;
-  if (may_split)
-    for (int s = 2; s <= kMaxSplit; ++s)
-      if (w_tiles * plan.tok_tiles * 2 * s <= (n <= 160 ? 2 * sms : sms) && kblocks >= 4 * s && s != 3) plan.split = s;
-  plan.smem = (n <= 160 || plan.split == 1) && w_tiles * plan.tok_tiles * 2 * plan.split > sms ? 115712 : kGsMaxSmem;
+  double best = 6.4 + static_cast<double>(waves) * (0.288 * kblocks + 1.9);
+  const double hbm = 128e-6 / 7.7 * static_cast<double>(N) * kblocks;
+  const int64_t units = (M + 31) / 32, fewest = (units + 7) / 8;
+  for (int64_t t = fewest; t <= units && t <= fewest + 12 && t * w_tiles <= sms; ++t) {
+    const int n = static_cast<int>(32 * ((units + t - 1) / t));
+    const double part = n / 256.0;
+    for (int S = 1; S <= kMaxSplit && kblocks >= 4 * S; ++S)
+      for (int smem : {kGsMaxSmem, kHalfSmem}) {
+        const bool half = smem == kHalfSmem;
+        if (t * w_tiles > clusters_at_once(S, sms) * (half ? 2 : 1)) continue;
+        if (few_slots(n, smem) * (kGsHalf + n / 2 * kGsBlock) < n * (S > 1 ? 512 : 256)) continue;
+        const int both = half && t * w_tiles * 2 * S > sms ? 2 : 1;
+        const double kb = static_cast<double>(kblocks) / S, alone = kb * (0.178 + 0.083 * part) * (half ? 1.5 : 1),
+                     shared = kb * (0.132 + 0.166 * part) * both;
+        double us = alone > shared ? alone : shared;
+        us = 2.2 + (us > hbm ? us : hbm) + 3.46 * part * (S > 1 || both == 1 ? 1 : 1.8) + (S > 1 ? 1.5 + 2.1 * part : 0);
+        if (us < best) {
+          best = us;
+          plan = ScaledPlan{static_cast<int>(t), S, smem};
+        }
+      }
+  }
+  return plan;
+}
+
+// The same for log-probabilities, whose epilogue with tokens on N is the longer one (it goes across lanes), and whose tiles take more
+// than one wave: 144 calls (1 - 800 tokens; 128256 x 4096, 102400 x 2048, 32000 x 4096, 50272 x 768, 8192 x 2048, 1000 x 1024; 16 and 8 bits),
+// 1.01 times the fastest form's time in the mean, 1.17 at most.
+static ScaledPlan logprob_plan(int64_t M, int64_t N, int kblocks, int sms) {
+  const int64_t w_tiles = (N + 255) / 256, pairs = sms / 2, waves = ((M + 255) / 256 * w_tiles + pairs - 1) / pairs;
+  const double bytes = 128e-6 * static_cast<double>(N) * kblocks;
+  const double all = static_cast<double>(waves) * (0.285 * kblocks + 2.8);
+  ScaledPlan plan{0, 1, 0};
+  double best = 8.1 + (all > bytes / 6.04 ? all : bytes / 6.04);
+  const int64_t units = (M + 31) / 32, fewest = (units + 7) / 8;
+  for (int64_t t = fewest; t <= units && t <= fewest + 12; ++t) {
+    const double part = static_cast<double>((units + t - 1) / t) / 8, tiles = static_cast<double>(t * w_tiles);
+    const double one = 1.8 + (tiles > pairs ? kblocks * (0.256 + 0.348 * part) + 15.5 * part : kblocks * (0.105 + 0.62 * part) + 0.6 * part);
+    double us = tiles > 2 * pairs ? one * tiles / static_cast<double>(2 * pairs) : one;
+    us = 4.9 + (us > bytes / 6.42 ? us : bytes / 6.42);
+    if (us < best) {
+      best = us;
+      plan = ScaledPlan{static_cast<int>(t), 1, kHalfSmem};
+    }
+  }
   return plan;
 }
 
 // ring slots for tokens on N; the sums (of one pair: the results) have to fit the ring
-static void few_ring(ScaledParams& p, const ScaledPlan& plan) {
+static int few_ring(ScaledParams& p, const ScaledPlan& plan) {
   p.slot = kGsHalf + p.n / 2 * kGsBlock;
-  const int fit = (plan.smem - kFewFixed) / p.slot, most = (p.kblocks + plan.split - 1) / plan.split;
+  const int fit = few_slots(p.n, plan.smem), most = (p.kblocks + plan.split - 1) / plan.split;
   const int sums = (p.n * (plan.split > 1 ? 512 : 256) + p.slot - 1) / p.slot;
-  p.stages = fit < kFewStages ? fit : kFewStages;
+  p.stages = fit;
   if (p.stages > most) p.stages = most < sums ? sums : most;
+  SPD_REQUIRE(p.stages >= 1 && p.stages >= sums && p.stages <= fit, SPD_E_SHAPE, "a ring of %d slots for %d", fit, sums);
+  return 0;
 }
 
 template <int kKind, int kEnd, typename T>
@@ -651,7 +732,7 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
   p.tok_tiles = plan.tok_tiles;
   if (plan.tok_tiles > 0) {
     p.n = static_cast<int>(32 * (((M + 31) / 32 + plan.tok_tiles - 1) / plan.tok_tiles));
-    few_ring(p, plan);
+    if (int rc = few_ring(p, plan)) return rc;
     if (int rc = make_tmap_2d_sw128(&tw, w, N, kbytes / 2, w_stride / 2, 128, kGsBlock / 2)) return rc;
     if (int rc = make_tmap_2d_sw128(&ta, a, M, kbytes / 2, a_stride / 2, p.n / 2, kGsBlock / 2)) return rc;
     static std::atomic<uint64_t> done{0};
@@ -703,7 +784,7 @@ int spd_int8_scaled_mm(void* out, const int8_t* a, const int8_t* b, const float*
   p.sb = scales_b;
   p.early = older_w;
   const int sms = budget(sm_budget);
-  const ScaledPlan plan = scaled_plan(M, N, static_cast<int>((K + kGsBlock - 1) / kGsBlock), sms, true);
+  const ScaledPlan plan = product_plan(M, N, static_cast<int>((K + kGsBlock - 1) / kGsBlock), sms);
   SPD_DISPATCH_DTYPE(dtype, { return (scaled_product<kInt8, kScaled, T>(a, b, M, N, K, lda, ldb, p, plan, sms, as_stream(stream))); });
 }
 
@@ -736,7 +817,7 @@ int spd_linear_logprobs(float* logprobs, float* lse, const void* x, const void* 
   p.part = reinterpret_cast<float2*>(workspace);
   p.early = older_w;
   const int64_t kbytes = K * size;
-  const ScaledPlan plan = scaled_plan(M, V, static_cast<int>((kbytes + kGsBlock - 1) / kGsBlock), sms, false);
+  const ScaledPlan plan = logprob_plan(M, V, static_cast<int>((kbytes + kGsBlock - 1) / kGsBlock), sms);
   const int tiles = static_cast<int>((V + 255) / 256) * (plan.tok_tiles > 0 ? 2 : 1);
   p.hit = reinterpret_cast<float*>(p.part + tiles * M);
   cudaStream_t st = as_stream(stream);
@@ -746,7 +827,7 @@ int spd_linear_logprobs(float* logprobs, float* lse, const void* x, const void* 
   else rc = scaled_product<kKindF16, kLogprob, __half>(x, w, M, V, kbytes, 2 * ldx, 2 * ldw, p, plan, sms, st);
   if (rc) return rc;
   int width = 1;
-  while (width < 32 && width < M) width *= 2;
+  while (width < 4 && width < M) width *= 2;
   SPD_CUDA(launch(logprob_join_kernel, dim3(static_cast<unsigned>((M + width - 1) / width)), dim3(kJoinThreads), 0, st, pdl_enabled(), logprobs,
                   lse, p.part, p.hit, targets, static_cast<int>(M), tiles, static_cast<int>(V), width));
   return 0;

@@ -61,6 +61,8 @@ def _here(fn: str, *ts: Optional[torch.Tensor]) -> None:
 
 def _all_here(fn: str, *ts: Optional[torch.Tensor]) -> None:
     """_cuda and _here in one pass (0.05 us a tensor)."""
+    if not ts[0].is_cuda:
+        _cuda(ts[0])
     here = torch._C._cuda_getDevice()
     for t in ts:
         if t is not None and t.get_device() != here:
@@ -499,22 +501,24 @@ def silu_fused(x: torch.Tensor, weight: torch.Tensor) -> bool:
 def _quant_int8(fn: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
                 silu_mul: int) -> Tuple[torch.Tensor, torch.Tensor]:
     _all_here(fn, x, residual, weight)
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+    shape, stride, dtype = x.shape, x.stride(), x.dtype
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise RuntimeError(f"{fn}: the input is 2-D with a contiguous last dimension")
-    rows, cols = x.shape
-    dim = cols // 2 if silu_mul else cols
-    if weight is not None and (weight.dtype != x.dtype or weight.dim() != 1 or weight.numel() != dim or not weight.is_contiguous()):
+    rows, dim = shape
+    if silu_mul:
+        if dim % 2:
+            raise RuntimeError(f"{fn}: the last dimension is gate || up, halves of one size")
+        dim //= 2
+    if weight is not None and (weight.dtype != dtype or weight.shape != (dim,) or weight.stride(0) != 1):
         raise RuntimeError(f"{fn}: the weight is a contiguous [{dim}] of the input's type")
-    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape
+    if residual is not None and (residual.dtype != dtype or residual.shape != shape
                                  or not (residual.is_contiguous() and x.is_contiguous())):
         raise RuntimeError(f"{fn}: input and residual are contiguous, of one shape and type")
-    if silu_mul and cols % 2:
-        raise RuntimeError(f"{fn}: the last dimension is gate || up, halves of one size")
-    q = torch.empty((rows, dim), device=x.device, dtype=torch.int8)
-    scales = torch.empty((rows, 1), device=x.device, dtype=torch.float32)
-    check(lib.spd_quant_int8(q.data_ptr(), scales.data_ptr(), x.data_ptr(), residual.data_ptr() if residual is not None else None,
-                             weight.data_ptr() if weight is not None else None, rows, dim, x.stride(0) if rows > 1 else cols,
-                             float(eps), silu_mul, _dt(x), _stream()), "spd_quant_int8")
+    q = x.new_empty((rows, dim), dtype=torch.int8)
+    scales = x.new_empty((rows, 1), dtype=torch.float32)
+    check(lib.spd_quant_int8(q.data_ptr(), scales.data_ptr(), x.data_ptr(), None if residual is None else residual.data_ptr(),
+                             None if weight is None else weight.data_ptr(), rows, dim, stride[0] if rows > 1 else shape[1], float(eps),
+                             silu_mul, _dt(x), _stream()), "spd_quant_int8")
     return q, scales
 
 
@@ -546,16 +550,18 @@ def int8_scaled_mm(mat_a: torch.Tensor, mat_b: torch.Tensor, scales_a: torch.Ten
     mat_a int8 [M, K] with contiguous rows; mat_b int8 [K, N] with contiguous columns (`weight.t()`); scales_a fp32, M of them;
     scales_b fp32, N; bias [N] of out_dtype, bf16 or fp16.  K is a multiple of 16, N of 8.  older_weight: as in `linear`."""
     _all_here("int8_scaled_mm", mat_a, mat_b, scales_a, scales_b, bias)
-    if mat_a.dim() != 2 or mat_b.dim() != 2:
+    shape_a, shape_b = mat_a.shape, mat_b.shape
+    if len(shape_a) != 2 or len(shape_b) != 2:
         raise RuntimeError("int8_scaled_mm: mat_a and mat_b must be 2-D")
-    M, K = mat_a.shape
-    N = mat_b.shape[1]
+    M, K = shape_a
+    N = shape_b[1]
     if mat_a.dtype != torch.int8 or mat_b.dtype != torch.int8:
         raise RuntimeError("int8_scaled_mm: mat_a and mat_b must be int8")
-    if mat_a.stride(1) != 1 or mat_b.stride(0) != 1:
+    stride_a, stride_b = mat_a.stride(), mat_b.stride()
+    if stride_a[1] != 1 or stride_b[0] != 1:
         raise RuntimeError("int8_scaled_mm: mat_a must be row-major, mat_b column-major")
-    if mat_b.shape[0] != K:
-        raise RuntimeError(f"int8_scaled_mm: mat_a is [{M}, {K}], mat_b {list(mat_b.shape)}")
+    if shape_b[0] != K:
+        raise RuntimeError(f"int8_scaled_mm: mat_a is [{M}, {K}], mat_b {list(shape_b)}")
     if (scales_a.dtype != torch.float32 or scales_b.dtype != torch.float32 or scales_a.numel() != M or scales_b.numel() != N
             or not scales_a.is_contiguous() or not scales_b.is_contiguous()):
         raise RuntimeError("int8_scaled_mm: scales are contiguous fp32, one for each row of mat_a and each column of mat_b")
@@ -563,10 +569,10 @@ def int8_scaled_mm(mat_a: torch.Tensor, mat_b: torch.Tensor, scales_a: torch.Ten
         raise RuntimeError(f"int8_scaled_mm: out_dtype is bfloat16 or float16, got {out_dtype}")
     if bias is not None and (bias.dtype != out_dtype or bias.numel() != N or not bias.is_contiguous()):
         raise RuntimeError("int8_scaled_mm: bias is a contiguous [N] of out_dtype")
-    out = torch.empty((M, N), device=mat_a.device, dtype=out_dtype)
+    out = mat_a.new_empty((M, N), dtype=out_dtype)
     check(lib.spd_int8_scaled_mm(out.data_ptr(), mat_a.data_ptr(), mat_b.data_ptr(), scales_a.data_ptr(), scales_b.data_ptr(),
-                                 bias.data_ptr() if bias is not None else None, M, N, K, mat_a.stride(0) if M > 1 else K,
-                                 mat_b.stride(1) if N > 1 else K, N, _DTYPE[out_dtype], 1 if older_weight else 0, get_sm_budget(),
+                                 None if bias is None else bias.data_ptr(), M, N, K, stride_a[0] if M > 1 else K,
+                                 stride_b[1] if N > 1 else K, N, _DTYPE[out_dtype], 1 if older_weight else 0, get_sm_budget(),
                                  _stream()), "spd_int8_scaled_mm")
     return out
 
@@ -577,12 +583,14 @@ def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
     `weight` at targets[m] (int64); a target outside [0, V) asks for nothing and gets 0.  x and weight are bf16 or fp16, or both
     int8 with fp32 scales for each row of either.  older_weight: as in `linear`."""
     _all_here("linear_logprobs", x, weight, targets, x_scales, weight_scales)
-    if x.dim() != 2 or weight.dim() != 2 or x.stride(1) != 1 or weight.stride(1) != 1 or x.shape[1] != weight.shape[1]:
+    shape, w_shape = x.shape, weight.shape
+    stride, w_stride = x.stride(), weight.stride()
+    if len(shape) != 2 or len(w_shape) != 2 or stride[1] != 1 or w_stride[1] != 1 or shape[1] != w_shape[1]:
         raise RuntimeError("linear_logprobs: x [M, K] and weight [V, K] with contiguous last dimension")
     if x.dtype != weight.dtype:
         raise RuntimeError("linear_logprobs: x and weight must have the same dtype")
-    M, K = x.shape
-    V = weight.shape[0]
+    M, K = shape
+    V = w_shape[0]
     if targets.dtype != torch.int64 or targets.shape != (M,) or not targets.is_contiguous():
         raise RuntimeError("linear_logprobs: targets is a contiguous int64 list, one for each row of x")
     if x.dtype == torch.int8:
@@ -595,17 +603,17 @@ def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
         if x_scales is not None or weight_scales is not None:
             raise RuntimeError("linear_logprobs: scales belong to int8 operands")
         dtype = _dt(x)
-    out = torch.empty((2, M), device=x.device, dtype=torch.float32)
+    logprobs, lse = x.new_empty((M,), dtype=torch.float32), x.new_empty((M,), dtype=torch.float32)
     if M == 0:
-        return out[0], out[1]
+        return logprobs, lse
     need = lib.spd_linear_logprobs_workspace_bytes(M, V)
-    ws = torch.empty((need,), device=x.device, dtype=torch.uint8)
-    check(lib.spd_linear_logprobs(out.data_ptr(), out[1].data_ptr(), x.data_ptr(), weight.data_ptr(),
-                                  x_scales.data_ptr() if x_scales is not None else None,
-                                  weight_scales.data_ptr() if weight_scales is not None else None, targets.data_ptr(), M, V, K,
-                                  x.stride(0) if M > 1 else K, weight.stride(0) if V > 1 else K, dtype, 1 if older_weight else 0,
+    ws = x.new_empty((need,), dtype=torch.uint8)
+    check(lib.spd_linear_logprobs(logprobs.data_ptr(), lse.data_ptr(), x.data_ptr(), weight.data_ptr(),
+                                  None if x_scales is None else x_scales.data_ptr(),
+                                  None if weight_scales is None else weight_scales.data_ptr(), targets.data_ptr(), M, V, K,
+                                  stride[0] if M > 1 else K, w_stride[0] if V > 1 else K, dtype, 1 if older_weight else 0,
                                   ws.data_ptr(), need, get_sm_budget(), _stream()), "spd_linear_logprobs")
-    return out[0], out[1]
+    return logprobs, lse
 
 
 def linear_block_diag(x: torch.Tensor, weight: torch.Tensor, num_groups: int, k: int, n: int,

@@ -127,7 +127,10 @@ def test_budget_of_sms_and_graphs(m):
         part = ops.linear_logprobs(x, w, targets)
     finally:
         ops.set_sm_budget(0)
-    assert torch.equal(want[0], part[0]) and torch.equal(want[1], part[1])
+    # a partition may cut the vocabulary into other tiles, whose sums are rounded in another order: held to the definition, as the
+    # whole device's are
+    check(x, w, None, None, targets, want)
+    check(x, w, None, None, targets, part)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
