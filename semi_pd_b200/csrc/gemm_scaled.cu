@@ -74,6 +74,7 @@ struct ScaledParams {
   int n_cols, m_rows;
   int kblocks;
   int tok_tiles, n;    // tokens on N: token tiles, MMA columns of each
+  int accs;            // accumulators that take k-blocks in turn (16-bit operands)
   int stages, slot;
   int x_tiles, y_tiles, panel;  // tokens on M
   int early;           // the weights are older than the kernel before this one: the first of them are fetched before it has ended
@@ -141,7 +142,8 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   const int S = static_cast<int>(cluster_nctarank() >> 1), s = static_cast<int>(crank >> 1);
   const int tile = blockIdx.x / (2 * S), wt = tile / p.tok_tiles, tt = tile - wt * p.tok_tiles;
   const int kb0 = s * p.kblocks / S, kb1 = (s + 1) * p.kblocks / S;
-  const int half = p.n >> 1, tmem_cols = p.n <= 32 ? 32 : p.n <= 64 ? 64 : p.n <= 128 ? 128 : 256;
+  const int accs = kKind == kInt8 ? 1 : p.accs, cols = p.n * accs;
+  const int half = p.n >> 1, tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
   const int tok_base = tt * p.n, tokens = min(p.n, p.m_rows - tok_base);
   const int row_base = wt * 256 + static_cast<int>(rank) * 128;
 
@@ -206,8 +208,8 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         const uint32_t wa = smem_u32(smem + stage * p.slot), aa = wa + kGsHalf;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          gs_mma<kKind>(tmem, umma_desc_sw128(wa + k * 32, 16, 1024), umma_desc_sw128(aa + k * 32, 16, 1024), idesc,
-                        (kb > kb0 || k > 0) ? 1u : 0u);
+          gs_mma<kKind>(tmem + ((kb - kb0) & (accs - 1)) * p.n, umma_desc_sw128(wa + k * 32, 16, 1024),
+                        umma_desc_sw128(aa + k * 32, 16, 1024), idesc, (kb - kb0 >= accs || k > 0) ? 1u : 0u);
         umma_commit_2cta_mc(&empty[stage], both);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
@@ -259,7 +261,17 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         }
       } else {
         float v[32], e[32];
-        if constexpr (kKind == kInt8) scales();
+        if constexpr (kKind == kInt8) {
+          scales();
+        } else {
+          for (int a = 1; a < accs; ++a) {
+            uint32_t more[32];
+            tmem_ld_32x32b_x32(taddr + a * p.n + c, more);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
+          }
+        }
         int hit[32];
 #pragma unroll
         for (int j = 0; j < 32; j += 4) *reinterpret_cast<int4*>(hit + j) = *reinterpret_cast<const int4*>(tok_target + c + j);
@@ -366,7 +378,53 @@ __device__ __forceinline__ void many_tile(const ScaledParams& p, int tile, int& 
   yt = y0 + r - xt * q;
 }
 
-template <int kKind, int kEnd, typename T>
+// One thread of each CTA: its 128 token rows and 128 weight rows of every k-block; the leader's barrier counts both CTAs' bytes.
+__device__ __forceinline__ void many_load(const CUtensorMap& tmA, const CUtensorMap& tmW, const ScaledParams& p, uint8_t* smem,
+                                          uint64_t* full, uint64_t* empty, uint32_t rank, int pair, int npairs, volatile int* dead) {
+  int stage = 0, phase = 0;
+  const uint32_t lead_full0 = map_to_rank(smem_u32(full), 0);
+  for (int tile = pair; tile < p.x_tiles * p.y_tiles; tile += npairs) {
+    int xt, yt;
+    many_tile(p, tile, xt, yt);
+    const int a_row = xt * 256 + static_cast<int>(rank) * 128, w_row = yt * 256 + static_cast<int>(rank) * 128;
+    for (int kb = 0; kb < p.kblocks; ++kb) {
+      mbar_wait_bounded(&empty[stage], phase ^ 1, dead);
+      if (rank == 0) mbar_expect_tx(&full[stage], 4 * kGsHalf);
+      uint8_t* slot = smem + stage * 2 * kGsHalf;
+      tma_load_2d_2cta(slot, &tmA, lead_full0 + stage * 8, kb * (kGsBlock / 2), a_row, kEvictNormal);
+      tma_load_2d_2cta(slot + kGsHalf, &tmW, lead_full0 + stage * 8, kb * (kGsBlock / 2), w_row, kEvictNormal);
+      if (++stage == kManyStages) { stage = 0; phase ^= 1; }
+    }
+  }
+}
+
+// One thread of the leader: the MMAs of every tile, `chunk` k-blocks into either accumulator in turn.
+template <int kKind>
+__device__ __forceinline__ void many_multiply(const ScaledParams& p, uint8_t* smem, uint64_t* full, uint64_t* empty, uint64_t* tfull,
+                                              uint64_t* tempty, uint32_t tmem, int pair, int npairs, int chunk, volatile int* dead) {
+  constexpr uint32_t idesc = gs_idesc<kKind>(256, 256);
+  int stage = 0, phase = 0, n = 0;
+  for (int tile = pair; tile < p.x_tiles * p.y_tiles; tile += npairs)
+    for (int kb0 = 0; kb0 < p.kblocks; kb0 += chunk, ++n) {
+      const int as = n & 1, kb1 = min(kb0 + chunk, p.kblocks);
+      mbar_wait_bounded(&tempty[as], ((n >> 1) & 1) ^ 1, dead);  // both CTAs have drained this accumulator
+      tc_fence_after_sync();
+      for (int kb = kb0; kb < kb1; ++kb) {
+        mbar_wait_bounded(&full[stage], phase, dead);
+        tc_fence_after_sync();
+        const uint32_t aa = smem_u32(smem + stage * 2 * kGsHalf), wa = aa + kGsHalf;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          gs_mma<kKind>(tmem + as * 256, umma_desc_sw128(aa + k * 32, 16, 1024), umma_desc_sw128(wa + k * 32, 16, 1024), idesc,
+                        (kb > kb0 || k > 0) ? 1u : 0u);
+        umma_commit_2cta_mc(&empty[stage], 0b11);
+        if (++stage == kManyStages) { stage = 0; phase ^= 1; }
+      }
+      umma_commit_2cta_mc(&tfull[as], 0b11);
+    }
+}
+
+template <typename T>
 __global__ void __launch_bounds__(kManyThreads, 1)
 many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const ScaledParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -412,44 +470,9 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   griddep_wait();
 
   if (warp == 0) {
-    if (elect_one()) {
-      int stage = 0, phase = 0;
-      const uint32_t lead_full0 = map_to_rank(smem_u32(full), 0);
-      for (int tile = pair; tile < num_tiles; tile += npairs) {
-        int xt, yt;
-        many_tile(p, tile, xt, yt);
-        const int a_row = xt * 256 + static_cast<int>(rank) * 128, w_row = yt * 256 + static_cast<int>(rank) * 128;
-        for (int kb = 0; kb < p.kblocks; ++kb) {
-          mbar_wait_bounded(&empty[stage], phase ^ 1, dead);
-          if (rank == 0) mbar_expect_tx(&full[stage], 4 * kGsHalf);
-          tma_load_2d_2cta(smem + stage * 2 * kGsHalf, &tmA, lead_full0 + stage * 8, kb * (kGsBlock / 2), a_row, kEvictNormal);
-          tma_load_2d_2cta(smem + stage * 2 * kGsHalf + kGsHalf, &tmW, lead_full0 + stage * 8, kb * (kGsBlock / 2), w_row, kEvictNormal);
-          if (++stage == kManyStages) { stage = 0; phase ^= 1; }
-        }
-      }
-    }
+    if (elect_one()) many_load(tmA, tmW, p, smem, full, empty, rank, pair, npairs, dead);
   } else if (warp == 1) {
-    if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = gs_idesc<kKind>(256, 256);
-      int stage = 0, phase = 0, n = 0;
-      for (int tile = pair; tile < num_tiles; tile += npairs, ++n) {
-        const int as = n & 1;
-        mbar_wait_bounded(&tempty[as], ((n >> 1) & 1) ^ 1, dead);  // both CTAs have drained this accumulator
-        tc_fence_after_sync();
-        for (int kb = 0; kb < p.kblocks; ++kb) {
-          mbar_wait_bounded(&full[stage], phase, dead);
-          tc_fence_after_sync();
-          const uint32_t aa = smem_u32(smem + stage * 2 * kGsHalf), wa = aa + kGsHalf;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            gs_mma<kKind>(tmem + as * 256, umma_desc_sw128(aa + k * 32, 16, 1024), umma_desc_sw128(wa + k * 32, 16, 1024), idesc,
-                          (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit_2cta_mc(&empty[stage], 0b11);
-          if (++stage == kManyStages) { stage = 0; phase ^= 1; }
-        }
-        umma_commit_2cta_mc(&tfull[as], 0b11);
-      }
-    }
+    if (rank == 0 && elect_one()) many_multiply<kInt8>(p, smem, full, empty, tfull, tempty, tmem, pair, npairs, p.kblocks, dead);
   } else if (warp >= 4) {
     const int q = warp & 3, et = threadIdx.x - 128;
     uint8_t* stage = sOut + q * kStageWarp;
@@ -462,79 +485,43 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int64_t m0 = static_cast<int64_t>(xt) * 256 + rank * 128 + q * 32;
       const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m_rows - m0));
       const float2* col = cols + as * 256;
-      if constexpr (kKind == kInt8) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = n0 + et + i * 128;
-          float2 sb = make_float2(0.f, 0.f);
-          if (c < p.n_cols) {
-            sb.x = p.sb[c];
-            if (kEnd == kScaled && p.bias) sb.y = to_f32<T>(reinterpret_cast<const T*>(p.bias)[c]);
-          }
-          cols[as * 256 + et + i * 128] = sb;
+      for (int i = 0; i < 2; ++i) {
+        const int c = n0 + et + i * 128;
+        float2 sb = make_float2(0.f, 0.f);
+        if (c < p.n_cols) {
+          sb.x = p.sb[c];
+          if (p.bias) sb.y = to_f32<T>(reinterpret_cast<const T*>(p.bias)[c]);
         }
-        // (one barrier a tile: a warp that is a tile ahead writes the other half, and cannot get two ahead)
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        cols[as * 256 + et + i * 128] = sb;
       }
-      const float sa = kKind == kInt8 && lane < rows ? p.sa[m0 + lane] : 1.f;
+      // (one barrier a tile: a warp that is a tile ahead writes the other half, and cannot get two ahead)
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const float sa = lane < rows ? p.sa[m0 + lane] : 1.f;
       mbar_wait_bounded(&tfull[as], (n >> 1) & 1, dead);
       tc_fence_after_sync();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + as * 256;
-      if constexpr (kEnd == kScaled) {
-        auto values = [&](int c, float (&v)[32]) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(taddr + c, r);
-          tmem_ld_wait();
+      auto values = [&](int c, float (&v)[32]) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(taddr + c, r);
+        tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float4 f = *reinterpret_cast<const float4*>(col + c + j);
-            v[j] = fmaf(gs_value<kKind>(r[j]) * sa, f.x, f.y);
-            v[j + 1] = fmaf(gs_value<kKind>(r[j + 1]) * sa, f.z, f.w);
-          }
-        };
-#pragma unroll 1
-        for (int c = 0; c < 256; c += 64) {
-          if (n0 + c >= p.n_cols) break;
-          float v[32];
-          values(c, v);
-          stage_put16<T>(stage, lane, 0, v);
-          values(c + 32, v);
-          stage_put16<T>(stage, lane, 1, v);
-          stage_out(stage, lane, reinterpret_cast<uint8_t*>(p.out) + (m0 * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
-                    min(64, p.n_cols - n0 - c) * 2);
+        for (int j = 0; j < 32; j += 2) {
+          const float4 f = *reinterpret_cast<const float4*>(col + c + j);
+          v[j] = fmaf(gs_value<kInt8>(r[j]) * sa, f.x, f.y);
+          v[j + 1] = fmaf(gs_value<kInt8>(r[j + 1]) * sa, f.z, f.w);
         }
-      } else {
-        const int64_t target = lane < rows ? p.target[m0 + lane] - n0 : -1;
-        LogSum all;
+      };
 #pragma unroll 1
-        for (int c = 0; c < 256; c += 32) {
-          if (n0 + c >= p.n_cols) break;
-          uint32_t r[32];
-          float v[32], top = -INFINITY;
-          tmem_ld_32x32b_x32(taddr + c, r);
-          tmem_ld_wait();
-          const int valid = p.n_cols - n0 - c;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            v[j] = kKind == kInt8 ? gs_value<kKind>(r[j]) * sa * col[c + j].x : __uint_as_float(r[j]);
-            if (j >= valid) v[j] = -INFINITY;
-            top = fmaxf(top, v[j]);
-          }
-          if (target >= c && target < c + 32 && target < c + valid) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (target == c + j) p.hit[m0 + lane] = v[j];
-          }
-          const float base = LogSum::base(top);
-          float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            s0 += fast_exp2(fmaf(v[j], kLog2e, -base));
-            s1 += fast_exp2(fmaf(v[j + 1], kLog2e, -base));
-          }
-          all.join(top, s0 + s1);
-        }
-        if (lane < rows) p.part[static_cast<int64_t>(yt) * p.m_rows + m0 + lane] = make_float2(all.m, all.s);
+      for (int c = 0; c < 256; c += 64) {
+        if (n0 + c >= p.n_cols) break;
+        float v[32];
+        values(c, v);
+        stage_put16<T>(stage, lane, 0, v);
+        values(c + 32, v);
+        stage_put16<T>(stage, lane, 1, v);
+        stage_out(stage, lane, reinterpret_cast<uint8_t*>(p.out) + (m0 * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
+                  min(64, p.n_cols - n0 - c) * 2);
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -552,6 +539,143 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   }
   cluster_sync_relaxed();  // the peer may still read this CTA's shared memory / signal its barriers
   if (warp == 2) tmem_dealloc_2cta(tmem, 512);
+}
+
+// Log-probabilities with tokens on M: 256 tokens x 256 vocabulary rows.  Eight warps take the accumulator, a lane with a token, its
+// 128 columns of one half kept in registers as fp32.  The tensor cores cut what does not fit behind the sum of 16-bit products, always
+// towards zero, and a long row adds that up (K = 4096: 1.1e-6 of the result); so a sum is taken out of TMEM after every 16 k-blocks and
+// added up in registers, while the other accumulator takes the next ones: a tenth of the error, no time (16 k-blocks take the MMAs
+// 8192 clk, taking 128 columns out 400).  8-bit sums are exact and come out once.
+constexpr int kLogThreads = 320;  // warp 0: TMA, 1: MMA and TMEM, 2-9: epilogue
+constexpr int kLogChunk = 16;     // k-blocks
+constexpr int kLogSmem = kManyRing + 2 * 256 * 4 + 256 + 1024;
+
+template <int kKind>
+__global__ void __launch_bounds__(kLogThreads, 1)
+many_logprobs_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const ScaledParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float* cols = reinterpret_cast<float*>(smem + kManyRing);         // [2][256] scales of a tile's vocabulary rows
+  uint64_t* full = reinterpret_cast<uint64_t*>(cols + 512);         // [stages]  (the leader's are the live ones)
+  uint64_t* empty = full + kManyStages;                             // [stages]
+  uint64_t* tfull = empty + kManyStages;                            // [2]
+  uint64_t* tempty = tfull + 2;                                     // [2]       (the leader's)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1, num_tiles = p.x_tiles * p.y_tiles;
+  const int chunk = kKind == kInt8 ? p.kblocks : kLogChunk;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+    *dead = 0;
+    for (int i = 0; i < kManyStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 16);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_2cta(tmem_slot, 512);
+    tmem_relinquish_2cta();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA signal
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+
+  if (warp == 0) {
+    if (elect_one()) many_load(tmA, tmW, p, smem, full, empty, rank, pair, npairs, dead);
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) many_multiply<kKind>(p, smem, full, empty, tfull, tempty, tmem, pair, npairs, chunk, dead);
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2, et = threadIdx.x - 64;
+    const uint32_t lead_tempty0 = map_to_rank(smem_u32(tempty), 0);
+    int n = 0, turn = 0;
+    for (int tile = pair; tile < num_tiles; tile += npairs, turn ^= 1) {
+      int xt, yt;
+      many_tile(p, tile, xt, yt);
+      const int n0 = yt * 256 + half * 128;
+      const int64_t m0 = static_cast<int64_t>(xt) * 256 + rank * 128 + q * 32;
+      const bool have = m0 + lane < p.m_rows;
+      const float* col = cols + turn * 256 + half * 128;
+      float sa = 1.f;
+      if constexpr (kKind == kInt8) {
+        cols[turn * 256 + et] = yt * 256 + et < p.n_cols ? p.sb[yt * 256 + et] : 0.f;
+        // (one barrier a tile: a warp that is a tile ahead writes the other half, and cannot get two ahead)
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (have) sa = p.sa[m0 + lane];
+      }
+      const int64_t target = have ? p.target[m0 + lane] - n0 : -1;
+      float v[128];
+      for (int kb0 = 0; kb0 < p.kblocks; kb0 += chunk, ++n) {
+        const int as = n & 1;
+        mbar_wait_bounded(&tfull[as], (n >> 1) & 1, dead);
+        tc_fence_after_sync();
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + as * 256 + half * 128;
+#pragma unroll
+        for (int c = 0; c < 128; c += 16) {
+          uint32_t r[16];
+          tmem_ld_32x32b_x16(taddr + c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[c + j] = kb0 == 0 ? gs_value<kKind>(r[j]) : v[c + j] + gs_value<kKind>(r[j]);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote_release(lead_tempty0 + as * 8);
+      }
+      const int valid = p.n_cols - n0;
+      if constexpr (kKind == kInt8) {
+#pragma unroll
+        for (int j = 0; j < 128; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(col + j);
+          v[j] = v[j] * sa * f.x;
+          v[j + 1] = v[j + 1] * sa * f.y;
+          v[j + 2] = v[j + 2] * sa * f.z;
+          v[j + 3] = v[j + 3] * sa * f.w;
+        }
+      }
+      if (target >= 0 && target < 128 && target < valid) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (target == j) p.hit[m0 + lane] = v[j];
+      }
+      if (valid < 128) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (j >= valid) v[j] = -INFINITY;
+      }
+      float top[4] = {v[0], v[1], v[2], v[3]}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 4; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], v[j]);
+      top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const float base = LogSum::base(top[0]);
+#pragma unroll
+      for (int j = 0; j < 128; ++j) sum[j & 3] += fast_exp2(fmaf(v[j], kLog2e, -base));
+      if (have) p.part[static_cast<int64_t>(yt * 2 + half) * p.m_rows + m0 + lane] = make_float2(top[0], (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    }
+  }
+
+  __syncwarp();  // the warps of the elected lanes come together before the barriers, which count whole warps
+  griddep_launch_dependents();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*dead) {
+    wait_drain();
+    if (threadIdx.x == 0) wait_report(p.wait_expired);
+  }
+  cluster_sync_relaxed();  // the peer may still read this CTA's shared memory / signal its barriers
+  if (warp == 1) tmem_dealloc_2cta(tmem, 512);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -686,21 +810,31 @@ static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
   return plan;
 }
 
+// 16-bit operands with tokens on N: k-blocks go to up to 8 accumulators in turn, as many as half of TMEM holds (see many_logprobs_kernel)
+static int few_accumulators(int n, int kblocks) {
+  int accs = 8;
+  while (accs > 1 && (accs * n > 256 || accs > kblocks)) accs /= 2;
+  return accs;
+}
+
 // The same for log-probabilities, whose epilogue with tokens on N is the longer one (it goes across lanes), and whose tiles take more
 // than one wave: 144 calls (1 - 800 tokens; 128256 x 4096, 102400 x 2048, 32000 x 4096, 50272 x 768, 8192 x 2048, 1000 x 1024; 16 and 8 bits),
-// 1.01 times the fastest form's time in the mean, 1.17 at most.
-static ScaledPlan logprob_plan(int64_t M, int64_t N, int kblocks, int sms) {
+// 1.01 times the fastest form's time in the mean, 1.13 at most.
+// Sums of 16-bit products stay with tokens on M where more than 32 k-blocks would come together in one accumulator: they are that much
+// less exact (64 in one 1.4e-6 of the result, 32 7e-7, 16 4e-7).
+static ScaledPlan logprob_plan(int64_t M, int64_t N, int kblocks, int sms, bool int8) {
   const int64_t w_tiles = (N + 255) / 256, pairs = sms / 2, waves = ((M + 255) / 256 * w_tiles + pairs - 1) / pairs;
   const double bytes = 128e-6 * static_cast<double>(N) * kblocks;
-  const double all = static_cast<double>(waves) * (0.285 * kblocks + 2.8);
   ScaledPlan plan{0, 1, 0};
-  double best = 8.1 + (all > bytes / 6.04 ? all : bytes / 6.04);
+  double best = 8.8 + static_cast<double>(waves) * (0.337 * kblocks + 1.65);
   const int64_t units = (M + 31) / 32, fewest = (units + 7) / 8;
   for (int64_t t = fewest; t <= units && t <= fewest + 12; ++t) {
-    const double part = static_cast<double>((units + t - 1) / t) / 8, tiles = static_cast<double>(t * w_tiles);
-    const double one = 1.8 + (tiles > pairs ? kblocks * (0.256 + 0.348 * part) + 15.5 * part : kblocks * (0.105 + 0.62 * part) + 0.6 * part);
+    const int n = static_cast<int>(32 * ((units + t - 1) / t));
+    if (!int8 && kblocks > 32 * few_accumulators(n, kblocks)) continue;
+    const double part = n / 256.0, tiles = static_cast<double>(t * w_tiles);
+    const double one = 0.4 + (tiles > pairs ? kblocks * (0.308 + 0.316 * part) + 17.9 * part : kblocks * (0.131 + 0.694 * part));
     double us = tiles > 2 * pairs ? one * tiles / static_cast<double>(2 * pairs) : one;
-    us = 4.9 + (us > bytes / 6.42 ? us : bytes / 6.42);
+    us = 6.2 + (us > bytes / 6.84 ? us : bytes / 6.84);
     if (us < best) {
       best = us;
       plan = ScaledPlan{static_cast<int>(t), 1, kHalfSmem};
@@ -735,6 +869,7 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
     if (int rc = few_ring(p, plan)) return rc;
     if (int rc = make_tmap_2d_sw128(&tw, w, N, kbytes / 2, w_stride / 2, 128, kGsBlock / 2)) return rc;
     if (int rc = make_tmap_2d_sw128(&ta, a, M, kbytes / 2, a_stride / 2, p.n / 2, kGsBlock / 2)) return rc;
+    p.accs = kKind == kInt8 ? 1 : few_accumulators(p.n, p.kblocks);
     static std::atomic<uint64_t> done{0};
     const int ctas = static_cast<int>((N + 255) / 256) * plan.tok_tiles * 2 * plan.split;
     return launch_pairs(few_tokens_kernel<kKind, kEnd, T>, done, ctas, 2 * plan.split, kFewThreads, p.stages * p.slot + kFewFixed, stream,
@@ -750,7 +885,8 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
   const int64_t tiles = static_cast<int64_t>(p.x_tiles) * p.y_tiles;
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
   static std::atomic<uint64_t> done{0};
-  return launch_pairs(many_tokens_kernel<kKind, kEnd, T>, done, 2 * pairs, 2, kManyThreads, kManySmem, stream, ta, tw, p);
+  if constexpr (kEnd == kScaled) return launch_pairs(many_tokens_kernel<T>, done, 2 * pairs, 2, kManyThreads, kManySmem, stream, ta, tw, p);
+  else return launch_pairs(many_logprobs_kernel<kKind>, done, 2 * pairs, 2, kLogThreads, kLogSmem, stream, ta, tw, p);
 }
 
 static int budget(int sm_budget) {
@@ -817,8 +953,8 @@ int spd_linear_logprobs(float* logprobs, float* lse, const void* x, const void* 
   p.part = reinterpret_cast<float2*>(workspace);
   p.early = older_w;
   const int64_t kbytes = K * size;
-  const ScaledPlan plan = logprob_plan(M, V, static_cast<int>((kbytes + kGsBlock - 1) / kGsBlock), sms);
-  const int tiles = static_cast<int>((V + 255) / 256) * (plan.tok_tiles > 0 ? 2 : 1);
+  const ScaledPlan plan = logprob_plan(M, V, static_cast<int>((kbytes + kGsBlock - 1) / kGsBlock), sms, dtype == SPD_I8);
+  const int tiles = static_cast<int>((V + 255) / 256) * 2;
   p.hit = reinterpret_cast<float*>(p.part + tiles * M);
   cudaStream_t st = as_stream(stream);
   int rc;
