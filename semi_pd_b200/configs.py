@@ -437,6 +437,9 @@ class ServerArgs:
     # "dummy": synthetic weights; "safetensors": <model_path>/model.safetensors; "auto": the file
     # when model_path is a folder that has one, else dummy; "external": load_weights() by the caller
     load_format: str = "dummy"
+    # "w8a8_int8": products of 8-bit integers, the weights quantised by row when they are loaded unless they come in 8 bits,
+    # activations by token (layers/quantization/w8a8_int8.py); None: as the weights are
+    quantization: Optional[str] = None
     tp_size: int = 1
     mem_fraction_static: Optional[float] = None
     max_total_tokens: Optional[int] = None
@@ -467,6 +470,7 @@ class ServerArgs:
         parser.add_argument("--model-path", type=str, default=ServerArgs.model_path)
         parser.add_argument("--dtype", type=str, default=ServerArgs.dtype)
         parser.add_argument("--load-format", type=str, default=ServerArgs.load_format)
+        parser.add_argument("--quantization", type=str, default=None, choices=["w8a8_int8"])
         parser.add_argument("--tp", "--tensor-parallel-size", dest="tp_size", type=int, default=1)
         parser.add_argument("--mem-fraction-static", type=float, default=None)
         parser.add_argument("--max-total-tokens", type=int, default=None)

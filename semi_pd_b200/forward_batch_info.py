@@ -87,8 +87,12 @@ class ModelWorkerBatch:
     extend_seq_lens: Optional[List[int]] = None
     extend_prefix_lens: Optional[List[int]] = None
     extend_logprob_start_lens: Optional[List[int]] = None
-    # logprobs are unsupported under semi-PD (semi_pd_decode_scheduler.py:354)
+    # the log-probabilities of the input tokens come back beside the logits (LogitsProcessor.input_token_logprobs); the semi-PD
+    # schedulers do not ask for them (semi_pd_decode_scheduler.py:354)
     return_logprob: bool = False
+    # [T] int64, device: the token whose log-probability every row is asked for, -1: none (logits_processor.py:
+    # extend_input_logprob_token_ids_gpu); None: the request's next token
+    extend_input_logprob_token_ids: Optional[torch.Tensor] = None
     sampling_info: object = None
     # TP > 1: all-gather the vocab-sharded logits (logits_processor.py:426-427).  The semi-PD
     # schedulers sample greedy ids from the (max, argmax) rows and never read the logits.
@@ -105,6 +109,7 @@ class LogitsProcessorOutput:
     hidden_states: Optional[torch.Tensor] = None
     # greedy ids when the argmax already ran inside the captured decode graph
     next_token_ids: Optional[torch.Tensor] = None
+    input_token_logprobs: Optional[torch.Tensor] = None  # return_logprob of an extend batch: fp32 [T]
 
 
 @dataclasses.dataclass
@@ -120,6 +125,7 @@ class ForwardBatch:
     seq_lens_sum: int
 
     return_logprob: bool = False
+    extend_input_logprob_token_ids: Optional[torch.Tensor] = None
     gather_logits: bool = True
     extend_logit_rows: Optional[torch.Tensor] = None
     positions: torch.Tensor = None
@@ -156,6 +162,7 @@ class ForwardBatch:
             out_cache_loc=batch.out_cache_loc,
             seq_lens_sum=batch.seq_lens_sum,
             return_logprob=batch.return_logprob,
+            extend_input_logprob_token_ids=batch.extend_input_logprob_token_ids,
             gather_logits=batch.gather_logits,
             extend_logit_rows=batch.extend_logit_rows,
             sampling_info=batch.sampling_info,

@@ -6,7 +6,7 @@ torch fallback.  Plain Python objects (no nn.Module / autograd: this is inferenc
 from __future__ import annotations
 
 import math
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -15,6 +15,13 @@ from .distributed import (get_current_comm, get_tensor_model_parallel_rank,
                           get_tensor_model_parallel_world_size, tensor_model_parallel_all_gather,
                           tensor_model_parallel_all_reduce)
 from .forward_batch_info import ForwardBatch, LogitsProcessorOutput
+
+
+class QuantizedTokens(NamedTuple):
+    """Activations in 8-bit integers, ready for the products that read them (ops.int8_scaled_mm)."""
+    q: torch.Tensor         # int8 [T, K]
+    scales: torch.Tensor    # fp32 [T, 1]
+    dtype: torch.dtype      # of the values that they stand for
 
 
 class RMSNorm:
@@ -43,6 +50,15 @@ class RMSNorm:
 
     __call__ = forward
 
+    def forward_quant(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        """forward() for a layer of 8-bit weights: the normed tokens as QuantizedTokens, quantised in the same pass."""
+        if residual is None:
+            return QuantizedTokens(*ops.rmsnorm_quant_int8(x, self.weight, self.variance_epsilon), x.dtype)
+        if getattr(x, "_spd_pending_all_reduce", False):  # the sum over the ranks comes first
+            x, residual = self.forward(x, residual)
+            return QuantizedTokens(*ops.per_token_quant_int8(x), x.dtype), residual
+        return QuantizedTokens(*ops.fused_add_rmsnorm_quant_int8(x, residual, self.weight, self.variance_epsilon), x.dtype), residual
+
 
 class SiluAndMul:
     """layers/activation.py:41-51."""
@@ -51,6 +67,9 @@ class SiluAndMul:
         return ops.silu_and_mul(x)
 
     __call__ = forward
+
+    def forward_quant(self, x: torch.Tensor) -> QuantizedTokens:
+        return QuantizedTokens(*ops.silu_and_mul_quant_int8(x), x.dtype)
 
 
 def _compute_inv_freq(rotary_dim: int, base: float) -> torch.Tensor:
@@ -123,17 +142,30 @@ def get_rope(head_size, rotary_dim, max_position, base, is_neox_style=True, rope
 
 
 class LinearBase:
-    """weight is [out_per_partition, in_per_partition], row-major (layers/linear.py:140-172)."""
+    """weight is [out_per_partition, in_per_partition], row-major (layers/linear.py:140-172).  An int8 weight has a scale for each
+    of its rows in `weight_scale` and takes its input in 8-bit integers (layers/quantization/w8a8_int8.py)."""
 
     def __init__(self, input_size: int, output_size: int):
         self.input_size = input_size
         self.output_size = output_size
         self.weight: torch.Tensor = None
+        self.weight_scale: Optional[torch.Tensor] = None  # fp32 [out_per_partition, 1]
+
+    def quantize_weight_int8(self) -> None:
+        """A 16-bit weight as 8-bit integers, a row's largest value 127."""
+        self.weight, self.weight_scale = ops.per_token_quant_int8(self.weight)
+
+    def _product(self, x: Union[torch.Tensor, QuantizedTokens]) -> torch.Tensor:
+        if self.weight_scale is None:
+            return ops.linear(x, self.weight)
+        if not isinstance(x, QuantizedTokens):
+            x = QuantizedTokens(*ops.per_token_quant_int8(x), x.dtype)
+        return ops.int8_scaled_mm(x.q, self.weight.t(), x.scales, self.weight_scale, x.dtype, older_weight=True)
 
 
 class ColumnParallelLinear(LinearBase):
-    def forward(self, x: torch.Tensor):
-        return ops.linear(x, self.weight), None
+    def forward(self, x: Union[torch.Tensor, QuantizedTokens]):
+        return self._product(x), None
 
     __call__ = forward
 
@@ -191,8 +223,8 @@ class RowParallelLinear(LinearBase):
         # a residual-add RMSNorm on the Llama path) runs the all-reduce fused with itself
         self.defer_reduce = defer_reduce
 
-    def forward(self, x: torch.Tensor):
-        out = ops.linear(x, self.weight)
+    def forward(self, x: Union[torch.Tensor, QuantizedTokens]):
+        out = self._product(x)
         if self.reduce_results and get_tensor_model_parallel_world_size() > 1:
             if self.defer_reduce:
                 out._spd_pending_all_reduce = True
@@ -262,6 +294,7 @@ class LogitsProcessor:
 
     def forward(self, input_ids, hidden_states, lm_head, forward_batch: ForwardBatch
                 ) -> LogitsProcessorOutput:
+        token_logprobs = self.input_token_logprobs(input_ids, hidden_states, lm_head, forward_batch)
         rows = self.logit_rows(forward_batch)
         pruned_states = hidden_states if rows is None else ops.gather_rows(hidden_states, rows)
         logits = ops.linear(pruned_states, lm_head.weight, out_f32=True)
@@ -275,9 +308,24 @@ class LogitsProcessor:
             if forward_batch.gather_logits and not torch.cuda.is_current_stream_capturing():
                 logits = tensor_model_parallel_all_gather(logits)
         logits = logits[:, : self.config.vocab_size]
-        return LogitsProcessorOutput(next_token_logits=logits, next_token_ids=next_ids)
+        return LogitsProcessorOutput(next_token_logits=logits, next_token_ids=next_ids, input_token_logprobs=token_logprobs)
 
     __call__ = forward
+
+    def input_token_logprobs(self, input_ids, hidden_states, lm_head, forward_batch: ForwardBatch) -> Optional[torch.Tensor]:
+        """return_logprob of an extend batch: fp32 [T], in row i the log-probability of the token behind token i — of
+        `extend_input_logprob_token_ids[i]` where the batch has them (-1: none), else of the request's next token in this batch
+        (0 in its last row).  One pass over the lm_head's rows; the logits of the T rows are not stored."""
+        if not forward_batch.return_logprob or not forward_batch.forward_mode.is_extend():
+            return None
+        if self.do_tensor_parallel_all_gather:
+            raise NotImplementedError("return_logprob with --tp > 1")
+        targets = forward_batch.extend_input_logprob_token_ids
+        if targets is None:
+            targets = torch.full_like(input_ids, -1)
+            targets[:-1] = input_ids[1:]
+            targets[forward_batch.extend_start_loc.long() - 1] = -1  # rows before a request's first, and the last row
+        return ops.linear_logprobs(hidden_states, lm_head.weight[: self.config.vocab_size], targets, older_weight=True)[0]
 
 
 class Sampler:

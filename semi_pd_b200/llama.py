@@ -3,6 +3,8 @@ order.  Differences, all fusions that remove HBM round trips:
   * RoPE + KV-cache write are one kernel (`RotaryEmbedding.forward_kvwrite`); attention is then
     called with save_kv_cache=False;
   * in the prefill regime the gate_up GEMM applies SiLU·mul in its epilogue;
+  * with quantization="w8a8_int8" (layers/quantization/w8a8_int8.py) a layer's four weights are 8-bit integers, and the norms and
+    SiLU·mul before them quantise their tokens in the same pass; embedding, lm_head and the final norm stay in 16 bits;
   * q, k, v are strided views of the qkv GEMM output (no split copies).
 """
 from __future__ import annotations
@@ -17,7 +19,7 @@ from . import ops
 from .attention_backend import RadixAttention
 from .distributed import get_tensor_model_parallel_rank, get_tensor_model_parallel_world_size
 from .forward_batch_info import ForwardBatch, LogitsProcessorOutput
-from .layers import (LogitsProcessor, MergedColumnParallelLinear, ParallelLMHead, QKVParallelLinear,
+from .layers import (LinearBase, LogitsProcessor, MergedColumnParallelLinear, ParallelLMHead, QKVParallelLinear,
                      RMSNorm, RowParallelLinear, SiluAndMul, VocabParallelEmbedding, get_rope)
 
 # SPD_FUSED_SILU_MIN_TOKENS: A/B knob (smaller batches go through the plain GEMM + SiLU·mul kernel)
@@ -33,6 +35,9 @@ class LlamaMLP:
         self.act_fn = SiluAndMul()
 
     def forward(self, x):
+        if self.gate_up_proj.weight_scale is not None:
+            gate_up, _ = self.gate_up_proj(x)
+            return self.down_proj(self.act_fn.forward_quant(gate_up))[0]
         if x.shape[0] >= _FUSED_SILU_MIN_TOKENS and ops.silu_fused(x, self.gate_up_proj.weight):
             x = self.gate_up_proj.forward_silu_mul(x)
         else:
@@ -102,16 +107,18 @@ class LlamaDecoderLayer:
 
     def forward(self, positions, hidden_states, forward_batch: ForwardBatch,
                 residual: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+        quantized = self.self_attn.qkv_proj.weight_scale is not None
+        norm = RMSNorm.forward_quant if quantized else RMSNorm.forward
         # Self Attention
         if residual is None:
             residual = hidden_states
-            hidden_states = self.input_layernorm(hidden_states)
+            hidden_states = norm(self.input_layernorm, hidden_states)
         else:
-            hidden_states, residual = self.input_layernorm(hidden_states, residual)
+            hidden_states, residual = norm(self.input_layernorm, hidden_states, residual)
         hidden_states = self.self_attn(positions=positions, hidden_states=hidden_states,
                                        forward_batch=forward_batch)
         # Fully Connected
-        hidden_states, residual = self.post_attention_layernorm(hidden_states, residual)
+        hidden_states, residual = norm(self.post_attention_layernorm, hidden_states, residual)
         hidden_states = self.mlp(hidden_states)
         return hidden_states, residual
 
@@ -139,10 +146,13 @@ class LlamaModel:
 
 
 class LlamaForCausalLM:
-    def __init__(self, config, dtype=torch.bfloat16, device="cuda"):
+    def __init__(self, config, dtype=torch.bfloat16, device="cuda", quantization: Optional[str] = None):
+        if quantization not in (None, "w8a8_int8"):
+            raise ValueError(f"quantization {quantization!r}: w8a8_int8 or none")
         self.config = config
         self.dtype = dtype
         self.device = device
+        self.quantization = quantization
         self.model = LlamaModel(config, dtype, device)
         if config.tie_word_embeddings:
             self.lm_head = self.model.embed_tokens
@@ -187,6 +197,25 @@ class LlamaForCausalLM:
             yield ("lm_head.weight", self.lm_head,
                    lambda w: ParallelLMHead.shard(w, tp_rank, tp_size))
 
+    def _scale_slots(self):
+        """(checkpoint name of the weight's scales, holder, shard function) of the weights that are 8-bit integers in a
+        quantised model: a row of the weight has one, so column-parallel shards take theirs, row-parallel ones all."""
+        if self.quantization is not None:
+            for name, holder, shard in self.named_slots():
+                if isinstance(holder, LinearBase):
+                    yield name + "_scale", holder, (lambda w: w) if isinstance(holder, RowParallelLinear) else shard
+
+    def _set_weight(self, holder, weight: torch.Tensor):
+        """A loaded shard: 8-bit integers stay (their scales are loaded beside them), 16-bit ones of a quantised model become such."""
+        if not isinstance(holder, LinearBase):
+            holder.weight = weight
+            return
+        if weight.dtype == torch.int8 and self.quantization is None:
+            raise ValueError("8-bit weights need quantization='w8a8_int8'")
+        holder.weight, holder.weight_scale = weight, None
+        if self.quantization is not None and weight.dtype != torch.int8:
+            holder.quantize_weight_int8()
+
     def full_shapes(self) -> Dict[str, Tuple[int, ...]]:
         cfg = self.config
         H, D = cfg.hidden_size, cfg.head_dim
@@ -207,18 +236,32 @@ class LlamaForCausalLM:
     def load_weights(self, weights: Iterable[Tuple[str, torch.Tensor]]):
         """Takes FULL (unsharded) tensors by checkpoint name; each rank keeps its TP shard."""
         slots = {name: (holder, shard) for name, holder, shard in self.named_slots()}
-        seen = set()
+        scales = {name: (holder, shard) for name, holder, shard in self._scale_slots()}
+        seen, loaded_scales = set(), {}
         for name, w in weights:
+            if name in scales:
+                holder, shard = scales[name]
+                loaded_scales[name] = (holder, shard(w.reshape(-1, 1).float()).to(self.device).contiguous())
+                continue
             if name not in slots:
                 if name == "lm_head.weight" and self.config.tie_word_embeddings:
                     continue
                 raise KeyError(f"unexpected parameter {name}")
             holder, shard = slots[name]
-            holder.weight = shard(w.to(self.dtype)).to(self.device).contiguous()
+            self._set_weight(holder, shard(w if w.dtype == torch.int8 else w.to(self.dtype)).to(self.device).contiguous())
             seen.add(name)
         missing = set(slots) - seen
         if missing:
             raise KeyError(f"missing parameters: {sorted(missing)[:4]} …")
+        for name, (holder, scale) in loaded_scales.items():
+            if holder.weight.dtype != torch.int8 or holder.weight_scale is not None:
+                raise ValueError(f"{name}: the weight did not come in 8-bit integers")
+            if scale.shape != (holder.weight.shape[0], 1):
+                raise ValueError(f"{name}: one scale for each of the weight's {holder.weight.shape[0]} rows, got {scale.numel()}")
+            holder.weight_scale = scale
+        for name, (holder, _) in scales.items():
+            if holder.weight_scale is None:
+                raise KeyError(f"missing parameters: ['{name}']")
 
     def dummy_full_weights(self, seed: int = 1234):
         """Yields (checkpoint name, FULL tensor) of the `--load-format dummy` model: one generator
@@ -248,8 +291,9 @@ class LlamaForCausalLM:
             if name not in slots:
                 continue
             holder, shard = slots[name]
-            holder.weight = shard(w).contiguous()
+            self._set_weight(holder, shard(w).contiguous())
 
     def state_dict(self) -> Dict[str, torch.Tensor]:
         """The local (sharded) parameters by checkpoint name."""
-        return {name: holder.weight for name, holder, _ in self.named_slots()}
+        weights = {name: holder.weight for name, holder, _ in self.named_slots()}
+        return {**weights, **{name: holder.weight_scale for name, holder, _ in self._scale_slots()}}

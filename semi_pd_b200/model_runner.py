@@ -99,7 +99,11 @@ class ModelRunner:
         model_type = getattr(self.model_config, "model_type", "llama")
         if self.dtype == torch.float32 and getattr(self.model_config, "layer_specs", None) is None:
             raise ValueError(f"--dtype float32: model_type {model_type!r} runs in 16-bit only")
-        self.model = get_model_class(model_type)(self.model_config, dtype=self.dtype, device=self.device)
+        quantization = self.server_args.quantization
+        if quantization is not None and (quantization != "w8a8_int8" or model_type != "llama"):
+            raise ValueError(f"--quantization {quantization}: w8a8_int8 of model_type 'llama' is supported, not of {model_type!r}")
+        kw = {} if quantization is None else {"quantization": quantization}
+        self.model = get_model_class(model_type)(self.model_config, dtype=self.dtype, device=self.device, **kw)
         fmt = self.server_args.load_format
         path = self.server_args.model_path
         if fmt == "auto":
@@ -217,6 +221,8 @@ class ModelRunner:
 
     def forward_extend(self, forward_batch: ForwardBatch, skip_attn_backend_init: bool = False
                        ) -> LogitsProcessorOutput:
+        if forward_batch.return_logprob and getattr(self.model_config, "layer_specs", None) is not None:
+            raise NotImplementedError(f"return_logprob: not of model_type {self.model_config.model_type!r}")
         if not skip_attn_backend_init:
             self.attn_backend.init_forward_metadata(forward_batch)
         return self.model.forward(forward_batch.input_ids, forward_batch.positions, forward_batch)

@@ -4,7 +4,7 @@ python/sglang/srt/managers/schedule_batch.py the semi-PD path exercises:
 `pre_allocated_req_pool_indices` variant the prefill worker uses, :923-935),
 `prepare_for_decode` (:1144-1207), `filter_batch` / `merge_batch` (:1209-1306),
 `check_decode_mem` / `retract_decode` (:1022-1125) and `get_model_worker_batch` (:1308-1370).
-Sampling is greedy-only; logprobs / grammar / multimodal are off this path
+Sampling is greedy-only; grammar / multimodal are off this path; `return_logprob` on a batch gives its input tokens' logprobs
 (managers/semi_pd_scheduler.py:207-209, semi_pd_decode_scheduler.py:354).
 """
 from __future__ import annotations
@@ -370,6 +370,8 @@ class ScheduleBatch:
             extend_seq_lens=self.extend_lens if extend else None,
             extend_prefix_lens=self.prefix_lens if extend else None,
             extend_logprob_start_lens=[0] * len(self.reqs) if extend else None,
+            return_logprob=getattr(self, "return_logprob", False),
+            extend_input_logprob_token_ids=getattr(self, "extend_input_logprob_token_ids", None) if extend else None,
             gather_logits=getattr(self, "gather_logits", True),
             extend_logit_rows=getattr(self, "extend_logit_rows", None) if extend else None)
 

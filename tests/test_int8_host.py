@@ -74,3 +74,58 @@ def test_there_is_no_cpu_path():
 
 def test_dtype_codes():
     assert _lib.SPD_I8 == 3 and "SPD_I8 3" in open(_lib.HEADER_PATH).read()
+
+
+def test_quantization_flag():
+    from semi_pd_b200.launch_server import prepare_server_args
+    assert prepare_server_args([]).quantization is None
+    assert prepare_server_args(["--quantization", "w8a8_int8"]).quantization == "w8a8_int8"
+    with pytest.raises(SystemExit):
+        prepare_server_args(["--quantization", "fp4"])
+
+
+def tiny(quantization="w8a8_int8"):
+    from semi_pd_b200.configs import get_model_config
+    from semi_pd_b200.llama import LlamaForCausalLM
+    return LlamaForCausalLM(get_model_config("tiny-llama-test"), device="cpu", quantization=quantization)
+
+
+def checkpoint(model, int8=True):
+    for name, shape in model.full_shapes().items():
+        if int8 and name.endswith("proj.weight"):
+            yield name, torch.ones(shape, dtype=torch.int8)
+            yield name + "_scale", torch.full((shape[0],), 0.5)
+        else:
+            yield name, torch.ones(shape, dtype=torch.bfloat16)
+
+
+def test_checkpoints_of_8_bit_weights():
+    m = tiny()
+    m.load_weights(checkpoint(m))
+    q = m.model.layers[1].self_attn.qkv_proj
+    assert q.weight.dtype == torch.int8 and q.weight_scale.shape == (q.weight.shape[0], 1) and q.weight_scale.dtype == torch.float32
+    assert m.lm_head.weight.dtype == torch.bfloat16
+    names = {n for n, _ in checkpoint(m)}
+    assert names == set(m.state_dict())
+    with pytest.raises(KeyError, match="missing"):
+        m.load_weights((n, w) for n, w in checkpoint(m) if n != "model.layers.0.mlp.down_proj.weight_scale")
+    with pytest.raises(ValueError, match="one scale"):
+        m.load_weights((n, w[:-1] if n == "model.layers.0.mlp.down_proj.weight_scale" else w) for n, w in checkpoint(m))
+    with pytest.raises(ValueError, match="quantization"):
+        plain = tiny(None)
+        plain.load_weights((n, w) for n, w in checkpoint(plain) if not n.endswith("_scale"))
+    with pytest.raises(KeyError, match="unexpected"):
+        plain.load_weights((n, w) for n, w in checkpoint(plain) if n.endswith("_scale"))
+    with pytest.raises(ValueError, match="quantization"):
+        tiny("int3")
+
+
+def test_shards_of_8_bit_weights():
+    from semi_pd_b200.layers import MergedColumnParallelLinear, QKVParallelLinear, RowParallelLinear
+    scale = torch.arange((4 + 2 * 2) * 8, dtype=torch.float32)[:, None]
+    parts = [QKVParallelLinear.shard(scale, 8, 4, 2, r, 2) for r in range(2)]
+    w = scale.expand(-1, 16).contiguous()
+    for r in range(2):
+        assert torch.equal(QKVParallelLinear.shard(w, 8, 4, 2, r, 2)[:, :1], parts[r])
+        assert torch.equal(MergedColumnParallelLinear.shard(w, r, 2)[:, :1], MergedColumnParallelLinear.shard(scale, r, 2))
+        assert RowParallelLinear.shard(w, r, 2).shape == (64, 8)
