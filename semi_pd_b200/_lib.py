@@ -295,6 +295,7 @@ def _load():
         fn.argtypes = args
     # the per-layer calls without ctypes (csrc/pycalls.cpp): the same functions of the same library
     try:
+        import torch  # noqa: F401  (its libraries, which the module's calls of tensors are linked to)
         from . import _calls
     except ImportError:  # not built, or built for another interpreter (its name is the file's): ctypes does all
         return lib
@@ -305,6 +306,14 @@ def _load():
 
 
 lib = _load()
+
+# the operators that take tensors in one call (csrc/tensorcalls.cpp), None where they are not built
+try:
+    from . import _calls as tensor_calls
+    if not hasattr(tensor_calls, "int8_scaled_mm"):
+        tensor_calls = None
+except ImportError:
+    tensor_calls = None
 
 
 class _Counter:

@@ -10,6 +10,9 @@
 #include <type_traits>
 
 #include "../../include/spd.h"
+#ifdef SPD_TORCH
+#include "tensorcalls.h"
+#endif
 
 namespace {
 
@@ -99,6 +102,9 @@ PyMethodDef calls[] = {
 // bind({name: (address, ctypes function)}) -> {name: function} for the names that are here
 PyObject* bind(PyObject*, PyObject* functions) {
   if (!PyDict_Check(functions)) return PyErr_Format(PyExc_TypeError, "bind takes a dict");
+#ifdef SPD_TORCH
+  spd_tensor_bind(functions);
+#endif
   PyObject* out = PyDict_New();
   for (PyMethodDef* m = calls; out && m->ml_name; ++m) {
     PyObject* pair = PyDict_GetItemString(functions, m->ml_name);  // borrowed
@@ -124,4 +130,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* m = PyModule_Create(&module);
+#ifdef SPD_TORCH
+  if (m && PyModule_AddFunctions(m, spd_tensor_methods) < 0) Py_CLEAR(m);
+#endif
+  return m;
+}

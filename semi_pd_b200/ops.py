@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import SPD_EPI_GELU, SPD_EPI_NONE, SPD_EPI_OLDER_W, SPD_EPI_SILU_MUL, check, lib
+from ._lib import SPD_EPI_GELU, SPD_EPI_NONE, SPD_EPI_OLDER_W, SPD_EPI_SILU_MUL, _Counter, check, lib, tensor_calls
 
 _DTYPE = {torch.bfloat16: _lib.SPD_BF16, torch.float16: _lib.SPD_F16}
 # the 32-bit capable operators (hybrid model family) additionally take float32
@@ -500,6 +500,11 @@ def silu_fused(x: torch.Tensor, weight: torch.Tensor) -> bool:
 # ------------------------------------------------------------------------------------------------
 def _quant_int8(fn: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
                 silu_mul: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    if tensor_calls is not None:
+        out = tensor_calls.quant_int8(x, residual, weight, eps, silu_mul)
+        if out is not None:
+            _Counter.launches += 1
+            return out
     _all_here(fn, x, residual, weight)
     shape, stride, dtype = x.shape, x.stride(), x.dtype
     if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
@@ -549,6 +554,11 @@ def int8_scaled_mm(mat_a: torch.Tensor, mat_b: torch.Tensor, scales_a: torch.Ten
     """scales_a[m] scales_b[n] (mat_a mat_b)[m, n] + bias[n], rounded once (sgl-kernel/python/sgl_kernel/gemm.py: int8_scaled_mm).
     mat_a int8 [M, K] with contiguous rows; mat_b int8 [K, N] with contiguous columns (`weight.t()`); scales_a fp32, M of them;
     scales_b fp32, N; bias [N] of out_dtype, bf16 or fp16.  K is a multiple of 16, N of 8.  older_weight: as in `linear`."""
+    if tensor_calls is not None:
+        out = tensor_calls.int8_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias, older_weight, get_sm_budget())
+        if out is not None:
+            _Counter.launches += 1
+            return out
     _all_here("int8_scaled_mm", mat_a, mat_b, scales_a, scales_b, bias)
     shape_a, shape_b = mat_a.shape, mat_b.shape
     if len(shape_a) != 2 or len(shape_b) != 2:
@@ -582,6 +592,11 @@ def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
     """(logprobs f32 [M], logsumexp f32 [M]) of the logits x @ weight.T [M, V], which are never stored: log-softmax over the rows of
     `weight` at targets[m] (int64); a target outside [0, V) asks for nothing and gets 0.  x and weight are bf16 or fp16, or both
     int8 with fp32 scales for each row of either.  older_weight: as in `linear`."""
+    if tensor_calls is not None:
+        out = tensor_calls.linear_logprobs(x, weight, targets, x_scales, weight_scales, older_weight, get_sm_budget())
+        if out is not None:
+            _Counter.launches += 2
+            return out
     _all_here("linear_logprobs", x, weight, targets, x_scales, weight_scales)
     shape, w_shape = x.shape, weight.shape
     stride, w_stride = x.stride(), weight.stride()
@@ -613,6 +628,7 @@ def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor
                                   None if weight_scales is None else weight_scales.data_ptr(), targets.data_ptr(), M, V, K,
                                   stride[0] if M > 1 else K, w_stride[0] if V > 1 else K, dtype, 1 if older_weight else 0,
                                   ws.data_ptr(), need, get_sm_budget(), _stream()), "spd_linear_logprobs")
+    _Counter.launches += 1  # the join
     return logprobs, lse
 
 

@@ -34,6 +34,8 @@ SCHEMAS = {
     "apply_rope_pos_ids_cos_sin_cache":
         "(Tensor q, Tensor k, Tensor! q_rope, Tensor! k_rope, Tensor cos_sin_cache, Tensor pos_ids, "
         "bool interleave, int cuda_stream) -> ()",
+    "int8_scaled_mm":
+        "(Tensor mat_a, Tensor mat_b, Tensor scales_a, Tensor scales_b, ScalarType out_dtype, Tensor? bias) -> Tensor",
 }
 
 _libs: Dict[str, torch.library.Library] = {}
@@ -77,6 +79,10 @@ def _apply_rope(q, k, q_rope, k_rope, cos_sin_cache, pos_ids, interleave, cuda_s
         ops.apply_rope_with_cos_sin_cache_inplace(pos_ids, q2, k2, head, cos_sin_cache, is_neox=not interleave)
 
 
+def _int8_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias):
+    return ops.int8_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias)
+
+
 class _Null:
     def __enter__(self):
         return self
@@ -86,7 +92,7 @@ class _Null:
 
 
 _IMPLS = {"rmsnorm": _rmsnorm, "fused_add_rmsnorm": _fused_add_rmsnorm, "silu_and_mul": _silu_and_mul,
-          "apply_rope_pos_ids_cos_sin_cache": _apply_rope}
+          "apply_rope_pos_ids_cos_sin_cache": _apply_rope, "int8_scaled_mm": _int8_scaled_mm}
 
 
 def register(namespace: str = "spd") -> torch.library.Library:

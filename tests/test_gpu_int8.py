@@ -276,3 +276,11 @@ def test_refusals():
                      (ops.silu_and_mul_quant_int8, (x[:, :33],))]:
         with pytest.raises(RuntimeError):
             fn(*args)
+
+
+def test_dispatcher_op():
+    import semi_pd_b200.torch_ops  # noqa: F401
+    a, b = int8_rows(4, 64, 1), int8_rows(16, 64, 2)
+    sa, sb, bias = torch.rand(4, 1, device=DEV), torch.rand(16, 1, device=DEV), torch.ones(16, device=DEV, dtype=torch.float16)
+    for kw in (None, bias):
+        assert torch.equal(torch.ops.spd.int8_scaled_mm(a, b.t(), sa, sb, torch.float16, kw), ops.int8_scaled_mm(a, b.t(), sa, sb, torch.float16, kw))
