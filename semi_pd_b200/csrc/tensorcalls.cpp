@@ -64,14 +64,15 @@ PyObject* pair(const at::Tensor& a, const at::Tensor& b) {
   return out;
 }
 
-// (x, residual | None, weight | None, eps, silu_mul)
+// (x, residual | None, weight | None, eps, silu_mul, sm_budget)
 PyObject* quant_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 5 || !quant_fn || !PyFloat_CheckExact(a[3]) || !PyLong_CheckExact(a[4])) Py_RETURN_NONE;
+  if (n != 6 || !quant_fn || !PyFloat_CheckExact(a[3]) || !PyLong_CheckExact(a[4]) || !PyLong_CheckExact(a[5])) Py_RETURN_NONE;
   const Here here;
   const at::Tensor *x = tensor(a[0], here.device), *residual = nullptr, *weight = nullptr;
   if (!x || !rows(*x) || x->scalar_type() == at::kChar || code(x->scalar_type()) < 0) Py_RETURN_NONE;
   const long silu = PyLong_AsLong(a[4]);
+  const int budget = static_cast<int>(PyLong_AsLong(a[5]));
   const int64_t count = x->size(0), cols = x->size(1), dim = silu ? cols / 2 : cols;
   if (silu && cols % 2) Py_RETURN_NONE;
   if (a[1] != Py_None) {
@@ -90,7 +91,7 @@ PyObject* quant_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return quant_fn(static_cast<int8_t*>(q.data_ptr()), static_cast<float*>(s.data_ptr()), x->data_ptr(),
                     residual ? residual->data_ptr() : nullptr, weight ? weight->data_ptr() : nullptr, count, dim,
                     count > 1 ? x->stride(0) : cols, static_cast<float>(PyFloat_AS_DOUBLE(a[3])), static_cast<int>(silu),
-                    code(x->scalar_type()), here.stream);
+                    code(x->scalar_type()), budget, here.stream);
   });
   if (rc) Py_RETURN_NONE;
   return pair(q, s);

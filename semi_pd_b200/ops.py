@@ -501,7 +501,7 @@ def silu_fused(x: torch.Tensor, weight: torch.Tensor) -> bool:
 def _quant_int8(fn: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
                 silu_mul: int) -> Tuple[torch.Tensor, torch.Tensor]:
     if tensor_calls is not None:
-        out = tensor_calls.quant_int8(x, residual, weight, eps, silu_mul)
+        out = tensor_calls.quant_int8(x, residual, weight, eps, silu_mul, get_sm_budget())
         if out is not None:
             _Counter.launches += 1
             return out
@@ -523,7 +523,7 @@ def _quant_int8(fn: str, x: torch.Tensor, residual: Optional[torch.Tensor], weig
     scales = x.new_empty((rows, 1), dtype=torch.float32)
     check(lib.spd_quant_int8(q.data_ptr(), scales.data_ptr(), x.data_ptr(), None if residual is None else residual.data_ptr(),
                              None if weight is None else weight.data_ptr(), rows, dim, stride[0] if rows > 1 else shape[1], float(eps),
-                             silu_mul, _dt(x), _stream()), "spd_quant_int8")
+                             silu_mul, _dt(x), get_sm_budget(), _stream()), "spd_quant_int8")
     return q, scales
 
 

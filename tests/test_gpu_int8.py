@@ -41,7 +41,8 @@ def close_quant(q, s, y, rel):
     assert near.float().mean() < 0.01
 
 
-SIZES = [(1, 16), (1, 4096), (3, 1024), (5, 1040), (33, 2064), (7, 8192), (2, 14336), (2, 16400), (3, 32768), (700, 256)]
+SIZES = [(1, 16), (1, 4096), (3, 1024), (5, 1040), (33, 2064), (7, 8192), (2, 14336), (2, 16400), (3, 32768), (700, 256), (1501, 4096), (901, 2064),
+         (601, 14336)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -284,3 +285,22 @@ def test_dispatcher_op():
     sa, sb, bias = torch.rand(4, 1, device=DEV), torch.rand(16, 1, device=DEV), torch.ones(16, device=DEV, dtype=torch.float16)
     for kw in (None, bias):
         assert torch.equal(torch.ops.spd.int8_scaled_mm(a, b.t(), sa, sb, torch.float16, kw), ops.int8_scaled_mm(a, b.t(), sa, sb, torch.float16, kw))
+
+
+@pytest.mark.parametrize("k", [1024, 4096, 14336])
+def test_rows_do_not_depend_on_their_number(k):
+    """A CTA a row and CTAs that take one row after another give the same bits, on the whole device and on a part of it."""
+    x, r = hidden(2000, 2 * k, torch.bfloat16, 1), hidden(2000, k, torch.bfloat16, 2)
+    w = (1 + 0.1 * torch.randn(k, generator=gen(3), device=DEV)).bfloat16()
+    n = x[:, :k].contiguous()
+    forms = [lambda m: ops.silu_and_mul_quant_int8(x[:m]), lambda m: ops.rmsnorm_quant_int8(n[:m], w),
+             lambda m: ops.fused_add_rmsnorm_quant_int8(n[:m], r[:m].clone(), w)]
+    for form in forms:
+        q, s = form(2000)
+        for m, sms in ((1, 0), (100, 0), (777, 0), (1999, 0), (2000, 40), (300, 16)):
+            ops.set_sm_budget(sms)
+            try:
+                q2, s2 = form(m)
+            finally:
+                ops.set_sm_budget(0)
+            assert torch.equal(q[:m], q2) and torch.equal(s[:m], s2)

@@ -24,11 +24,11 @@ def test_product_refuses(code, kw):
 
 def test_no_tokens_is_no_work():
     assert mm(M=0) == 0
-    assert lib.spd_quant_int8(A, A, A, None, None, 0, 64, 64, 0.0, 0, 0, None) == 0
+    assert lib.spd_quant_int8(A, A, A, None, None, 0, 64, 64, 0.0, 0, 0, 0, None) == 0
 
 
 def quant(q=A, s=A, x=A, residual=None, weight=None, rows=2, dim=64, stride=64, silu=0, dtype=0):
-    return lib.spd_quant_int8(q, s, x, residual, weight, rows, dim, stride, 1e-5, silu, dtype, None)
+    return lib.spd_quant_int8(q, s, x, residual, weight, rows, dim, stride, 1e-5, silu, dtype, 0, None)
 
 
 @pytest.mark.parametrize("code,kw", [
