@@ -37,11 +37,28 @@ struct QuantParams {
   float eps;
 };
 
-__device__ __forceinline__ uint32_t pack_s8(float a, float b, float c, float d) {
-  uint32_t hi, lo;
-  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(__float2int_rn(d)), "r"(__float2int_rn(c)));
-  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(lo) : "r"(__float2int_rn(b)), "r"(__float2int_rn(a)), "r"(hi));
-  return lo;
+// Four products rounded to integers of 8 bits, halves to even.  Added to 1.5 * 2^23, whose last place is 1, a float of that size holds
+// its integer in two's complement in its lowest byte; the conversion instruction goes at the rate of the exponentials (SiLU * mul of
+// 8192 x 14336 in 100 us with it).
+__device__ __forceinline__ uint32_t pack_s8(float a, float b, float c, float d, float k) {
+  constexpr float kPlace = 12582912.f;
+  const uint32_t lo = __byte_perm(__float_as_uint(fmaf(a, k, kPlace)), __float_as_uint(fmaf(b, k, kPlace)), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(fmaf(c, k, kPlace)), __float_as_uint(fmaf(d, k, kPlace)), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+
+// max(top, |y|) that lets NaN through
+__device__ __forceinline__ float max_abs(float top, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(y)));
+  return r;
+}
+
+// g / (1 + e^-g): the exponential to 2^-22, the quotient to an ulp more
+__device__ __forceinline__ float silu_flushed(float g) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(-1.4426950408889634f * g)));
+  return g * r;
 }
 
 template <typename T>
@@ -57,7 +74,7 @@ __device__ __forceinline__ void unpack8(const uint4& u, float* f) {
 
 // y of one piece of 8, from x and what stands beside it (the residual, or up); *sum: x + residual for memory
 template <typename T, int kForm>
-__device__ __forceinline__ void quant_piece(const uint4& x, const uint4& beside, const uint4& w, float (&y)[8], float& ss, uint32_t& top,
+__device__ __forceinline__ void quant_piece(const uint4& x, const uint4& beside, const uint4& w, float (&y)[8], float& ss, float& top,
                                             uint4* sum) {
   unpack8<T>(x, y);
   float f[8];
@@ -79,10 +96,10 @@ __device__ __forceinline__ void quant_piece(const uint4& x, const uint4& beside,
   if constexpr (kForm == kQuantSilu) {
     unpack8<T>(beside, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = silu_f32(y[j]) * f[j];
+    for (int j = 0; j < 8; ++j) y[j] = silu_flushed(y[j]) * f[j];
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
+  for (int j = 0; j < 8; ++j) top = max_abs(top, y[j]);
 }
 
 // The factor on y (before the norm's own) and the row's scale, from the row's maximum and sum of squares
@@ -97,7 +114,7 @@ __device__ __forceinline__ float quant_factor(uint32_t top, float ss, const Quan
 }
 
 __device__ __forceinline__ uint2 quant_pack(const float (&y)[8], float k) {
-  return make_uint2(pack_s8(y[0] * k, y[1] * k, y[2] * k, y[3] * k), pack_s8(y[4] * k, y[5] * k, y[6] * k, y[7] * k));
+  return make_uint2(pack_s8(y[0], y[1], y[2], y[3], k), pack_s8(y[4], y[5], y[6], y[7], k));
 }
 
 // x as it is stays packed until it is multiplied: its maximum is taken over pairs of 16 bits, and 32 registers a thread leave room for
@@ -119,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, (quant_ctas<kForm, kThreads, kVecs>(
   uint4* r = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.residual) + row * p.x_stride);
   float y[kForm == kQuantPlain ? 1 : kVecs][8];
   uint4 raw[kForm == kQuantPlain ? kVecs : 1];
-  float ss = 0.f;
+  float ss = 0.f, most = 0.f;
   uint32_t top = 0;
   if constexpr (kForm == kQuantPlain) {
 #pragma unroll
@@ -143,10 +160,11 @@ __global__ void __launch_bounds__(kThreads, (quant_ctas<kForm, kThreads, kVecs>(
         if constexpr (kForm == kQuantAddNorm) beside = r[v];
         if constexpr (kForm == kQuantSilu) beside = x[p.vecs + v];
         if constexpr (kHasNorm) w = reinterpret_cast<const uint4*>(p.w)[v];
-        quant_piece<T, kForm>(x[v], beside, w, y[i], ss, top, &sum);
+        quant_piece<T, kForm>(x[v], beside, w, y[i], ss, most, &sum);
         if constexpr (kForm == kQuantAddNorm) r[v] = sum;
       }
     }
+    top = __float_as_uint(most);
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   top = __reduce_max_sync(0xffffffffu, top);
@@ -179,8 +197,8 @@ __global__ void __launch_bounds__(kThreads, (quant_ctas<kForm, kThreads, kVecs>(
 
 // Many rows of 32-bit values: a CTA takes rows one after another, and while a row is worked on the next one is on its way into shared
 // memory.  A thread copies and reads its own pieces, so only the row's reduction needs a barrier (in turn in two places, one a row).
-// us, a CTA a row / this: SiLU, 8192 x 14336 127 / 100 (floor 90), 1300 x 14336 22.8 / 19.3 (14.2); residual and norm, 4099 x 4096
-// 19.4 / 18.2 (18.0).  Results are the same bits: the sums are over the same pieces in the same order.
+// us, a CTA a row / this: SiLU, 8192 x 14336 125 / 97 (floor 90), 1300 x 14336 22.5 / 18.3 (14.2); residual and norm, 4099 x 4096
+// 19.6 / 18.3 (18.0).  Results are the same bits: the sums are over the same pieces in the same order.
 template <typename T, int kForm, int kThreads, int kVecs>
 __global__ void __launch_bounds__(kThreads) quant_int8_rows_kernel(const QuantParams p) {
   constexpr bool kHasNorm = kForm == kQuantNorm || kForm == kQuantAddNorm;
@@ -225,19 +243,18 @@ __global__ void __launch_bounds__(kThreads) quant_int8_rows_kernel(const QuantPa
     fetch(row + gridDim.x, turn ^ 1);
     cp_async_wait<1>();
     float y[kVecs][8];
-    float ss = 0.f;
-    uint32_t top = 0;
+    float ss = 0.f, most = 0.f;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int v = threadIdx.x + i * kThreads;
       if (v < p.vecs) {
         uint4 beside{}, sum;
         if constexpr (kIn == 2) beside = *place(turn, 1, i);
-        quant_piece<T, kForm>(*place(turn, 0, i), beside, w[kHasNorm ? i : 0], y[i], ss, top, &sum);
+        quant_piece<T, kForm>(*place(turn, 0, i), beside, w[kHasNorm ? i : 0], y[i], ss, most, &sum);
         if constexpr (kForm == kQuantAddNorm) row_of(row, 1)[v] = sum;
       }
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
     if constexpr (kHasNorm) ss = warp_sum(ss);
     if (lane == 0) {
       tops[turn][warp] = top;
@@ -301,6 +318,7 @@ static int launch_quant(const QuantParams& p, int sms, cudaStream_t stream) {
   } else {
     // 32-bit values: 2 pieces a thread (8192 x 8192 with a residual 77 us, 4 pieces 84; 4099 x 4096 19.5, 4 pieces 21.3)
     if (p.vecs <= 256) return launch_quant_sized<T, kForm, 256, 1>(p, sms, stream);
+    if (kForm == kQuantNorm && p.vecs <= 512) return launch_quant_sized<T, kForm, 128, 4>(p, sms, stream);  // 4099 x 4096 10.2, 2 pieces 12.0
     if (p.vecs <= 512) return launch_quant_sized<T, kForm, 256, 2>(p, sms, stream);
     if (p.vecs <= 1024) return launch_quant_sized<T, kForm, 512, 2>(p, sms, stream);
   }
