@@ -101,6 +101,11 @@ constexpr int kFewStages = 12;    // at most
 constexpr int kFewFixed = 1024 + 256 + 2048;  // alignment, barriers, a scale and a target for each token
 constexpr int kMaxSplit = 4;
 
+// TMEM columns of a CTA, and the least shared memory that it takes: its share of the SM's, so that whatever CTAs are on an SM
+// together never wait for one another's columns.
+__host__ __device__ constexpr int few_columns(int cols) { return cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256; }
+constexpr int few_least_smem(int cols) { return few_columns(cols) * (233472 / 512) - 1024; }
+
 __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
   int4 v;
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -142,8 +147,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   const int S = static_cast<int>(cluster_nctarank() >> 1), s = static_cast<int>(crank >> 1);
   const int tile = blockIdx.x / (2 * S), wt = tile / p.tok_tiles, tt = tile - wt * p.tok_tiles;
   const int kb0 = s * p.kblocks / S, kb1 = (s + 1) * p.kblocks / S;
-  const int accs = kKind == kInt8 ? 1 : p.accs, cols = p.n * accs;
-  const int half = p.n >> 1, tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+  const int accs = kKind == kInt8 ? 1 : p.accs, half = p.n >> 1, tmem_cols = few_columns(p.n * accs);
   const int tok_base = tt * p.n, tokens = min(p.n, p.m_rows - tok_base);
   const int row_base = wt * 256 + static_cast<int>(rank) * 128;
 
@@ -198,6 +202,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     }
     __syncwarp();
   } else if (warp == 5) {
+    griddep_wait();  // (the tokens come behind it; a bounded wait for them starts there)
     if (rank == 0 && elect_one()) {
       const uint32_t idesc = gs_idesc<kKind>(256, p.n);
       const uint16_t both = static_cast<uint16_t>(0b11 << leader);
@@ -870,9 +875,10 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
     if (int rc = make_tmap_2d_sw128(&tw, w, N, kbytes / 2, w_stride / 2, 128, kGsBlock / 2)) return rc;
     if (int rc = make_tmap_2d_sw128(&ta, a, M, kbytes / 2, a_stride / 2, p.n / 2, kGsBlock / 2)) return rc;
     p.accs = kKind == kInt8 ? 1 : few_accumulators(p.n, p.kblocks);
+    const int need = p.stages * p.slot + kFewFixed, least = few_least_smem(p.n * p.accs), smem = need > least ? need : least;
     static std::atomic<uint64_t> done{0};
     const int ctas = static_cast<int>((N + 255) / 256) * plan.tok_tiles * 2 * plan.split;
-    return launch_pairs(few_tokens_kernel<kKind, kEnd, T>, done, ctas, 2 * plan.split, kFewThreads, p.stages * p.slot + kFewFixed, stream,
+    return launch_pairs(few_tokens_kernel<kKind, kEnd, T>, done, ctas, 2 * plan.split, kFewThreads, smem, stream,
                         tw, ta, p);
   }
   if (int rc = make_tmap_2d_sw128(&tw, w, N, kbytes / 2, w_stride / 2, 128, kGsBlock / 2)) return rc;

@@ -304,3 +304,51 @@ def test_rows_do_not_depend_on_their_number(k):
             finally:
                 ops.set_sm_budget(0)
             assert torch.equal(q[:m], q2) and torch.equal(s[:m], s2)
+
+
+@pytest.mark.parametrize("m,n", [(70000, 32768), (200, 11000000)])
+def test_offsets_beyond_32_bits(m, n):
+    """Outputs of more than 2^31 elements: the last rows and columns are where they belong."""
+    a, b = int8_rows(m, 16, 1), int8_rows(n, 16, 2)
+    sa, sb = torch.rand(m, device=DEV), torch.rand(n, device=DEV)
+    out = ops.int8_scaled_mm(a, b.t(), sa, sb, torch.float16)
+    assert out.numel() > 2 ** 31
+    for r in (slice(0, 3), slice(m // 2, m // 2 + 3), slice(m - 3, m)):
+        for c in (slice(0, 300), slice(n // 2, n // 2 + 300), slice(n - 300, n)):
+            want, tol = product(a[r], b[c], sa[r], sb[c], None, torch.float16)
+            fits = want.abs() < 65000  # (fp16 overflows beyond)
+            assert (((out[r, c].double() - want).abs() <= tol) | ~fits).all()
+    del out
+    torch.cuda.empty_cache()
+
+
+def test_quant_of_more_than_32_bits_of_elements():
+    x = torch.empty(70000, 32768, device=DEV, dtype=torch.bfloat16)
+    for part in x.split(10000):
+        part.normal_()
+    q, s = ops.per_token_quant_int8(x)
+    for r in (slice(0, 2), slice(65000, 65002), slice(69998, 70000)):
+        want, scale = quantised(x[r].double())
+        assert torch.equal(q[r].double(), want)
+    w = torch.ones(32768, device=DEV, dtype=torch.bfloat16)
+    q2, s2 = ops.rmsnorm_quant_int8(x, w, 1e-5)
+    for r in (slice(0, 2), slice(69998, 70000)):
+        v = x[r].double()
+        close_quant(q2[r], s2[r], v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-5), (32768 / 512 + 20) * 2.0 ** -24)
+    del x, q, q2
+    torch.cuda.empty_cache()
+
+
+def test_behind_a_long_kernel():
+    """Waits inside a product start when the kernel before it is done, whatever that takes."""
+    a, b = int8_rows(8, 1024, 1), int8_rows(512, 1024, 2)
+    sa, sb = torch.rand(8, device=DEV), torch.rand(512, device=DEV)
+    want = ops.int8_scaled_mm(a, b.t(), sa, sb, torch.bfloat16)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(int(4e9))
+    out = ops.int8_scaled_mm(a, b.t(), sa, sb, torch.bfloat16, older_weight=True)
+    q, s = ops.per_token_quant_int8(out)
+    out2 = ops.int8_scaled_mm(q, int8_rows(64, 512, 3).t(), s, sb[:64], torch.bfloat16, older_weight=True)
+    torch.cuda.synchronize()
+    ops.check_waits()
+    assert torch.equal(out, want) and out2.isfinite().all()

@@ -150,3 +150,22 @@ def test_refusals():
                  (x[:, :60], w[:, :60], t), (x[:, 1:33], w[:, :32], t), (xi[:, :56], wi[:, :56], t, xs, ws)]:
         with pytest.raises(RuntimeError):
             ops.linear_logprobs(*args)
+
+
+def test_two_streams_at_once():
+    """Calls of both forms on two streams beside one another, each with a workspace of its own."""
+    sets = []
+    for m, v, k, dtype in ((16, 30000, 1024, torch.bfloat16), (400, 20000, 512, torch.float16), (64, 30000, 1024, torch.int8)):
+        x, w, xs, ws = operands(m, v, k, dtype)
+        t = torch.arange(m, device=DEV) * 7
+        sets.append((x, w, t, xs, ws, ops.linear_logprobs(x, w, t, xs, ws)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(30):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append([ops.linear_logprobs(*s[:5]) for s in sets[i % 2:] + sets[:i % 2]])
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        for (lp, lse), s in zip(outs, sets[i % 2:] + sets[:i % 2]):
+            assert torch.equal(lp, s[5][0]) and torch.equal(lse, s[5][1])
