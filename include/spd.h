@@ -905,7 +905,7 @@ int spd_gated_group_norm(void* out, const float* y, const void* z, const void* w
 int spd_quant_int8(int8_t* q, float* scales, const void* x, void* residual, const void* weight, int64_t rows, int64_t dim,
                    int64_t x_stride, float eps, int silu_mul, int dtype, int sm_budget, spd_stream_t stream);
 /* out[m][n] = scales_a[m] * scales_b[n] * sum_k a[m][k] b[n][k] + bias[n], rounded once to dtype (bf16 or fp16; bias of that type
- * or NULL).  a [M, K], b [N, K] int8, their sums exact.  K, lda, ldb multiples of 16, N and ldc of 8; K <= 131072.
+ * or NULL).  a [M, K], b [N, K] int8, their sums exact.  K, lda, ldb multiples of 16, N and ldc of 8; K < 131072.
  * older_w: as SPD_EPI_OLDER_W.  No workspace. */
 int spd_int8_scaled_mm(void* out, const int8_t* a, const int8_t* b, const float* scales_a, const float* scales_b, const void* bias,
                        int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int dtype, int older_w,

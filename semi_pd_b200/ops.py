@@ -553,7 +553,7 @@ def int8_scaled_mm(mat_a: torch.Tensor, mat_b: torch.Tensor, scales_a: torch.Ten
                    bias: Optional[torch.Tensor] = None, older_weight: bool = False) -> torch.Tensor:
     """scales_a[m] scales_b[n] (mat_a mat_b)[m, n] + bias[n], rounded once (sgl-kernel/python/sgl_kernel/gemm.py: int8_scaled_mm).
     mat_a int8 [M, K] with contiguous rows; mat_b int8 [K, N] with contiguous columns (`weight.t()`); scales_a fp32, M of them;
-    scales_b fp32, N; bias [N] of out_dtype, bf16 or fp16.  K is a multiple of 16, N of 8.  older_weight: as in `linear`."""
+    scales_b fp32, N; bias [N] of out_dtype, bf16 or fp16.  K is a multiple of 16 below 131072, N of 8.  older_weight: as in `linear`."""
     if tensor_calls is not None:
         out = tensor_calls.int8_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias, older_weight, get_sm_budget())
         if out is not None:

@@ -166,8 +166,9 @@ def test_product(m, n, k, dtype):
 
 @pytest.mark.parametrize("m", [3, 40, 160, 600])
 def test_sums_that_need_32_bits_are_exact(m):
-    k, n = 131072, 264
-    a, b = torch.full((m, k), -128, device=DEV, dtype=torch.int8), torch.full((n, k), -127, device=DEV, dtype=torch.int8)
+    k, n = 131056, 264
+    a, b = torch.full((m, k), -128, device=DEV, dtype=torch.int8), torch.full((n, k), -128, device=DEV, dtype=torch.int8)
+    b[1] = 127
     a[:, 5] = torch.arange(m, device=DEV).remainder(100).to(torch.int8)
     ones = torch.ones(max(m, n), device=DEV)
     scale = 2.0 ** -20

@@ -17,7 +17,8 @@ def mm(out=A, a=A, b=A, sa=A, sb=A, bias=None, M=4, N=64, K=64, lda=64, ldb=64, 
     (-1, dict(out=None)), (-1, dict(a=None)), (-1, dict(b=None)), (-1, dict(sa=None)), (-1, dict(sb=None)), (-1, dict(M=-1)),
     (-1, dict(N=0)), (-1, dict(K=0)), (-1, dict(dtype=2)), (-1, dict(dtype=7)), (-1, dict(lda=48)), (-1, dict(ldb=48)), (-1, dict(ldc=56)),
     (-2, dict(K=56)), (-2, dict(N=60)), (-2, dict(lda=72)), (-2, dict(ldb=72)), (-2, dict(ldc=68)), (-2, dict(a=A + 8)),
-    (-2, dict(b=A + 1)), (-2, dict(out=A + 2)), (-3, dict(K=131088, lda=131088, ldb=131088)), (-1, dict(M=1 << 31))])
+    (-2, dict(b=A + 1)), (-2, dict(out=A + 2)), (-3, dict(K=131072, lda=131072, ldb=131072)),
+    (-3, dict(M=1 << 27, N=1 << 20, ldc=1 << 20)), (-1, dict(M=1 << 31))])
 def test_product_refuses(code, kw):
     assert mm(**kw) == code and lib.spd_last_error_string()
 
@@ -49,7 +50,8 @@ def score(lp=A, lse=A, x=A, w=A, xs=None, ws=None, t=A, M=2, V=100, K=64, ldx=64
     (-1, dict(M=-1, room=0)), (-1, dict(V=0, room=0)), (-1, dict(K=0)), (-1, dict(dtype=2)), (-1, dict(ldx=56)), (-1, dict(ldw=56)),
     (-1, dict(xs=A)), (-1, dict(ws=A)), (-1, dict(dtype=3)), (-1, dict(dtype=3, xs=A)), (-2, dict(K=60)), (-2, dict(ldx=68)),
     (-2, dict(ldw=68)), (-2, dict(dtype=3, xs=A, ws=A, K=56, ldx=56, ldw=56)), (-2, dict(x=A + 2)), (-2, dict(w=A + 2)),
-    (-2, dict(work=A + 4)), (-4, dict(room=39))])
+    (-2, dict(work=A + 4)), (-4, dict(room=39)), (-3, dict(dtype=3, xs=A, ws=A, K=131072, ldx=131072, ldw=131072)),
+    (-3, dict(M=1 << 27, V=1 << 20))])
 def test_logprobs_refuse(code, kw):
     assert score(**kw) == code
 
