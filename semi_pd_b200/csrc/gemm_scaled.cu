@@ -795,7 +795,7 @@ static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
   for (int64_t t = fewest; t <= units && t <= fewest + 12 && t * w_tiles <= sms; ++t) {
     const int n = static_cast<int>(32 * ((units + t - 1) / t));
     const double part = n / 256.0;
-    for (int S = 1; S <= kMaxSplit && kblocks >= 4 * S; ++S)
+    for (int S = 1; S <= kMaxSplit && (S == 1 || kblocks >= 4 * S); ++S)
       for (int smem : {kGsMaxSmem, kHalfSmem}) {
         const bool half = smem == kHalfSmem;
         if (t * w_tiles > clusters_at_once(S, sms) * (half ? 2 : 1)) continue;
