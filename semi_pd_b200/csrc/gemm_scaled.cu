@@ -76,7 +76,8 @@ struct ScaledParams {
   int tok_tiles, n;    // tokens on N: token tiles, MMA columns of each
   int accs;            // accumulators that take k-blocks in turn (16-bit operands)
   int stages, slot;
-  int x_tiles, y_tiles, panel;  // tokens on M
+  int x_tiles, y_tiles, panel;             // tokens on M
+  uint64_t by_panel, by_width, by_last;    // reciprocals of a panel's tiles, of its width and the last one's (see quotient)
   int early;           // the weights are older than the kernel before this one: the first of them are fetched before it has ended
   unsigned* wait_expired;
 };
@@ -373,13 +374,21 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
 constexpr int kManyThreads = 256;  // warp 0: TMA, 1: MMA, 2: TMEM, 4-7: epilogue
 constexpr int kManyStages = 6;
 constexpr int kManyRing = kManyStages * 2 * kGsHalf;
-constexpr int kManySmem = kManyRing + 4 * kStageWarp + 2 * 256 * 8 + 256 + 1024;
+constexpr int kManyStage = 32 * 128;  // 64 columns of a warp's 32 rows
+constexpr int kManySmem = kManyRing + 4 * kManyStage + 2 * 256 * 8 + 256 + 1024;
 static_assert(kManySmem <= kGsMaxSmem, "shared memory of a CTA");
 
+// n / d of non-negative n, d < 2^31 for a reciprocal ceil(2^64 / d), exact (it is less than 1 too large, and n d < 2^64); 0 stands for
+// 2^64.  The compiler's division took an epilogue warp 150 clk, four of them a tile.
+__host__ inline uint64_t reciprocal(int d) { return ~uint64_t{0} / d + 1; }
+__device__ __forceinline__ int quotient(int n, uint64_t reciprocal) {
+  return reciprocal ? static_cast<int>(__umul64hi(static_cast<uint64_t>(n), reciprocal)) : n;
+}
+
 __device__ __forceinline__ void many_tile(const ScaledParams& p, int tile, int& xt, int& yt) {
-  const int per_panel = p.x_tiles * p.panel, pn = tile / per_panel, r = tile - pn * per_panel;
-  const int y0 = pn * p.panel, q = min(p.panel, p.y_tiles - y0);
-  xt = r / q;
+  const int pn = quotient(tile, p.by_panel), r = tile - pn * p.x_tiles * p.panel;
+  const int y0 = pn * p.panel, whole = y0 + p.panel <= p.y_tiles, q = whole ? p.panel : p.y_tiles - y0;
+  xt = quotient(r, whole ? p.by_width : p.by_last);
   yt = y0 + r - xt * q;
 }
 
@@ -431,11 +440,12 @@ __device__ __forceinline__ void many_multiply(const ScaledParams& p, uint8_t* sm
 
 template <typename T>
 __global__ void __launch_bounds__(kManyThreads, 1)
-many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const ScaledParams p) {
+many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ CUtensorMap tmO, const ScaledParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* sOut = smem + kManyRing;                                          // kStageWarp per epilogue warp
-  float2* cols = reinterpret_cast<float2*>(sOut + 4 * kStageWarp);           // [2][256] (scale, bias) of a tile's columns
+  uint8_t* sOut = smem + kManyRing;                                          // kManyStage per epilogue warp
+  float2* cols = reinterpret_cast<float2*>(sOut + 4 * kManyStage);           // [2][256] (scale, bias) of a tile's columns
   uint64_t* full = reinterpret_cast<uint64_t*>(cols + 512);                  // [stages]  (the leader's are the live ones)
   uint64_t* empty = full + kManyStages;                                      // [stages]
   uint64_t* tfull = empty + kManyStages;                                     // [2]
@@ -480,58 +490,85 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     if (rank == 0 && elect_one()) many_multiply<kInt8>(p, smem, full, empty, tfull, tempty, tmem, pair, npairs, p.kblocks, dead);
   } else if (warp >= 4) {
     const int q = warp & 3, et = threadIdx.x - 128;
-    uint8_t* stage = sOut + q * kStageWarp;
+    uint8_t* stage = sOut + q * kManyStage;
     const uint32_t lead_tempty0 = map_to_rank(smem_u32(tempty), 0);
+    // An epilogue shorter than this bounds products of few k-blocks (256 x 256 results: 9000 clk a tile at first, five k-blocks of
+    // MMAs take 2700).  So: a tile's scales and biases are fetched a tile ahead (1000 clk; the bias as it is in memory, to convert
+    // it would wait for it), the accumulator is given back by an arrival that does not wait for the stores (a releasing one: 1700),
+    // and the results leave by TMA, a warp's 64 columns while it works on the next.  8000 x 4096 x 256 34.5 -> 25.6 us,
+    // 8192 x 4096 x 1024 40.7 -> 31.2, 6061 x 14984 x 528 104 -> 83 (of which 20 for the stores; to fill such an output takes 49),
+    // 4099 x 6144 x 4096 68.3 -> 67.5.  Not taken: eight warps (25.1, 30.6, 84, 67.7); integers to fp32 by halves for every second
+    // value, for the conversions' rate of 16 a clk (28.5, 33.6, 86).
+    float sb[2], sa = 1.f;
+    T bias[2];
+    auto fetch = [&](int tile) {
+      int xt, yt;
+      many_tile(p, tile, xt, yt);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = yt * 256 + et + i * 128;
+        const bool in = c < p.n_cols;
+        sb[i] = in ? p.sb[c] : 0.f;
+        bias[i] = in && p.bias ? reinterpret_cast<const T*>(p.bias)[c] : from_f32<T>(0.f);
+      }
+      const int64_t m = static_cast<int64_t>(xt) * 256 + rank * 128 + q * 32 + lane;
+      sa = m < p.m_rows ? p.sa[m] : 1.f;
+    };
+    if (pair < num_tiles) fetch(pair);
     int n = 0;
     for (int tile = pair; tile < num_tiles; tile += npairs, ++n) {
       int xt, yt;
       many_tile(p, tile, xt, yt);
-      const int as = n & 1, n0 = yt * 256;
+      const int as = n & 1, n0 = yt * 256, columns = min(256, p.n_cols - n0);
       const int64_t m0 = static_cast<int64_t>(xt) * 256 + rank * 128 + q * 32;
       const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m_rows - m0));
       const float2* col = cols + as * 256;
+      const float row_scale = sa;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = n0 + et + i * 128;
-        float2 sb = make_float2(0.f, 0.f);
-        if (c < p.n_cols) {
-          sb.x = p.sb[c];
-          if (p.bias) sb.y = to_f32<T>(reinterpret_cast<const T*>(p.bias)[c]);
-        }
-        cols[as * 256 + et + i * 128] = sb;
-      }
+      for (int i = 0; i < 2; ++i) cols[as * 256 + et + i * 128] = make_float2(sb[i], to_f32<T>(bias[i]));
       // (one barrier a tile: a warp that is a tile ahead writes the other half, and cannot get two ahead)
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      const float sa = lane < rows ? p.sa[m0 + lane] : 1.f;
+      if (tile + npairs < num_tiles) fetch(tile + npairs);
       mbar_wait_bounded(&tfull[as], (n >> 1) & 1, dead);
       tc_fence_after_sync();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + as * 256;
-      auto values = [&](int c, float (&v)[32]) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(taddr + c, r);
-        tmem_ld_wait();
+      auto values = [&](int c, const uint32_t (&r)[32], uint4 (&out)[4]) {
+        float v[32];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           const float4 f = *reinterpret_cast<const float4*>(col + c + j);
-          v[j] = fmaf(gs_value<kInt8>(r[j]) * sa, f.x, f.y);
-          v[j + 1] = fmaf(gs_value<kInt8>(r[j + 1]) * sa, f.z, f.w);
+          v[j] = fmaf(gs_value<kInt8>(r[j]) * row_scale, f.x, f.y);
+          v[j + 1] = fmaf(gs_value<kInt8>(r[j + 1]) * row_scale, f.z, f.w);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          out[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                              pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
       };
 #pragma unroll 1
-      for (int c = 0; c < 256; c += 64) {
-        if (n0 + c >= p.n_cols) break;
-        float v[32];
-        values(c, v);
-        stage_put16<T>(stage, lane, 0, v);
-        values(c + 32, v);
-        stage_put16<T>(stage, lane, 1, v);
-        stage_out(stage, lane, reinterpret_cast<uint8_t*>(p.out) + (m0 * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
-                  min(64, p.n_cols - n0 - c) * 2);
+      for (int c = 0; c < columns; c += 64) {
+        uint32_t r0[32], r1[32];
+        uint4 o[2][4];
+        tmem_ld_32x32b_x32(taddr + c, r0);
+        tmem_ld_32x32b_x32(taddr + c + 32, r1);
+        tmem_ld_wait();
+        values(c, r0, o[0]);
+        values(c + 32, r1, o[1]);
+        if (c + 64 >= columns) tc_fence_before_sync();
+        if (lane == 0) bulk_wait_group_read0();  // the copy of the last 64 columns has read them
+        __syncwarp();
+        if (c + 64 >= columns && lane == 0) mbar_arrive_remote_relaxed(lead_tempty0 + as * 8);  // the accumulator is free
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) * 16)) = o[i >> 2][i & 3];
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && rows > 0) {
+          tma_store_2d(&tmO, stage, n0 + c, static_cast<int>(m0));
+          bulk_commit_group();
+        }
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote_release(lead_tempty0 + as * 8);
     }
+    if (lane == 0) bulk_wait_group0();
   }
 
   __syncwarp();  // the warps of the elected lanes come together before the barriers, which count whole warps
@@ -637,7 +674,8 @@ many_logprobs_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote_release(lead_tempty0 + as * 8);
+        // (a releasing arrival would wait for the last tile's stores: 4000 x 50272 x 768, 8 bits 176 us instead of 153)
+        if (lane == 0) mbar_arrive_remote_relaxed(lead_tempty0 + as * 8);
       }
       const int valid = p.n_cols - n0;
       if constexpr (kKind == kInt8) {
@@ -740,9 +778,9 @@ static int allow_smem(K kern, std::atomic<uint64_t>& done) {
   return 0;
 }
 
-template <typename K>
+template <typename K, typename... Args>
 static int launch_pairs(K kern, std::atomic<uint64_t>& done, int ctas, int cluster, int threads, int smem, cudaStream_t stream,
-                        const CUtensorMap& t0, const CUtensorMap& t1, const ScaledParams& p) {
+                        const Args&... args) {
   if (int rc = allow_smem(kern, done)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
@@ -758,7 +796,7 @@ static int launch_pairs(K kern, std::atomic<uint64_t>& done, int ctas, int clust
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  SPD_CUDA(cudaLaunchKernelEx(&cfg, kern, t0, t1, p));
+  SPD_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
   return 0;
 }
 
@@ -783,13 +821,14 @@ static int clusters_at_once(int S, int sms) {
 
 // Every form's time in us as fitted to 162 products (1 - 3000 tokens; 1024 x 8192, 4096 x 4096 to 4096 x 14336, 5000 x 1360, 5632 x 1024,
 // 6144 x 4096, 8192 x 8192, 16384 x 2048, 28672 x 4096), weights out of L2; the form chosen took 1.02 times the fastest one's time in the
-// mean, 1.19 at most.  Tokens on N, all tiles at once: a k-block of 128 bytes takes a pair 0.18 to 0.26 (half the ring: 1.5 times
+// mean, 1.19 at most (120 others, 100 - 3000 tokens, K from 144 on: 1.02, 1.32 at 400 x 4096 x 256).  Tokens on N, all tiles at once: a k-block of 128 bytes takes a pair 0.18 to 0.26 (half the ring: 1.5 times
 // that), two pairs on an SM 0.13 to 0.30 each, the weights 7.7 GB/ms; then the epilogue, longer where two CTAs on an SM are in it
-// at once, and the pairs' sums.  Tokens on M: 0.29 a k-block and 1.9 a tile.
+// at once, and the pairs' sums.  Tokens on M: 0.29 a k-block and 1 a tile, 2.8 at least.
 static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
   const int64_t w_tiles = (N + 255) / 256, waves = ((M + 255) / 256 * w_tiles + sms / 2 - 1) / (sms / 2);
   ScaledPlan plan{0, 1, 0};
-  double best = 6.4 + static_cast<double>(waves) * (0.288 * kblocks + 1.9);
+  const double tile = 0.288 * kblocks + 1;
+  double best = 6.4 + static_cast<double>(waves) * (tile > 2.8 ? tile : 2.8);
   const double hbm = 128e-6 / 7.7 * static_cast<double>(N) * kblocks;
   const int64_t units = (M + 31) / 32, fewest = (units + 7) / 8;
   for (int64_t t = fewest; t <= units && t <= fewest + 12 && t * w_tiles <= sms; ++t) {
@@ -889,11 +928,17 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
   // weight tiles of a rasterisation panel: as many as stay in L2 beside what else passes (gemm.cu)
   const int64_t q = (40ll << 20) / (256 * kbytes);
   p.panel = static_cast<int>(q < 1 ? 1 : q < p.y_tiles ? q : p.y_tiles);
+  p.by_panel = reciprocal(p.x_tiles * p.panel);
+  p.by_width = reciprocal(p.panel);
+  p.by_last = p.y_tiles % p.panel ? reciprocal(p.y_tiles % p.panel) : p.by_width;
   const int64_t tiles = static_cast<int64_t>(p.x_tiles) * p.y_tiles;
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
   static std::atomic<uint64_t> done{0};
-  if constexpr (kEnd == kScaled) return launch_pairs(many_tokens_kernel<T>, done, 2 * pairs, 2, kManyThreads, kManySmem, stream, ta, tw, p);
-  else return launch_pairs(many_logprobs_kernel<kKind>, done, 2 * pairs, 2, kLogThreads, kLogSmem, stream, ta, tw, p);
+  if constexpr (kEnd == kScaled) {
+    CUtensorMap to;
+    if (int rc = make_tmap_2d_sw128(&to, p.out, M, N, p.ldc, 32, 64)) return rc;
+    return launch_pairs(many_tokens_kernel<T>, done, 2 * pairs, 2, kManyThreads, kManySmem, stream, ta, tw, to, p);
+  } else return launch_pairs(many_logprobs_kernel<kKind>, done, 2 * pairs, 2, kLogThreads, kLogSmem, stream, ta, tw, p);
 }
 
 static int budget(int sm_budget) {
