@@ -20,7 +20,6 @@
 #include "common.cuh"
 #include "pair.cuh"
 #include "ptx.cuh"
-#include "row_stage.cuh"
 #include "tmap.cuh"
 
 namespace spd {

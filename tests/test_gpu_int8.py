@@ -353,3 +353,47 @@ def test_behind_a_long_kernel():
     torch.cuda.synchronize()
     ops.check_waits()
     assert torch.equal(out, want) and out2.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1700, 8200, 528), (5000, 4104, 16), (600, 24008, 4096), (4100, 10248, 1040)])
+def test_product_of_many_tiles(m, n, k, dtype):
+    # (more tiles than pairs of CTAs, ragged at both edges; 24008 x 4096: three panels of weights, the last one narrower)
+    a, b = int8_rows(m, k, 21), int8_rows(n, k, 22)
+    sa = torch.rand(m, 1, generator=gen(23), device=DEV) * 0.02 / k ** 0.5
+    sb = torch.rand(n, 1, generator=gen(24), device=DEV) + 0.1
+    bias = torch.randn(n, generator=gen(25), device=DEV).to(dtype)
+    for b_ in (bias, None):
+        out = ops.int8_scaled_mm(a, b.t(), sa, sb, dtype, b_)
+        want, tol = product(a, b, sa, sb, b_, dtype)
+        assert ((out.double() - want).abs() <= tol).all()
+        for _ in range(3):
+            assert torch.equal(out, ops.int8_scaled_mm(a, b.t(), sa, sb, dtype, b_))
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 264, 144), (150, 1000, 528), (700, 1000, 144), (2100, 4104, 528)])
+def test_results_inside_a_wider_buffer(m, n, k):
+    # (a caller of the library: what is beside and behind the results stays as it was)
+    from semi_pd_b200 import _lib
+    a, b = int8_rows(m, k, 31), int8_rows(n, k, 32)
+    sa = torch.rand(m, 1, generator=gen(33), device=DEV) * 0.02 / k ** 0.5
+    sb = torch.rand(n, 1, generator=gen(34), device=DEV) + 0.1
+    buf = torch.full((m + 3, n + 24), 77.0, device=DEV, dtype=torch.bfloat16)
+    _lib.check(_lib.lib.spd_int8_scaled_mm(buf[1:, 8:].data_ptr(), a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), None, m, n, k, k, k,
+                                           n + 24, 0, 0, 0, torch.cuda.current_stream().cuda_stream), "spd_int8_scaled_mm")
+    assert torch.equal(buf[1:m + 1, 8:n + 8], ops.int8_scaled_mm(a, b.t(), sa, sb, torch.bfloat16))
+    buf[1:m + 1, 8:n + 8] = 77.0
+    assert (buf == 77.0).all()
+
+
+@pytest.mark.parametrize("k", [48, 528])
+def test_integer_results_are_exact(k):
+    # (scales of 1 and sums below 2^11: every result is a number of both types; each of the forms)
+    for m, n in ((3, 512), (180, 2056), (900, 8200), (2500, 4104)):
+        g = gen(m)
+        a = torch.randint(-1, 2, (m, k), generator=g, device=DEV, dtype=torch.int8)
+        b = torch.randint(-1, 2, (n, k), generator=g, device=DEV, dtype=torch.int8)
+        a[:, k // 2:] = 0
+        b[:, 256:] = 0  # at most 256 products of 1: exact in bf16
+        one_a, one_b = torch.ones(m, 1, device=DEV), torch.ones(n, 1, device=DEV)
+        assert torch.equal(ops.int8_scaled_mm(a, b.t(), one_a, one_b, torch.bfloat16).double(), a.double() @ b.double().t())
