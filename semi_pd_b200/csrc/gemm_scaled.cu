@@ -822,31 +822,37 @@ static int clusters_at_once(int S, int sms) {
   return share < most ? share : most;
 }
 
-// Every form's time in us as fitted to 162 products (1 - 3000 tokens; 1024 x 8192, 4096 x 4096 to 4096 x 14336, 5000 x 1360, 5632 x 1024,
-// 6144 x 4096, 8192 x 8192, 16384 x 2048, 28672 x 4096), weights out of L2; the form chosen took 1.02 times the fastest one's time in the
-// mean, 1.19 at most (120 others, 100 - 3000 tokens, K from 144 on: 1.02, 1.32 at 400 x 4096 x 256).  Tokens on N, all tiles at once: a k-block of 128 bytes takes a pair 0.18 to 0.26 (half the ring: 1.5 times
-// that), two pairs on an SM 0.13 to 0.30 each, the weights 7.7 GB/ms; then the epilogue, longer where two CTAs on an SM are in it
-// at once, and the pairs' sums.  Tokens on M: 0.29 a k-block and 1 a tile, 2.8 at least.
+// Every form's time in us as fitted to 264 products (1 - 2000 tokens; 22 weights of 1024 x 2048 to 28672 x 4096, K from 144 to 14336),
+// weights out of memory, in a row of such calls; the form chosen took 1.01 times the fastest one's time in the mean, 1.13 at most.
+// Tokens on N, all tiles at once: a k-block of 128 bytes takes a pair 0.15 to 0.24 (half the ring: 1.65 times that), two pairs on an
+// SM 0.09 to 0.29 each; the weights 8.6 GB/ms, and two thirds of that again for every further tile of tokens that reads them.  Where the
+// next call's CTAs fit beside this one's, what their rings hold is on its way before this one ends: 0.4 of that share.  Then the
+// epilogue, the pairs' sums, and what CTAs and tiles cost each other.  Tokens on M: 0.29 a k-block and 1 a tile, 2.8 at least.
 static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
   const int64_t w_tiles = (N + 255) / 256, waves = ((M + 255) / 256 * w_tiles + sms / 2 - 1) / (sms / 2);
   ScaledPlan plan{0, 1, 0};
   const double tile = 0.288 * kblocks + 1;
   double best = 6.4 + static_cast<double>(waves) * (tile > 2.8 ? tile : 2.8);
-  const double hbm = 128e-6 / 7.7 * static_cast<double>(N) * kblocks;
+  const double pass = 128e-6 / 7.7 * static_cast<double>(N) * kblocks;
   const int64_t units = (M + 31) / 32, fewest = (units + 7) / 8;
   for (int64_t t = fewest; t <= units && t <= fewest + 12 && t * w_tiles <= sms; ++t) {
     const int n = static_cast<int>(32 * ((units + t - 1) / t));
-    const double part = n / 256.0;
+    const double part = n / 256.0, weights = pass * (0.9 + 0.67 * static_cast<double>(t - 1));
     for (int S = 1; S <= kMaxSplit && (S == 1 || kblocks >= 4 * S); ++S)
       for (int smem : {kGsMaxSmem, kHalfSmem}) {
         const bool half = smem == kHalfSmem;
+        const int slots = few_slots(n, smem);
+        const int64_t ctas = t * w_tiles * 2 * S;
         if (t * w_tiles > clusters_at_once(S, sms) * (half ? 2 : 1)) continue;
-        if (few_slots(n, smem) * (kGsHalf + n / 2 * kGsBlock) < n * (S > 1 ? 512 : 256)) continue;
-        const int both = half && t * w_tiles * 2 * S > sms ? 2 : 1;
-        const double kb = static_cast<double>(kblocks) / S, alone = kb * (0.178 + 0.083 * part) * (half ? 1.5 : 1),
-                     shared = kb * (0.132 + 0.166 * part) * both;
+        if (slots * (kGsHalf + n / 2 * kGsBlock) < n * (S > 1 ? 512 : 256)) continue;
+        const bool two = half && ctas > sms;
+        const double kb = static_cast<double>(kblocks) / S, alone = kb * (0.15 + 0.085 * part) * (half ? 1.65 : 1),
+                     shared = kb * (0.09 + 0.2 * part) * (two ? 2 : 1);
         double us = alone > shared ? alone : shared;
-        us = 2.2 + (us > hbm ? us : hbm) + 3.46 * part * (S > 1 || both == 1 ? 1 : 1.8) + (S > 1 ? 1.5 + 2.1 * part : 0);
+        if (us < weights) us = weights;
+        if (ctas <= (half ? sms : sms / 2)) us *= 1 - 0.4 * (slots < kb ? slots / kb : 1);
+        us += 2.7 + 2.7 * part * (two && S == 1 ? 0.9 : 1) + (S > 1 ? 0.3 + 3.7 * part : 0) + 0.25 * static_cast<double>(ctas) / sms +
+              (t > 1 ? 0.3 : 0);
         if (us < best) {
           best = us;
           plan = ScaledPlan{static_cast<int>(t), S, smem};
