@@ -101,10 +101,10 @@ constexpr int kFewStages = 12;    // at most
 constexpr int kFewFixed = 1024 + 256 + 2048;  // alignment, barriers, a scale and a target for each token
 constexpr int kMaxSplit = 4;
 
-// TMEM columns of a CTA, and the least shared memory that it takes: its share of the SM's, so that whatever CTAs are on an SM
-// together never wait for one another's columns.
+// TMEM columns of a CTA, 256 at most: CTAs with tokens on N take at least half of the SM's shared memory (kHalfSmem), CTAs with tokens
+// on M, which take all columns, all of it.  So whatever of these are on an SM together never wait for one another's columns: a CTA
+// that did, while its peer holds another SM's, could close a circle of waits.
 __host__ __device__ constexpr int few_columns(int cols) { return cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256; }
-constexpr int few_least_smem(int cols) { return few_columns(cols) * (233472 / 512) - 1024; }
 
 __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
   int4 v;
@@ -379,7 +379,7 @@ constexpr int kManyStages = 6;
 constexpr int kManyRing = kManyStages * 2 * kGsHalf;
 constexpr int kManyStage = 32 * 128;  // 64 columns of a warp's 32 rows
 constexpr int kManySmem = kManyRing + 4 * kManyStage + 2 * 256 * 8 + 256 + 1024;
-static_assert(kManySmem <= kGsMaxSmem, "shared memory of a CTA");
+static_assert(kManySmem <= kGsMaxSmem, "shared memory of a CTA");  // (a launch asks for kGsMaxSmem: see few_columns)
 
 // n / d of non-negative n, d < 2^31 for a reciprocal ceil(2^64 / d), exact (it is less than 1 too large, and n d < 2^64); 0 stands for
 // 2^64.  The compiler's division took an epilogue warp 150 clk, four of them a tile.
@@ -593,7 +593,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 // 8192 clk, taking 128 columns out 400).  8-bit sums are exact and come out once.
 constexpr int kLogThreads = 320;  // warp 0: TMA, 1: MMA and TMEM, 2-9: epilogue
 constexpr int kLogChunk = 16;     // k-blocks
-constexpr int kLogSmem = kManyRing + 2 * 256 * 4 + 256 + 1024;
+static_assert(kManyRing + 2 * 256 * 4 + 256 + 1024 <= kGsMaxSmem, "shared memory of a CTA");
 
 template <int kKind>
 __global__ void __launch_bounds__(kLogThreads, 1)
@@ -927,7 +927,7 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
     if (kEnd == kScaled && plan.split == 1)
       if (int rc = make_tmap_2d_sw128(&to, p.out, M, N, p.ldc, 32, 64)) return rc;
     p.accs = kKind == kInt8 ? 1 : few_accumulators(p.n, p.kblocks);
-    const int need = p.stages * p.slot + kFewFixed, least = few_least_smem(p.n * p.accs), smem = need > least ? need : least;
+    const int need = p.stages * p.slot + kFewFixed, smem = need > kHalfSmem ? need : kHalfSmem;
     static std::atomic<uint64_t> done{0};
     const int ctas = static_cast<int>((N + 255) / 256) * plan.tok_tiles * 2 * plan.split;
     return launch_pairs(few_tokens_kernel<kKind, kEnd, T>, done, ctas, 2 * plan.split, kFewThreads, smem, stream,
@@ -949,8 +949,8 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
   if constexpr (kEnd == kScaled) {
     CUtensorMap to;
     if (int rc = make_tmap_2d_sw128(&to, p.out, M, N, p.ldc, 32, 64)) return rc;
-    return launch_pairs(many_tokens_kernel<T>, done, 2 * pairs, 2, kManyThreads, kManySmem, stream, ta, tw, to, p);
-  } else return launch_pairs(many_logprobs_kernel<kKind>, done, 2 * pairs, 2, kLogThreads, kLogSmem, stream, ta, tw, p);
+    return launch_pairs(many_tokens_kernel<T>, done, 2 * pairs, 2, kManyThreads, kGsMaxSmem, stream, ta, tw, to, p);
+  } else return launch_pairs(many_logprobs_kernel<kKind>, done, 2 * pairs, 2, kLogThreads, kGsMaxSmem, stream, ta, tw, p);
 }
 
 static int budget(int sm_budget) {

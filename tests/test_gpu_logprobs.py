@@ -169,3 +169,26 @@ def test_two_streams_at_once():
     for i, outs in enumerate(got):
         for (lp, lse), s in zip(outs, sets[i % 2:] + sets[:i % 2]):
             assert torch.equal(lp, s[5][0]) and torch.equal(lse, s[5][1])
+
+
+def test_beside_products_of_few_values():
+    # (CTAs with one k-block in their ring and 32 columns of TMEM, on the SMs of CTAs that take all columns)
+    g = gen(40)
+    a = torch.randint(-127, 128, (8, 128), generator=g, device=DEV, dtype=torch.int8)
+    b = torch.randint(-127, 128, (8192, 128), generator=g, device=DEV, dtype=torch.int8)
+    sa, sb = torch.rand(8, 1, generator=g, device=DEV), torch.rand(8192, 1, generator=g, device=DEV)
+    x, w, _, _ = operands(600, 32000, 2048, torch.bfloat16)
+    targets = torch.randint(0, 32000, (600,), generator=g, device=DEV)
+    want_product = ops.int8_scaled_mm(a, b.t(), sa, sb, torch.bfloat16)
+    want = ops.linear_logprobs(x, w, targets)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    products, scores = [], []
+    for _ in range(20):
+        with torch.cuda.stream(one):
+            scores.append(ops.linear_logprobs(x, w, targets))
+        with torch.cuda.stream(two):
+            products += [ops.int8_scaled_mm(a, b.t(), sa, sb, torch.bfloat16) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, want_product) for p in products)
+    assert all(torch.equal(s[0], want[0]) and torch.equal(s[1], want[1]) for s in scores)
