@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) quant_int8_rows_kernel(const QuantPa
 
 // CTAs of a kernel that run on an SM at once, asked once for every device (kKern: kernels of one type keep apart)
 template <auto kKern>
-static int resident_ctas( int threads, int smem, int* out) {
+static int resident_ctas(int threads, int smem, int* out) {
   static std::atomic<int> known[64];
   int dev = 0;
   SPD_CUDA(cudaGetDevice(&dev));
