@@ -75,6 +75,7 @@ struct ScaledParams {
   int tok_tiles, n;    // tokens on N: token tiles, MMA columns of each
   int accs;            // accumulators that take k-blocks in turn (16-bit operands)
   int stages, slot;
+  int to_l2;           // k-blocks of weights behind the ring's that a CTA asks into L2
   int x_tiles, y_tiles, panel;             // tokens on M
   uint64_t by_panel, by_width, by_last;    // reciprocals of a panel's tiles, of its width and the last one's (see quotient)
   int early;           // the weights are older than the kernel before this one: the first of them are fetched before it has ended
@@ -188,6 +189,7 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         if (rank == 0) mbar_expect_tx(&full[i], bytes);
         load_w(i, kb0 + i);
       }
+      for (int kb = kb0 + ahead; kb < min(kb1, kb0 + ahead + p.to_l2); ++kb) tma_prefetch_2d(&tmW, kb * (kGsBlock / 2), row_base);
       if (p.early) griddep_wait();
       int stage = 0, phase = 0;
       const int a_row = tok_base + static_cast<int>(rank) * half;
@@ -809,6 +811,14 @@ struct ScaledPlan {
 };
 constexpr int kHalfSmem = 113 * 1024;  // of a CTA that shares its SM with another
 
+// Weights that a call with one tile of tokens asks into L2 behind what its rings hold, while it waits for the tokens and for the kernel
+// before it: memory does not pause there.  us, without / 8, 16, 24 MB: 1 x 28672 x 4096 21.4 / 21.1, 20.7, 20.4; 1 x 4096 x 4096 5.8 / 5.5,
+// 5.4, 5.5; 16 x 5120 x 5120 7.7 / 7.5, 7.3, 7.2; 40 x 4096 x 14336 14.4 / 14.3, 14.1, 14.3 (64 MB: 15.2); behind a kernel that leaves nothing
+// to overlap 64 x 28672 x 4096 23.2 / 22.6, 21.9, 21.8, 1 x 8192 x 3584 9.8 / 9.9, 10.2, 10.2.  With several tiles of tokens it costs time:
+// 256 x 6144 x 4096 10.8 / 11.5; so it does in a part of the SMs, which memory does not bound: a decode step of Llama-3-8B, 32 requests
+// on 72 SMs 4.22 / 4.33 ms (on all of them 2.95 / 2.95).  Single lines asked for by the epilogue's warps: 21.1 instead of 20.7.
+constexpr int kAheadInL2 = 16 << 20;
+
 // Shared memory for the ring of a CTA with tokens on N: `slots` of what it takes for n tokens
 static int few_slots(int n, int smem) {
   const int slots = (smem - kFewFixed) / (kGsHalf + n / 2 * kGsBlock);
@@ -930,6 +940,7 @@ static int scaled_product(const void* a, const void* w, int64_t M, int64_t N, in
     const int need = p.stages * p.slot + kFewFixed, smem = need > kHalfSmem ? need : kHalfSmem;
     static std::atomic<uint64_t> done{0};
     const int ctas = static_cast<int>((N + 255) / 256) * plan.tok_tiles * 2 * plan.split;
+    p.to_l2 = kEnd == kScaled && plan.tok_tiles == 1 && sms >= device_sm_count_cached() ? kAheadInL2 / kGsHalf / ctas : 0;
     return launch_pairs(few_tokens_kernel<kKind, kEnd, T>, done, ctas, 2 * plan.split, kFewThreads, smem, stream,
                         tw, ta, to, p);
   }

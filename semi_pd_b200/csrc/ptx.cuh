@@ -154,6 +154,10 @@ __device__ __forceinline__ void cp_async_wait() {
 // ------------------------------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor) — 2D tiled load, completion on an mbarrier
 // ------------------------------------------------------------------------------------------------
+// a box of a tensor into L2
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int32_t c_inner, int32_t c_outer) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(c_inner), "r"(c_outer) : "memory");
+}
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(tmap) : "memory");
