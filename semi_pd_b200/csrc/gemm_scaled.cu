@@ -837,15 +837,19 @@ static int clusters_at_once(int S, int sms) {
 // Tokens on N, all tiles at once: a k-block of 128 bytes takes a pair 0.15 to 0.24 (half the ring: 1.65 times that), two pairs on an
 // SM 0.09 to 0.29 each; the weights 8.6 GB/ms, and two thirds of that again for every further tile of tokens that reads them.  Where the
 // next call's CTAs fit beside this one's, what their rings hold is on its way before this one ends: 0.4 of that share.  Then the
-// epilogue, the pairs' sums, and what CTAs and tiles cost each other.  Tokens on M: 0.29 a k-block and 1 a tile, 2.8 at least.
+// epilogue, the pairs' sums, and what CTAs and tiles cost each other.  Tokens on M: 0.29 a k-block and 1 a tile, 2.8 at least, and the
+// weights of a single row of tiles at 5.3 GB/ms.
+// More tiles than run at once, one of tokens: 57344 x 8192 of 1 token 74 us (tokens on M 111), of 160 87 (104), 128256 x 4096 of 1 80 (131),
+// of 100 94 (97), of 256 125 (105).
 static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
   const int64_t w_tiles = (N + 255) / 256, waves = ((M + 255) / 256 * w_tiles + sms / 2 - 1) / (sms / 2);
   ScaledPlan plan{0, 1, 0};
   const double tile = 0.288 * kblocks + 1;
   double best = 6.4 + static_cast<double>(waves) * (tile > 2.8 ? tile : 2.8);
   const double pass = 128e-6 / 7.7 * static_cast<double>(N) * kblocks;
+  if (M <= 256 && best < 6.4 + 1.45 * pass) best = 6.4 + 1.45 * pass;
   const int64_t units = (M + 31) / 32, fewest = (units + 7) / 8;
-  for (int64_t t = fewest; t <= units && t <= fewest + 12 && t * w_tiles <= sms; ++t) {
+  for (int64_t t = fewest; t <= units && t <= fewest + 12 && (t == 1 || t * w_tiles <= sms); ++t) {
     const int n = static_cast<int>(32 * ((units + t - 1) / t));
     const double part = n / 256.0, weights = pass * (0.9 + 0.67 * static_cast<double>(t - 1));
     for (int S = 1; S <= kMaxSplit && (S == 1 || kblocks >= 4 * S); ++S)
@@ -853,7 +857,9 @@ static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
         const bool half = smem == kHalfSmem;
         const int slots = few_slots(n, smem);
         const int64_t ctas = t * w_tiles * 2 * S;
-        if (t * w_tiles > clusters_at_once(S, sms) * (half ? 2 : 1)) continue;
+        const int64_t at_once = clusters_at_once(S, sms) * (half ? 2 : 1);
+        const bool several = t * w_tiles > at_once;
+        if (several && (t > 1 || S > 1 || !half)) continue;
         if (slots * (kGsHalf + n / 2 * kGsBlock) < n * (S > 1 ? 512 : 256)) continue;
         const bool two = half && ctas > sms;
         const double kb = static_cast<double>(kblocks) / S, alone = kb * (0.15 + 0.085 * part) * (half ? 1.65 : 1),
@@ -863,6 +869,10 @@ static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
         if (ctas <= (half ? sms : sms / 2)) us *= 1 - 0.4 * (slots < kb ? slots / kb : 1);
         us += 2.7 + 2.7 * part * (two && S == 1 ? 0.9 : 1) + (S > 1 ? 0.3 + 3.7 * part : 0) + 0.25 * static_cast<double>(ctas) / sms +
               (t > 1 ? 0.3 : 0);
+        if (several) {
+          us = static_cast<double>((w_tiles + at_once - 1) / at_once) * (1.2 * shared + 2.7 + 5.3 * part);
+          if (us < 1.22 * pass + 4) us = 1.22 * pass + 4;
+        }
         if (us < best) {
           best = us;
           plan = ScaledPlan{static_cast<int>(t), S, smem};

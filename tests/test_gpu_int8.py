@@ -397,3 +397,20 @@ def test_integer_results_are_exact(k):
         b[:, 256:] = 0  # at most 256 products of 1: exact in bf16
         one_a, one_b = torch.ones(m, 1, device=DEV), torch.ones(n, 1, device=DEV)
         assert torch.equal(ops.int8_scaled_mm(a, b.t(), one_a, one_b, torch.bfloat16).double(), a.double() @ b.double().t())
+
+
+@pytest.mark.parametrize("sms", [0, 8, 72])
+@pytest.mark.parametrize("m,n,k", [(1, 40008, 528), (3, 60000, 144), (100, 80024, 272), (250, 39000, 1040)])
+def test_more_weight_tiles_than_run_at_once(m, n, k, sms):
+    a, b = int8_rows(m, k, 41), int8_rows(n, k, 42)
+    sa = torch.rand(m, 1, generator=gen(43), device=DEV) * 0.02 / k ** 0.5
+    sb = torch.rand(n, 1, generator=gen(44), device=DEV) + 0.1
+    bias = torch.randn(n, generator=gen(45), device=DEV).bfloat16()
+    ops.set_sm_budget(sms)
+    try:
+        outs = [ops.int8_scaled_mm(a, b.t(), sa, sb, torch.bfloat16, bias, older_weight=older) for older in (False, True, True)]
+    finally:
+        ops.set_sm_budget(0)
+    want, tol = product(a, b, sa, sb, bias, torch.bfloat16)
+    for out in outs:
+        assert ((out.double() - want).abs() <= tol).all()
