@@ -189,7 +189,8 @@ few_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         if (rank == 0) mbar_expect_tx(&full[i], bytes);
         load_w(i, kb0 + i);
       }
-      for (int kb = kb0 + ahead; kb < min(kb1, kb0 + ahead + p.to_l2); ++kb) tma_prefetch_2d(&tmW, kb * (kGsBlock / 2), row_base);
+      const int asked = row_base < p.n_cols ? min(kb1, kb0 + ahead + p.to_l2) : 0;
+      for (int kb = kb0 + ahead; kb < asked; ++kb) tma_prefetch_2d(&tmW, kb * (kGsBlock / 2), row_base);
       if (p.early) griddep_wait();
       int stage = 0, phase = 0;
       const int a_row = tok_base + static_cast<int>(rank) * half;

@@ -414,3 +414,15 @@ def test_more_weight_tiles_than_run_at_once(m, n, k, sms):
     want, tol = product(a, b, sa, sb, bias, torch.bfloat16)
     for out in outs:
         assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 8, 60000), (1, 136, 131056), (40, 264, 30000), (200, 520, 40016)])
+def test_long_rows_of_few_columns(m, n, k):
+    # (far more k-blocks than the rings hold, and CTAs whose weight rows are all behind the last)
+    a, b = int8_rows(m, k, 51), int8_rows(n, k, 52)
+    sa = torch.rand(m, 1, generator=gen(53), device=DEV) * 0.02 / k ** 0.5
+    sb = torch.rand(n, 1, generator=gen(54), device=DEV) + 0.1
+    for older in (True, False):
+        out = ops.int8_scaled_mm(a, b.t(), sa, sb, torch.bfloat16, older_weight=older)
+        want, tol = product(a, b, sa, sb, None, torch.bfloat16)
+        assert ((out.double() - want).abs() <= tol).all()
