@@ -11,7 +11,8 @@
 // Rounding.  For 16-bit y the result is the exact one, halves away from zero: with X and A the integer significands (at most 11
 // bits) of |y| and of the largest, y / s = 127 X 2^-e / A lies on a half or at least 1 / (2 A 2^e) beside it, relative to itself
 // at least 1 / (254 X) > 2^-19; the factor 1 + 2^-20 on 127 / max is above the three roundings of 2^-24 in the way and below that
-// distance, so it moves halves up and nothing else over a border.
+// distance, so it moves halves up and nothing else over a border.  32-bit y has no such distance, and no factor (with it SiLU * mul
+// of 7800 rows of 14336 had 194 integers that 64 bits give otherwise, without 23; plain fp32 has 22).
 //
 // A NaN or an infinity in a row makes its scale NaN or infinite, and with it everything that the row is multiplied into: the
 // maximum is taken over the bits of |y|, which order NaN above infinity above numbers.
@@ -54,7 +55,9 @@ __device__ __forceinline__ float max_abs(float top, float y) {
   return r;
 }
 
-// g / (1 + e^-g): the exponential to 2^-22, the quotient to an ulp more
+// g / (1 + e^-g).  The exponential is good to (2 + 1.2 |g|) 2^-23, for its argument is rounded at g log2 e; 1 + e^-g has that error only
+// for negative g, and there g e^g falls faster than the error grows: next to the row's maximum it is below 2^-22.  With expf: as many
+// integers that 64 bits give otherwise, and 8192 x 14336 in 109 us instead of 95.
 __device__ __forceinline__ float silu_flushed(float g) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(-1.4426950408889634f * g)));
@@ -110,7 +113,7 @@ __device__ __forceinline__ float quant_factor(uint32_t top, float ss, const Quan
   float most = __uint_as_float(top) * c;
   most = most < 1e-10f ? 1e-10f : most;  // (NaN stays)
   scale = __fdiv_rn(most, 127.f);
-  return __fdiv_rn(127.f, most) * (kHasNorm ? c : 1.f + 0x1p-20f);
+  return __fdiv_rn(127.f, most) * (kHasNorm ? c : kForm == kQuantPlain ? 1.f + 0x1p-20f : 1.f);
 }
 
 __device__ __forceinline__ uint2 quant_pack(const float (&y)[8], float k) {
