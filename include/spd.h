@@ -910,6 +910,11 @@ int spd_quant_int8(int8_t* q, float* scales, const void* x, void* residual, cons
 int spd_int8_scaled_mm(void* out, const int8_t* a, const int8_t* b, const float* scales_a, const float* scales_b, const void* bias,
                        int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int dtype, int older_w,
                        int sm_budget, spd_stream_t stream);
+/* Token tiles of such a product with tokens on N, 0: tiles of 256 x 256.  *split: pairs of CTAs over which a cluster cuts K;
+ * *ctas_per_sm: 2 where they take half of an SM's shared memory.  clusters: how many clusters of 1, 2, ... 8 CTAs run at once on
+ * sm_budget SMs, one CTA an SM, -1: not known (the whole device's share), or NULL: as the driver says of the device.  A call on a partition asks
+ * for its own stream. */
+int spd_int8_scaled_mm_tiles(int64_t M, int64_t N, int64_t K, int sm_budget, const int* clusters, int* split, int* ctas_per_sm);
 /* The log-softmax of x w^T over the V rows of w at one of them for every row of x, without the products reaching memory:
  * lse[m] = log sum_v exp l[m][v], logprobs[m] = l[m][targets[m]] - lse[m]; a target outside [0, V) asks for nothing and gets 0.
  * (S/layers/logits_processor.py: input_token_logprobs.)  l is the fp32 accumulator; SPD_I8: times scales_x[m] scales_w[v].

@@ -107,6 +107,7 @@ SIGNATURES = {
     "spd_kv_compact": (_i, [_p, _i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i, _p]),
     "spd_quant_int8": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _i, _i, _i, _p]),
     "spd_int8_scaled_mm": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _p]),
+    "spd_int8_scaled_mm_tiles": (_i, [_i64, _i64, _i64, _i, _p, _p, _p]),
     "spd_linear_logprobs_workspace_bytes": (_i64, [_i64, _i64]),
     "spd_linear_logprobs": (_i, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _i, _p, _i64, _i, _p]),
     "spd_comm_create": (_i, [_i, _i, _i64, C.POINTER(_p), _p]),

@@ -279,15 +279,15 @@ int gemm_pair_split(void* C, const void* A, const void* W, int64_t M, int64_t N,
   SPD_DISPATCH_DTYPE(dtype, { return launch_split<T, false>(tw, ta, p, w_tiles * tok_tiles, split, stream); });
 }
 
-// Clusters of 2 `split` CTAs that the choice below reckons with on `sms` SMs when the driver says that `found` run at once
-// (-1: there is no device to ask).  0 is an answer: no cluster of this size fits.
-static int split_room(int split, int found, int sms) {
-  static const int b200[kPtMaxSplit + 1] = {0, 74, 33, 22, 15};
+// Clusters of `ctas` CTAs, one CTA an SM, to reckon with on `sms` SMs when the driver says that `found` run at once (-1: there is no
+// device to ask).  0 is an answer: no cluster of this size fits.
+int cluster_room(int ctas, int found, int sms) {
+  static const int b200[2 * kPtMaxSplit + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
   if (found < 0) {
     const int whole = device_sm_count_cached();
-    found = sms >= whole ? b200[split] : b200[split] * sms / whole;
+    found = sms >= whole ? b200[ctas] : b200[ctas] * sms / whole;
   }
-  const int most = sms / (2 * split);
+  const int most = sms / ctas;
   return found < most ? found : most;
 }
 
@@ -295,19 +295,19 @@ static int split_room(int split, int found, int sms) {
 // of SMs does not tell (whole B200: 74, 33, 22, 15 clusters of 2, 4, 6, 8 CTAs; 76 SMs beside 72: 38, 15, 9, 6, the 72: 36, 18, 9, 9;
 // 108 beside 40: 54, 23, 13, 10).  Reckoned by number, 4096 x 14336 got 16 clusters of four on the 76 SMs, two waves: 23 us of
 // one token became 48.  A query takes 1 us of host time, so the whole device is asked once.
-static int split_clusters(int split, int sms, cudaStream_t stream) {
-  static std::atomic<int> cached[kPtMaxSplit + 1];  // the whole device's answer + 2
+int clusters_found(int ctas, int sms, cudaStream_t stream) {
+  static std::atomic<int> cached[2 * kPtMaxSplit + 1];  // the whole device's answer + 2
   const bool whole = sms >= device_sm_count_cached();
-  int n = whole ? cached[split].load(std::memory_order_relaxed) - 2 : -2;
+  int n = whole ? cached[ctas].load(std::memory_order_relaxed) - 2 : -2;
   if (n > -2) return n;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(2 * split);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPtThreads);
   cfg.dynamicSmemBytes = kPtMaxSmem;
   cfg.stream = whole ? nullptr : stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2 * split;
+  attr[0].val.clusterDim.x = ctas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -318,12 +318,12 @@ static int split_clusters(int split, int sms, cudaStream_t stream) {
     cudaGetLastError();
     n = -1;  // no device to ask (the choice of kernel can be asked for without one)
   }
-  if (whole) cached[split].store(n + 2, std::memory_order_relaxed);
+  if (whole) cached[ctas].store(n + 2, std::memory_order_relaxed);
   return n;
 }
 
 int gemm_cluster_ctas(int64_t M, int64_t N, int64_t K, int sms);
-int split_room_of(int split, int found, int sms) { return split >= 1 && split <= kPtMaxSplit ? split_room(split, found, sms) : 0; }
+int split_room_of(int split, int found, int sms) { return split >= 1 && split <= kPtMaxSplit ? cluster_room(2 * split, found, sms) : 0; }
 
 // The tiles of a GEMM on few weight tiles, 0: the other kernels.  *split = pairs per tile in a cluster (this kernel), 0: tiles
 // of gemm_pair_swap.cu that one wave holds.  scratch: the call has the workspace that stream-K wants.
@@ -355,7 +355,7 @@ int gemm_split_tiles(int64_t M, int64_t N, int64_t K, int epilogue, int out_f32,
   int room[kPtMaxSplit + 1];
   for (int s = 1; s <= kPtMaxSplit; ++s) {
     const bool may = w_tiles * 2 * s <= sms && 8 * (s - 1) <= kb;
-    room[s] = !may ? 0 : split_room(s, s == 1 ? pairs : split_clusters(s, sms, on), sms);
+    room[s] = !may ? 0 : cluster_room(2 * s, s == 1 ? pairs : clusters_found(2 * s, sms, on), sms);
   }
   double best = 0, swap = 0;
   int tiles = 0, swap_tiles = 0;

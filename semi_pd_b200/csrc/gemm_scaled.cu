@@ -826,13 +826,45 @@ static int few_slots(int n, int smem) {
   return slots < kFewStages ? slots : kFewStages;
 }
 
-// Clusters of 2 S CTAs that run at once, one CTA an SM (a partition: by its share of the SMs, of 6 and more CTAs less one; 16 x 5120 x 5120 on
-// 72 SMs, 20 tiles of 6 CTAs, two on an SM, went in two rounds: 14.2 us, 20 of 4 CTAs 9.1)
-static int clusters_at_once(int S, int sms) {
-  static const int b200[kMaxSplit + 1] = {0, 74, 33, 22, 15};
-  const int share = b200[S] * sms / 148 - (sms < 148 && S > 2 ? 1 : 0), most = sms / (2 * S);
-  return share < most ? share : most;
-}
+// Clusters of `ctas` CTAs, one CTA an SM, that run at once as the driver says of a stream, and how many of them to reckon with
+// (gemm_pair_split.cu): a partition's SMs stand on the chip as they do, which their number does not tell.
+int clusters_found(int ctas, int sms, cudaStream_t stream);
+int cluster_room(int ctas, int found, int sms);
+
+// Clusters of 2 S CTAs that run at once, one CTA an SM or two.  The driver counts one CTA an SM, whatever a CTA takes of it, so two an SM are
+// twice that at least; a cluster of 6 or 8 CTAs finds room where one of half as many fits, unless the SMs stand in small groups, which the
+// two counts tell by being far apart.  Clusters of 4, 6, 8 with two CTAs an SM that ran at once (CTAs noted when they began) / twice the
+// driver's count / its count for half the CTAs: whole B200 71, 45, 33 / 66, 44, 30 / 74, 45, 33; 76 SMs 33, 21, 15 / 30, 18, 12 / 38, 21, 15;
+// 72 36, 19, 18 / 36, 18, 18 / 36, 18, 18; 108 50, 30, 23 / 46, 26, 20 / 54, 30, 23; 52 18, 12, 9 / 18, 12, 6 / 26, 12, 9; 36 10, 4, 3 / 10, 4, 2 /
+// 18, 6, 5.  One too many is a second round: 20 tiles of 6 CTAs, 16 x 5120 x 5120 on 72 SMs, 14.2 us, of 4 CTAs 9.1; 36 of 4 CTAs,
+// 256 x 2304 x 8192 on 76, 22.2, 36 of 2 CTAs 15.8.  One too few costs less: 20 of 6, 64 x 5120 x 5120 on 76, 10.2, of 2 11.0.
+struct Clusters {
+  int sms;
+  cudaStream_t stream;
+  const int* found;  // the driver's answers for 1 - 8 CTAs where a caller has them, or null
+  int at_once[kMaxSplit + 1][2];
+  bool asked[kMaxSplit + 1][2];  // the others are as many as there are SMs for
+
+  Clusters(int sms, cudaStream_t stream, const int* found) : sms(sms), stream(stream), found(found) {
+    const bool whole = sms >= device_sm_count_cached();
+    for (int S = 1; S <= kMaxSplit; ++S)
+      for (int half = 0; half < 2; ++half) {
+        at_once[S][half] = half ? sms / S : sms / (2 * S);
+        asked[S][half] = S == 1;
+        if (S > 1 && (found || whole)) ask(S, half);
+      }
+  }
+  // (1 us of host time in a partition for each answer of the driver's)
+  void ask(int S, int half) {
+    at_once[S][half] = room(2 * S) * (half ? 2 : 1);
+    if (half && S > 2) {
+      const int more = room(S);
+      if (more > at_once[S][half] && 4 * more <= 5 * at_once[S][half]) at_once[S][half] = more;
+    }
+    asked[S][half] = true;
+  }
+  int room(int ctas) const { return cluster_room(ctas, found ? found[ctas - 1] : clusters_found(ctas, sms, stream), sms); }
+};
 
 // Every form's time in us as fitted to 264 products (1 - 2000 tokens; 22 weights of 1024 x 2048 to 28672 x 4096, K from 144 to 14336),
 // weights out of memory, in a row of such calls; the form chosen took 1.01 times the fastest one's time in the mean, 1.13 at most.
@@ -843,7 +875,13 @@ static int clusters_at_once(int S, int sms) {
 // weights of a single row of tiles at 5.3 GB/ms.
 // More tiles than run at once, one of tokens: 57344 x 8192 of 1 token 74 us (tokens on M 111), of 160 87 (104), 128256 x 4096 of 1 80 (131),
 // of 100 94 (97), of 256 125 (105).
-static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
+//
+// By the driver's counts, and not by the share of the whole device's that a partition has ("one fewer" of 6 and 8 CTAs), us before / now:
+// 76 SMs 16 x 4096 x 4096 13.5 / 7.5, 64 x 4096 x 14336 29.2 / 16.2, 256 x 1024 x 8192 20.3 / 10.3; 72 256 x 2304 x 8192 15.8 / 13.0;
+// 108 1 x 3584 x 8192 14.8 / 8.5; 36 64 x 3584 x 8192 24.0 / 15.2; whole 640 x 2304 x 14336 22.5 / 20.3.  Of 284 products (5 partitions) none
+// takes 4 % longer.
+static ScaledPlan fastest_plan(int64_t M, int64_t N, int kblocks, const Clusters& clusters) {
+  const int sms = clusters.sms;
   const int64_t w_tiles = (N + 255) / 256, waves = ((M + 255) / 256 * w_tiles + sms / 2 - 1) / (sms / 2);
   ScaledPlan plan{0, 1, 0};
   const double tile = 0.288 * kblocks + 1;
@@ -859,7 +897,7 @@ static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
         const bool half = smem == kHalfSmem;
         const int slots = few_slots(n, smem);
         const int64_t ctas = t * w_tiles * 2 * S;
-        const int64_t at_once = clusters_at_once(S, sms) * (half ? 2 : 1);
+        const int64_t at_once = clusters.at_once[S][half];
         const bool several = t * w_tiles > at_once;
         if (several && (t > 1 || S > 1 || !half)) continue;
         if (slots * (kGsHalf + n / 2 * kGsBlock) < n * (S > 1 ? 512 : 256)) continue;
@@ -882,6 +920,16 @@ static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, int sms) {
       }
   }
   return plan;
+}
+
+// The fastest of the forms that fit: the driver is asked only about those that would be it.
+static ScaledPlan product_plan(int64_t M, int64_t N, int kblocks, Clusters clusters) {
+  for (;;) {
+    const ScaledPlan plan = fastest_plan(M, N, kblocks, clusters);
+    const int half = plan.smem == kHalfSmem;
+    if (clusters.asked[plan.split][half]) return plan;
+    clusters.ask(plan.split, half);
+  }
 }
 
 // 16-bit operands with tokens on N: k-blocks go to up to 8 accumulators in turn, as many as half of TMEM holds (see many_logprobs_kernel)
@@ -1007,8 +1055,18 @@ int spd_int8_scaled_mm(void* out, const int8_t* a, const int8_t* b, const float*
   p.sb = scales_b;
   p.early = older_w;
   const int sms = budget(sm_budget);
-  const ScaledPlan plan = product_plan(M, N, static_cast<int>((K + kGsBlock - 1) / kGsBlock), sms);
+  const ScaledPlan plan = product_plan(M, N, static_cast<int>((K + kGsBlock - 1) / kGsBlock), {sms, as_stream(stream), nullptr});
   SPD_DISPATCH_DTYPE(dtype, { return (scaled_product<kInt8, kScaled, T>(a, b, M, N, K, lda, ldb, p, plan, sms, as_stream(stream))); });
+}
+
+int spd_int8_scaled_mm_tiles(int64_t M, int64_t N, int64_t K, int sm_budget, const int* clusters, int* split, int* ctas_per_sm) {
+  SPD_REQUIRE(M > 0 && N > 0 && K > 0 && M <= 0x7fffff00 && N <= 0x7fffff00 && K < 131072 && split && ctas_per_sm, SPD_E_BADARG,
+              "spd_int8_scaled_mm_tiles: bad arguments");
+  const int sms = budget(sm_budget);
+  const ScaledPlan plan = product_plan(M, N, static_cast<int>((K + kGsBlock - 1) / kGsBlock), {sms, nullptr, clusters});
+  *split = plan.split;
+  *ctas_per_sm = plan.tok_tiles > 0 && plan.smem == kHalfSmem ? 2 : 1;
+  return plan.tok_tiles;
 }
 
 int64_t spd_linear_logprobs_workspace_bytes(int64_t M, int64_t V) {
