@@ -31,6 +31,13 @@ def pytest_collection_modifyitems(config, items):
             item.add_marker(skip)
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    """Inputs that a test draws without a generator are the same in every run."""
+    import torch
+    torch.manual_seed(0)
+
+
 @pytest.fixture(scope="session")
 def golden():
     import torch
