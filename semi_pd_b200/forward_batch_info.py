@@ -91,7 +91,7 @@ class ModelWorkerBatch:
     # schedulers do not ask for them (semi_pd_decode_scheduler.py:354)
     return_logprob: bool = False
     # [T] int64, device: the token whose log-probability every row is asked for, -1: none (logits_processor.py:
-    # extend_input_logprob_token_ids_gpu); None: the request's next token
+    # extend_input_logprob_token_ids_gpu); None: the request's next token in this batch
     extend_input_logprob_token_ids: Optional[torch.Tensor] = None
     sampling_info: object = None
     # TP > 1: all-gather the vocab-sharded logits (logits_processor.py:426-427).  The semi-PD

@@ -4,8 +4,8 @@ python/sglang/srt/managers/schedule_batch.py the semi-PD path exercises:
 `pre_allocated_req_pool_indices` variant the prefill worker uses, :923-935),
 `prepare_for_decode` (:1144-1207), `filter_batch` / `merge_batch` (:1209-1306),
 `check_decode_mem` / `retract_decode` (:1022-1125) and `get_model_worker_batch` (:1308-1370).
-Sampling is greedy-only; grammar / multimodal are off this path; `return_logprob` on a batch gives its input tokens' logprobs
-(managers/semi_pd_scheduler.py:207-209, semi_pd_decode_scheduler.py:354).
+Sampling is greedy-only; grammar / multimodal are off this path (managers/semi_pd_scheduler.py:207-209,
+semi_pd_decode_scheduler.py:354); `return_logprob` on a batch gives its input tokens' logprobs.
 """
 from __future__ import annotations
 
@@ -116,11 +116,34 @@ class ScheduleBatch:
         self.decoding_reqs = None
         self._shared = None   # (groups of the last step, SharedPrefix, its lists)
         self._compacted = False   # some request may have dropped tokens
+        # the log-probabilities of an extend batch's input tokens (schedule_batch.py: return_logprob); a decode batch has none
+        self.return_logprob = False
+        self._logprob_token_ids: Optional[torch.Tensor] = None
+        self._logprob_token_ids_used = False
 
     @classmethod
     def init_new(cls, reqs, req_to_token_pool, token_to_kv_pool_allocator, device=None):
         return cls(reqs, req_to_token_pool, token_to_kv_pool_allocator,
                    device or req_to_token_pool.device)
+
+    @property
+    def extend_input_logprob_token_ids(self) -> Optional[torch.Tensor]:
+        """[T] int64: tokens of the caller's own whose log-probabilities the rows of the next extend batch are asked for (-1: none),
+        set before or after prepare_for_extend; a batch that is prepared again has used them up.  None: every row's next token of
+        its request, behind a chunk's last row too, as far as it is known."""
+        return self._logprob_token_ids
+
+    @extend_input_logprob_token_ids.setter
+    def extend_input_logprob_token_ids(self, ids: Optional[torch.Tensor]):
+        self._logprob_token_ids, self._logprob_token_ids_used = ids, False
+
+    def _next_input_tokens(self) -> torch.Tensor:
+        ids = []
+        for r, pre in zip(self.reqs, self.prefix_lens):
+            end = len(r.fill_ids)
+            known = r.fill_ids + (r.origin_input_ids + r.output_ids)[end:end + 1]
+            ids += known[pre + 1:] + [-1] * (end + 1 - len(known)) if end > pre else []
+        return self._h2d(ids, torch.int64)
 
     def batch_size(self):
         return len(self.reqs)
@@ -150,6 +173,8 @@ class ScheduleBatch:
         req_to_token.  Prefill-side call: adopts the request slots the decode side chose and reads
         out_cache_loc back from the shared req_to_token table (schedule_batch.py:923-935)."""
         self.forward_mode = ForwardMode.EXTEND
+        if self._logprob_token_ids_used:
+            self.extend_input_logprob_token_ids = None
         bs = len(self.reqs)
         reqs = self.reqs
         if any(r.dropped_tokens for r in reqs):
@@ -360,6 +385,13 @@ class ScheduleBatch:
         global _bid
         _bid += 1
         extend = self.forward_mode.is_extend()
+        logprob = extend and self.return_logprob
+        token_ids = None
+        if extend:
+            token_ids = self._logprob_token_ids
+            self._logprob_token_ids_used = True
+            if token_ids is None and logprob:
+                token_ids = self._next_input_tokens()
         return ModelWorkerBatch(
             bid=_bid, forward_mode=self.forward_mode, input_ids=self.input_ids,
             req_pool_indices=self.req_pool_indices, seq_lens=self.seq_lens,
@@ -370,8 +402,8 @@ class ScheduleBatch:
             extend_seq_lens=self.extend_lens if extend else None,
             extend_prefix_lens=self.prefix_lens if extend else None,
             extend_logprob_start_lens=[0] * len(self.reqs) if extend else None,
-            return_logprob=getattr(self, "return_logprob", False),
-            extend_input_logprob_token_ids=getattr(self, "extend_input_logprob_token_ids", None) if extend else None,
+            return_logprob=logprob,
+            extend_input_logprob_token_ids=token_ids,
             gather_logits=getattr(self, "gather_logits", True),
             extend_logit_rows=getattr(self, "extend_logit_rows", None) if extend else None)
 
