@@ -87,8 +87,9 @@ class ModelWorkerBatch:
     extend_seq_lens: Optional[List[int]] = None
     extend_prefix_lens: Optional[List[int]] = None
     extend_logprob_start_lens: Optional[List[int]] = None
-    # the log-probabilities of the input tokens come back beside the logits (LogitsProcessor.input_token_logprobs); the semi-PD
-    # schedulers do not ask for them (semi_pd_decode_scheduler.py:354)
+    # extend: the log-probabilities of the input tokens, of all rows, come back beside the logits
+    # (LogitsProcessor.input_token_logprobs); decode batches, --tp > 1 and the hybrid families refuse it, the semi-PD schedulers
+    # do not ask for them (semi_pd_decode_scheduler.py:354)
     return_logprob: bool = False
     # [T] int64, device: the token whose log-probability every row is asked for, -1: none (logits_processor.py:
     # extend_input_logprob_token_ids_gpu); None: the request's next token in this batch

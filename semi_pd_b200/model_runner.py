@@ -234,6 +234,8 @@ class ModelRunner:
     def forward(self, forward_batch: ForwardBatch, skip_attn_backend_init: bool = False
                 ) -> LogitsProcessorOutput:
         set_current_comm(self.tp_comm)
+        if forward_batch.return_logprob and forward_batch.forward_mode.is_decode():
+            raise NotImplementedError("return_logprob of a decode batch: log-probabilities are those of an extend batch's tokens")
         if (forward_batch.forward_mode.is_cuda_graph() and self.cuda_graph_runner
                 and self.cuda_graph_runner.can_run(forward_batch)):
             return self.cuda_graph_runner.replay(forward_batch,
