@@ -153,7 +153,10 @@ class LinearBase:
 
     def quantize_weight_int8(self) -> None:
         """A 16-bit weight as 8-bit integers, a row's largest value 127."""
-        self.weight, self.weight_scale = ops.per_token_quant_int8(self.weight)
+        self.weight, scale = ops.per_token_quant_int8(self.weight)
+        # A copy: the products read the weight before they wait for this library's kernels right before them (older_weight), each of
+        # which lets the next one in early, the quantisation of this weight among them; behind a copy all of it is there.
+        self.weight_scale = scale.clone()
 
     def _product(self, x: Union[torch.Tensor, QuantizedTokens]) -> torch.Tensor:
         if self.weight_scale is None:
