@@ -205,16 +205,25 @@ class LlamaForCausalLM:
                 if isinstance(holder, LinearBase):
                     yield name + "_scale", holder, (lambda w: w) if isinstance(holder, RowParallelLinear) else shard
 
-    def _set_weight(self, holder, weight: torch.Tensor):
+    def _set_weight(self, name: str, holder, weight: torch.Tensor):
         """A loaded shard: 8-bit integers stay (their scales are loaded beside them), 16-bit ones of a quantised model become such."""
-        if not isinstance(holder, LinearBase):
-            holder.weight = weight
-            return
-        if weight.dtype == torch.int8 and self.quantization is None:
-            raise ValueError("8-bit weights need quantization='w8a8_int8'")
-        holder.weight, holder.weight_scale = weight, None
-        if self.quantization is not None and weight.dtype != torch.int8:
-            holder.quantize_weight_int8()
+        linear = isinstance(holder, LinearBase)
+        if weight.dtype == torch.int8:
+            if self.quantization is None:
+                raise ValueError(f"{name}: 8-bit weights need quantization='w8a8_int8'")
+            if not linear:
+                raise ValueError(f"{name}: only the weights of products are 8-bit integers")
+        if linear and self.quantization is not None:
+            rows, cols = weight.shape
+            most = 131071 if weight.dtype == torch.int8 else 32768  # (what ops.int8_scaled_mm and ops.per_token_quant_int8 take)
+            if rows % 8 or cols % 16 or cols > most:
+                raise ValueError(f"{name}: a shard of {rows} x {cols} in 8-bit integers; rows are a multiple of 8, columns of 16 and "
+                                 f"at most {most}")
+        holder.weight = weight
+        if linear:
+            holder.weight_scale = None
+            if self.quantization is not None and weight.dtype != torch.int8:
+                holder.quantize_weight_int8()
 
     def full_shapes(self) -> Dict[str, Tuple[int, ...]]:
         cfg = self.config
@@ -248,7 +257,7 @@ class LlamaForCausalLM:
                     continue
                 raise KeyError(f"unexpected parameter {name}")
             holder, shard = slots[name]
-            self._set_weight(holder, shard(w if w.dtype == torch.int8 else w.to(self.dtype)).to(self.device).contiguous())
+            self._set_weight(name, holder, shard(w if w.dtype == torch.int8 else w.to(self.dtype)).to(self.device).contiguous())
             seen.add(name)
         missing = set(slots) - seen
         if missing:
@@ -291,7 +300,7 @@ class LlamaForCausalLM:
             if name not in slots:
                 continue
             holder, shard = slots[name]
-            self._set_weight(holder, shard(w).contiguous())
+            self._set_weight(name, holder, shard(w).contiguous())
 
     def state_dict(self) -> Dict[str, torch.Tensor]:
         """The local (sharded) parameters by checkpoint name."""
