@@ -51,8 +51,10 @@ class RMSNorm:
     __call__ = forward
 
     def forward_quant(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
-        """forward() for a layer of 8-bit weights: the normed tokens as QuantizedTokens, quantised in the same pass."""
+        """forward() for a layer of 8-bit weights: the normed tokens as QuantizedTokens, quantised in the same pass.  Behind a sum over
+        the ranks, whose kernel writes the normed tokens in 16 bits, they are quantised from those."""
         if residual is None:
+            assert not getattr(x, "_spd_pending_all_reduce", False)
             return QuantizedTokens(*ops.rmsnorm_quant_int8(x, self.weight, self.variance_epsilon), x.dtype)
         if getattr(x, "_spd_pending_all_reduce", False):  # the sum over the ranks comes first
             x, residual = self.forward(x, residual)

@@ -1,4 +1,5 @@
 """A layer that quantises its weight: what its products may read early is behind a copy in the stream."""
+import pytest
 import torch
 
 from semi_pd_b200 import layers
@@ -25,3 +26,21 @@ def test_a_copy_stands_between_the_quantisation_and_the_products(monkeypatch):
     assert order == ["quant", "clone"]
     assert torch.equal(layer.weight, quantised[0]) and torch.equal(layer.weight_scale.as_subclass(torch.Tensor), quantised[1])
     assert layer.weight_scale.data_ptr() != quantised[1].data_ptr()
+
+
+def test_a_sum_over_the_ranks_is_not_left_out(monkeypatch):
+    calls = []
+    for name in ("rmsnorm_quant_int8", "fused_add_rmsnorm_quant_int8", "per_token_quant_int8"):
+        monkeypatch.setattr(layers.ops, name, lambda x, *a, name=name: (calls.append(name), (x, x))[1])
+    norm = layers.RMSNorm(16)
+    x = torch.zeros(2, 16)
+    norm.forward_quant(x)
+    norm.forward_quant(x, torch.zeros(2, 16))
+    assert calls == ["rmsnorm_quant_int8", "fused_add_rmsnorm_quant_int8"]
+    x._spd_pending_all_reduce = True
+    with pytest.raises(AssertionError):
+        norm.forward_quant(x)
+    reduced = torch.ones(2, 16)
+    monkeypatch.setattr(layers.RMSNorm, "forward", lambda self, x, residual: (reduced, residual + 1))
+    tokens, residual = norm.forward_quant(x, torch.zeros(2, 16))
+    assert tokens.q is reduced and residual.sum() == 32 and calls[2:] == ["per_token_quant_int8"]
