@@ -867,7 +867,7 @@ struct Clusters {
 };
 
 // Every form's time in us as fitted to 264 products (1 - 2000 tokens; 22 weights of 1024 x 2048 to 28672 x 4096, K from 144 to 14336),
-// weights out of memory, in a row of such calls; the form chosen took 1.01 times the fastest one's time in the mean, 1.13 at most.
+// weights out of memory, in a row of such calls; the form chosen took 1.013 times the fastest one's time in the mean, 1.12 at most.
 // Tokens on N, all tiles at once: a k-block of 128 bytes takes a pair 0.15 to 0.24 (half the ring: 1.65 times that), two pairs on an
 // SM 0.09 to 0.29 each; the weights 8.6 GB/ms, and two thirds of that again for every further tile of tokens that reads them.  Where the
 // next call's CTAs fit beside this one's, what their rings hold is on its way before this one ends: 0.4 of that share.  Then the
